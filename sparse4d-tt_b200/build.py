@@ -1,12 +1,14 @@
-"""Build ``lib/libs4d_dfa.so`` (the C ABI of ``include/s4d_dfa.h``) for sm_100a with nvcc.
+"""Build ``lib/libs4d_dfa.so`` (the C ABI of ``include/s4d_dfa.h``) and ``lib/libs4d_decoder.so``
+(``include/s4d_decoder.h``) for sm_100a with nvcc.
 
     python sparse4d-tt_b200/build.py [--verbose-ptxas]
 
-The library is built in-tree so that it travels with the repository; nothing is installed.
+The libraries are built in-tree so that they travel with the repository; nothing is installed.
 """
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -20,6 +22,9 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libs4d_dfa.so")
 SOURCES = ["capi.cu", "kps_project.cu", "dfa_gather.cu", "kps_noalloc.cu", "linear_tc.cu", "camera_encoder.cu", "pack_maps.cu",
            "instance_bank.cu", "peer.cu", "layer_norm.cu"]
+# The decoder's operators: each source is compiled by itself, several at a time.
+DECODER_LIB_PATH = os.path.join(LIB_DIR, "libs4d_decoder.so")
+DECODER_SOURCES = ["decoder_capi.cu", "decoder_norm.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -28,6 +33,45 @@ def nvcc_path() -> str:
         if cand and os.path.exists(cand):
             return cand
     raise RuntimeError("nvcc not found (set NVCC or put /usr/local/cuda/bin on PATH)")
+
+
+def _run(cmd, what: str, verbose_ptxas: bool) -> None:
+    if verbose_ptxas:
+        cmd = [cmd[0], "-Xptxas", "-v", *cmd[1:]]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"nvcc failed building {what}")
+    if verbose_ptxas:
+        sys.stdout.write(res.stderr)
+
+
+def build_decoder(verbose_ptxas: bool = False, force: bool = False) -> str:
+    """``libs4d_decoder.so``: objects newer than their source and every header are kept."""
+    obj_dir = os.path.join(LIB_DIR, "obj")
+    headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".cuh")]
+    headers += [os.path.join(INCLUDE, h) for h in os.listdir(INCLUDE)] + [os.path.abspath(__file__)]
+    newest_header = max(os.path.getmtime(h) for h in headers)
+    os.makedirs(obj_dir, exist_ok=True)
+    flags = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
+             "-I", INCLUDE, "-I", CSRC]
+    objs, jobs = [], []
+    for s in DECODER_SOURCES:
+        src, obj = os.path.join(CSRC, s), os.path.join(obj_dir, s[:-3] + ".o")
+        objs.append(obj)
+        if force or verbose_ptxas or not os.path.exists(obj) or os.path.getmtime(obj) < max(newest_header,
+                                                                                            os.path.getmtime(src)):
+            jobs.append((src, obj))
+    with concurrent.futures.ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
+        for f in [pool.submit(_run, [nvcc_path(), *flags, "-c", "-o", obj, src], os.path.basename(src), verbose_ptxas)
+                  for src, obj in jobs]:
+            f.result()
+    if jobs or not os.path.exists(DECODER_LIB_PATH) or any(os.path.getmtime(o) > os.path.getmtime(DECODER_LIB_PATH)
+                                                           for o in objs):
+        _run([nvcc_path(), *ARCH_FLAGS, "--shared", "-o", DECODER_LIB_PATH + ".tmp", *objs, "-lcudart"],
+             "libs4d_decoder.so", False)
+        os.replace(DECODER_LIB_PATH + ".tmp", DECODER_LIB_PATH)
+    return DECODER_LIB_PATH
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:
@@ -60,3 +104,4 @@ if __name__ == "__main__":
     ap.add_argument("--force", action="store_true")
     a = ap.parse_args()
     print(build(a.verbose_ptxas, a.force))
+    print(build_decoder(a.verbose_ptxas, a.force))

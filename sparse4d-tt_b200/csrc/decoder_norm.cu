@@ -1,0 +1,470 @@
+// LayerNorm rows of any width up to 16384, forward and backward (f32, bf16, f16).
+//
+// Forward, one row r of N values:   n = (x - mean) rstd,  y = n w + b.
+// Backward, with g = dy w:          dx = rstd (g - mean(g) - n mean(g n)),
+//                                   dw = sum_r dy n,  db = sum_r dy.
+// Both are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.
+// So each row is read once, into the registers of a group of W warps (16 values a thread at most:
+// W = 1 up to 512 columns, 2 up to 1024, ... 32 up to 16384), in 16-byte vectors where the row
+// pointers and strides allow it and single elements otherwise; the mean and then the variance of
+// the deviations from it (no cancellation for rows far from zero) are reduced by shuffles and,
+// for W > 1, through shared memory.
+//
+// The sums over rows for dw and db stay in registers: a block keeps its columns and walks the rows
+// with the stride of a grid that just fills the SMs, adds its row groups through shared memory
+// and writes one fp32 partial row per block; a second launch adds the partial rows in block order.
+// No atomics: the order of every addition depends on the sizes alone.
+#include "decoder_types.cuh"
+
+namespace s4d {
+namespace {
+
+struct NormParams {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const void* bias;
+  void* y;   // forward: y; backward: dx (may be null)
+  float* mean;
+  float* rstd;
+  float* partial;  // [gridDim.x, 2, width]: dw then db of each block, or null
+  int64_t x_ld, dy_ld, y_ld;
+  int64_t rows;
+  int width;
+  int param_f32;  // weight and bias are f32 (else T)
+  float eps;
+};
+
+constexpr int kNormMaxWidth = 16384;
+constexpr int kEpt = 16;  // values a thread holds of one row
+
+template <int W>
+struct Group {
+  static constexpr int kWarps = W < 8 ? 8 : W;      // warps of a block
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRows = kWarps / W;          // rows a block holds at a time
+};
+
+// Sum over the W warps of a group; every thread gets it.  `red` holds one value per warp and is
+// used once between two block barriers.
+template <int W>
+__device__ __forceinline__ float group_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (W > 1) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    const float* r = red + warp / W * W;
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += r[i];
+  }
+  return v;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_param(const void* p, bool f32, int col, float (&f)[VEC]) {
+  if (f32) {
+    const float* q = static_cast<const float*>(p) + col;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = __ldg(q + i);
+  } else {
+    const T* q = static_cast<const T*>(p) + col;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_f32<T>(q[i]);
+  }
+}
+
+// Chunk k of a thread covers columns [col, col + VEC), col = (k * 32 W + thread of the group) VEC.
+template <typename T, int W, int VEC, int K>
+__global__ void __launch_bounds__(Group<W>::kThreads) norm_forward_kernel(const NormParams p) {
+  __shared__ float red[2][Group<W>::kWarps];
+  const int gt = threadIdx.x % (32 * W);
+  const int64_t row = int64_t(blockIdx.x) * Group<W>::kRows + threadIdx.x / (32 * W);
+  const bool live = row < p.rows;
+  if (W == 1 && !live) return;  // whole warps: no block barrier below
+  const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.x_ld;
+  float v[K][VEC];
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = (k * 32 * W + gt) * VEC;
+    if (live && col < p.width) {
+      load_vec<T, VEC>(xr + col, v[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[k][i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s += v[k][i];
+  const float inv = 1.0f / float(p.width);
+  const float mean = group_sum<W>(s, red[0]) * inv;
+  float q = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if ((k * 32 * W + gt) * VEC < p.width) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float d = v[k][i] - mean;
+        q = fmaf(d, d, q);
+      }
+    }
+  }
+  const float rstd = 1.0f / sqrtf(group_sum<W>(q, red[1]) * inv + p.eps);
+  if (!live) return;
+  if (gt == 0 && p.mean != nullptr) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  T* yr = static_cast<T*>(p.y) + row * p.y_ld;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = (k * 32 * W + gt) * VEC;
+    if (col >= p.width) break;
+    float o[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = (v[k][i] - mean) * rstd;
+    if (p.weight != nullptr) {
+      float w[VEC];
+      load_param<T, VEC>(p.weight, p.param_f32, col, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] *= w[i];
+    }
+    if (p.bias != nullptr) {
+      float b[VEC];
+      load_param<T, VEC>(p.bias, p.param_f32, col, b);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] += b[i];
+    }
+    store_vec<T, VEC>(yr + col, o);
+  }
+}
+
+template <typename T, int W, int VEC, int K>
+__global__ void __launch_bounds__(Group<W>::kThreads) norm_backward_kernel(const NormParams p) {
+  constexpr int R = Group<W>::kRows;
+  __shared__ float red[2][2][Group<W>::kWarps];  // two sums, two buffers: one barrier a row
+  // partial sums of the block's other row groups, one 32-column-wide slice of a warp at a time
+  __shared__ float join[R > 1 ? 2 * R * 32 * W * VEC : 1];
+  const int group = threadIdx.x / (32 * W), gt = threadIdx.x % (32 * W);
+  griddep_launch_dependents();  // the reduction waits for this whole launch before it reads
+  float w[K][VEC], aw[K][VEC], ab[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = (k * 32 * W + gt) * VEC;
+    if (p.weight != nullptr && col < p.width) {
+      load_param<T, VEC>(p.weight, p.param_f32, col, w[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[k][i] = 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) aw[k][i] = 0.0f, ab[k][i] = 0.0f;
+  }
+  const float inv = 1.0f / float(p.width);
+  int buf = 0;
+  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += int64_t(gridDim.x) * R, buf ^= 1) {
+    const int64_t row = base + group;
+    const bool live = row < p.rows;
+    const int64_t r = live ? row : 0;
+    const T* xr = static_cast<const T*>(p.x) + r * p.x_ld;
+    const T* dyr = static_cast<const T*>(p.dy) + r * p.dy_ld;
+    float n[K][VEC], g[K][VEC];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * 32 * W + gt) * VEC;
+      if (live && col < p.width) {
+        load_vec<T, VEC>(xr + col, n[k]);
+        load_vec<T, VEC>(dyr + col, g[k]);
+      }
+    }
+    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool in = live && (k * 32 * W + gt) * VEC < p.width;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float nn = in ? (n[k][i] - mean) * rstd : 0.0f, d = in ? g[k][i] : 0.0f;
+        aw[k][i] = fmaf(d, nn, aw[k][i]);
+        ab[k][i] += d;
+        n[k][i] = nn;
+        g[k][i] = d * w[k][i];
+        s1 += g[k][i];
+        s2 = fmaf(g[k][i], nn, s2);
+      }
+    }
+    if (p.y == nullptr) continue;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    }
+    if constexpr (W > 1) {
+      const int warp = threadIdx.x >> 5;
+      if ((threadIdx.x & 31) == 0) red[buf][0][warp] = s1, red[buf][1][warp] = s2;
+      __syncthreads();
+      const int w0 = warp / W * W;
+      s1 = s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) s1 += red[buf][0][w0 + i], s2 += red[buf][1][w0 + i];
+    }
+    if (!live) continue;
+    s1 *= inv, s2 *= inv;
+    T* dxr = static_cast<T*>(p.y) + row * p.y_ld;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * 32 * W + gt) * VEC;
+      if (col >= p.width) break;
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = rstd * (g[k][i] - s1 - n[k][i] * s2);
+      store_vec<T, VEC>(dxr + col, o);
+    }
+  }
+  if (p.partial == nullptr) return;
+  float* pw = p.partial + int64_t(blockIdx.x) * 2 * p.width;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = (k * 32 * W + gt) * VEC;
+    if constexpr (R > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        join[(group * VEC + i) * 32 * W + gt] = aw[k][i];
+        join[((R + group) * VEC + i) * 32 * W + gt] = ab[k][i];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float a = 0.0f, b = 0.0f;
+          for (int j = 0; j < R; ++j) {
+            a += join[(j * VEC + i) * 32 * W + gt];
+            b += join[((R + j) * VEC + i) * 32 * W + gt];
+          }
+          aw[k][i] = a, ab[k][i] = b;
+        }
+      }
+    }
+    if (group == 0 && col < p.width) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) pw[col + i] = aw[k][i], pw[p.width + col + i] = ab[k][i];
+    }
+  }
+}
+
+// dw and db from the blocks' partial rows: 32 columns a block, its 32 warps each adding every
+// 32nd partial row, then the 32 sums in warp order.
+template <typename P>
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* partial, int blocks, int width, P* dweight,
+                                                           P* dbias) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane;
+  P* out = blockIdx.y == 0 ? dweight : dbias;
+  griddep_wait();
+  if (out == nullptr) return;
+  const float* src = partial + int64_t(blockIdx.y) * width + col;
+  float s = 0.0f;
+  if (col < width) {
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += 32) s += src[int64_t(b) * 2 * width];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < width) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sums[i][lane];
+    out[col] = from_f32<P>(s);
+  }
+}
+
+// Warps a row is spread over: the fewest that hold it at kEpt values a thread.
+int warps_for(int64_t width) {
+  int w = 1;
+  while (int64_t(w) * 32 * kEpt < width) w *= 2;
+  return w;
+}
+
+int rows_per_block(int w) { return w < 8 ? 8 / w : 1; }
+
+// Blocks of the backward launch: enough to fill the SMs at the registers its threads need (16
+// warps an SM: two blocks of 256 threads, one of 512 or 1024), fewer when there are fewer rows.
+int64_t backward_blocks(int64_t rows, int64_t width) {
+  const int w = warps_for(width), r = rows_per_block(w);
+  const int64_t need = (rows + r - 1) / r;
+  const int64_t fill = int64_t(device_sms()) * (w <= 8 ? 2 : 1);
+  return need < fill ? need : fill;
+}
+
+template <typename T, int W, int VEC, int K>
+int launch_norm(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
+  const dim3 grid{static_cast<unsigned>(blocks)};
+  if (backward) {
+    norm_backward_kernel<T, W, VEC, K><<<grid, Group<W>::kThreads, 0, st>>>(p);
+    return cuda_check(cudaGetLastError(), "norm_backward_kernel launch");
+  }
+  norm_forward_kernel<T, W, VEC, K><<<grid, Group<W>::kThreads, 0, st>>>(p);
+  return cuda_check(cudaGetLastError(), "norm_forward_kernel launch");
+}
+
+template <typename T, int VEC>
+int dispatch_width(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
+  constexpr int K = kEpt / VEC;
+  switch (warps_for(p.width)) {
+    case 1:
+      // narrow rows: only as many chunks as the width needs (a decoder row of 256 is half of 512)
+      if constexpr (K > 1) {
+        if (p.width <= 32 * kEpt / 2) return launch_norm<T, 1, VEC, K / 2>(backward, p, blocks, st);
+      }
+      return launch_norm<T, 1, VEC, K>(backward, p, blocks, st);
+    case 2: return launch_norm<T, 2, VEC, K>(backward, p, blocks, st);
+    case 4: return launch_norm<T, 4, VEC, K>(backward, p, blocks, st);
+    case 8: return launch_norm<T, 8, VEC, K>(backward, p, blocks, st);
+    case 16: return launch_norm<T, 16, VEC, K>(backward, p, blocks, st);
+    default: return launch_norm<T, 32, VEC, K>(backward, p, blocks, st);
+  }
+}
+
+bool vector_rows(const void* p, int64_t ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+
+template <typename T>
+int dispatch_vector(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = p.width % VEC == 0 && vector_rows(p.x, p.x_ld, sizeof(T)) && vector_rows(p.y, p.y_ld, sizeof(T)) &&
+                   vector_rows(p.dy, p.dy_ld, sizeof(T));
+  return vec ? dispatch_width<T, VEC>(backward, p, blocks, st) : dispatch_width<T, 1>(backward, p, blocks, st);
+}
+
+int dispatch_type(bool backward, int dtype, const NormParams& p, int64_t blocks, cudaStream_t st) {
+  switch (dtype) {
+    case S4D_DTYPE_F32: return dispatch_vector<float>(backward, p, blocks, st);
+    case S4D_DTYPE_BF16: return dispatch_vector<__nv_bfloat16>(backward, p, blocks, st);
+    default: return dispatch_vector<__half>(backward, p, blocks, st);
+  }
+}
+
+int type_size(int dtype) { return dtype == S4D_DTYPE_F32 ? 4 : 2; }
+
+bool aligned_to(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % uintptr_t(size) == 0; }
+
+// The checks both directions share (fn names the entry point).
+int check_norm(const char* fn, int dtype, int param_dtype, int64_t rows, int64_t width, int64_t ld_a, int64_t ld_b,
+               int64_t ld_out) {
+  if (dtype != S4D_DTYPE_F32 && dtype != S4D_DTYPE_BF16 && dtype != S4D_DTYPE_F16) {
+    set_error("%s: unknown dtype", fn);
+    return S4D_ERR_INVALID_ARG;
+  }
+  if (param_dtype != S4D_DTYPE_F32 && param_dtype != dtype) {
+    set_error("%s: weight and bias must be f32 or of the input's dtype", fn);
+    return S4D_ERR_INVALID_ARG;
+  }
+  if (rows < 0 || width <= 0) {
+    set_error("%s: rows must be >= 0 and width >= 1", fn);
+    return S4D_ERR_INVALID_ARG;
+  }
+  if (width > kNormMaxWidth) {
+    set_error("%s: width must be <= %d", fn, kNormMaxWidth);
+    return S4D_ERR_UNSUPPORTED_SHAPE;
+  }
+  int64_t span = 0;
+  if (ld_a < 0 || ld_b < 0 || (rows > 1 && ld_out < width)) {
+    set_error("%s: row strides must be >= 0, the output's >= width", fn);
+    return S4D_ERR_INVALID_ARG;
+  }
+  if (rows > 0x7fffffff || !size_product({rows, ld_a}, int64_t(1) << 46, &span) ||
+      !size_product({rows, ld_b}, int64_t(1) << 46, &span) || !size_product({rows, ld_out}, int64_t(1) << 46, &span)) {
+    set_error("%s: too many rows or elements", fn);
+    return S4D_ERR_UNSUPPORTED_SHAPE;
+  }
+  return S4D_OK;
+}
+
+}  // namespace
+}  // namespace s4d
+
+using namespace s4d;
+
+extern "C" {
+
+int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void* weight, const void* bias, int param_dtype,
+                     void* y, int64_t y_ld, float* mean, float* rstd, int64_t rows, int64_t width, float eps,
+                     void* stream) {
+  set_error("%s", "");
+  const int st = check_norm("s4d_norm_forward", dtype, param_dtype, rows, width, x_ld, 0, y_ld);
+  if (st != S4D_OK) return st;
+  if (!(eps >= 0.0f)) return fail(S4D_ERR_INVALID_ARG, "s4d_norm_forward: eps must be >= 0");
+  if (rows == 0) return S4D_OK;
+  if (x == nullptr || y == nullptr) return fail(S4D_ERR_INVALID_ARG, "s4d_norm_forward: null pointer");
+  if ((mean == nullptr) != (rstd == nullptr))
+    return fail(S4D_ERR_INVALID_ARG, "s4d_norm_forward: mean and rstd go together");
+  const int size = type_size(dtype), psize = type_size(param_dtype);
+  if (!aligned_to(x, size) || !aligned_to(y, size) || !aligned_to(weight, psize) || !aligned_to(bias, psize) ||
+      !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return fail(S4D_ERR_INVALID_ARG, "s4d_norm_forward: misaligned pointer");
+  NormParams p{};
+  p.x = x, p.x_ld = x_ld, p.weight = weight, p.bias = bias, p.y = y, p.y_ld = y_ld;
+  p.mean = mean, p.rstd = rstd, p.rows = rows, p.width = int(width), p.eps = eps;
+  p.param_f32 = param_dtype == S4D_DTYPE_F32;
+  const int r = rows_per_block(warps_for(width));
+  return dispatch_type(false, dtype, p, (rows + r - 1) / r, static_cast<cudaStream_t>(stream));
+}
+
+size_t s4d_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
+  if (rows <= 0 || width <= 0 || width > kNormMaxWidth || rows > 0x7fffffff) return 0;
+  return size_t(backward_blocks(rows, width)) * 2 * size_t(width) * sizeof(float);
+}
+
+int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, const void* weight,
+                      int param_dtype, const float* mean, const float* rstd, void* dx, int64_t dx_ld, void* dweight,
+                      void* dbias, int64_t rows, int64_t width, void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("%s", "");
+  int st = check_norm("s4d_norm_backward", dtype, param_dtype, rows, width, x_ld, dy_ld, dx == nullptr ? width : dx_ld);
+  if (st != S4D_OK) return st;
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  if (rows > 0 && (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr))
+    return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: null pointer");
+  const int size = type_size(dtype), psize = type_size(param_dtype);
+  if (!aligned_to(dy, size) || !aligned_to(x, size) || !aligned_to(dx, size) || !aligned_to(weight, psize) ||
+      !aligned_to(dweight, psize) || !aligned_to(dbias, psize) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: misaligned pointer");
+  const int64_t blocks = rows > 0 ? backward_blocks(rows, width) : 0;
+  if (sums && rows > 0 &&
+      (workspace == nullptr || !aligned_to(workspace, 16) ||
+       workspace_bytes < s4d_norm_backward_workspace_bytes(rows, width)))
+    return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: missing, misaligned or small workspace");
+  cudaStream_t stm = static_cast<cudaStream_t>(stream);
+  if (rows > 0 && (sums || dx != nullptr)) {
+    NormParams p{};
+    p.x = x, p.x_ld = x_ld, p.dy = dy, p.dy_ld = dy_ld, p.weight = weight, p.y = dx, p.y_ld = dx == nullptr ? 0 : dx_ld;
+    p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd), p.rows = rows, p.width = int(width);
+    p.param_f32 = param_dtype == S4D_DTYPE_F32;
+    p.partial = sums ? static_cast<float*>(workspace) : nullptr;
+    st = dispatch_type(true, dtype, p, blocks, stm);
+    if (st != S4D_OK) return st;
+  }
+  if (!sums) return S4D_OK;
+  const dim3 grid(unsigned((width + 31) / 32), 2);
+  const float* partial = static_cast<const float*>(workspace);
+  cudaError_t e;
+  if (param_dtype == S4D_DTYPE_F32)
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<float>, grid, dim3(1024), 0, stm, partial, int(blocks), int(width),
+                   static_cast<float*>(dweight), static_cast<float*>(dbias));
+  else if (param_dtype == S4D_DTYPE_BF16)
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<__nv_bfloat16>, grid, dim3(1024), 0, stm, partial, int(blocks),
+                   int(width), static_cast<__nv_bfloat16*>(dweight), static_cast<__nv_bfloat16*>(dbias));
+  else
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<__half>, grid, dim3(1024), 0, stm, partial, int(blocks), int(width),
+                   static_cast<__half*>(dweight), static_cast<__half*>(dbias));
+  return cuda_check(e, "norm_reduce_kernel launch");
+}
+
+}  // extern "C"
