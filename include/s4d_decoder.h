@@ -2,6 +2,9 @@
  * s4d_decoder.h -- C ABI of the decoder's dense operators on B200 (sm_100a), the layers that
  * stand around the DeformableFeatureAggregation path of s4d_dfa.h:
  *
+ *   s4d_attention_forward               attention over shared or own heads with scores capped by a
+ *                                       tanh, a bias by distance, a document mask and a valid length
+ *                                       per batch entry, for one query or many.
  *   s4d_norm_forward / _backward        LayerNorm rows of any width up to 16384 in f32, bf16 or
  *                                       f16, with the gradients of the input, weight and bias.
  *
@@ -47,6 +50,54 @@ S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int6
                               const void* weight, int param_dtype, const float* mean, const float* rstd, void* dx,
                               int64_t dx_ld, void* dweight, void* dbias, int64_t rows, int64_t width,
                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention.  For batch entry b, head h (shared head g = h / (heads / kv_heads)), query i, key j:
+ *   x = scale q_i.k_j;  z = softcap tanh(x / softcap), or x when softcap is 0;
+ *   s = z - slope_{b,i,h} |q_pos_i - k_pos_j|   (Euclidean, pos_dim 1 or 2 coordinates);
+ *   key j is seen when j < k_len[b] and q_segment_i == k_segment_j >= 0;
+ *   out_i = sum_j softmax_j(s) v_j over the seen keys, 0 for a query that sees none;
+ *   lse_i = log sum_j exp(s), -inf for such a query.
+ * What q, k, v and the positions hold at pairs that are not seen never reaches out: an infinity or
+ * a NaN there changes nothing.
+ *
+ *   dtype         S4D_DTYPE_BF16 or S4D_DTYPE_F16, of q, k, v and out
+ *   q             [batch, queries, heads, dim], k and v [batch, keys, kv_heads, dim]: unit stride along
+ *                 dim, the other strides (elements: batch, row, head) positive multiples of 8, 16-byte
+ *                 aligned; the stride of an axis of one entry is not used
+ *   dim           a multiple of 8, 8 to 128; heads a multiple of kv_heads
+ *   out           [batch, queries, heads, dim] contiguous, 16-byte aligned
+ *   lse           [batch, heads, queries] f32, or NULL
+ *   slopes        f32 with strides (elements: batch, query, head; 0 allowed), when pos_dim > 0
+ *   q_pos, k_pos  [batch, queries | keys, pos_dim] f32 contiguous, when pos_dim > 0
+ *   q_segment, k_segment  [batch, queries | keys] int32 contiguous, both or neither NULL
+ *   k_len         [batch] int32 or NULL (all keys); values outside 0 .. keys are clamped
+ *   workspace     s4d_attention_forward_workspace_bytes(args) bytes, 16-byte aligned, used by this call
+ *                 only while it runs (0 bytes: may be NULL)
+ *   error_flag    int32 or NULL: S4D_FLAG_WAIT_TIMEOUT as in s4d_dfa.h
+ * P is rounded to `dtype` for its product with v; sums and softmax statistics are f32.  Equal calls
+ * give equal bits.  batch and the axes may be 0; rows of one shared head (queries * heads /
+ * kv_heads) and keys must stay below 2^31.
+ */
+typedef struct s4d_attention_args {
+  int64_t batch, queries, keys, heads, kv_heads, dim, pos_dim;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  void* out;
+  float* lse;
+  const float* slopes;
+  int64_t slope_stride[3];
+  const float *q_pos, *k_pos;
+  const int32_t *q_segment, *k_segment, *k_len;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* error_flag;
+  float scale, softcap;
+  int32_t dtype;
+} s4d_attention_args;
+
+S4D_API size_t s4d_attention_forward_workspace_bytes(const s4d_attention_args* args);
+S4D_API int s4d_attention_forward(const s4d_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -22,10 +22,24 @@ DTYPES = {torch.float32: L.S4D_DTYPE_F32, torch.bfloat16: L.S4D_DTYPE_BF16, torc
 
 _i64, _int, _p, _sz, _f = C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_float
 
+
+
+class AttentionArgs(C.Structure):
+    """``s4d_attention_args``.  ``keep`` (not part of the struct) holds the tensors it points to."""
+
+    _fields_ = [(n, _i64) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "pos_dim")] + [
+        ("q", _p), ("k", _p), ("v", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
+        ("out", _p), ("lse", _p), ("slopes", _p), ("slope_stride", _i64 * 3), ("q_pos", _p), ("k_pos", _p),
+        ("q_segment", _p), ("k_segment", _p), ("k_len", _p), ("workspace", _p), ("workspace_bytes", _sz),
+        ("error_flag", _p), ("scale", _f), ("softcap", _f), ("dtype", C.c_int32)]
+
+
 # name -> (restype, argtypes); one entry per function of include/s4d_decoder.h
 SIGNATURES = {
     "s4d_decoder_abi_version": (_int, []),
     "s4d_decoder_last_error": (C.c_char_p, []),
+    "s4d_attention_forward_workspace_bytes": (_sz, [C.POINTER(AttentionArgs)]),
+    "s4d_attention_forward": (_int, [C.POINTER(AttentionArgs), _p]),
     "s4d_norm_forward": (_int, [_p, _i64, _int, _p, _p, _int, _p, _i64, _p, _p, _i64, _i64, _f, _p]),
     "s4d_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "s4d_norm_backward": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _p, _p, _p, _i64, _p, _p, _i64, _i64, _p, _sz,

@@ -22,9 +22,11 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libs4d_dfa.so")
 SOURCES = ["capi.cu", "kps_project.cu", "dfa_gather.cu", "kps_noalloc.cu", "linear_tc.cu", "camera_encoder.cu", "pack_maps.cu",
            "instance_bank.cu", "peer.cu", "layer_norm.cu"]
-# The decoder's operators: each source is compiled by itself, several at a time.
+# The decoder's operators: each (source, defines) is compiled by itself, several at a time.
 DECODER_LIB_PATH = os.path.join(LIB_DIR, "libs4d_decoder.so")
-DECODER_SOURCES = ["decoder_capi.cu", "decoder_norm.cu"]
+DECODER_SOURCES = [("decoder_capi.cu",), ("decoder_norm.cu",), ("decoder_attention.cu",),
+                   ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=64"),
+                   ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=128")]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -56,15 +58,16 @@ def build_decoder(verbose_ptxas: bool = False, force: bool = False) -> str:
     flags = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
              "-I", INCLUDE, "-I", CSRC]
     objs, jobs = [], []
-    for s in DECODER_SOURCES:
-        src, obj = os.path.join(CSRC, s), os.path.join(obj_dir, s[:-3] + ".o")
+    for name, *defs in DECODER_SOURCES:
+        src, obj = os.path.join(CSRC, name), os.path.join(obj_dir, "_".join([name[:-3], *(d.split("=")[-1] for d in defs)])
+                                                          + ".o")
         objs.append(obj)
         if force or verbose_ptxas or not os.path.exists(obj) or os.path.getmtime(obj) < max(newest_header,
                                                                                             os.path.getmtime(src)):
-            jobs.append((src, obj))
+            jobs.append((src, obj, defs))
     with concurrent.futures.ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
-        for f in [pool.submit(_run, [nvcc_path(), *flags, "-c", "-o", obj, src], os.path.basename(src), verbose_ptxas)
-                  for src, obj in jobs]:
+        for f in [pool.submit(_run, [nvcc_path(), *flags, *defs, "-c", "-o", obj, src], os.path.basename(src),
+                              verbose_ptxas) for src, obj, defs in jobs]:
             f.result()
     if jobs or not os.path.exists(DECODER_LIB_PATH) or any(os.path.getmtime(o) > os.path.getmtime(DECODER_LIB_PATH)
                                                            for o in objs):

@@ -1,0 +1,209 @@
+// extern "C" entry points of the decoder's attention (include/s4d_decoder.h): argument validation on
+// the host, tensor maps and the choice of launches.
+#include <mutex>
+
+#include "decoder_attention.cuh"
+
+namespace s4d {
+namespace {
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(f);
+  });
+  return fn;
+}
+
+bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Strides of [batch, rows, heads] for addressing: those of an axis with one entry (or none) are 0.
+struct Strides {
+  int64_t b, n, h;
+  Strides(const int64_t* s, int64_t batch, int64_t rows, int64_t heads)
+      : b(batch > 1 ? s[0] : 0), n(rows > 1 ? s[1] : 0), h(heads > 1 ? s[2] : 0) {}
+  // Positive multiples of 8 elements below 2^37 where the axis has more than one entry, and an extent
+  // that stays below 2^46 elements.
+  bool ok(int64_t batch, int64_t rows, int64_t heads) const {
+    const int64_t st[3] = {b, n, h}, ext[3] = {batch, rows, heads};
+    for (int i = 0; i < 3; ++i) {
+      int64_t span = 0;
+      if (ext[i] > 1 && (st[i] <= 0 || st[i] % 8 != 0 || st[i] >= (int64_t(1) << 37) ||
+                         !size_product({ext[i], st[i]}, int64_t(1) << 46, &span)))
+        return false;
+    }
+    return true;
+  }
+};
+
+// Tensor map of [B, N, heads, D] 16-bit elements, loaded in boxes of 64 columns x box_rows rows of one
+// head with the 128-byte swizzle; columns past D and rows past N are zero.
+int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t heads, int64_t rows, int64_t batch,
+             const Strides& s, int box_rows) {
+  EncodeTiledFn fn = encode_tiled();
+  if (fn == nullptr) return fail(S4D_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
+  // an axis of one entry still needs a stride the encoder takes
+  const int64_t row_bytes = dim * 2 >= 16 ? (dim * 2 + 15) / 16 * 16 : 16;
+  const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(batch)};
+  const cuuint64_t strides[3] = {cuuint64_t(s.h > 0 ? s.h * 2 : row_bytes), cuuint64_t(s.n > 0 ? s.n * 2 : row_bytes),
+                                 cuuint64_t(s.b > 0 ? s.b * 2 : row_bytes)};
+  const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(map, dtype == S4D_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (CUresult %d) for [%lld, %lld, %lld, %lld]", int(r), (long long)batch,
+              (long long)rows, (long long)heads, (long long)dim);
+    return S4D_ERR_CUDA;
+  }
+  return S4D_OK;
+}
+
+constexpr int64_t kMaxRows = int64_t(1) << 31;
+
+// Checks of sizes and of the arguments that forward and backward share; fn names the entry point.
+int check_args(const char* fn, const s4d_attention_args* a) {
+#define S4D_BAD(status, text)         \
+  do {                                \
+    set_error("%s: %s", fn, text);    \
+    return status;                    \
+  } while (0)
+  if (a == nullptr) S4D_BAD(S4D_ERR_INVALID_ARG, "null args");
+  if (a->dtype != S4D_DTYPE_BF16 && a->dtype != S4D_DTYPE_F16) S4D_BAD(S4D_ERR_INVALID_ARG, "dtype must be bf16 or f16");
+  if (a->batch < 0 || a->queries < 0 || a->keys < 0 || a->heads <= 0 || a->kv_heads <= 0)
+    S4D_BAD(S4D_ERR_INVALID_ARG, "bad sizes");
+  if (a->heads % a->kv_heads != 0) S4D_BAD(S4D_ERR_INVALID_ARG, "heads must be a multiple of kv_heads");
+  if (a->dim < 8 || a->dim > 128 || a->dim % 8 != 0)
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "dim must be a multiple of 8 from 8 to 128");
+  if (a->pos_dim < 0 || a->pos_dim > 2) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "pos_dim must be 0, 1 or 2");
+  if (!(a->scale > -INFINITY && a->scale < INFINITY)) S4D_BAD(S4D_ERR_INVALID_ARG, "scale must be finite");
+  if (!(a->softcap >= 0.0f && a->softcap < INFINITY)) S4D_BAD(S4D_ERR_INVALID_ARG, "softcap must be finite and >= 0");
+  int64_t n = 0;
+  if (!size_product({a->queries, a->heads / a->kv_heads}, kMaxRows, &n) || a->keys >= kMaxRows ||
+      a->batch >= kMaxRows || a->heads >= (1 << 20) ||
+      !size_product({a->batch, a->queries, a->heads, a->dim}, int64_t(1) << 46, &n) ||
+      !size_product({a->batch, a->keys, a->kv_heads, a->dim}, int64_t(1) << 46, &n))
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "too many rows or elements");
+  if ((a->q_segment == nullptr) != (a->k_segment == nullptr))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "q_segment and k_segment go together");
+  if (a->batch == 0) return S4D_OK;
+  if (!aligned_to(a->q, 16) || !aligned_to(a->k, 16) || !aligned_to(a->v, 16) || !aligned_to(a->out, 16) ||
+      !aligned_to(a->lse, 4) || !aligned_to(a->slopes, 4) || !aligned_to(a->q_pos, 4) || !aligned_to(a->k_pos, 4) ||
+      !aligned_to(a->q_segment, 4) || !aligned_to(a->k_segment, 4) || !aligned_to(a->k_len, 4) ||
+      !aligned_to(a->error_flag, 4))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "misaligned pointer");
+  if (a->queries > 0 && (a->q == nullptr || a->out == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "null q or out");
+  if (a->keys > 0 && (a->k == nullptr || a->v == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "null k or v");
+  if (a->pos_dim > 0 && ((a->queries > 0 && (a->q_pos == nullptr || a->slopes == nullptr)) ||
+                         (a->keys > 0 && a->k_pos == nullptr)))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "null slopes or positions");
+  if (!Strides(a->q_stride, a->batch, a->queries, a->heads).ok(a->batch, a->queries, a->heads) ||
+      !Strides(a->k_stride, a->batch, a->keys, a->kv_heads).ok(a->batch, a->keys, a->kv_heads) ||
+      !Strides(a->v_stride, a->batch, a->keys, a->kv_heads).ok(a->batch, a->keys, a->kv_heads))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "strides of q, k and v must be positive multiples of 8 elements");
+  return S4D_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Parts of the keys.  A tile of 128 rows and one shared head is one CTA, and two of them share an SM:
+// with fewer CTAs than that the keys are cut until the SMs are full, but not below two tiles of 128
+// keys a part, since a part costs a launch's start and the join reads it again.
+int64_t key_splits(const s4d_attention_args& a) {
+  const int64_t ctas = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), kAttnRows);
+  const int64_t tiles = ceil_div(a.keys, kAttnRows);
+  const int64_t least = ceil_div(tiles, kAttnMaxTiles);
+  int64_t splits = 1;
+  if (ctas > 0 && ctas < 2 * device_sms()) splits = ceil_div(2 * device_sms(), ctas);
+  if (splits > tiles / 2) splits = tiles / 2;
+  if (splits < least) splits = least;
+  if (splits < 1) splits = 1;
+  // as many parts as there are after each got the same number of tiles
+  return tiles == 0 ? 1 : ceil_div(tiles, ceil_div(tiles, splits));
+}
+
+size_t forward_workspace(const s4d_attention_args& a) {
+  const int64_t splits = key_splits(a);
+  return splits == 1 ? 0 : size_t(splits) * size_t(a.batch * a.queries * a.heads) * size_t(a.dim + 1) * sizeof(float);
+}
+
+AttnParams fill(const s4d_attention_args& a) {
+  AttnParams p{};
+  const Strides q(a.q_stride, a.batch, a.queries, a.heads);
+  p.q = a.q, p.q_sb = q.b, p.q_sn = q.n, p.q_sh = q.h;
+  p.out = a.out, p.lse = a.lse;
+  p.slopes = a.slopes, p.sl_b = a.slope_stride[0], p.sl_n = a.slope_stride[1], p.sl_h = a.slope_stride[2];
+  p.q_pos = a.q_pos, p.k_pos = a.k_pos, p.q_seg = a.q_segment, p.k_seg = a.k_segment, p.k_len = a.k_len;
+  p.nq = a.queries, p.nk = a.keys;
+  p.batch = int(a.batch), p.heads = int(a.heads), p.kv_heads = int(a.kv_heads), p.rep = int(a.heads / a.kv_heads);
+  p.dim = int(a.dim), p.scale = a.scale, p.cap = a.softcap;
+  p.error_flag = a.error_flag;
+  p.wait_limit_ns = kWaitLimitNs;
+  return p;
+}
+
+// A map of k or v; without keys one of q's memory, which no kernel then reads.
+int key_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, const int64_t* stride, int box_rows) {
+  if (a.keys == 0) return make_map(map, a.q, a.dtype, a.dim, 1, 1, 1, Strides(stride, 1, 1, 1), box_rows);
+  return make_map(map, base, a.dtype, a.dim, a.kv_heads, a.keys, a.batch, Strides(stride, a.batch, a.keys, a.kv_heads),
+                  box_rows);
+}
+
+}  // namespace
+}  // namespace s4d
+
+using namespace s4d;
+
+extern "C" {
+
+size_t s4d_attention_forward_workspace_bytes(const s4d_attention_args* args) {
+  if (args == nullptr || args->batch <= 0 || args->queries <= 0 || args->keys < 0 || args->heads <= 0 ||
+      args->kv_heads <= 0 || args->heads % args->kv_heads != 0 || args->dim <= 0 || args->dim > 128)
+    return 0;
+  int64_t n = 0;
+  if (!size_product({args->batch, args->queries, args->heads, args->dim}, int64_t(1) << 46, &n) || args->keys >= kMaxRows)
+    return 0;
+  return forward_workspace(*args);
+}
+
+int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
+  const char* fn = "s4d_attention_forward";
+  set_error("%s", "");
+  int st = check_args(fn, args);
+  if (st != S4D_OK) return st;
+  const s4d_attention_args& a = *args;
+  if (a.batch == 0 || a.queries == 0) return S4D_OK;
+  AttnParams p = fill(a);
+  const int64_t splits = key_splits(a), tiles = ceil_div(a.keys, kAttnRows);
+  int64_t ctas = 0;
+  if (!size_product({a.batch, a.kv_heads, ceil_div(a.queries * p.rep, kAttnRows), splits}, kMaxRows, &ctas) ||
+      ceil_div(a.batch * a.queries * a.heads, 8) >= kMaxRows)
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "too many row tiles");
+  const size_t need = forward_workspace(a);
+  if (need > 0 && (a.workspace == nullptr || !aligned_to(a.workspace, 16) || a.workspace_bytes < need))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "missing, misaligned or small workspace");
+  p.splits = int(splits);
+  p.tiles_per_split = ceil_div(tiles, splits);
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_lse = p.part_o + (splits > 1 ? splits * a.batch * a.queries * a.heads * a.dim : 0);
+  CUtensorMap km, vm;
+  st = key_map(&km, a, a.k, a.k_stride, kAttnRows);
+  if (st == S4D_OK) st = key_map(&vm, a, a.v, a.v_stride, kAttnRows);
+  if (st != S4D_OK) return st;
+  cudaStream_t stm = static_cast<cudaStream_t>(stream);
+  return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, km, vm, stm)
+                     : launch_attention_forward_d128(a.dtype, int(a.pos_dim), p, km, vm, stm);
+}
+
+}  // extern "C"

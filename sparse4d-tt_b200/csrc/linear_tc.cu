@@ -28,6 +28,7 @@
 #include <mutex>
 
 #include "params.cuh"
+#include "tc_ptx.cuh"
 
 namespace s4d {
 namespace {
@@ -38,68 +39,8 @@ constexpr int kThreads = 192;
 constexpr int kStages = 4;
 constexpr int kATile = kBM * kBK * 4;  // 8 KiB
 constexpr int kStageChunk = 32 * 32 * 4;  // one 32x32 fp32 output box (4 KiB)
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
-// ---- PTX wrappers ---------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// Waits until the phase with `parity` has completed.  Returns false without waiting further
-// once another role of the CTA has given up (abort_flag set), or after limit_ns, in which case it
-// sets abort_flag itself.  With abort_flag == nullptr only the time limit applies.
-//
-// Two kinds of waits use it.  The pipeline waits (TMA producer on an empty stage, MMA issuer on a
-// full stage, epilogue on the accumulator) pass the CTA's abort flag and the launch's limit
-// (WfcParams / OprojParams::wait_limit_ns, 2 s unless a caller lowered it through
-// s4d_set_tc_wait_limit_ns).  The teardown waits -- the producer's drain of the loads it issued
-// and the MMA issuer's wait for the MMAs it issued -- pass no flag and always kWaitLimitNs: they
-// are what guarantees that no copy is still landing in shared memory and no MMA still writing
-// tensor memory when the CTA frees it and exits, whatever the pipeline waits decided.
-__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                          unsigned long long limit_ns = kWaitLimitNs) {
-  if (mbar_test(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  for (;;) {
-    if (mbar_test(bar, parity)) return true;
-    if (abort_flag != nullptr && *abort_flag) return false;
-    if (now_ns() - t0 > limit_ns) {
-      if (abort_flag != nullptr) *abort_flag = 1;
-      return false;
-    }
-  }
-}
+// ---- PTX wrappers of these kernels alone ------------------------------------------------------
 
 // 2-D tiled TMA load of one box of `map` at (x, y), completion counted on `bar`.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -121,21 +62,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read_le1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// Generic-proxy shared-memory writes become visible to the async proxy (TMA, tensor cores).
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 // D[tmem] (+)= A[smem] . B[smem]^T, both K-major TF32, fp32 accumulate.
 __device__ __forceinline__ void mma_tf32(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -144,11 +70,6 @@ __device__ __forceinline__ void mma_tf32(uint32_t d, uint64_t a, uint64_t b, uin
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-// Arrives once on `bar` when every tcgen05.mma issued so far by this thread has completed.
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Shared-memory matrix descriptor of a K-major tile of 64-byte rows stored with the 64-byte
@@ -166,20 +87,6 @@ __device__ __forceinline__ uint64_t sw64_desc(uint32_t saddr) {
 // 10-12 = 2), both K-major (bits 15, 16 = 0), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
 __host__ __device__ constexpr uint32_t tf32_idesc(int n) {
   return (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
-}
-
-// 32 consecutive accumulator columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // ---- shared pieces of the two kernels ------------------------------------------------------
