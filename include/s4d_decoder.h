@@ -2,7 +2,7 @@
  * s4d_decoder.h -- C ABI of the decoder's dense operators on B200 (sm_100a), the layers that
  * stand around the DeformableFeatureAggregation path of s4d_dfa.h:
  *
- *   s4d_attention_forward               attention over shared or own heads with scores capped by a
+ *   s4d_attention_forward / _backward   attention over shared or own heads with scores capped by a
  *                                       tanh, a bias by distance, a document mask and a valid length
  *                                       per batch entry, for one query or many.
  *   s4d_norm_forward / _backward        LayerNorm rows of any width up to 16384 in f32, bf16 or
@@ -94,10 +94,28 @@ typedef struct s4d_attention_args {
   int32_t* error_flag;
   float scale, softcap;
   int32_t dtype;
+  int32_t dslopes_per_row; /* backward only, from here on */
+  const void* dout;
+  int64_t dout_stride[3];
+  void *dq, *dk, *dv;
+  float* dslopes;
 } s4d_attention_args;
 
 S4D_API size_t s4d_attention_forward_workspace_bytes(const s4d_attention_args* args);
 S4D_API int s4d_attention_forward(const s4d_attention_args* args, void* stream);
+
+/* Gradients of s4d_attention_forward for bf16, from the same arguments, its out and lse, and dout.
+ *   dout     [batch, queries, heads, dim], strides as q's
+ *   dq       [batch, queries, heads, dim] contiguous; dk, dv [batch, keys, kv_heads, dim] contiguous, or
+ *            both NULL when not wanted; all 16-byte aligned
+ *   dslopes  f32, or NULL: [batch, queries, heads] when dslopes_per_row, else [heads], the sum over all
+ *            rows.  Positions have no gradient.
+ *   workspace  s4d_attention_backward_workspace_bytes(args) bytes, 16-byte aligned
+ * No atomics: equal calls give equal bits.  Pairs that are not seen take no part, whatever q, k, v,
+ * dout and the positions hold there; gradients of rows that see nothing or are seen by nothing are 0.
+ * At most 524288 queries and keys. */
+S4D_API size_t s4d_attention_backward_workspace_bytes(const s4d_attention_args* args);
+S4D_API int s4d_attention_backward(const s4d_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -9,14 +9,14 @@ Public API:
   chained_camera_terms                                      -- next layer's camera terms beside this gather
   InstanceBank, project_anchors                             -- temporal instances (instance_bank.py)
   Sparse4DHead, HeadGraph, preprocess_head_parameters       -- the decoder chain around the DFA (head.py)
-  decoder_attention_forward                                 -- biased, capped, masked attention (attention.py)
+  decoder_attention, decoder_attention_forward / _backward  -- biased, capped, masked attention (attention.py)
   decoder_norm, decoder_norm_forward / _backward            -- LayerNorm with gradients (norm.py)
 The operators run hand-written sm_100a CUDA kernels from lib/libs4d_dfa.so through the C ABI
 of include/s4d_dfa.h, the decoder_* ones from lib/libs4d_decoder.so (include/s4d_decoder.h); each
 library is loaded on first use and its absence raises.
 """
 from . import synthetic  # noqa: F401
-from .attention import decoder_attention_forward  # noqa: F401
+from .attention import decoder_attention, decoder_attention_backward, decoder_attention_forward  # noqa: F401
 from .dfa import DeformableFeatureAggregation, preprocess_dfa_parameters  # noqa: F401
 from .graph import DFAStack, PipelinedDFAStack, capture, chained_camera_terms  # noqa: F401
 from .head import HeadGraph, Sparse4DHead, preprocess_head_parameters  # noqa: F401

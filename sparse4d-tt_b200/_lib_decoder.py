@@ -31,7 +31,9 @@ class AttentionArgs(C.Structure):
         ("q", _p), ("k", _p), ("v", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
         ("out", _p), ("lse", _p), ("slopes", _p), ("slope_stride", _i64 * 3), ("q_pos", _p), ("k_pos", _p),
         ("q_segment", _p), ("k_segment", _p), ("k_len", _p), ("workspace", _p), ("workspace_bytes", _sz),
-        ("error_flag", _p), ("scale", _f), ("softcap", _f), ("dtype", C.c_int32)]
+        ("error_flag", _p), ("scale", _f), ("softcap", _f), ("dtype", C.c_int32),
+        ("dslopes_per_row", C.c_int32), ("dout", _p), ("dout_stride", _i64 * 3), ("dq", _p), ("dk", _p), ("dv", _p),
+        ("dslopes", _p)]
 
 
 # name -> (restype, argtypes); one entry per function of include/s4d_decoder.h
@@ -40,6 +42,8 @@ SIGNATURES = {
     "s4d_decoder_last_error": (C.c_char_p, []),
     "s4d_attention_forward_workspace_bytes": (_sz, [C.POINTER(AttentionArgs)]),
     "s4d_attention_forward": (_int, [C.POINTER(AttentionArgs), _p]),
+    "s4d_attention_backward_workspace_bytes": (_sz, [C.POINTER(AttentionArgs)]),
+    "s4d_attention_backward": (_int, [C.POINTER(AttentionArgs), _p]),
     "s4d_norm_forward": (_int, [_p, _i64, _int, _p, _p, _int, _p, _i64, _p, _p, _i64, _i64, _f, _p]),
     "s4d_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "s4d_norm_backward": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _p, _p, _p, _i64, _p, _p, _i64, _i64, _p, _sz,

@@ -16,8 +16,9 @@ sequence), the segments its denoising groups (or packed documents; a negative id
 head, ``kv_heads`` that divide ``heads``, any number of queries from one to many: few queries over
 many keys are split along the keys.
 
-* ``decoder_attention_forward`` -- the pass by itself, for programs that keep their own buffers
-  (no autograd; capturable in a CUDA graph).
+* ``decoder_attention`` -- differentiable in q, k, v and the slopes (bf16).
+* ``decoder_attention_forward`` / ``decoder_attention_backward`` -- the two passes by themselves, for
+  programs that keep their own buffers (no autograd; capturable in a CUDA graph).
 
 There is no CPU path: CPU tensors are rejected.
 """
@@ -155,3 +156,82 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
         st = lib.s4d_attention_forward(C.byref(a), _stream_ptr(dev))
     D.check(name, st)
     return out, lse
+
+
+def decoder_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
+                               scale: Optional[float] = None, softcap: float = 0.0, slopes: Optional[Tensor] = None,
+                               q_pos: Optional[Tensor] = None, k_pos: Optional[Tensor] = None,
+                               q_segment: Optional[Tensor] = None, k_segment: Optional[Tensor] = None,
+                               k_len: Optional[Tensor] = None, need_dkv: bool = True, need_dslopes: bool = True,
+                               error_flag: Optional[Tensor] = None
+                               ) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """``(dq, dk, dv, dslopes)`` of ``decoder_attention_forward`` from its output's gradient ``dout`` (like
+    ``q``), its arguments and its results, in bf16 (``dslopes`` fp32, like ``slopes``; None without them).
+    ``need_dkv`` / ``need_dslopes`` False leave those out (None).  Positions have no gradient.  No
+    atomics: equal calls give equal bits."""
+    name = "decoder_attention_backward"
+    dev, a = _fill(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
+    _require_cuda(name, q, dout, out, lse)
+    _check_dtype(name, q, (torch.bfloat16,), "q")
+    for what, t in (("dout", dout), ("out", out)):
+        _check_dtype(name, t, (q.dtype,), what)
+        _require(t.shape == q.shape, lambda: f"{name}: {what} must be {list(q.shape)}, got {list(t.shape)}")
+    _require(out.is_contiguous() and out.data_ptr() % 16 == 0, lambda: f"{name}: out must be contiguous")
+    _check_dtype(name, lse, (torch.float32,), "lse")
+    _require(tuple(lse.shape) == (a.batch, a.heads, a.queries) and lse.is_contiguous(),
+             lambda: f"{name}: lse must be a contiguous [{a.batch}, {a.heads}, {a.queries}] tensor")
+    dout = _operand(dout)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=dev) if need_dkv else None for _ in range(2))
+    ds = torch.empty(slopes.shape, dtype=torch.float32, device=dev) if slopes is not None and need_dslopes else None
+    a.out, a.lse, a.dout, a.dq, a.dk, a.dv, a.dslopes = (out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(),
+                                                         _ptr(dk), _ptr(dv), _ptr(ds))
+    a.dout_stride[:] = dout.stride()[:3]
+    a.dslopes_per_row = int(ds is not None and ds.dim() == 3)
+    if a.batch == 0:
+        if ds is not None:
+            ds.zero_()
+        return dq, dk, dv, ds
+    lib = D.lib()
+    with D.on_device(dev):
+        need = lib.s4d_attention_backward_workspace_bytes(C.byref(a))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        a.workspace, a.workspace_bytes = _ptr(ws), need
+        st = lib.s4d_attention_backward(C.byref(a), _stream_ptr(dev))
+    D.check(name, st)
+    return dq, dk, dv, ds
+
+
+class _DecoderAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, scale, softcap, q_pos, k_pos, q_segment, k_segment, k_len):
+        rest = (q_pos, k_pos, q_segment, k_segment, k_len)
+        out, lse = decoder_attention_forward(q, k, v, scale, softcap, slopes, *rest)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, *rest)
+        ctx.scale, ctx.softcap = scale, softcap
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, slopes, *rest = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv, ds = decoder_attention_backward(dout, q, k, v, out, lse, ctx.scale, ctx.softcap, slopes, *rest,
+                                                    need_dkv=need[1] or need[2], need_dslopes=need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, ds, *([None] * 7))
+
+
+def decoder_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None, softcap: float = 0.0,
+                      slopes: Optional[Tensor] = None, q_pos: Optional[Tensor] = None, k_pos: Optional[Tensor] = None,
+                      q_segment: Optional[Tensor] = None, k_segment: Optional[Tensor] = None,
+                      k_len: Optional[Tensor] = None) -> Tensor:
+    """``out`` of ``decoder_attention_forward``, differentiable (first derivatives) in ``q``, ``k``, ``v`` and
+    ``slopes``.  Gradients are for bf16: fp16 inputs that require one are rejected (dS of a long row lies
+    in fp16's subnormal range), and so are positions that require one."""
+    name = "decoder_attention"
+    if torch.is_grad_enabled():
+        for what, t in (("q_pos", q_pos), ("k_pos", k_pos)):
+            _require(t is None or not t.requires_grad, lambda: f"{name}: {what} has no gradient; detach it")
+        if q.dtype != torch.bfloat16 and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
+            raise TypeError(f"{name}: gradients are implemented for torch.bfloat16, got {q.dtype}")
+    return _DecoderAttention.apply(q, k, v, slopes, scale, softcap, q_pos, k_pos, q_segment, k_segment, k_len)

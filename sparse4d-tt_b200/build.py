@@ -26,7 +26,9 @@ SOURCES = ["capi.cu", "kps_project.cu", "dfa_gather.cu", "kps_noalloc.cu", "line
 DECODER_LIB_PATH = os.path.join(LIB_DIR, "libs4d_decoder.so")
 DECODER_SOURCES = [("decoder_capi.cu",), ("decoder_norm.cu",), ("decoder_attention.cu",),
                    ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=64"),
-                   ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=128")]
+                   ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=128"),
+                   ("decoder_attention_backward.cu", "-DS4D_HEAD_DIM=64"),
+                   ("decoder_attention_backward.cu", "-DS4D_HEAD_DIM=128")]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -160,6 +160,41 @@ int key_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, con
                   box_rows);
 }
 
+// A map of q or dout; without queries one of k's memory, which no kernel then reads.
+int query_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, const int64_t* stride, int box_rows) {
+  if (a.queries == 0) return make_map(map, a.k, a.dtype, a.dim, 1, 1, 1, Strides(stride, 1, 1, 1), box_rows);
+  return make_map(map, base, a.dtype, a.dim, a.heads, a.queries, a.batch, Strides(stride, a.batch, a.queries, a.heads),
+                  box_rows);
+}
+
+// dslopes of one slope per head: the sum of every row's, one head a block, its rows added in an order
+// that depends on the sizes alone.
+__global__ void __launch_bounds__(512) slope_sum_kernel(const float* rows, int64_t n, int heads, float* out) {
+  __shared__ float part[16];
+  const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t r = threadIdx.x; r < n; r += 4 * 512)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (r + u * 512 < n) s[u] += rows[(r + u * 512) * heads + h];
+  float v = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    v = 0.0f;
+    for (int w = 0; w < 16; ++w) v += part[w];
+    out[h] = v;
+  }
+}
+
+size_t backward_workspace(const s4d_attention_args& a) {
+  const size_t rows = size_t(a.batch) * size_t(a.queries) * size_t(a.heads) * sizeof(float);
+  const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
+  return rows + (sum ? rows : 0);
+}
+
 }  // namespace
 }  // namespace s4d
 
@@ -204,6 +239,68 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, km, vm, stm)
                      : launch_attention_forward_d128(a.dtype, int(a.pos_dim), p, km, vm, stm);
+}
+
+size_t s4d_attention_backward_workspace_bytes(const s4d_attention_args* args) {
+  int64_t n = 0;
+  if (args == nullptr || args->batch <= 0 || args->queries <= 0 || args->heads <= 0 ||
+      !size_product({args->batch, args->queries, args->heads}, int64_t(1) << 46, &n))
+    return 0;
+  return backward_workspace(*args);
+}
+
+int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
+  const char* fn = "s4d_attention_backward";
+  set_error("%s", "");
+  int st = check_args(fn, args);
+  if (st != S4D_OK) return st;
+  const s4d_attention_args& a = *args;
+  if (a.dtype != S4D_DTYPE_BF16) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for bf16");
+  if (ceil_div(a.queries, 64) > kAttnMaxTiles || ceil_div(a.keys, 64) > kAttnMaxTiles)
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 524288 queries and keys");
+  if (a.batch == 0) return S4D_OK;
+  if ((a.dk == nullptr) != (a.dv == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "dk and dv go together");
+  if (!aligned_to(a.dout, 16) || !aligned_to(a.dq, 16) || !aligned_to(a.dk, 16) || !aligned_to(a.dv, 16) ||
+      !aligned_to(a.dslopes, 4))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "misaligned pointer");
+  if (a.queries > 0 && (a.dout == nullptr || a.dq == nullptr || a.lse == nullptr))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "null dout, dq or lse");
+  if (a.dslopes != nullptr && a.pos_dim == 0) S4D_BAD(S4D_ERR_INVALID_ARG, "dslopes without a distance bias");
+  if (!Strides(a.dout_stride, a.batch, a.queries, a.heads).ok(a.batch, a.queries, a.heads))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "strides of dout must be positive multiples of 8 elements");
+  const size_t need = backward_workspace(a);
+  if (a.queries > 0 && (a.workspace == nullptr || !aligned_to(a.workspace, 16) || a.workspace_bytes < need))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "missing, misaligned or small workspace");
+  AttnParams p = fill(a);
+  int64_t ctas = 0;
+  if (!size_product({a.batch, a.kv_heads, ceil_div(a.queries * p.rep, kAttnRows)}, kMaxRows, &ctas) ||
+      !size_product({a.batch, a.kv_heads, ceil_div(a.keys, kAttnRows)}, kMaxRows, &ctas))
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "too many row tiles");
+  const Strides d(a.dout_stride, a.batch, a.queries, a.heads);
+  p.dout = a.dout, p.do_sb = d.b, p.do_sn = d.n, p.do_sh = d.h;
+  p.dq = a.dq, p.dk = a.dk, p.dv = a.dv;
+  p.splits = 1;
+  p.delta = static_cast<float*>(a.workspace);
+  const int64_t rows = a.batch * a.queries;
+  const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
+  p.dslopes = sum ? p.delta + rows * a.heads : a.dslopes;
+  cudaStream_t stm = static_cast<cudaStream_t>(stream);
+  if (a.queries > 0 || a.keys > 0) {
+    AttnBackwardMaps m;
+    st = key_map(&m.k64, a, a.k, a.k_stride, 64);
+    if (st == S4D_OK) st = key_map(&m.v64, a, a.v, a.v_stride, 64);
+    if (st == S4D_OK) st = key_map(&m.k128, a, a.k, a.k_stride, 128);
+    if (st == S4D_OK) st = key_map(&m.v128, a, a.v, a.v_stride, 128);
+    if (st == S4D_OK) st = query_map(&m.q64, a, a.q, a.q_stride, 64);
+    if (st == S4D_OK) st = query_map(&m.do64, a, a.dout, a.dout_stride, 64);
+    if (st == S4D_OK)
+      st = a.dim <= 64 ? launch_attention_backward_d64(int(a.pos_dim), p, m, stm)
+                       : launch_attention_backward_d128(int(a.pos_dim), p, m, stm);
+    if (st != S4D_OK) return st;
+  }
+  if (!sum) return S4D_OK;
+  slope_sum_kernel<<<dim3(unsigned(a.heads)), 512, 0, stm>>>(p.dslopes, rows, p.heads, a.dslopes);
+  return cuda_check(cudaGetLastError(), "slope_sum_kernel launch");
 }
 
 }  // extern "C"

@@ -398,6 +398,13 @@ int launch_attention_forward_d64(int dtype, int pos, const AttnParams& p, const 
 int launch_attention_forward_d128(int dtype, int pos, const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm,
                                   cudaStream_t st);
 
+// Maps of the backward kernels, named by the rows of their boxes.
+struct AttnBackwardMaps {
+  CUtensorMap k64, v64, k128, v128, q64, do64;
+};
+int launch_attention_backward_d64(int pos, const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st);
+int launch_attention_backward_d128(int pos, const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st);
+
 // The dynamic shared-memory limit of `kernel`, set once per device; `done` is the caller's record.
 template <typename K>
 int set_kernel_smem(K kernel, size_t bytes, const char* what, bool (&done)[64]) {

@@ -12,19 +12,21 @@ def half_step(t):
 
 def reference(q, k, v, scale=None, softcap=0.0, slopes=None, q_pos=None, k_pos=None, q_segment=None, k_segment=None,
               k_len=None, dout=None):
-    """A dict in fp64: ``out``, ``lse``, with ``dout`` also ``dq``, ``dk``, ``dv`` and ``dslopes [B, Nq, H]``,
-    and the sums of magnitudes the bounds are made of.  Values at masked pairs take no part, whatever
-    they are.  Loops over batch entries and heads."""
+    """A dict in fp64: ``out``, ``lse`` and ``out_abs`` = sum P |V|; with ``dout`` also ``dq``, ``dk``, ``dv`` and
+    ``dslopes [B, Nq, H]`` and the bound of each before its own last rounding (``*_tol``).  Values at
+    masked pairs take no part, whatever they are.  Loops over batch entries and heads."""
     B, Nq, H, D = q.shape
     Nk, G = k.shape[1], k.shape[2]
     dev = q.device
     scale = D ** -0.5 if scale is None else scale
     z = lambda *s: torch.zeros(*s, dtype=torch.float64, device=dev)  # noqa: E731
     r = dict(out=z(B, Nq, H, D), lse=torch.full((B, H, Nq), -math.inf, dtype=torch.float64, device=dev),
-             out_abs=z(B, Nq, H, D), spread=z(B, Nq, H))
+             out_abs=z(B, Nq, H, D))
     if dout is not None:
-        r.update(dq=z(B, Nq, H, D), dk=z(B, Nk, G, D), dv=z(B, Nk, G, D), dslopes=z(B, Nq, H), dq_abs=z(B, Nq, H, D),
-                 dk_abs=z(B, Nk, G, D), dv_abs=z(B, Nk, G, D), dslopes_abs=z(B, Nq, H))
+        h16 = half_step(q.dtype)
+        e = score_error(q, k, scale, softcap, slopes, q_pos, k_pos)
+        for n, shape in (("dq", (B, Nq, H, D)), ("dk", (B, Nk, G, D)), ("dv", (B, Nk, G, D)), ("dslopes", (B, Nq, H))):
+            r[n], r[n + "_tol"] = z(*shape), z(*shape)
     for b in range(B):
         ok = torch.ones(Nq, Nk, dtype=torch.bool, device=dev)
         if k_len is not None:
@@ -58,18 +60,25 @@ def reference(q, k, v, scale=None, softcap=0.0, slopes=None, q_pos=None, k_pos=N
             dp = dO @ V.T
             delta = (p * dp).sum(1, keepdim=True)
             ds = p * (dp - delta)
-            if dist is not None:
-                r["dslopes"][b, :, h] = -(ds * dist).sum(1)
-                r["dslopes_abs"][b, :, h] = (p * (dO.abs() @ V.abs().T + delta.abs()) * dist).sum(1)
             dx = ds * (1 - t * t) if softcap else ds
             r["dq"][b, :, h] = scale * dx @ K
             r["dk"][b, :, g] += scale * dx.T @ Q
             r["dv"][b, :, g] += p.T @ dO
-            # what the roundings scale with: dS itself, and P |dO| (|V| + |out|) for the row term
-            row = p * (dO.abs() * (p @ V).abs()).sum(1, keepdim=True)
-            r["dq_abs"][b, :, h] = abs(scale) * (dx.abs() + row) @ K.abs()
-            r["dk_abs"][b, :, g] += abs(scale) * (dx.abs() + row).T @ Q.abs()
-            r["dv_abs"][b, :, g] += p.T @ dO.abs()
+            # Bounds.  A weight is off by 2 e (score and log-sum-exp); dP by D u of its products; delta
+            # by h of |dO| |out| (out is rounded) and D u; the cap's derivative by 16 u; dX and P are
+            # rounded to the type once (h); sums over N terms by N u.
+            row = p * (dO.abs() * r["out"][b, :, h].abs()).sum(1, keepdim=True)
+            mag = p * (dO.abs() @ V.abs().T) + row
+            off = 2 * e * ds.abs() + 16 * U * ds.abs() + (D + 8) * U * mag
+            dx_off = (h16 + max(Nq, Nk) * U) * dx.abs() + off + h16 * row
+            r["dq_tol"][b, :, h] = abs(scale) * dx_off @ K.abs()
+            r["dk_tol"][b, :, g] += abs(scale) * dx_off.T @ Q.abs()
+            r["dv_tol"][b, :, g] += (h16 + 2 * e + max(Nq, Nk) * U) * p.T @ dO.abs()
+            if dist is not None:
+                r["dslopes"][b, :, h] = -(ds * dist).sum(1)
+                # delta's rounding cancels up to the error of sum P = 1
+                r["dslopes_tol"][b, :, h] = ((off + Nk * U * mag + (2 * e + Nk * U) * h16 * row) * dist).sum(1) \
+                    + (2 * e + Nk * U) * h16 * row.sum(1) * (p * dist).sum(1)
     return r
 
 

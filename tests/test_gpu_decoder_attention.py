@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from attention_ref import U, half_step, reference, score_error
-from sparse4d_tt_b200 import decoder_attention_forward
+from sparse4d_tt_b200 import decoder_attention, decoder_attention_backward, decoder_attention_forward
 from sparse4d_tt_b200.graph import capture
 
 pytestmark = pytest.mark.gpu
@@ -215,3 +215,198 @@ def test_equal_bits_streams_and_graphs(cuda_device):
         assert all(torch.equal(x, y) for x, y in zip(first, other))
         q.neg_()
         assert torch.equal(a.replay()[0], call()[0]) and not torch.equal(call()[0], first[0])
+
+
+# ---- gradients --------------------------------------------------------------------------------------
+
+
+def check_backward(q, k, v, how, dout, grads, out=None):
+    ref = reference(q, k, v, **how, dout=dout)
+    h = half_step(q.dtype)
+    names = ("dq", "dk", "dv") + (("dslopes",) if "slopes" in how else ())
+    assert (grads[3] is None) == ("slopes" not in how)
+    for n, got in zip(names, grads):
+        want, tol = ref[n], ref[n + "_tol"]
+        if n == "dslopes":
+            if how["slopes"].dim() == 1:
+                tol = tol.sum((0, 1)) + want.shape[0] * want.shape[1] * U * want.abs().sum((0, 1))
+                want = want.sum((0, 1))
+            tol = tol + 2 * U * want.abs()
+        else:
+            tol = (1 + h) * tol + h * want.abs()
+        assert got.shape == want.shape, n
+        err = (got.double() - want).abs()
+        assert (err <= tol).all(), (n, (err - tol).max(), err.max())
+
+
+def gradients(q, k, v, how, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    dout = torch.randn(q.shape, generator=g).to(q.dtype).cuda()
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    return dout, decoder_attention_backward(dout, q, k, v, out, lse, **how)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D", [
+    (1, 1, 1, 1, 1, 64), (2, 5, 3, 2, 2, 64), (1, 128, 128, 2, 1, 64), (1, 129, 257, 3, 3, 64), (1, 900, 900, 4, 4, 64),
+    (1, 200, 300, 6, 2, 32), (2, 77, 130, 4, 4, 8), (1, 150, 401, 4, 2, 128), (1, 300, 140, 3, 1, 96), (2, 65, 128, 5, 5, 72),
+    (1, 1, 1500, 4, 2, 128), (3, 400, 2, 2, 2, 64),
+])
+def test_gradients_plain(cuda_device, B, Nq, Nk, H, G, D):
+    q, k, v, how = make(B, Nq, Nk, H, G, D)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pos,slopes", [(1, "head"), (2, "head"), (2, "row"), (0, None)])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_gradients_bias_and_cap(cuda_device, D, pos, slopes, cap):
+    q, k, v, how = make(2, 190, 333, 4, 2, D, pos=pos, slopes=slopes, cap=cap)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+
+
+@pytest.mark.parametrize("q_ids,k_ids", [
+    (ids(300, 80, 20), ids(300, 80, 20)), (ids(128, 128, 128), ids(128, 128, 128)), (ids(10, -5, 200, 1), ids(3, 90, -7, 1)),
+    ([i % 3 for i in range(150)], [i % 4 for i in range(290)]), ([-1] * 40, [0] * 60), ([5] * 40, [7] * 500),
+])
+@pytest.mark.parametrize("k_len", [None, [260, 0]])
+def test_gradients_documents(cuda_device, q_ids, k_ids, k_len):
+    q, k, v, how = make(2, len(q_ids), len(k_ids), 4, 2, 64, segments=(q_ids, k_ids), k_len=k_len, pos=1)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+
+
+def test_gradients_valid_lengths(cuda_device):
+    lens = [0, 1, 127, 128, 129, 600, 700, -3]
+    q, k, v, how = make(8, 100, 600, 2, 1, 64, k_len=lens, cap=10.0)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+    assert not grads[0][0].any() and not grads[1][7].any() and not grads[1][1, 1:].any() and not grads[2][2, 127:].any()
+
+
+def test_gradients_without_keys_queries_or_batch(cuda_device):
+    q, k, v, how = make(2, 5, 3, 2, 1, 64, pos=2)
+    full = dict(how)
+    how["k_pos"] = full["k_pos"][:, :0]
+    _, (dq, dk, dv, ds) = gradients(q, k[:, :0], v[:, :0], how)
+    assert not dq.any() and dk.shape == (2, 0, 1, 64) and not ds.any()
+    how = dict(full, q_pos=full["q_pos"][:, :0])
+    _, (dq, dk, dv, ds) = gradients(q[:, :0], k, v, how)
+    assert dq.shape == (2, 0, 2, 64) and not dk.any() and not dv.any() and not ds.any()
+    how = dict(full, q_pos=full["q_pos"][:0], k_pos=full["k_pos"][:0])
+    _, (dq, dk, dv, ds) = gradients(q[:0], k[:0], v[:0], how)
+    assert dk.shape == (0, 3, 1, 64) and not ds.any()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_ignore_values_behind_masks(cuda_device, bad):
+    """Infinities and NaNs in padding, past the valid length and in another document, in keys, values,
+    queries and the output's gradient."""
+    sizes = ids(150, 60, 90, -20)
+    q, k, v, how = make(2, 320, 320, 4, 2, 64, segments=(sizes, sizes), k_len=[320, 280], pos=2, slopes="row", cap=20.0)
+    dout, clean = gradients(q, k, v, how)
+    t = [x.clone() for x in (q, k, v, dout)]
+    how = dict(how, q_pos=how["q_pos"].clone(), k_pos=how["k_pos"].clone())
+    for x in t + [how["q_pos"], how["k_pos"]]:
+        x[:, 300:] = bad                       # padding ids
+    for x in (t[1], t[2], how["k_pos"]):
+        x[1, 280:] = bad                       # past the valid length
+    for x in (t[1], t[3]):
+        x[:, 155:170] = bad                    # document 1
+    q2, k2, v2, dout2 = t
+    out, lse = decoder_attention_forward(q2, k2, v2, **how)
+    got = decoder_attention_backward(dout2, q2, k2, v2, out, lse, **how)
+    keep = torch.tensor([s in (0, 2) for s in sizes], device="cuda")
+    how_ref = dict(how, q_pos=how["q_pos"].nan_to_num(0, 0, 0), k_pos=how["k_pos"].nan_to_num(0, 0, 0))
+    ref = reference(*(x.nan_to_num(0, 0, 0) for x in (q2, k2, v2)), **how_ref, dout=dout2.nan_to_num(0, 0, 0))
+    for n, g, c in zip(("dq", "dk", "dv", "dslopes"), got, clean):
+        assert torch.isfinite(g[:, keep]).all(), n
+        want, tol = ref[n][:, keep], ref[n + "_tol"][:, keep]
+        if n != "dslopes":
+            tol = 1.01 * tol + half_step(torch.bfloat16) * want.abs()
+        assert ((g[:, keep].double() - want).abs() <= tol + 2 * U * want.abs()).all(), n
+        assert not g[:, 300:].any(), n
+    assert not got[1][1, 280:].any() and not got[2][1, 280:].any()
+    assert not torch.isfinite(got[0][:, 160]).any()
+
+
+def test_gradients_strides_expanded_and_parts(cuda_device):
+    q, k, v, how = make(2, 100, 150, 4, 4, 64, pos=1)
+    dout, want = gradients(q, k, v, how)
+    qkv = [x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for x in (q, k, v, dout)]
+    out, lse = decoder_attention_forward(*qkv[:3], **how)
+    got = decoder_attention_backward(qkv[3], *qkv[:3], out, lse, **how)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    one = decoder_attention_backward(dout[:, :1].expand(-1, 100, -1, -1), q, k, v, out, lse, **how)
+    two = decoder_attention_backward(dout[:, :1].expand(-1, 100, -1, -1).contiguous(), q, k, v, out, lse, **how)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    part = decoder_attention_backward(dout, q, k, v, out, lse, **how, need_dkv=False, need_dslopes=False)
+    assert torch.equal(part[0], want[0]) and part[1:] == (None, None, None)
+
+
+def test_gradients_equal_bits_and_graphs(cuda_device):
+    q, k, v, how = make(2, 700, 900, 4, 2, 64, pos=2)
+    dout = torch.randn_like(q)
+
+    def step():
+        out, lse = decoder_attention_forward(q, k, v, **how)
+        return (out, *decoder_attention_backward(dout, q, k, v, out, lse, **how))
+
+    first = [t.clone() for t in step()]
+    a, b = capture(step), capture(step)
+    for run in (a.replay, step, b.replay, a.replay, b.replay):
+        assert all(torch.equal(x, y) for x, y in zip(first, run()))
+    dout.neg_()
+    assert torch.equal(a.replay()[1], step()[1]) and torch.equal(a.replay()[1], -first[1])
+
+
+def test_autograd(cuda_device):
+    """Through autograd: expanded (shared) keys get the sum of their uses, slopes and leaves the sum of
+    two calls; only what requires a gradient gets one."""
+    q, k, v, how = make(2, 60, 90, 4, 4, 64, pos=2, cap=8.0)
+    dout, want = gradients(q, k, v, how)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, how["slopes"])]
+    rest = {n: how[n] for n in ("q_pos", "k_pos", "softcap")}
+    (decoder_attention(*leaves[:3], slopes=leaves[3], **rest).float() * dout.float()).sum().backward()
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    (decoder_attention(*leaves[:3], slopes=leaves[3], **rest).float() * dout.float()).sum().backward()
+    assert torch.allclose(leaves[0].grad.float(), 2 * want[0].float())
+    ql = q.clone().requires_grad_()
+    decoder_attention(ql, k, v, slopes=how["slopes"], **rest).backward(dout)
+    assert torch.equal(ql.grad, want[0])
+    kl = k[:, :, :1].clone().requires_grad_()
+    decoder_attention(q, kl.expand(-1, -1, 4, -1), v[:, :, :1].expand(-1, -1, 4, -1)).backward(dout)
+    ks = k[:, :, :1].clone().requires_grad_()
+    decoder_attention(q, ks, v[:, :, :1]).backward(dout)
+    # the expanded form rounds four gradients to bf16 and their sum, the shared one its sum once
+    big = kl.grad.float().abs().max()
+    assert (kl.grad.float() - ks.grad.float()).abs().max() <= 6 * half_step(torch.bfloat16) * 2 * big
+    with pytest.raises(TypeError, match="bfloat16"):
+        decoder_attention(q.half().requires_grad_(), k.half(), v.half())
+    with pytest.raises(ValueError, match="q_pos"):
+        decoder_attention(q, k, v, slopes=how["slopes"], q_pos=how["q_pos"].clone().requires_grad_(), k_pos=how["k_pos"])
+    with torch.no_grad():
+        assert decoder_attention(q.half(), k.half(), v.half()).dtype == torch.float16
+
+
+def test_gradient_against_differences(cuda_device):
+    """The gradient of a loss against central differences of the 64-bit definition, along random
+    directions: the definition's derivative is the kernels' up to their own bounds (3 % covers the
+    bf16 roundings of a sum of about 10^4 terms of either sign at these sizes)."""
+    q, k, v, how = make(1, 40, 50, 2, 1, 64, pos=2, cap=6.0)
+    dout, grads = gradients(q, k, v, how)
+    g = torch.Generator().manual_seed(9)
+    base = dict(q=q.double(), k=k.double(), v=v.double(), slopes=how["slopes"].double())
+
+    def loss(x):
+        args = dict(how, slopes=x["slopes"])
+        return (reference(x["q"], x["k"], x["v"], **args)["out"] * dout.double()).sum().item()
+
+    for name, got in zip(("q", "k", "v", "slopes"), grads):
+        d = torch.randn(base[name].shape, generator=g).double().cuda().sign() * got.double().sign()
+        up, down = dict(base), dict(base)
+        up[name], down[name] = base[name] + 1e-5 * d, base[name] - 1e-5 * d
+        want = (loss(up) - loss(down)) / 2e-5
+        have = (got.double() * d).sum().item()
+        assert abs(want - have) <= 0.03 * got.double().abs().sum().item(), (name, want, have)
