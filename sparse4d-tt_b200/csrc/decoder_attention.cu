@@ -71,6 +71,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t
 }
 
 constexpr int64_t kMaxRows = int64_t(1) << 31;
+constexpr int kKeyTile = 64;  // keys of a forward tile
 
 // Checks of sizes and of the arguments that forward and backward share; fn names the entry point.
 int check_args(const char* fn, const s4d_attention_args* a) {
@@ -118,15 +119,15 @@ int check_args(const char* fn, const s4d_attention_args* a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Parts of the keys.  A tile of 128 rows and one shared head is one CTA, and two of them share an SM:
-// with fewer CTAs than that the keys are cut until the SMs are full, but not below two tiles of 128
+// with fewer CTAs than that the keys are cut until the SMs are full, but not below four tiles of 64
 // keys a part, since a part costs a launch's start and the join reads it again.
 int64_t key_splits(const s4d_attention_args& a) {
   const int64_t ctas = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), kAttnRows);
-  const int64_t tiles = ceil_div(a.keys, kAttnRows);
+  const int64_t tiles = ceil_div(a.keys, kKeyTile);
   const int64_t least = ceil_div(tiles, kAttnMaxTiles);
   int64_t splits = 1;
   if (ctas > 0 && ctas < 2 * device_sms()) splits = ceil_div(2 * device_sms(), ctas);
-  if (splits > tiles / 2) splits = tiles / 2;
+  if (splits > tiles / 4) splits = tiles / 4;
   if (splits < least) splits = least;
   if (splits < 1) splits = 1;
   // as many parts as there are after each got the same number of tiles
@@ -220,7 +221,7 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
   const s4d_attention_args& a = *args;
   if (a.batch == 0 || a.queries == 0) return S4D_OK;
   AttnParams p = fill(a);
-  const int64_t splits = key_splits(a), tiles = ceil_div(a.keys, kAttnRows);
+  const int64_t splits = key_splits(a), tiles = ceil_div(a.keys, kKeyTile);
   int64_t ctas = 0;
   if (!size_product({a.batch, a.kv_heads, ceil_div(a.queries * p.rep, kAttnRows), splits}, kMaxRows, &ctas) ||
       ceil_div(a.batch * a.queries * a.heads, 8) >= kMaxRows)
@@ -233,8 +234,8 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
   p.part_o = static_cast<float*>(a.workspace);
   p.part_lse = p.part_o + (splits > 1 ? splits * a.batch * a.queries * a.heads * a.dim : 0);
   CUtensorMap km, vm;
-  st = key_map(&km, a, a.k, a.k_stride, kAttnRows);
-  if (st == S4D_OK) st = key_map(&vm, a, a.v, a.v_stride, kAttnRows);
+  st = key_map(&km, a, a.k, a.k_stride, kKeyTile);
+  if (st == S4D_OK) st = key_map(&vm, a, a.v, a.v_stride, kKeyTile);
   if (st != S4D_OK) return st;
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, km, vm, stm)

@@ -72,6 +72,43 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Two fp32 values in one 64-bit register: an instruction of the score loops does two scores, which
+// leaves the issue slots to the special-function unit.  Each half is rounded as the scalar
+// instruction would.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -107,14 +144,26 @@ struct ScoreConst {
 };
 
 // 2 / (1 + e^2y): tanh(y) = 1 - that
-__device__ __forceinline__ float tanh_rest(float acc, float k1) { return 2.0f * rcp(1.0f + ex2(acc * k1)); }
+__device__ __forceinline__ F2 tanh_rest(F2 acc, float k1) {
+  float a, b;
+  split(mul2(acc, f2(k1)), a, b);
+  split(add2(f2(ex2(a), ex2(b)), f2(1.0f)), a, b);
+  return mul2(f2(rcp(a), rcp(b)), f2(2.0f));
+}
 
+// Distances of one point (x, y) to two points given by their negated coordinates.
 template <int POS>
-__device__ __forceinline__ float distance(float ax, float ay, float bx, float by) {
-  const float dx = ax - bx;
-  if constexpr (POS == 1) return fabsf(dx);
-  const float dy = ay - by;
-  return sqrt_approx(fmaf(dx, dx, dy * dy));
+__device__ __forceinline__ F2 distance(F2 x, F2 y, F2 nx, F2 ny) {
+  const F2 dx = add2(x, nx);
+  float a, b;
+  if constexpr (POS == 1) {
+    split(dx, a, b);
+    return f2(fabsf(a), fabsf(b));
+  } else {
+    const F2 dy = add2(y, ny);
+    split(fma2(dx, dx, mul2(dy, dy)), a, b);
+    return f2(sqrt_approx(a), sqrt_approx(b));
+  }
 }
 
 // ---- tensor memory and tensor cores ----------------------------------------------------------------

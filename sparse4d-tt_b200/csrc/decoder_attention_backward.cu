@@ -56,62 +56,88 @@ struct Dkv {
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
-// One score: its weight, its gradient dS and (CAP) the cap's derivative 1 - tanh^2 = rest (2 - rest).
-template <int POS, bool CAP>
-__device__ __forceinline__ void score_terms(float acc, const ScoreConst& k, float slope2, float dist, float lse2,
-                                            float dp, float delta, bool seen, float& p, float& ds, float& dx) {
-  float s, deriv = 1.0f;
+// Two scores: their weights, gradients dS and (CAP) the cap's derivative 1 - tanh^2 = rest (2 - rest).
+struct Terms {
+  F2 p, ds, dx;
+};
+template <int POS, bool CAP, bool MASKED>
+__device__ __forceinline__ Terms score_terms(F2 acc, const ScoreConst& k, F2 nslope, F2 dist, F2 nlse2, F2 dp,
+                                             F2 ndelta, bool seen0, bool seen1) {
+  F2 s, deriv;
   if constexpr (CAP) {
-    const float rest = tanh_rest(acc, k.k1);
-    s = fmaf(-k.c, rest, k.c);
-    deriv = rest * (2.0f - rest);
+    const F2 rest = tanh_rest(acc, k.k1);
+    s = fma2(f2(-k.c), rest, f2(k.c));
+    deriv = mul2(rest, fma2(f2(-1.0f), rest, f2(2.0f)));
   } else {
-    s = acc * k.k1;
+    s = mul2(acc, f2(k.k1));
   }
-  if constexpr (POS > 0) s = fmaf(-slope2, dist, s);
-  p = seen ? ex2(s - lse2) : 0.0f;
-  ds = seen ? p * (dp - delta) : 0.0f;
-  dx = CAP ? (seen ? ds * deriv : 0.0f) : ds;  // the derivative of a masked NaN is one too
+  if constexpr (POS > 0) s = fma2(nslope, dist, s);
+  float a, b;
+  split(add2(s, nlse2), a, b);
+  a = ex2(a), b = ex2(b);
+  if constexpr (MASKED) a = seen0 ? a : 0.0f, b = seen1 ? b : 0.0f;
+  Terms r;
+  r.p = f2(a, b);
+  r.ds = mul2(r.p, add2(dp, ndelta));
+  r.dx = CAP ? mul2(r.ds, deriv) : r.ds;
+  if constexpr (MASKED) {  // dP and the derivative of a masked pair may be no numbers
+    split(r.ds, a, b);
+    r.ds = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
+    split(r.dx, a, b);
+    r.dx = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
+  }
+  return r;
 }
 
+__device__ __forceinline__ F2 half_of(const float4& v, int u) { return u == 0 ? f2(v.x, v.y) : f2(v.z, v.w); }
+__device__ __forceinline__ F2 pair_of(const uint32_t* r) { return f2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+__device__ __forceinline__ uint32_t pack(F2 v) {
+  float a, b;
+  split(v, a, b);
+  return pack2<T>(a, b);
+}
+
+// One chunk of 32 keys of a query row.  aux arrays of a tile: -x, -y, segment.
 template <int POS, bool CAP, bool MASKED>
 __device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[32], const uint32_t (&pr)[32], uint32_t (&w)[16],
                                          const ScoreConst& k, float slope2, float qx, float qy, int seg, float lse2,
-                                         float delta, const float* kx, const float* ky, const int* ks, float (&sums)[3]) {
-  float r0 = 0.0f, r1 = 0.0f, e1 = 0.0f;
+                                         float delta, const float* aux, float (&sums)[3]) {
+  F2 r0 = f2(0.0f), r1 = r0, e1 = r0;
+  const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), nlse2 = f2(-lse2), ndelta = f2(-delta);
 #pragma unroll
   for (int j4 = 0; j4 < 32; j4 += 4) {
     float4 x4, y4;
     int4 s4;
-    if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(kx + j4);
-    if constexpr (POS > 1) y4 = *reinterpret_cast<const float4*>(ky + j4);
-    if constexpr (MASKED) s4 = *reinterpret_cast<const int4*>(ks + j4);
-    float dx[4];
+    if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(aux + j4);
+    if constexpr (POS > 1) y4 = *reinterpret_cast<const float4*>(aux + kCols + j4);
+    if constexpr (MASKED) s4 = *reinterpret_cast<const int4*>(aux + 2 * kCols + j4);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float dist = 0.0f;
+    for (int u = 0; u < 4; u += 2) {
+      bool seen0 = true, seen1 = true;
+      if constexpr (MASKED) seen0 = (u == 0 ? s4.x : s4.z) == seg, seen1 = (u == 0 ? s4.y : s4.w) == seg;
+      F2 dist = f2(0.0f);
+      if constexpr (POS > 0) dist = distance<POS>(x2, y2, half_of(x4, u), POS > 1 ? half_of(y4, u) : x2);
+      const Terms t = score_terms<POS, CAP, MASKED>(pair_of(sr + j4 + u), k, nslope, dist, nlse2, pair_of(pr + j4 + u),
+                                                    ndelta, seen0, seen1);
       if constexpr (POS > 0) {
-        const float bx = u == 0 ? x4.x : u == 1 ? x4.y : u == 2 ? x4.z : x4.w;
-        float by = 0.0f;
-        if constexpr (POS > 1) by = u == 0 ? y4.x : u == 1 ? y4.y : u == 2 ? y4.z : y4.w;
-        dist = distance<POS>(qx, qy, bx, by);
+        if constexpr (MASKED) {
+          float a, b;
+          split(dist, a, b);
+          dist = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
+        }
+        r0 = add2(r0, t.ds);
+        r1 = fma2(t.ds, dist, r1);
+        e1 = fma2(t.p, dist, e1);
       }
-      bool seen = true;
-      if constexpr (MASKED) seen = (u == 0 ? s4.x : u == 1 ? s4.y : u == 2 ? s4.z : s4.w) == seg;
-      float p, ds;
-      score_terms<POS, CAP>(__uint_as_float(sr[j4 + u]), k, slope2, dist, lse2, __uint_as_float(pr[j4 + u]), delta,
-                            seen, p, ds, dx[u]);
-      if constexpr (POS > 0) {
-        if (MASKED && !seen) dist = 0.0f;
-        r0 += ds;
-        r1 = fmaf(ds, dist, r1);
-        e1 = fmaf(p, dist, e1);
-      }
+      w[(j4 + u) / 2] = pack(t.dx);
     }
-    w[j4 / 2] = pack2<T>(dx[0], dx[1]);
-    w[j4 / 2 + 1] = pack2<T>(dx[2], dx[3]);
   }
-  if constexpr (POS > 0) sums[0] += r0, sums[1] += r1, sums[2] += e1;
+  if constexpr (POS > 0) {
+    float a, b;
+    split(r0, a, b), sums[0] += a + b;
+    split(r1, a, b), sums[1] += a + b;
+    split(e1, a, b), sums[2] += a + b;
+  }
 }
 
 template <int DP, int POS, bool CAP>
@@ -269,7 +295,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       }
       p.delta[lse_row] = delta;
     }
-    float* aux = reinterpret_cast<float*>(smem + S::kAux);  // [2][3][64]: x, y, segment of the keys
+    float* aux = reinterpret_cast<float*>(smem + S::kAux);  // [2][3][64]: -x, -y, segment of the keys
     float nx = 0.0f, ny = 0.0f;
     int ns = -1;
     auto fetch = [&](int t) {
@@ -278,8 +304,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const bool in = j < valid;
       ns = in ? (p.k_seg != nullptr ? max(-1, __ldg(p.k_seg + b * p.nk + j)) : 0) : -1;
       if constexpr (POS > 0) {
-        nx = in ? __ldg(p.k_pos + (b * p.nk + j) * POS) : 0.0f;
-        if constexpr (POS > 1) ny = in ? __ldg(p.k_pos + (b * p.nk + j) * POS + 1) : 0.0f;
+        nx = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS) : 0.0f;
+        if constexpr (POS > 1) ny = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS + 1) : 0.0f;
       }
     };
     fetch(t0);
@@ -315,10 +341,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           tmem_ld_wait(pr);
           const float* cx = bx + c * 32;
           if (masked)
-            dq_chunk<POS, CAP, true>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, cx + kCols,
-                                     reinterpret_cast<const int*>(cx + 2 * kCols), sums);
+            dq_chunk<POS, CAP, true>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, sums);
           else
-            dq_chunk<POS, CAP, false>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, cx + kCols, nullptr, sums);
+            dq_chunk<POS, CAP, false>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, sums);
           tmem_st16(tmem + lanes + c * 16, w);
         }
         tmem_st_wait();
@@ -364,11 +389,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
 }
 
-// One chunk of 32 query columns of a key's row.  aux arrays of a tile: lse2, delta, x, y, slope2, segment.
+// One chunk of 32 query columns of a key's row.  aux arrays of a tile: -lse2, -delta, -x, -y, -slope2, segment.
 template <int POS, bool CAP, bool MASKED>
 __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[32], const uint32_t (&pr)[32], uint32_t (&wp)[16],
                                           uint32_t (&wd)[16], const ScoreConst& k, float kx, float ky, int seg,
                                           const float* aux) {
+  const F2 x2 = f2(kx), y2 = f2(ky);
 #pragma unroll
   for (int j4 = 0; j4 < 32; j4 += 4) {
     const float4 l4 = *reinterpret_cast<const float4*>(aux + j4);
@@ -379,29 +405,20 @@ __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[32], const uint32
     if constexpr (POS > 1) y4 = *reinterpret_cast<const float4*>(aux + 3 * kCols + j4);
     if constexpr (POS > 0) sl4 = *reinterpret_cast<const float4*>(aux + 4 * kCols + j4);
     if constexpr (MASKED) s4 = *reinterpret_cast<const int4*>(aux + 5 * kCols + j4);
-    float pv[4], dx[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float dist = 0.0f, slope2 = 0.0f;
+    for (int u = 0; u < 4; u += 2) {
+      bool seen0 = true, seen1 = true;
+      if constexpr (MASKED) seen0 = (u == 0 ? s4.x : s4.z) == seg, seen1 = (u == 0 ? s4.y : s4.w) == seg;
+      F2 dist = f2(0.0f), nslope = dist;
       if constexpr (POS > 0) {
-        const float bx = u == 0 ? x4.x : u == 1 ? x4.y : u == 2 ? x4.z : x4.w;
-        float by = 0.0f;
-        if constexpr (POS > 1) by = u == 0 ? y4.x : u == 1 ? y4.y : u == 2 ? y4.z : y4.w;
-        dist = distance<POS>(bx, by, kx, ky);
-        slope2 = u == 0 ? sl4.x : u == 1 ? sl4.y : u == 2 ? sl4.z : sl4.w;
+        dist = distance<POS>(x2, y2, half_of(x4, u), POS > 1 ? half_of(y4, u) : x2);
+        nslope = half_of(sl4, u);
       }
-      bool seen = true;
-      if constexpr (MASKED) seen = (u == 0 ? s4.x : u == 1 ? s4.y : u == 2 ? s4.z : s4.w) == seg;
-      const float lse2 = u == 0 ? l4.x : u == 1 ? l4.y : u == 2 ? l4.z : l4.w;
-      const float delta = u == 0 ? d4.x : u == 1 ? d4.y : u == 2 ? d4.z : d4.w;
-      float ds;
-      score_terms<POS, CAP>(__uint_as_float(sr[j4 + u]), k, slope2, dist, lse2, __uint_as_float(pr[j4 + u]), delta,
-                            seen, pv[u], ds, dx[u]);
+      const Terms t = score_terms<POS, CAP, MASKED>(pair_of(sr + j4 + u), k, nslope, dist, half_of(l4, u),
+                                                    pair_of(pr + j4 + u), half_of(d4, u), seen0, seen1);
+      wp[(j4 + u) / 2] = pack(t.p);
+      wd[(j4 + u) / 2] = pack(t.dx);
     }
-    wp[j4 / 2] = pack2<T>(pv[0], pv[1]);
-    wp[j4 / 2 + 1] = pack2<T>(pv[2], pv[3]);
-    wd[j4 / 2] = pack2<T>(dx[0], dx[1]);
-    wd[j4 / 2 + 1] = pack2<T>(dx[2], dx[3]);
   }
 }
 
@@ -527,7 +544,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
         if constexpr (POS > 1) ky = __ldg(p.k_pos + (b * p.nk + key) * POS + 1);
       }
     }
-    // [2][6][64]: lse2, delta, x, y, slope2, segment of the queries; threads 0-63 carry the first two
+    // [2][6][64]: -lse2, -delta, -x, -y, -slope2, segment of the queries; threads 0-63 carry the first two
     // of their query one tile ahead, threads 64-127 the others
     float* aux = reinterpret_cast<float*>(smem + S::kAux);
     float c0 = 0.0f, c1 = 0.0f, c2 = 0.0f;
@@ -541,13 +558,13 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
       if (tid < kCols) {
         const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
         const float l = in ? __ldg(p.lse + r) : -INFINITY;
-        c0 = l == -INFINITY ? INFINITY : l * kLog2e;  // no key seen: weights of 2^-inf
-        c1 = in ? p.delta[r] : 0.0f;
+        c0 = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
+        c1 = in ? -p.delta[r] : 0.0f;
       } else {
         if constexpr (POS > 0) {
-          c0 = in ? __ldg(p.q_pos + (b * p.nq + i) * POS) : 0.0f;
-          if constexpr (POS > 1) c1 = in ? __ldg(p.q_pos + (b * p.nq + i) * POS + 1) : 0.0f;
-          c2 = in ? __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
+          c0 = in ? -__ldg(p.q_pos + (b * p.nq + i) * POS) : 0.0f;
+          if constexpr (POS > 1) c1 = in ? -__ldg(p.q_pos + (b * p.nq + i) * POS + 1) : 0.0f;
+          c2 = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
         }
         c3 = in ? (p.q_seg != nullptr ? max(-1, __ldg(p.q_seg + b * p.nq + i)) : 0) : -1;
       }

@@ -2,21 +2,23 @@
 // the allowed keys, in one pass over the keys with a running maximum m and sum l per row.
 //
 // One CTA owns 128 rows of one shared head: row r is query r / rep of head g rep + r % rep, so that
-// the rep heads that share keys read them once.  It walks the keys in tiles of 128:
+// the rep heads that share keys read them once.  It walks the keys in tiles of 64:
 //   warp 4      loads K and V tiles by TMA into rings of shared memory;
-//   warp 5      issues S = Q K^T into 128 tensor-memory columns, and once P is there O += P V, with
-//               P read from tensor memory and V as an MN-major operand;
-//   warps 0-3   one row a thread: scores from tensor memory, cap, bias and mask in registers, the
-//               row maximum without a shuffle, P = 2^(s - m) back over S as 16-bit pairs.
+//   warp 5      issues S = Q K^T for the next tile into one of two score buffers in tensor memory (64
+//               columns each), and once P of this tile is there O += P V, with P read from tensor
+//               memory and V as an MN-major operand;
+//   warps 0-3   one row a thread: scores from tensor memory, cap, bias and mask in registers (two
+//               scores an instruction), the row maximum without a shuffle, P = 2^(s - m) back over S
+//               as 16-bit pairs.
 // O is only rescaled when a row's maximum grew by more than 2^8 since the last time: P then stays
 // under 2^8, which costs no precision in a float.  P is rounded to the inputs' type because the
 // tensor cores multiply it with V in that type; l adds the unrounded values in fp32.
 //
 // What bounds it: a score costs one exponential (16 a clock on an SM), a second special-function
 // instruction with a 2-D distance and two more with a cap, against 4 D flops: for D = 64 the
-// exponentials take four times as long as the products.  So two CTAs share an SM (256 tensor-memory
-// columns and at most 113 KB of shared memory each): one's products run under the other's
-// exponentials, and neither needs a second score buffer.
+// exponentials take four times as long as the products.  So the row threads must not wait: the next
+// tile's scores are always under way, and two CTAs share an SM (256 tensor-memory columns and at
+// most 113 KB of shared memory each).
 //
 // Few rows and many keys: the keys are cut into parts, each CTA writes its part's normalised O and
 // log-sum-exp, and a second launch joins them.
@@ -25,47 +27,54 @@
 namespace s4d {
 namespace {
 
+constexpr int kKeys = 64;  // keys of a tile
+
 template <int DP>
 struct Fwd {
-  static constexpr int kBlock = kAttnRows * 128;       // 64 columns of a 128-row tile
-  static constexpr int kTile = DP / 64 * kBlock;
-  static constexpr int kStages = DP == 64 ? 2 : 1;     // of K and of V
-  static constexpr int kK = kTile, kV = kK + kStages * kTile, kAux = kV + kStages * kTile;
-  // x, y of the keys and their segments, two buffers; barriers; tensor-memory slot, abort, skip[2]
-  static constexpr int kBars = kAux + 2 * 3 * kAttnRows * 4;
-  static constexpr int kNumBars = 4 * kStages + 3;
+  static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kKeys * 128;  // 64 columns of Q, of K or V
+  static constexpr int kQ = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
+  static constexpr int kStages = DP == 64 ? 4 : 2;     // of K and of V
+  static constexpr int kK = kQ, kV = kK + kStages * kTile, kAux = kV + kStages * kTile;
+  // negated x, y of the keys and their segments, two buffers; barriers; tensor-memory slot, abort, skip[2]
+  static constexpr int kBars = kAux + 2 * 3 * kKeys * 4;
+  static constexpr int kNumBars = 4 * kStages + 6;
   static constexpr int kCtl = kBars + kNumBars * 8;
   static constexpr int kKinds = kCtl + 16;
-  static constexpr uint32_t kCols = 256;  // S / P: 128, O: DP
+  static constexpr uint32_t kCols = 256;  // S / P: 2 x 64, O: DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
-template <typename T, int DP, int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void scores(uint32_t (&r)[128], const ScoreConst& k, float slope2, float qx, float qy,
-                                       int seg, const float* kx, const float* ky, const int* ks, float& mx) {
+// The 64 scores of a row, in base 2, and their maximum.
+template <int POS, bool CAP, bool MASKED>
+__device__ __forceinline__ void scores(uint32_t (&r)[64], const ScoreConst& k, float slope2, float qx, float qy,
+                                       int seg, const float* aux, float& mx) {
+  const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), k1 = f2(k.k1), c = f2(k.c), nc = f2(-k.c);
 #pragma unroll
-  for (int j4 = 0; j4 < 128; j4 += 4) {
+  for (int j4 = 0; j4 < kKeys; j4 += 4) {
     float4 x4, y4;
     int4 s4;
-    if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(kx + j4);
-    if constexpr (POS > 1) y4 = *reinterpret_cast<const float4*>(ky + j4);
-    if constexpr (MASKED) s4 = *reinterpret_cast<const int4*>(ks + j4);
+    if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(aux + j4);
+    if constexpr (POS > 1) y4 = *reinterpret_cast<const float4*>(aux + kKeys + j4);
+    if constexpr (MASKED) s4 = *reinterpret_cast<const int4*>(aux + 2 * kKeys + j4);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float acc = __uint_as_float(r[j4 + u]);
-      float s = CAP ? fmaf(-k.c, tanh_rest(acc, k.k1), k.c) : acc * k.k1;
+    for (int u = 0; u < 4; u += 2) {
+      const F2 acc = f2(__uint_as_float(r[j4 + u]), __uint_as_float(r[j4 + u + 1]));
+      F2 s = CAP ? fma2(nc, tanh_rest(acc, k.k1), c) : mul2(acc, k1);
       if constexpr (POS > 0) {
-        const float bx = u == 0 ? x4.x : u == 1 ? x4.y : u == 2 ? x4.z : x4.w;
-        float by = 0.0f;
-        if constexpr (POS > 1) by = u == 0 ? y4.x : u == 1 ? y4.y : u == 2 ? y4.z : y4.w;
-        s = fmaf(-slope2, distance<POS>(qx, qy, bx, by), s);
+        const F2 nx = u == 0 ? f2(x4.x, x4.y) : f2(x4.z, x4.w);
+        F2 ny = nx;
+        if constexpr (POS > 1) ny = u == 0 ? f2(y4.x, y4.y) : f2(y4.z, y4.w);
+        s = fma2(nslope, distance<POS>(x2, y2, nx, ny), s);
       }
+      float a, b;
+      split(s, a, b);
       if constexpr (MASKED) {
-        const int kseg = u == 0 ? s4.x : u == 1 ? s4.y : u == 2 ? s4.z : s4.w;
-        s = kseg == seg ? s : -INFINITY;
+        a = (u == 0 ? s4.x : s4.z) == seg ? a : -INFINITY;
+        b = (u == 0 ? s4.y : s4.w) == seg ? b : -INFINITY;
       }
-      mx = fmaxf(mx, s);
-      r[j4 + u] = __float_as_uint(s);
+      mx = max3(mx, a, b);
+      r[j4 + u] = __float_as_uint(a);
+      r[j4 + u + 1] = __float_as_uint(b);
     }
   }
 }
@@ -79,28 +88,28 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const uint32_t k_full = sbase + S::kBars, k_empty = k_full + 8 * S::kStages, v_full = k_empty + 8 * S::kStages,
-                 v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, p_full = s_full + 8,
-                 o_full = p_full + 8;
+                 v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, p_full = s_full + 16,
+                 pv_done = p_full + 16, o_full = pv_done + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip_pv = abort_flag + 1;
   unsigned char* kinds = smem + S::kKinds;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // blockIdx.x = ((b G + g) row tiles + row tile) splits + split
+  // blockIdx.x = ((b G + g) row tiles + row tile) splits + part
   const int64_t rows = p.nq * p.rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
   int64_t u = blockIdx.x;
-  const int split = int(u % p.splits);
+  const int part = int(u % p.splits);
   u /= p.splits;
   const int64_t row0 = u % row_tiles * kAttnRows;
   u /= row_tiles;
   const int g = int(u % p.kv_heads), b = int(u / p.kv_heads);
 
   // keys of this part
-  const int64_t first = split * p.tiles_per_split;
+  const int64_t first = part * p.tiles_per_split;
   int64_t valid = p.nk;
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
-  const int64_t all_tiles = (valid + kAttnRows - 1) / kAttnRows;
+  const int64_t all_tiles = (valid + kKeys - 1) / kKeys;
   const int tiles = int(max(int64_t(0), min(p.tiles_per_split, all_tiles - first)));
 
   if (threadIdx.x == 0) {
@@ -110,8 +119,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       mbar_init(v_full + 8 * s, 1);
       mbar_init(v_empty + 8 * s, 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, kAttnRows);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full + 8 * s, 1);
+      mbar_init(p_full + 8 * s, kAttnRows);
+    }
+    mbar_init(pv_done, 1);
     mbar_init(o_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const int64_t i0 = row0 / p.rep, i1 = (min(rows, row0 + kAttnRows) - 1) / p.rep;
       own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
     }
-    classify_tiles(kinds, first, tiles, kAttnRows, valid, segs ? p.k_seg + b * p.nk : nullptr, own, true);
+    classify_tiles(kinds, first, tiles, kKeys, valid, segs ? p.k_seg + b * p.nk : nullptr, own, true);
   }
   const uint32_t rep = uint32_t(p.rep);  // rows of a shared head stay below 2^31
   // Q: 16-byte pieces, zero past the last row and column, in the swizzled layout TMA gives K and V
@@ -135,13 +147,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     if (row < rows && d * 8 < p.dim)
       v = ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + int64_t(uint32_t(row) / rep) * p.q_sn + (g * p.rep + uint32_t(row) % rep) * p.q_sh +
                     d * 8);
-    *reinterpret_cast<uint4*>(smem + (d / 8) * S::kBlock + r * 128 + (((d & 7) ^ (r & 7)) << 4)) = v;
+    *reinterpret_cast<uint4*>(smem + (d / 8) * S::kOwnBlock + r * 128 + (((d & 7) ^ (r & 7)) << 4)) = v;
   }
   fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 2 * kKeys;
   const int t0 = next_tile(kinds, -1, tiles);
 
   if (warp == 4) {
@@ -150,15 +162,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages + 1) & 1;
-        const int key = int((first + t) * kAttnRows);
+        const int key = int((first + t) * kKeys);
         if (n >= S::kStages && !mbar_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        load_tile<DP, kAttnRows>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, key, b);
+        load_tile<DP, kKeys>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, key, b);
         if (n >= S::kStages && !mbar_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
           // the K load is out: it may not land in the memory of a CTA that is gone
           mbar_wait(k_full + 8 * s, (n / S::kStages) & 1, nullptr);
           break;
         }
-        load_tile<DP, kAttnRows>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, key, b);
+        load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, key, b);
       }
       for (int i = max(0, n - S::kStages); i < n; ++i) {
         mbar_wait(k_full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
@@ -167,21 +179,32 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     }
   } else if (warp == 5) {
     if (lane == 0) {
-      int n = 0;
-      for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+      // S of tile n, n counting the walked tiles
+      auto issue_scores = [&](int n) {
         const int s = n % S::kStages;
-        const uint32_t parity = (n / S::kStages) & 1;
-        if (!mbar_wait(k_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
+        if (!mbar_wait(k_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns)) return false;
         tc_fence_after();
-        mma_scores<T, DP>(tmem, sbase, S::kBlock, sbase + S::kK + s * S::kTile, S::kBlock, 128);
+        mma_scores<T, DP>(tmem + (n & 1) * kKeys, sbase, S::kOwnBlock, sbase + S::kK + s * S::kTile, S::kBlock, kKeys);
         mma_commit(k_empty + 8 * s);
-        mma_commit(s_full);
-        if (!mbar_wait(v_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        if (!mbar_wait(p_full, n & 1, abort_flag, p.wait_limit_ns)) break;
+        mma_commit(s_full + 8 * (n & 1));
+        return true;
+      };
+      int n = 0;
+      bool ok = t0 >= tiles || issue_scores(0);
+      for (int t = t0; ok && t < tiles; ++n) {
+        const int s = n % S::kStages, next = next_tile(kinds, t, tiles);
+        // The next scores go over P of the tile before this one, whose product with V is issued: the
+        // tensor cores work in order.
+        if (next < tiles && !(ok = issue_scores(n + 1))) break;
+        ok = mbar_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns) &&
+             mbar_wait(p_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
+        if (!ok) break;
         tc_fence_after();
         if (!(kinds[t] == kTileMasked && skip_pv[n & 1]))
-          mma_accumulate<T, DP, kAttnRows>(tmem_o, tmem, sbase + S::kV + s * S::kTile, n > 0);
+          mma_accumulate<T, DP, kKeys>(tmem_o, tmem + (n & 1) * kKeys, sbase + S::kV + s * S::kTile, n > 0);
         mma_commit(v_empty + 8 * s);
+        mma_commit(pv_done);
+        t = next;
       }
       mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
       mbar_wait(o_full, 0, nullptr);
@@ -207,18 +230,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       seg = __ldg(p.q_seg + b * p.nq + i);
       if (seg < 0) seg = -2;
     }
-    float* kx = reinterpret_cast<float*>(smem + S::kAux);  // [2][3][128]: x, y, segment
-    // this thread's key of a tile: position and segment, loaded one tile ahead
+    float* aux = reinterpret_cast<float*>(smem + S::kAux);  // [2][3][64]: -x, -y, segment
+    // threads 0-63: a key of the next tile, loaded one tile ahead
     float nx = 0.0f, ny = 0.0f;
     int ns = -1;
     auto fetch = [&](int t) {
-      if (t >= tiles) return;
-      const int64_t j = (first + t) * kAttnRows + tid;
+      if (t >= tiles || tid >= kKeys) return;
+      const int64_t j = (first + t) * kKeys + tid;
       const bool in = j < valid;
       ns = in ? (p.k_seg != nullptr ? max(-1, __ldg(p.k_seg + b * p.nk + j)) : 0) : -1;
       if constexpr (POS > 0) {
-        nx = in ? __ldg(p.k_pos + (b * p.nk + j) * POS) : 0.0f;
-        if constexpr (POS > 1) ny = in ? __ldg(p.k_pos + (b * p.nk + j) * POS + 1) : 0.0f;
+        nx = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS) : 0.0f;
+        if constexpr (POS > 1) ny = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS + 1) : 0.0f;
       }
     };
     fetch(t0);
@@ -228,32 +251,38 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     for (int t = t0; t < tiles; ++n) {
       const int next = next_tile(kinds, t, tiles);
       const bool masked = kinds[t] == kTileMasked;
-      const float* bx = kx + (n & 1) * 3 * 128;
-      kx[(n & 1) * 3 * 128 + tid] = nx;
-      kx[(n & 1) * 3 * 128 + 128 + tid] = ny;
-      reinterpret_cast<int*>(kx)[(n & 1) * 3 * 128 + 256 + tid] = ns;
+      float* bx = aux + (n & 1) * 3 * kKeys;
+      if (tid < kKeys) {
+        bx[tid] = nx;
+        bx[kKeys + tid] = ny;
+        reinterpret_cast<int*>(bx)[2 * kKeys + tid] = ns;
+      }
       rows_sync();
       fetch(next);
       bool bad = false;  // a masked tile whose V holds values that are no numbers
+      const unsigned char* vt = smem + S::kV + n % S::kStages * S::kTile;
+      const uint32_t tmem_s = tmem + lanes + (n & 1) * kKeys;
       if (masked) {
-        const int s = n % S::kStages;
-        if (!dead) dead = !warp_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
-        bad = rows_any(!dead && row_not_finite<T, DP>(smem + S::kV + s * S::kTile, S::kBlock, tid));
+        if (!dead) dead = !warp_wait(v_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
+        bad = rows_any(!dead && tid < kKeys && row_not_finite<T, DP>(vt, S::kBlock, tid));
         if (tid == 0) skip_pv[n & 1] = bad;
       }
-      if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
       if (!dead && warp_live) {
-        uint32_t r[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_async(tmem + lanes + c * 32, r + c * 32);
+        uint32_t r[kKeys];
+        tmem_ld32_async(tmem_s, r);
+        tmem_ld32_async(tmem_s + 32, r + 32);
         tmem_ld_wait(r);
         float mx = -INFINITY;
         if (masked)
-          scores<T, DP, POS, CAP, true>(r, k, slope2, qx, qy, seg, bx, bx + 128, reinterpret_cast<const int*>(bx + 256), mx);
+          scores<POS, CAP, true>(r, k, slope2, qx, qy, seg, bx, mx);
         else
-          scores<T, DP, POS, CAP, false>(r, k, slope2, qx, qy, seg, bx, bx + 128, nullptr, mx);
+          scores<POS, CAP, false>(r, k, slope2, qx, qy, seg, bx, mx);
         const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
-        if (__any_sync(0xffffffffu, grow)) {
+        const bool any_grow = __any_sync(0xffffffffu, grow);
+        if (n > 0 && (any_grow || bad))  // O is about to change outside the tensor cores
+          dead = !warp_wait(pv_done, (n - 1) & 1, abort_flag, p.wait_limit_ns);
+        if (any_grow && !dead) {
           const float f = grow ? ex2(m - mx) : 1.0f;  // 0 for a row's first keys
           if (grow) m = mx;
           l *= f;
@@ -269,28 +298,26 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m;  // no key yet: every score is -inf, every weight 0
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const F2 nbase = f2(m == -INFINITY ? 0.0f : -m);  // no key yet: every score is -inf, every weight 0
+        F2 sum[2] = {f2(0.0f), f2(0.0f)};
+        uint32_t w[kKeys / 2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float a = ex2(__uint_as_float(r[c * 64 + 2 * e]) - base);
-            const float d = ex2(__uint_as_float(r[c * 64 + 2 * e + 1]) - base);
-            sum[e & 3] += a + d;
-            w[e] = pack2<T>(a, d);
-          }
-          tmem_st32(tmem + lanes + c * 32, w);
+        for (int e = 0; e < kKeys / 2; ++e) {
+          float a, d;
+          split(add2(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), nbase), a, d);
+          a = ex2(a), d = ex2(d);
+          sum[e & 1] = add2(sum[e & 1], f2(a, d));
+          w[e] = pack2<T>(a, d);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(tmem_s, w);
+        float a, d;
+        split(add2(sum[0], sum[1]), a, d);
+        l += a + d;
         tmem_st_wait();
-        if (bad)
-          accumulate_nonzero<T, DP, kAttnRows>(tmem_o + lanes, tmem + lanes,
-                                               smem + S::kV + n % S::kStages * S::kTile, n == 0);
+        if (bad && !dead) accumulate_nonzero<T, DP, kKeys>(tmem_o + lanes, tmem_s, vt, n == 0);
       }
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(p_full + 8 * (n & 1));
       t = next;
     }
     // O / l, the log-sum-exp, and zeros for rows without a key
@@ -303,7 +330,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const float lse = any ? (m + log2f(l)) * kLn2 : -INFINITY;
       if (live) {
         if (p.splits > 1)
-          p.part_lse[split * all_rows + lse_row] = lse;
+          p.part_lse[part * all_rows + lse_row] = lse;
         else if (p.lse != nullptr)
           p.lse[lse_row] = lse;
       }
@@ -318,7 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         for (int e = 0; e < 32; ++e) f[e] = any ? __uint_as_float(o[e]) * inv : 0.0f;
         if (!live) continue;
         if (p.splits > 1) {
-          float* dst = p.part_o + (split * all_rows + out_row) * p.dim + c * 32;
+          float* dst = p.part_o + (part * all_rows + out_row) * p.dim + c * 32;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (c * 32 + e * 4 < p.dim)
