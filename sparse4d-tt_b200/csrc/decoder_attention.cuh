@@ -20,7 +20,6 @@
 
 namespace s4d {
 
-constexpr int kAttnThreads = 192;   // warps 0-3: one score row a thread; 4: TMA; 5: tensor cores
 constexpr int kAttnRows = 128;      // rows of a tile = tensor-memory lanes
 constexpr int kAttnMaxTiles = 8192; // tiles of the other axis one CTA walks (its table of tile kinds)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -294,18 +293,21 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * ROWS * 128, map, bar, c * 64, h, n, b);
 }
 
-// Barriers of the 128 row threads (the other warps take no part).  Every row thread passes the same
-// number of them whatever happens: one that gave up waiting goes on through its loop without work.
-__device__ __forceinline__ void rows_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool rows_any(bool v) {
+// Barriers of row threads (the other warps take no part).  Every row thread passes the same number of
+// them whatever happens: one that gave up waiting goes on through its loop without work.
+// barrier_sync / barrier_any: `threads` threads meet at barrier `id`; any: whether one brought true.
+__device__ __forceinline__ void barrier_sync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool v) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 2, 128, p;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(uint32_t(v))
+      : "r"(id), "r"(threads), "r"(uint32_t(v))
       : "memory");
   return r != 0;
 }
@@ -415,13 +417,13 @@ __device__ __forceinline__ SegRange seg_range(const int32_t* ids, int n) {
 __device__ __forceinline__ void classify_tiles(unsigned char* kinds, int64_t first, int tiles, int rows, int64_t valid,
                                                const int32_t* ids, const SegRange& own, bool own_whole) {
   if (ids == nullptr) {
-    for (int t = threadIdx.x; t < tiles; t += kAttnThreads) {
+    for (int t = threadIdx.x; t < tiles; t += blockDim.x) {
       const int64_t r0 = (first + t) * rows;
       kinds[t] = r0 >= valid ? kTileSkip : (own_whole && r0 + rows <= valid ? kTileFull : kTileMasked);
     }
     return;
   }
-  for (int t = threadIdx.x >> 5; t < tiles; t += kAttnThreads / 32) {
+  for (int t = threadIdx.x >> 5; t < tiles; t += blockDim.x / 32) {
     const int64_t r0 = (first + t) * rows;
     const int n = int(valid - r0 < rows ? (valid > r0 ? valid - r0 : 0) : rows);
     const SegRange r = seg_range(ids + r0, n);

@@ -27,6 +27,7 @@ namespace {
 
 using T = __nv_bfloat16;
 constexpr int kCols = 64;  // rows of a walked tile
+constexpr int kAttnThreads = 192;  // warps 0-3: one score row a thread; 4: TMA; 5: tensor cores
 
 template <int DP>
 struct Dq {
@@ -321,13 +322,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         bx[kCols + tid] = ny;
         reinterpret_cast<int*>(bx)[2 * kCols + tid] = ns;
       }
-      rows_sync();
+      barrier_sync(1, kAttnRows);
       fetch(next);
       bool bad = false;
       const unsigned char* kt = smem + S::kK + n % S::kStages * S::kTile;
       if (masked) {
         if (!dead) dead = !warp_wait(k_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
-        bad = rows_any(!dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
+        bad = barrier_any(2, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
         if (tid == 0) skip[n & 1] = bad;
       }
       if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
@@ -586,14 +587,14 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
         bx[4 * kCols + e] = c2;
         reinterpret_cast<int*>(bx)[5 * kCols + e] = c3;
       }
-      rows_sync();
+      barrier_sync(1, kAttnRows);
       fetch(next_hh, next);
       bool bad = false;
       const int s = n % S::kStages;
       const unsigned char *qt = smem + S::kQ + s * 2 * S::kTile, *dot = qt + S::kTile;
       if (masked) {
         if (!dead) dead = !warp_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
-        bad = rows_any(!dead && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, e));
+        bad = barrier_any(2, kAttnRows, !dead && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, e));
         if (tid == 0) skip[n & 1] = bad;
       }
       if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
