@@ -45,10 +45,10 @@ struct Strides {
   }
 };
 
-// Tensor map of [B, N, heads, D] 16-bit elements, loaded in boxes of 64 columns x box_rows rows of one
-// head with the 128-byte swizzle; columns past D and rows past N are zero.
+// Tensor map of [B, N, heads, D] 16-bit elements, loaded in boxes of 64 columns x box_heads heads x box_rows
+// rows with the 128-byte swizzle; columns past D and rows past N are zero.
 int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t heads, int64_t rows, int64_t batch,
-             const Strides& s, int box_rows) {
+             const Strides& s, int box_rows, int box_heads = 1) {
   EncodeTiledFn fn = encode_tiled();
   if (fn == nullptr) return fail(S4D_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   // an axis of one entry still needs a stride the encoder takes
@@ -56,7 +56,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t
   const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(batch)};
   const cuuint64_t strides[3] = {cuuint64_t(s.h > 0 ? s.h * 2 : row_bytes), cuuint64_t(s.n > 0 ? s.n * 2 : row_bytes),
                                  cuuint64_t(s.b > 0 ? s.b * 2 : row_bytes)};
-  const cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_heads), cuuint32_t(box_rows), 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r =
       fn(map, dtype == S4D_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
@@ -119,24 +119,28 @@ int check_args(const char* fn, const s4d_attention_args* a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Parts of the keys.  A tile of 128 rows and one shared head is one CTA, and two of them share an SM:
-// with fewer CTAs than that the keys are cut until the SMs are full, but not below four tiles of 64
-// keys a part, since a part costs a launch's start and the join reads it again.
+// with fewer CTAs than that the keys are cut until the SMs are full, but not below two tiles of 64
+// keys a part (one for each stream of row warps).  Up to 11 parts become at most 8, which one cluster
+// joins in shared memory: a second launch and its pass over memory cost more than a quarter of the
+// CTAs brings.
 int64_t key_splits(const s4d_attention_args& a) {
   const int64_t ctas = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), kAttnRows);
-  const int64_t tiles = ceil_div(a.keys, kKeyTile);
+  const int64_t tiles = ceil_div(a.keys, kKeyTile), most = 2 * device_sms();
   const int64_t least = ceil_div(tiles, kAttnMaxTiles);
-  int64_t splits = 1;
-  if (ctas > 0 && ctas < 2 * device_sms()) splits = ceil_div(2 * device_sms(), ctas);
-  if (splits > tiles / 4) splits = tiles / 4;
+  int64_t splits = ctas > 0 ? most / ctas : 1;
+  if (splits > tiles / 2) splits = tiles / 2;
+  if (splits > 8 && splits < 12) splits = 8;
   if (splits < least) splits = least;
   if (splits < 1) splits = 1;
   // as many parts as there are after each got the same number of tiles
   return tiles == 0 ? 1 : ceil_div(tiles, ceil_div(tiles, splits));
 }
 
+int cluster_of(int64_t splits) { return splits <= 8 ? int(splits) : 1; }
+
 size_t forward_workspace(const s4d_attention_args& a) {
   const int64_t splits = key_splits(a);
-  return splits == 1 ? 0 : size_t(splits) * size_t(a.batch * a.queries * a.heads) * size_t(a.dim + 1) * sizeof(float);
+  return splits == cluster_of(splits) ? 0 : size_t(splits) * size_t(a.batch * a.queries * a.heads) * size_t(a.dim + 1) * sizeof(float);
 }
 
 AttnParams fill(const s4d_attention_args& a) {
@@ -168,24 +172,28 @@ int query_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, c
                   box_rows);
 }
 
-// dslopes of one slope per head: the sum of every row's, one head a block, its rows added in an order
-// that depends on the sizes alone.
-__global__ void __launch_bounds__(512) slope_sum_kernel(const float* rows, int64_t n, int heads, float* out) {
-  __shared__ float part[16];
+// dslopes of one slope per head: the sum of every row's ([B, H, Nq]), one head a block, its rows added
+// in an order that depends on the sizes alone.
+__global__ void __launch_bounds__(1024) slope_sum_kernel(const float* rows, int batch, int64_t nq, int heads, float* out) {
+  __shared__ float part[32];
   const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t r = threadIdx.x; r < n; r += 4 * 512)
+  float s[8] = {};
+  griddep_wait();
+  for (int b = 0; b < batch; ++b) {
+    const float* src = rows + (int64_t(b) * heads + h) * nq;
+    for (int64_t r = threadIdx.x; r < nq; r += 8 * 1024)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (r + u * 512 < n) s[u] += rows[(r + u * 512) * heads + h];
-  float v = (s[0] + s[1]) + (s[2] + s[3]);
+      for (int u = 0; u < 8; ++u)
+        if (r + u * 1024 < nq) s[u] += src[r + u * 1024];
+  }
+  float v = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (lane == 0) part[warp] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
     v = 0.0f;
-    for (int w = 0; w < 16; ++w) v += part[w];
+    for (int w = 0; w < 32; ++w) v += part[w];
     out[h] = v;
   }
 }
@@ -230,16 +238,23 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
   if (need > 0 && (a.workspace == nullptr || !aligned_to(a.workspace, 16) || a.workspace_bytes < need))
     S4D_BAD(S4D_ERR_INVALID_ARG, "missing, misaligned or small workspace");
   p.splits = int(splits);
+  p.cluster = cluster_of(splits);
   p.tiles_per_split = ceil_div(tiles, splits);
   p.part_o = static_cast<float*>(a.workspace);
-  p.part_lse = p.part_o + (splits > 1 ? splits * a.batch * a.queries * a.heads * a.dim : 0);
-  CUtensorMap km, vm;
-  st = key_map(&km, a, a.k, a.k_stride, kKeyTile);
-  if (st == S4D_OK) st = key_map(&vm, a, a.v, a.v_stride, kKeyTile);
+  p.part_lse = p.part_o + (need > 0 ? splits * a.batch * a.queries * a.heads * a.dim : 0);
+  AttnForwardMaps m;
+  st = key_map(&m.k, a, a.k, a.k_stride, kKeyTile);
+  if (st == S4D_OK) st = key_map(&m.v, a, a.v, a.v_stride, kKeyTile);
+  // a box of 128 / rep queries of all the heads that share keys (the kernel gathers Q itself for a rep
+  // that does not divide 128: the map is then not used)
+  const bool whole = kAttnRows % p.rep == 0;
+  if (st == S4D_OK)
+    st = make_map(&m.q, a.q, a.dtype, a.dim, a.heads, a.queries, a.batch, Strides(a.q_stride, a.batch, a.queries, a.heads),
+                  whole ? kAttnRows / p.rep : 1, whole ? p.rep : 1);
   if (st != S4D_OK) return st;
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
-  return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, km, vm, stm)
-                     : launch_attention_forward_d128(a.dtype, int(a.pos_dim), p, km, vm, stm);
+  return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, m, stm)
+                     : launch_attention_forward_d128(a.dtype, int(a.pos_dim), p, m, stm);
 }
 
 size_t s4d_attention_backward_workspace_bytes(const s4d_attention_args* args) {
@@ -285,6 +300,7 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   const int64_t rows = a.batch * a.queries;
   const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
   p.dslopes = sum ? p.delta + rows * a.heads : a.dslopes;
+  p.dslopes_by_head = sum;
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   if (a.queries > 0 || a.keys > 0) {
     AttnBackwardMaps m;
@@ -300,8 +316,9 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
     if (st != S4D_OK) return st;
   }
   if (!sum) return S4D_OK;
-  slope_sum_kernel<<<dim3(unsigned(a.heads)), 512, 0, stm>>>(p.dslopes, rows, p.heads, a.dslopes);
-  return cuda_check(cudaGetLastError(), "slope_sum_kernel launch");
+  return cuda_check(launch_pdl(true, slope_sum_kernel, dim3(unsigned(a.heads)), dim3(1024), 0, stm,
+                               static_cast<const float*>(p.dslopes), p.batch, p.nq, p.heads, a.dslopes),
+                    "slope_sum_kernel launch");
 }
 
 }  // extern "C"

@@ -41,14 +41,16 @@ struct AttnParams {
   int batch, heads, kv_heads, rep, dim;
   float scale, cap;
   // forward over parts of the keys
-  int splits;
+  int splits;   // parts
+  int cluster;  // CTAs that join their parts in shared memory: splits, or 1 (joined by a second launch)
   int64_t tiles_per_split;
   float* part_o;    // [splits, B, Nq, H, D]
   float* part_lse;  // [splits, B, H, Nq]
   // backward
   void *dq, *dk, *dv;
   float* delta;    // [B, H, Nq]
-  float* dslopes;  // [B, Nq, H] or null
+  float* dslopes;  // [B, Nq, H], by head [B, H, Nq], or null
+  int dslopes_by_head;
   int32_t* error_flag;
   unsigned long long wait_limit_ns;
 };
@@ -412,17 +414,10 @@ __device__ __forceinline__ SegRange seg_range(const int32_t* ids, int n) {
   return {lo, hi, all && lo == hi};
 }
 
-// Kind of every tile of `rows` ids in [first, first + tiles) of an axis with `valid` ids of which
-// `total` exist, for an own tile with range `own`; ids null: no segments.  All warps of the CTA.
+// Kind of every tile of `rows` ids in [first, first + tiles) of an axis with `valid` ids, for an own tile
+// with range `own` (own_whole: none of its rows is past the end).  All warps of the CTA.
 __device__ __forceinline__ void classify_tiles(unsigned char* kinds, int64_t first, int tiles, int rows, int64_t valid,
                                                const int32_t* ids, const SegRange& own, bool own_whole) {
-  if (ids == nullptr) {
-    for (int t = threadIdx.x; t < tiles; t += blockDim.x) {
-      const int64_t r0 = (first + t) * rows;
-      kinds[t] = r0 >= valid ? kTileSkip : (own_whole && r0 + rows <= valid ? kTileFull : kTileMasked);
-    }
-    return;
-  }
   for (int t = threadIdx.x >> 5; t < tiles; t += blockDim.x / 32) {
     const int64_t r0 = (first + t) * rows;
     const int n = int(valid - r0 < rows ? (valid > r0 ? valid - r0 : 0) : rows);
@@ -434,20 +429,54 @@ __device__ __forceinline__ void classify_tiles(unsigned char* kinds, int64_t fir
   }
 }
 
-// The next tile after t that is walked (tiles: none).
-__device__ __forceinline__ int next_tile(const unsigned char* kinds, int t, int tiles) {
-  do ++t;
-  while (t < tiles && kinds[t] == kTileSkip);
-  return t;
+// The tiles a CTA walks: by the table of kinds, or without segments all of them, the first `whole` of
+// them full and the others masked (the axis ends in the last one, or the own tile is not whole).
+struct TileWalk {
+  const unsigned char* kinds;
+  int tiles, whole;
+  __device__ __forceinline__ bool masked(int t) const { return kinds != nullptr ? kinds[t] == kTileMasked : t >= whole; }
+  __device__ __forceinline__ int next(int t) const {
+    ++t;
+    if (kinds != nullptr)
+      while (t < tiles && kinds[t] == kTileSkip) ++t;
+    return t;
+  }
+  __device__ __forceinline__ int first() const { return next(-1); }
+};
+
+// ---- clusters -----------------------------------------------------------------------------------------
+
+// All threads of all CTAs of the cluster, none of whose waits before it is without a limit.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Shared-memory address `addr` of this CTA in CTA `rank` of the cluster, and loads from there.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 peer_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 peer_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
 
+struct AttnForwardMaps {
+  CUtensorMap q, k, v;  // boxes of 128 rows of the heads of a shared head; of 64 keys
+};
 // One translation unit for each padded head dimension.
-int launch_attention_forward_d64(int dtype, int pos, const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                                 cudaStream_t st);
-int launch_attention_forward_d128(int dtype, int pos, const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                                  cudaStream_t st);
+int launch_attention_forward_d64(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
+int launch_attention_forward_d128(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
 
 // Maps of the backward kernels, named by the rows of their boxes.
 struct AttnBackwardMaps {

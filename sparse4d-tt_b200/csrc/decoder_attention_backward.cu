@@ -64,7 +64,7 @@ struct Terms {
 template <int POS, bool CAP, bool MASKED>
 __device__ __forceinline__ Terms score_terms(F2 acc, const ScoreConst& k, F2 nslope, F2 dist, F2 nlse2, F2 dp,
                                              F2 ndelta, bool seen0, bool seen1) {
-  F2 s, deriv;
+  F2 s, deriv = f2(1.0f);
   if constexpr (CAP) {
     const F2 rest = tanh_rest(acc, k.k1);
     s = fma2(f2(-k.c), rest, f2(k.c));
@@ -183,14 +183,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 5) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
-  {
-    const bool segs = p.q_seg != nullptr;
-    SegRange own{0, 0, true};
-    if (segs) {
-      const int64_t i0 = row0 / p.rep, i1 = (min(rows, row0 + kAttnRows) - 1) / p.rep;
-      own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
-    }
-    classify_tiles(kinds, 0, tiles, kCols, valid, segs ? p.k_seg + b * p.nk : nullptr, own, true);
+  TileWalk walk{nullptr, tiles, int(valid / kCols)};
+  if (p.q_seg != nullptr) {
+    const int64_t i0 = row0 / p.rep, i1 = (min(rows, row0 + kAttnRows) - 1) / p.rep;
+    const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
+    classify_tiles(kinds, 0, tiles, kCols, valid, p.k_seg + b * p.nk, own, true);
+    walk.kinds = kinds;
   }
   for (int c = threadIdx.x; c < 2 * kAttnRows * (DP / 8); c += kAttnThreads) {
     const bool is_do = c >= kAttnRows * (DP / 8);
@@ -210,12 +208,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_dp = tmem + kCols, tmem_o = tmem + 2 * kCols;
-  const int t0 = next_tile(kinds, -1, tiles);
+  const int t0 = walk.first();
 
   if (warp == 4) {
     if (lane == 0) {
       int n = 0;
-      for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages + 1) & 1;
         // V first: its stage is free once dP is there, K's only after dQ
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   } else if (warp == 5) {
     if (lane == 0) {
       int n = 0;
-      for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages) & 1;
         const uint32_t kt = sbase + S::kK + s * S::kTile, vt = sbase + S::kV + s * S::kTile;
@@ -249,7 +247,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         mma_commit(s_full);
         if (!mbar_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns)) break;
         tc_fence_after();
-        if (!(kinds[t] == kTileMasked && skip[n & 1])) mma_accumulate<T, DP, kCols>(tmem_o, tmem, kt, n > 0);
+        if (!(walk.masked(t) && skip[n & 1])) mma_accumulate<T, DP, kCols>(tmem_o, tmem, kt, n > 0);
         mma_commit(k_empty + 8 * s);
       }
       mma_commit(o_full);
@@ -314,8 +312,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     bool dead = false;
     int n = 0;
     for (int t = t0; t < tiles; ++n) {
-      const int next = next_tile(kinds, t, tiles);
-      const bool masked = kinds[t] == kTileMasked;
+      const int next = walk.next(t);
+      const bool masked = walk.masked(t);
       float* bx = aux + (n & 1) * 3 * kCols;
       if (tid < kCols) {
         bx[tid] = nx;
@@ -359,7 +357,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (POS > 0 && live && p.dslopes != nullptr) {
         // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits, so
         // dS is off by P times that sum, and sum dS dist by that times sum P dist.
-        p.dslopes[out_row] = -fmaf(-sums[0], sums[2], sums[1]);
+        p.dslopes[p.dslopes_by_head ? lse_row : out_row] = -fmaf(-sums[0], sums[2], sums[1]);
       }
 #pragma unroll
       for (int c = 0; c < DP / 32; ++c) {
@@ -464,18 +462,18 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 5) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
-  {
-    const bool segs = p.k_seg != nullptr;
-    const bool whole = key0 + kAttnRows <= valid;
-    SegRange own{0, 0, true};
-    if (segs) own = seg_range(p.k_seg + b * p.nk + key0, int(min(valid - key0, int64_t(kAttnRows))));
-    classify_tiles(kinds, 0, tiles, kCols, p.nq, segs ? p.q_seg + b * p.nq : nullptr, own, whole);
+  const bool own_whole = key0 + kAttnRows <= valid;
+  TileWalk walk{nullptr, tiles, own_whole ? int(p.nq / kCols) : 0};
+  if (p.k_seg != nullptr) {
+    const SegRange own = seg_range(p.k_seg + b * p.nk + key0, int(min(valid - key0, int64_t(kAttnRows))));
+    classify_tiles(kinds, 0, tiles, kCols, p.nq, p.q_seg + b * p.nq, own, own_whole);
+    walk.kinds = kinds;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_dp = tmem + kCols, tmem_dv = tmem + 2 * kCols, tmem_dk = tmem_dv + DP;
-  const int t0 = next_tile(kinds, -1, tiles);
+  const int t0 = walk.first();
   const bool work = t0 < tiles;
 
   if (warp == 4) {
@@ -488,7 +486,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
       int n = 0;
       bool ok = true;
       for (int hh = 0; hh < p.rep && ok; ++hh)
-        for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+        for (int t = t0; t < tiles; t = walk.next(t), ++n) {
           const int s = n % S::kStages;
           if (n >= S::kStages && !mbar_wait(empty + 8 * s, (n / S::kStages + 1) & 1, abort_flag, p.wait_limit_ns)) {
             ok = false;
@@ -510,7 +508,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
       int n = 0;
       bool ok = !work || mbar_wait(own_full, 0, abort_flag, p.wait_limit_ns);
       for (int hh = 0; hh < p.rep && ok; ++hh)
-        for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+        for (int t = t0; t < tiles; t = walk.next(t), ++n) {
           const int s = n % S::kStages;
           const uint32_t qt = sbase + S::kQ + s * 2 * S::kTile, dot = qt + S::kTile;
           if (!(ok = mbar_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns))) break;
@@ -520,7 +518,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
           mma_commit(s_full);
           if (!(ok = mbar_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns))) break;
           tc_fence_after();
-          if (!(kinds[t] == kTileMasked && skip[n & 1])) {
+          if (!(walk.masked(t) && skip[n & 1])) {
             mma_accumulate<T, DP, kCols>(tmem_dv, tmem, dot, n > 0);
             mma_accumulate<T, DP, kCols>(tmem_dk, tmem_dp, qt, n > 0);
           }
@@ -574,9 +572,9 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
     bool dead = false;
     if (work) fetch(0, t0);
     while (work && hh < p.rep) {
-      int next = next_tile(kinds, t, tiles), next_hh = hh;
+      int next = walk.next(t), next_hh = hh;
       if (next >= tiles) next = t0, ++next_hh;
-      const bool masked = kinds[t] == kTileMasked;
+      const bool masked = walk.masked(t);
       float* bx = aux + (n & 1) * 6 * kCols;
       if (tid < kCols) {
         bx[e] = c0;
@@ -675,13 +673,13 @@ int launch(const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st) {
   if (p.nq > 0) {
     const int64_t row_tiles = (p.nq * p.rep + kAttnRows - 1) / kAttnRows;
     attention_dq_kernel<DP, POS, CAP><<<dim3(unsigned(row_tiles * groups)), kAttnThreads,
-                                        Dq<DP>::smem((p.nk + kCols - 1) / kCols), st>>>(m.k64, m.v64, p);
+                                        Dq<DP>::smem(p.q_seg != nullptr ? (p.nk + kCols - 1) / kCols : 0), st>>>(m.k64, m.v64, p);
     rc = cuda_check(cudaGetLastError(), "attention_dq_kernel launch");
   }
   if (rc == S4D_OK && p.nk > 0 && p.dk != nullptr) {
     const int64_t key_tiles = (p.nk + kAttnRows - 1) / kAttnRows;
     attention_dkv_kernel<DP, POS, CAP><<<dim3(unsigned(key_tiles * groups)), kAttnThreads,
-                                         Dkv<DP>::smem((p.nq + kCols - 1) / kCols), st>>>(m.k128, m.v128, m.q64, m.do64, p);
+                                         Dkv<DP>::smem(p.q_seg != nullptr ? (p.nq + kCols - 1) / kCols : 0), st>>>(m.k128, m.v128, m.q64, m.do64, p);
     rc = cuda_check(cudaGetLastError(), "attention_dkv_kernel launch");
   }
   return rc;

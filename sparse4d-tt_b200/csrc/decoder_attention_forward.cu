@@ -22,8 +22,9 @@
 // warps, one for the even and one for the odd tiles, each with its own O, m and l, joined at the
 // end (at D = 128 tensor memory holds one O).
 //
-// Few rows and many keys: the keys are cut into parts, each CTA writes its part's normalised O and
-// log-sum-exp, and a second launch joins them.
+// Few rows and many keys: the keys are cut into parts, a CTA each.  Up to eight parts are one cluster:
+// every CTA leaves its O, m and l in shared memory and each joins a share of the rows from its peers'.
+// More parts write normalised O and log-sum-exp to memory and a second launch joins them.
 #include "decoder_attention.cuh"
 
 namespace s4d {
@@ -43,7 +44,7 @@ struct Fwd {
   // per row warp: negated x, y of the keys and their segments (after the last tile: m and l of its
   // rows); barriers; tensor-memory slot, abort, skip[2]
   static constexpr int kBars = kAux + kWarps * 3 * kKeys * 4;
-  static constexpr int kNumBars = 4 * kStages + 7;
+  static constexpr int kNumBars = 4 * kStages + 8;
   static constexpr int kCtl = kBars + kNumBars * 8;
   static constexpr int kKinds = kCtl + 16;
   static constexpr uint32_t kCols = 256;  // S / P: 2 x 64, O: DP
@@ -100,38 +101,33 @@ __device__ __forceinline__ void weights(const uint32_t (&r)[32], F2 nbase, F2 (&
 
 template <typename T, int DP, int POS, bool CAP>
 __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
-    attention_forward_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
-                             const AttnParams p) {
+    attention_forward_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                             const __grid_constant__ CUtensorMap vm, const AttnParams p) {
   using S = Fwd<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const uint32_t k_full = sbase + S::kBars, k_empty = k_full + 8 * S::kStages, v_full = k_empty + 8 * S::kStages,
                  v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, p_full = s_full + 16,
-                 pv_done = p_full + 16, o_full = pv_done + 16;
+                 pv_done = p_full + 16, o_full = pv_done + 16, q_full = o_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip_pv = abort_flag + 1;
   unsigned char* kinds = smem + S::kKinds;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // blockIdx.x = ((b G + g) row tiles + row tile) splits + part
-  const int64_t rows = p.nq * p.rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
-  int64_t u = blockIdx.x;
-  const int part = int(u % p.splits);
-  u /= p.splits;
-  const int64_t row0 = u % row_tiles * kAttnRows;
+  // blockIdx.x = ((b G + g) row tiles + row tile) splits + part; rank in the cluster: part % cluster
+  const uint32_t rep = uint32_t(p.rep);  // rows of a shared head stay below 2^31
+  const uint32_t rows = uint32_t(p.nq) * rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
+  uint32_t u = blockIdx.x;
+  const int part = int(u % uint32_t(p.splits));
+  u /= uint32_t(p.splits);
+  const int64_t row0 = int64_t(u % row_tiles) * kAttnRows;
   u /= row_tiles;
-  const int g = int(u % p.kv_heads), b = int(u / p.kv_heads);
+  const int g = int(u % uint32_t(p.kv_heads)), b = int(u / uint32_t(p.kv_heads));
+  const int64_t first = part * p.tiles_per_split;  // this part's first tile
 
-  // keys of this part
-  const int64_t first = part * p.tiles_per_split;
-  int64_t valid = p.nk;
-  if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
-  const int64_t all_tiles = (valid + kKeys - 1) / kKeys;
-  const int tiles = int(max(int64_t(0), min(p.tiles_per_split, all_tiles - first)));
-
-  if (threadIdx.x == 0) {
+  if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(k_full + 8 * s, 1);
       mbar_init(k_empty + 8 * s, 1);
@@ -144,41 +140,108 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       mbar_init(pv_done + 8 * s, 1);
     }
     mbar_init(o_full, 1);
+    mbar_init(q_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kCols);
-  {
-    const bool segs = p.q_seg != nullptr;
-    SegRange own{0, 0, true};
-    if (segs) {
-      const int64_t i0 = row0 / p.rep, i1 = (min(rows, row0 + kAttnRows) - 1) / p.rep;
-      own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
+  griddep_wait();
+  int64_t valid = p.nk;
+  if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
+  const int tiles = int(max(int64_t(0), min(p.tiles_per_split, (valid + kKeys - 1) / kKeys - first)));
+  TileWalk walk{nullptr, tiles, int(max(int64_t(0), min(int64_t(tiles), valid / kKeys - first)))};
+  const bool q_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
+  int loaded = 0;                                // tiles already asked for (the TMA thread)
+  if (warp == S::kWarps && lane == 0) {
+    if (q_by_tma) {
+      mbar_expect_tx(q_full, S::kQ);
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c)
+        tma_load_4d(sbase + c * S::kOwnBlock, &qm, q_full, c * 64, g * p.rep, int(uint32_t(row0) / rep), b);
     }
-    classify_tiles(kinds, first, tiles, kKeys, valid, segs ? p.k_seg + b * p.nk : nullptr, own, true);
+    // without segments every tile is walked: the first loads need not wait for the other warps
+    if (p.q_seg == nullptr)
+      for (; loaded < min(S::kStages, tiles); ++loaded) {
+        const int key = int((first + loaded) * kKeys);
+        load_tile<DP, kKeys>(sbase + S::kK + loaded * S::kTile, &km, k_full + 8 * loaded, g, key, b);
+        load_tile<DP, kKeys>(sbase + S::kV + loaded * S::kTile, &vm, v_full + 8 * loaded, g, key, b);
+      }
   }
-  const uint32_t rep = uint32_t(p.rep);  // rows of a shared head stay below 2^31
-  // Q: 16-byte pieces, zero past the last row and column, in the swizzled layout TMA gives K and V
-  for (int c = threadIdx.x; c < kAttnRows * (DP / 8); c += S::kThreads) {
-    const int r = c / (DP / 8), d = c % (DP / 8);
-    const int64_t row = row0 + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < rows && d * 8 < p.dim)
-      v = ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + int64_t(uint32_t(row) / rep) * p.q_sn + (g * p.rep + uint32_t(row) % rep) * p.q_sh +
-                    d * 8);
-    *reinterpret_cast<uint4*>(smem + (d / 8) * S::kOwnBlock + r * 128 + (((d & 7) ^ (r & 7)) << 4)) = v;
+  if (p.q_seg != nullptr) {
+    const int64_t i0 = row0 / rep, i1 = (min(int64_t(rows), row0 + kAttnRows) - 1) / rep;
+    const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
+    classify_tiles(kinds, first, tiles, kKeys, valid, p.k_seg + b * p.nk, own, true);
+    walk.kinds = kinds;
   }
-  fence_proxy_async();
+  // The row threads' own values and their first tile's keys
+  const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
+  const int64_t row = row0 + tid;
+  const bool live = row < rows;
+  const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
+  const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
+  const int64_t left = valid - first * kKeys;  // keys of this part and after it
+  const int64_t at0 = b * p.nk + first * kKeys;
+  float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
+  int seg = 0;  // own segment: -2 (matches nothing) or >= 0; without segments 0
+  // two keys of the next tile a lane, loaded one tile ahead
+  float2 nx = make_float2(0.0f, 0.0f), ny = nx;
+  int2 ns = make_int2(0, 0);
+  auto fetch = [&](int t) {
+    if (t >= tiles) return;
+    const int64_t j = int64_t(t) * kKeys + 2 * lane;
+    const bool in0 = j < left, in1 = j + 1 < left;
+    if (p.k_seg != nullptr) {
+      ns.x = in0 ? __ldg(p.k_seg + at0 + j) : -1;
+      ns.y = in1 ? __ldg(p.k_seg + at0 + j + 1) : -1;
+    }
+    if constexpr (POS > 0) {
+      const float* kp = p.k_pos + (at0 + j) * POS;
+      nx.x = in0 ? -__ldg(kp) : 0.0f;
+      nx.y = in1 ? -__ldg(kp + POS) : 0.0f;
+      if constexpr (POS > 1) {
+        ny.x = in0 ? -__ldg(kp + 1) : 0.0f;
+        ny.y = in1 ? -__ldg(kp + POS + 1) : 0.0f;
+      }
+    }
+  };
+  if (warp < S::kWarps) {
+    if constexpr (POS > 0) {
+      slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
+      qx = __ldg(p.q_pos + (b * p.nq + i) * POS);
+      if constexpr (POS > 1) qy = __ldg(p.q_pos + (b * p.nq + i) * POS + 1);
+    }
+    if (p.q_seg != nullptr) {
+      seg = __ldg(p.q_seg + b * p.nq + i);
+      if (seg < 0) seg = -2;
+    } else {
+      fetch(stream);  // without segments stream s begins with tile s
+    }
+  }
+  // Q where TMA cannot gather it: 16-byte pieces, zero past the last row and column, in the swizzled
+  // layout TMA gives K and V
+  if (!q_by_tma) {
+    for (int c = threadIdx.x; c < kAttnRows * (DP / 8); c += S::kThreads) {
+      const int r = c / (DP / 8), d = c % (DP / 8);
+      const uint32_t at = uint32_t(row0) + r;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (at < rows && d * 8 < p.dim)
+        v = ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + int64_t(at / rep) * p.q_sn +
+                      int64_t(g * rep + at % rep) * p.q_sh + d * 8);
+      *reinterpret_cast<uint4*>(smem + (d / 8) * S::kOwnBlock + r * 128 + (((d & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_proxy_async();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  griddep_launch_dependents();  // tensor memory is allocated: a kernel behind this one cannot take it away
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + 2 * kKeys;
-  const int t0 = next_tile(kinds, -1, tiles);
+  const int t0 = walk.first();
 
   if (warp == S::kWarps) {
     if (lane == 0) {
-      int n = 0;
-      for (int t = t0; t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+      int n = loaded;
+      for (int t = loaded > 0 ? loaded : t0; t < tiles; t = walk.next(t), ++n) {
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages + 1) & 1;
         const int key = int((first + t) * kKeys);
@@ -191,9 +254,10 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         }
         load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, key, b);
       }
-      for (int i = max(0, n - S::kStages); i < n; ++i) {
-        mbar_wait(k_full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
-        mbar_wait(v_full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
+      if (q_by_tma) mbar_wait(q_full, 0, nullptr);
+      for (int e = max(0, n - S::kStages); e < n; ++e) {
+        mbar_wait(k_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
+        mbar_wait(v_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
       }
     }
   } else if (warp == S::kWarps + 1) {
@@ -210,86 +274,54 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       };
       // the scores of two tiles are out before the first P is waited for, and tile n + 2's follow the
       // product of P of tile n, whose buffer they go over: the tensor cores work in order
-      const int t1 = next_tile(kinds, t0, tiles);
-      bool ok = t0 >= tiles || (issue_scores(0) && (t1 >= tiles || issue_scores(1)));
-      int n = 0, ahead = t1 < tiles ? next_tile(kinds, t1, tiles) : tiles;
-      for (int t = t0; ok && t < tiles; t = next_tile(kinds, t, tiles), ++n) {
+      const int t1 = walk.next(t0);
+      bool ok = t0 >= tiles || ((!q_by_tma || mbar_wait(q_full, 0, abort_flag, p.wait_limit_ns)) && issue_scores(0) && (t1 >= tiles || issue_scores(1)));
+      int n = 0, ahead = t1 < tiles ? walk.next(t1) : tiles;
+      for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
         const int s = n % S::kStages;
         ok = mbar_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns) &&
              mbar_wait(p_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
         if (!ok) break;
         tc_fence_after();
-        if (!(kinds[t] == kTileMasked && skip_pv[n & 1]))
+        if (!(walk.masked(t) && skip_pv[n & 1]))
           mma_accumulate<T, DP, kKeys>(tmem_o + n % S::kStreams * DP, tmem + (n & 1) * kKeys,
                                        sbase + S::kV + s * S::kTile, n >= S::kStreams);
         mma_commit(v_empty + 8 * s);
         mma_commit(pv_done + 8 * (n % S::kStreams));
         if (ahead < tiles) {
           ok = issue_scores(n + 2);
-          ahead = next_tile(kinds, ahead, tiles);
+          ahead = walk.next(ahead);
         }
       }
       mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
       mbar_wait(o_full, 0, nullptr);
     }
   } else {
-    const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
-    const int64_t row = row0 + tid;
-    const bool live = row < rows;
-    const int64_t i = live ? uint32_t(row) / rep : 0;
-    const int h = g * p.rep + (live ? int(uint32_t(row) % rep) : 0);
     const bool warp_live = row0 + warp % 4 * 32 < rows;
     const ScoreConst k(p);
-    float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
-    if constexpr (POS > 0) {
-      slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
-      qx = __ldg(p.q_pos + (b * p.nq + i) * POS);
-      if constexpr (POS > 1) qy = __ldg(p.q_pos + (b * p.nq + i) * POS + 1);
-    }
-    // segments: own -2 (matches nothing) or >= 0; keys -1 when masked; without segments 0 and 0 / -1
-    int seg = 0;
-    if (p.q_seg != nullptr) {
-      seg = __ldg(p.q_seg + b * p.nq + i);
-      if (seg < 0) seg = -2;
-    }
     float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 3 * kKeys;  // [3][64]: -x, -y, segment
-    // two keys of the next tile a lane, loaded one tile ahead
-    float2 nx = make_float2(0.0f, 0.0f), ny = nx;
-    int2 ns = make_int2(-1, -1);
-    auto fetch = [&](int t) {
-      if (t >= tiles) return;
-      const int64_t j = (first + t) * kKeys + 2 * lane;
-      const int64_t at = b * p.nk + j;
-      const bool in0 = j < valid, in1 = j + 1 < valid;
-      ns.x = in0 ? (p.k_seg != nullptr ? max(-1, __ldg(p.k_seg + at)) : 0) : -1;
-      ns.y = in1 ? (p.k_seg != nullptr ? max(-1, __ldg(p.k_seg + at + 1)) : 0) : -1;
-      if constexpr (POS > 0) {
-        nx.x = in0 ? -__ldg(p.k_pos + at * POS) : 0.0f;
-        nx.y = in1 ? -__ldg(p.k_pos + (at + 1) * POS) : 0.0f;
-        if constexpr (POS > 1) {
-          ny.x = in0 ? -__ldg(p.k_pos + at * POS + 1) : 0.0f;
-          ny.y = in1 ? -__ldg(p.k_pos + (at + 1) * POS + 1) : 0.0f;
-        }
-      }
-    };
     auto nth = [&](int t, int steps) {  // `steps` walked tiles on
-      for (int e = 0; e < steps && t < tiles; ++e) t = next_tile(kinds, t, tiles);
+      for (int e = 0; e < steps && t < tiles; ++e) t = walk.next(t);
       return t;
     };
     int t = nth(t0, stream);
-    fetch(t);
+    if (walk.kinds != nullptr) fetch(t);
     float m = -INFINITY, l = 0.0f;
     bool dead = false;
     int n = stream;
     for (; t < tiles; n += S::kStreams) {
       const int next = nth(t, S::kStreams);
-      const bool masked = kinds[t] == kTileMasked, first_tile = n == stream;
+      const bool masked = walk.masked(t), first_tile = n == stream;
       if (POS > 0 || masked) {
         __syncwarp();
         if constexpr (POS > 0) *reinterpret_cast<float2*>(aux + 2 * lane) = nx;
         if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kKeys + 2 * lane) = ny;
-        *reinterpret_cast<int2*>(aux + 2 * kKeys + 2 * lane) = ns;
+        if (masked) {  // -1: a key that no row sees (rows have ids >= 0, or -2)
+          const int64_t j = int64_t(t) * kKeys + 2 * lane;
+          *reinterpret_cast<int2*>(aux + 2 * kKeys + 2 * lane) =
+              make_int2(j < left ? max(-1, ns.x) : -1, j + 1 < left ? max(-1, ns.y) : -1);
+        }
         __syncwarp();
       }
       fetch(next);
@@ -371,35 +403,40 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       mbar_arrive(p_full + 8 * (n & 1));
       t = next;
     }
-    // O / l, the log-sum-exp, and zeros for rows without a key.  Two streams: each takes half of the
-    // columns and adds what both have there.
+    // With two streams each takes half of the columns and adds what both have there.
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
-    float m1 = -INFINITY, l1 = 0.0f;  // the other stream's
+    float2* ml = reinterpret_cast<float2*>(smem + S::kAux);  // [128] m, l; the keys' values go with them
+    float m1 = -INFINITY, l1 = 0.0f;                         // the other stream's
     if constexpr (S::kStreams == 2) {
-      float* ml = reinterpret_cast<float*>(smem + S::kAux);  // the keys' values are not needed any more ...
-      barrier_sync(3, S::kWarps * 32);                       // ... by any warp
-      ml[stream * 256 + tid] = m;
-      ml[stream * 256 + 128 + tid] = l;
+      // o_full: every row thread has handed in its last P, so none reads its keys' values any more
+      ml[stream * 128 + tid] = make_float2(m, l);
       barrier_sync(3, S::kWarps * 32);
-      m1 = ml[(stream ^ 1) * 256 + tid];
-      l1 = ml[(stream ^ 1) * 256 + 128 + tid];
+      m1 = ml[(stream ^ 1) * 128 + tid].x, l1 = ml[(stream ^ 1) * 128 + tid].y;
     }
-    if (!dead && warp_live) {
-      const bool any0 = l != 0.0f, any1 = l1 != 0.0f;  // else tensor memory holds nothing of this row
-      const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
-      float f0 = S::kStreams == 2 ? ex2(m - base) : 1.0f, f1 = ex2(m1 - base);
-      const float total = S::kStreams == 2 ? fmaf(l, f0, l1 * f1) : l;
-      const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
+    float f0 = S::kStreams == 2 ? ex2(m - base) : 1.0f, f1 = S::kStreams == 2 ? ex2(m1 - base) : 0.0f;
+    // a CTA that gave up makes its rows NaN
+    const float total = dead ? __int_as_float(0x7fc00000) : S::kStreams == 2 ? fmaf(l, f0, l1 * f1) : l;
+    const bool any0 = l != 0.0f, any1 = l1 != 0.0f;  // else tensor memory holds nothing of this row
+    const int64_t out_row = (b * p.nq + i) * p.heads + h;
+    if (p.cluster > 1) {
+      // O (not yet divided by l) and m, l stay in shared memory for the cluster: O over the K and V tiles,
+      // which nothing reads any more, 16-byte piece j of row r at j ^ (r & 7)
+      if constexpr (S::kStreams == 2) barrier_sync(3, S::kWarps * 32);
+      if (stream == 0) ml[tid] = make_float2(top, total);
+    } else {
+      const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // no key: zeros
       f0 *= inv, f1 *= inv;
-      const int64_t out_row = (b * p.nq + i) * p.heads + h, lse_row = (int64_t(b) * p.heads + h) * p.nq + i;
-      const int64_t all_rows = int64_t(p.batch) * p.nq * p.heads;
-      const float lse = total != 0.0f ? (top + log2f(total)) * kLn2 : -INFINITY;
       if (live && stream == 0) {
+        const int64_t lse_row = (int64_t(b) * p.heads + h) * p.nq + i;
+        const float lse = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
         if (p.splits > 1)
-          p.part_lse[part * all_rows + lse_row] = lse;
+          p.part_lse[part * (int64_t(p.batch) * p.nq * p.heads) + lse_row] = lse;
         else if (p.lse != nullptr)
           p.lse[lse_row] = lse;
       }
+    }
+    if (!dead && warp_live) {
 #pragma unroll
       for (int c0 = 0; c0 < DP / 32 / S::kStreams; ++c0) {
         const int c = c0 + stream * (DP / 32 / S::kStreams);
@@ -416,14 +453,18 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
 #pragma unroll
           for (int e = 0; e < 32; ++e) f[e] = any1 ? fmaf(__uint_as_float(o[e]), f1, f[e]) : f[e];
         }
-        if (!live) continue;
-        if (p.splits > 1) {
-          float* dst = p.part_o + (part * all_rows + out_row) * p.dim + c * 32;
+        if (p.cluster > 1) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(smem + S::kK + tid * (DP * 4) + (((c * 8 + e) ^ (tid & 7)) << 4)) =
+                make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        } else if (live && p.splits > 1) {
+          float* dst = p.part_o + (part * (int64_t(p.batch) * p.nq * p.heads) + out_row) * p.dim + c * 32;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (c * 32 + e * 4 < p.dim)
               *reinterpret_cast<float4*>(dst + e * 4) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-        } else {
+        } else if (live) {
           T* dst = static_cast<T*>(p.out) + out_row * p.dim + c * 32;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -436,12 +477,66 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (p.cluster > 1)
+    cluster_sync();
+  else
+    __syncthreads();
   if (warp == S::kWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kCols);
   }
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  if (p.cluster == 1) return;
+
+  // The cluster's rows: DP / 8 lanes a row, 8 columns a lane; this CTA takes rows part, part + cluster, ...
+  constexpr int kLanes = DP / 8, kRowsPerWarp = 32 / kLanes;
+  const int col = lane % kLanes * 8;
+  for (int r = part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && row0 + r < rows;
+       r += p.cluster * kRowsPerWarp * (S::kThreads / 32)) {
+    const uint32_t at = uint32_t(row0) + r, qi = rep == 1 ? at : at / rep, hh = g * rep + (at - qi * rep);
+    const int64_t out_row = (b * p.nq + qi) * p.heads + hh, lse_row = (int64_t(b) * p.heads + hh) * p.nq + qi;
+    const uint32_t at_ml = sbase + S::kAux + r * 8, at_o = sbase + S::kK + r * (DP * 4);
+    const uint32_t piece0 = at_o + (((col / 4) ^ (r & 7)) << 4), piece1 = at_o + (((col / 4 + 1) ^ (r & 7)) << 4);
+    // four peers at a time, all their loads before the first use
+    float top = -INFINITY, total = 0.0f;
+    float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
+    for (int s0 = 0; s0 < p.cluster; s0 += 4) {
+      float2 v[4];
+      float4 x[4], y[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t peer = min(s0 + s, p.cluster - 1);
+        v[s] = peer_f2(peer_addr(at_ml, peer));
+        x[s] = peer_f4(peer_addr(piece0, peer));
+        y[s] = peer_f4(peer_addr(piece1, peer));
+      }
+      float high = top;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s0 + s < p.cluster) high = fmaxf(high, v[s].x);
+      const float base = high == -INFINITY ? 0.0f : high, old = ex2(top - base);
+      top = high;
+      total *= old;
+      o0.x *= old, o0.y *= old, o0.z *= old, o0.w *= old, o1.x *= old, o1.y *= old, o1.z *= old, o1.w *= old;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (s0 + s >= p.cluster) continue;
+        const float w = ex2(v[s].x - base);  // 0 for a part without keys
+        total = fmaf(v[s].y, w, total);
+        o0.x = fmaf(w, x[s].x, o0.x), o0.y = fmaf(w, x[s].y, o0.y), o0.z = fmaf(w, x[s].z, o0.z),
+        o0.w = fmaf(w, x[s].w, o0.w);
+        o1.x = fmaf(w, y[s].x, o1.x), o1.y = fmaf(w, y[s].y, o1.y), o1.z = fmaf(w, y[s].z, o1.z),
+        o1.w = fmaf(w, y[s].w, o1.w);
+      }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // no key: zeros
+    if (col == 0 && p.lse != nullptr) p.lse[lse_row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+    if (col < p.dim)
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * p.dim + col) =
+          make_uint4(pack2<T>(o0.x * inv, o0.y * inv), pack2<T>(o0.z * inv, o0.w * inv),
+                     pack2<T>(o1.x * inv, o1.y * inv), pack2<T>(o1.z * inv, o1.w * inv));
+  }
+  cluster_sync();  // the peers still read this CTA's shared memory
 }
 
 // Joins the parts of one row: o = sum_s 2^(lse_s - lse) o_s.  One warp a row, lanes along D.
@@ -479,24 +574,42 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
 }
 
 template <typename T, int DP, int POS, bool CAP>
-int launch(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+int launch(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
   static bool smem_set[64] = {};
   const int rc = set_kernel_smem(attention_forward_kernel<T, DP, POS, CAP>, Fwd<DP>::smem(kAttnMaxTiles),
                                  "cudaFuncSetAttribute(attention_forward_kernel)", smem_set);
   if (rc != S4D_OK) return rc;
   const int64_t row_tiles = (p.nq * p.rep + kAttnRows - 1) / kAttnRows;
-  const dim3 grid(unsigned(row_tiles * p.kv_heads * p.batch * p.splits));
-  attention_forward_kernel<T, DP, POS, CAP><<<grid, Fwd<DP>::kThreads, Fwd<DP>::smem(p.tiles_per_split), st>>>(km, vm, p);
-  return cuda_check(cudaGetLastError(), "attention_forward_kernel launch");
+  const int64_t ctas = row_tiles * p.kv_heads * p.batch * p.splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(Fwd<DP>::kThreads);
+  cfg.dynamicSmemBytes = Fwd<DP>::smem(p.q_seg != nullptr ? p.tiles_per_split : 0);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  // one wave of CTAs: their start overlaps the end of the kernel ahead
+  if (ctas <= 2 * device_sms()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = unsigned(p.cluster);
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  return cuda_check(cudaLaunchKernelEx(&cfg, attention_forward_kernel<T, DP, POS, CAP>, m.q, m.k, m.v, p),
+                    "attention_forward_kernel launch");
 }
 
 template <typename T, int DP>
-int by_scores(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st, int pos) {
+int by_scores(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st, int pos) {
   const bool cap = p.cap > 0.0f;
   switch (pos) {
-    case 0: return cap ? launch<T, DP, 0, true>(p, km, vm, st) : launch<T, DP, 0, false>(p, km, vm, st);
-    case 1: return cap ? launch<T, DP, 1, true>(p, km, vm, st) : launch<T, DP, 1, false>(p, km, vm, st);
-    default: return cap ? launch<T, DP, 2, true>(p, km, vm, st) : launch<T, DP, 2, false>(p, km, vm, st);
+    case 0: return cap ? launch<T, DP, 0, true>(p, m, st) : launch<T, DP, 0, false>(p, m, st);
+    case 1: return cap ? launch<T, DP, 1, true>(p, m, st) : launch<T, DP, 1, false>(p, m, st);
+    default: return cap ? launch<T, DP, 2, true>(p, m, st) : launch<T, DP, 2, false>(p, m, st);
   }
 }
 
@@ -505,11 +618,11 @@ int by_scores(const AttnParams& p, const CUtensorMap& km, const CUtensorMap& vm,
 // This source is compiled once for each padded head dimension.
 #define S4D_CAT2(a, b) a##b
 #define S4D_CAT(a, b) S4D_CAT2(a, b)
-int S4D_CAT(launch_attention_forward_d, S4D_HEAD_DIM)(int dtype, int pos, const AttnParams& p, const CUtensorMap& km,
-                                                     const CUtensorMap& vm, cudaStream_t st) {
-  int rc = dtype == S4D_DTYPE_BF16 ? by_scores<__nv_bfloat16, S4D_HEAD_DIM>(p, km, vm, st, pos)
-                                   : by_scores<__half, S4D_HEAD_DIM>(p, km, vm, st, pos);
-  if (rc != S4D_OK || p.splits == 1) return rc;
+int S4D_CAT(launch_attention_forward_d, S4D_HEAD_DIM)(int dtype, int pos, const AttnParams& p,
+                                                     const AttnForwardMaps& m, cudaStream_t st) {
+  int rc = dtype == S4D_DTYPE_BF16 ? by_scores<__nv_bfloat16, S4D_HEAD_DIM>(p, m, st, pos)
+                                   : by_scores<__half, S4D_HEAD_DIM>(p, m, st, pos);
+  if (rc != S4D_OK || p.splits == p.cluster) return rc;
   const int64_t rows = int64_t(p.batch) * p.nq * p.heads;
   const dim3 grid(unsigned((rows + 7) / 8));
   const cudaError_t e = dtype == S4D_DTYPE_BF16

@@ -63,16 +63,23 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
   return v;
 }
 
+// VEC parameters from column col, as 16-byte vectors where the rows are (the pointer is checked with them).
 template <typename T, int VEC>
 __device__ __forceinline__ void load_param(const void* p, bool f32, int col, float (&f)[VEC]) {
   if (f32) {
     const float* q = static_cast<const float*>(p) + col;
+    if constexpr (VEC % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = __ldg(q + i);
+      for (int i = 0; i < VEC; i += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(q + i));
+        f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = __ldg(q + i);
+    }
   } else {
-    const T* q = static_cast<const T*>(p) + col;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = to_f32<T>(q[i]);
+    load_vec<T, VEC>(static_cast<const T*>(p) + col, f);
   }
 }
 
@@ -340,7 +347,7 @@ template <typename T>
 int dispatch_vector(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = p.width % VEC == 0 && vector_rows(p.x, p.x_ld, sizeof(T)) && vector_rows(p.y, p.y_ld, sizeof(T)) &&
-                   vector_rows(p.dy, p.dy_ld, sizeof(T));
+                   vector_rows(p.dy, p.dy_ld, sizeof(T)) && vector_rows(p.weight, 0, 4) && vector_rows(p.bias, 0, 4);
   return vec ? dispatch_width<T, VEC>(backward, p, blocks, st) : dispatch_width<T, 1>(backward, p, blocks, st);
 }
 
