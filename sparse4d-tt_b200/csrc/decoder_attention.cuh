@@ -242,6 +242,17 @@ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn) {
   return (1u << 4) | (t << 7) | (t << 10) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
 
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -314,10 +325,26 @@ __device__ __forceinline__ bool barrier_any(int id, int threads, bool v) {
   return r != 0;
 }
 
+// mbar_wait (tc_ptx.cuh) with sleeping tests.
+__device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                           unsigned long long limit_ns) {
+  constexpr uint32_t kNap = 20000;  // ns
+  if (mbar_test_sleep(bar, parity, kNap)) return true;
+  const unsigned long long t0 = now_ns();
+  for (;;) {
+    if (mbar_test_sleep(bar, parity, kNap)) return true;
+    if (*abort_flag) return false;
+    if (now_ns() - t0 > limit_ns) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // Warp-uniform bounded wait (the tensor-memory loads behind it are warp-collective).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           unsigned long long limit_ns) {
-  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit_ns));
+  const bool ok = __all_sync(0xffffffffu, sleep_wait(bar, parity, abort_flag, limit_ns));
   tc_fence_after();
   return ok;
 }

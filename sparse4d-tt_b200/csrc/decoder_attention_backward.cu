@@ -217,9 +217,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages + 1) & 1;
         // V first: its stage is free once dP is there, K's only after dQ
-        if (n >= S::kStages && !mbar_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
+        if (n >= S::kStages && !sleep_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
         load_tile<DP, kCols>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, t * kCols, b);
-        if (n >= S::kStages && !mbar_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
+        if (n >= S::kStages && !sleep_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
           mbar_wait(v_full + 8 * s, (n / S::kStages) & 1, nullptr);
           break;
         }
@@ -237,15 +237,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages) & 1;
         const uint32_t kt = sbase + S::kK + s * S::kTile, vt = sbase + S::kV + s * S::kTile;
-        if (!mbar_wait(v_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
+        if (!sleep_wait(v_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
         tc_fence_after();
         mma_scores<T, DP>(tmem_dp, sbase + S::kDo, S::kOwnBlock, vt, S::kBlock, kCols);
         mma_commit(v_empty + 8 * s);
-        if (!mbar_wait(k_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
+        if (!sleep_wait(k_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
         tc_fence_after();
         mma_scores<T, DP>(tmem, sbase, S::kOwnBlock, kt, S::kBlock, kCols);
         mma_commit(s_full);
-        if (!mbar_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns)) break;
+        if (!sleep_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns)) break;
         tc_fence_after();
         if (!(walk.masked(t) && skip[n & 1])) mma_accumulate<T, DP, kCols>(tmem_o, tmem, kt, n > 0);
         mma_commit(k_empty + 8 * s);
@@ -327,9 +327,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (masked) {
         if (!dead) dead = !warp_wait(k_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
         bad = barrier_any(2, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
-        if (tid == 0) skip[n & 1] = bad;
       }
       if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
+      // only now: this tile's scores follow the products that read the flag's last value
+      if (masked && tid == 0) skip[n & 1] = bad;
       if (!dead && warp_live) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
       for (int hh = 0; hh < p.rep && ok; ++hh)
         for (int t = t0; t < tiles; t = walk.next(t), ++n) {
           const int s = n % S::kStages;
-          if (n >= S::kStages && !mbar_wait(empty + 8 * s, (n / S::kStages + 1) & 1, abort_flag, p.wait_limit_ns)) {
+          if (n >= S::kStages && !sleep_wait(empty + 8 * s, (n / S::kStages + 1) & 1, abort_flag, p.wait_limit_ns)) {
             ok = false;
             break;
           }
@@ -506,17 +507,17 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
   } else if (warp == 5) {
     if (lane == 0) {
       int n = 0;
-      bool ok = !work || mbar_wait(own_full, 0, abort_flag, p.wait_limit_ns);
+      bool ok = !work || sleep_wait(own_full, 0, abort_flag, p.wait_limit_ns);
       for (int hh = 0; hh < p.rep && ok; ++hh)
         for (int t = t0; t < tiles; t = walk.next(t), ++n) {
           const int s = n % S::kStages;
           const uint32_t qt = sbase + S::kQ + s * 2 * S::kTile, dot = qt + S::kTile;
-          if (!(ok = mbar_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns))) break;
+          if (!(ok = sleep_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns))) break;
           tc_fence_after();
           mma_scores<T, DP>(tmem, sbase, S::kOwnBlock, qt, S::kBlock, kCols);
           mma_scores<T, DP>(tmem_dp, sbase + S::kV, S::kOwnBlock, dot, S::kBlock, kCols);
           mma_commit(s_full);
-          if (!(ok = mbar_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns))) break;
+          if (!(ok = sleep_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns))) break;
           tc_fence_after();
           if (!(walk.masked(t) && skip[n & 1])) {
             mma_accumulate<T, DP, kCols>(tmem_dv, tmem, dot, n > 0);
@@ -593,9 +594,10 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
       if (masked) {
         if (!dead) dead = !warp_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
         bad = barrier_any(2, kAttnRows, !dead && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, e));
-        if (tid == 0) skip[n & 1] = bad;
       }
       if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
+      // only now: this tile's scores follow the products that read the flag's last value
+      if (masked && tid == 0) skip[n & 1] = bad;
       if (!dead) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {

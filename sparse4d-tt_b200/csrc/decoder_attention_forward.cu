@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip_pv = abort_flag + 1;
   unsigned char* kinds = smem + S::kKinds;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // blockIdx.x = ((b G + g) row tiles + row tile) splits + part; rank in the cluster: part % cluster
   const uint32_t rep = uint32_t(p.rep);  // rows of a shared head stay below 2^31
@@ -245,9 +245,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         const int s = n % S::kStages;
         const uint32_t parity = (n / S::kStages + 1) & 1;
         const int key = int((first + t) * kKeys);
-        if (n >= S::kStages && !mbar_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
+        if (n >= S::kStages && !sleep_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
         load_tile<DP, kKeys>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, key, b);
-        if (n >= S::kStages && !mbar_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
+        if (n >= S::kStages && !sleep_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
           // the K load is out: it may not land in the memory of a CTA that is gone
           mbar_wait(k_full + 8 * s, (n / S::kStages) & 1, nullptr);
           break;
@@ -261,41 +261,50 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       }
     }
   } else if (warp == S::kWarps + 1) {
-    if (lane == 0) {
-      // S of tile n, n counting the walked tiles
-      auto issue_scores = [&](int n) {
-        const int s = n % S::kStages;
-        if (!mbar_wait(k_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns)) return false;
-        tc_fence_after();
+    // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one
+    // lane issues.
+    const uint32_t leader = elect_one();
+    // S of tile n, n counting the walked tiles
+    auto issue_scores = [&](int n) {
+      const int s = n % S::kStages;
+      if (!warp_wait(k_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns)) return false;
+      if (leader) {
         mma_scores<T, DP>(tmem + (n & 1) * kKeys, sbase, S::kOwnBlock, sbase + S::kK + s * S::kTile, S::kBlock, kKeys);
         mma_commit(k_empty + 8 * s);
         mma_commit(s_full + 8 * (n & 1));
-        return true;
-      };
-      // the scores of two tiles are out before the first P is waited for, and tile n + 2's follow the
-      // product of P of tile n, whose buffer they go over: the tensor cores work in order
-      const int t1 = walk.next(t0);
-      bool ok = t0 >= tiles || ((!q_by_tma || mbar_wait(q_full, 0, abort_flag, p.wait_limit_ns)) && issue_scores(0) && (t1 >= tiles || issue_scores(1)));
-      int n = 0, ahead = t1 < tiles ? walk.next(t1) : tiles;
-      for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
-        const int s = n % S::kStages;
-        ok = mbar_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns) &&
-             mbar_wait(p_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
-        if (!ok) break;
-        tc_fence_after();
+      }
+      __syncwarp();
+      return true;
+    };
+    // the scores of two tiles are out before the first P is waited for, and tile n + 2's follow the
+    // product of P of tile n, whose buffer they go over: the tensor cores work in order
+    const int t1 = walk.next(t0);
+    bool ok = t0 >= tiles || ((!q_by_tma || warp_wait(q_full, 0, abort_flag, p.wait_limit_ns)) && issue_scores(0) &&
+                              (t1 >= tiles || issue_scores(1)));
+    int n = 0, ahead = t1 < tiles ? walk.next(t1) : tiles;
+    for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
+      const int s = n % S::kStages;
+      ok = warp_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns) &&
+           warp_wait(p_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
+      if (!ok) break;
+      if (leader) {
         if (!(walk.masked(t) && skip_pv[n & 1]))
           mma_accumulate<T, DP, kKeys>(tmem_o + n % S::kStreams * DP, tmem + (n & 1) * kKeys,
                                        sbase + S::kV + s * S::kTile, n >= S::kStreams);
         mma_commit(v_empty + 8 * s);
         mma_commit(pv_done + 8 * (n % S::kStreams));
-        if (ahead < tiles) {
-          ok = issue_scores(n + 2);
-          ahead = walk.next(ahead);
-        }
       }
+      __syncwarp();
+      if (ahead < tiles) {
+        ok = issue_scores(n + 2);
+        ahead = walk.next(ahead);
+      }
+    }
+    if (leader) {
       mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
       mbar_wait(o_full, 0, nullptr);
     }
+    __syncwarp();
   } else {
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool warp_live = row0 + warp % 4 * 32 < rows;
@@ -331,9 +340,10 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       if (masked) {
         if (!dead) dead = !warp_wait(v_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
         bad = barrier_any(1 + stream, kAttnRows, !dead && tid < kKeys && row_not_finite<T, DP>(vt, S::kBlock, tid));
-        if (tid == 0) skip_pv[n & 1] = bad;
       }
       if (!dead) dead = !warp_wait(s_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
+      // only now: this tile's scores follow the product that read the flag's last value
+      if (masked && tid == 0) skip_pv[n & 1] = bad;
       if (!dead && warp_live) {
         // With two streams a thread has 96 registers: the first half of the scores waits in tensor memory.
         uint32_t r0[32], r1[32];

@@ -42,6 +42,20 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+// The same, but the thread may sleep up to `hint_ns` for the phase: a thread that polls takes issue
+// slots from the warps it waits for.
+__device__ __forceinline__ bool mbar_test_sleep(uint32_t bar, uint32_t parity, uint32_t hint_ns) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(hint_ns)
+      : "memory");
+  return done != 0;
+}
+
 // Waits until the phase with `parity` has completed.  Returns false without waiting further
 // once another role of the CTA has given up (abort_flag set), or after limit_ns, in which case it
 // sets abort_flag itself.  With abort_flag == nullptr only the time limit applies.
