@@ -44,7 +44,8 @@ S4D_API int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void*
  * dweight and dbias are sums over all rows, held in f32 and added in an order that depends on the
  * sizes alone, so that equal calls give equal bits.  rows = 0 writes zeros to them.
  * workspace: s4d_norm_backward_workspace_bytes(rows, width) bytes, 16-byte aligned, read and
- * written by this call only while it runs (may be NULL when neither dweight nor dbias is wanted). */
+ * written by this call only while it runs (may be NULL when that is 0 or neither dweight nor dbias is
+ * wanted). */
 S4D_API size_t s4d_norm_backward_workspace_bytes(int64_t rows, int64_t width);
 S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype,
                               const void* weight, int param_dtype, const float* mean, const float* rstd, void* dx,

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -24,26 +25,28 @@ _i64, _int, _p, _sz, _f = C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_float
 
 
 
-class AttentionArgs(C.Structure):
-    """``s4d_attention_args``.  ``keep`` (not part of the struct) holds the tensors it points to."""
-
-    _fields_ = [(n, _i64) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "pos_dim")] + [
-        ("q", _p), ("k", _p), ("v", _p), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3),
-        ("out", _p), ("lse", _p), ("slopes", _p), ("slope_stride", _i64 * 3), ("q_pos", _p), ("k_pos", _p),
-        ("q_segment", _p), ("k_segment", _p), ("k_len", _p), ("workspace", _p), ("workspace_bytes", _sz),
-        ("error_flag", _p), ("scale", _f), ("softcap", _f), ("dtype", C.c_int32),
-        ("dslopes_per_row", C.c_int32), ("dout", _p), ("dout_stride", _i64 * 3), ("dq", _p), ("dk", _p), ("dv", _p),
-        ("dslopes", _p)]
+# s4d_attention_args as one format of the struct module: packing all fields at once costs a few microseconds
+# less a call than setting them one by one.  Pointers are 0 for NULL.
+ATTENTION_ARGS = struct.Struct(
+    "@7q"   # batch, queries, keys, heads, kv_heads, dim, pos_dim
+    "3P"    # q, k, v
+    "9q"    # strides of q, k, v
+    "3P3q"  # out, lse, slopes and their strides
+    "5P"    # q_pos, k_pos, q_segment, k_segment, k_len
+    "PNP"   # workspace, workspace_bytes, error_flag
+    "2f2i"  # scale, softcap, dtype, dslopes_per_row
+    "P3q"   # dout and its strides
+    "4P")   # dq, dk, dv, dslopes
 
 
 # name -> (restype, argtypes); one entry per function of include/s4d_decoder.h
 SIGNATURES = {
     "s4d_decoder_abi_version": (_int, []),
     "s4d_decoder_last_error": (C.c_char_p, []),
-    "s4d_attention_forward_workspace_bytes": (_sz, [C.POINTER(AttentionArgs)]),
-    "s4d_attention_forward": (_int, [C.POINTER(AttentionArgs), _p]),
-    "s4d_attention_backward_workspace_bytes": (_sz, [C.POINTER(AttentionArgs)]),
-    "s4d_attention_backward": (_int, [C.POINTER(AttentionArgs), _p]),
+    "s4d_attention_forward_workspace_bytes": (_sz, [C.c_char_p]),
+    "s4d_attention_forward": (_int, [C.c_char_p, _p]),
+    "s4d_attention_backward_workspace_bytes": (_sz, [C.c_char_p]),
+    "s4d_attention_backward": (_int, [C.c_char_p, _p]),
     "s4d_norm_forward": (_int, [_p, _i64, _int, _p, _p, _int, _p, _i64, _p, _p, _i64, _i64, _f, _p]),
     "s4d_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "s4d_norm_backward": (_int, [_p, _i64, _p, _i64, _int, _p, _int, _p, _p, _p, _i64, _p, _p, _i64, _i64, _p, _sz,
@@ -53,6 +56,7 @@ SIGNATURES = {
 # Version of include/s4d_decoder.h these bindings are written for (s4d_decoder_abi_version()).
 ABI_VERSION = 1
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _lib = None
 _lock = threading.Lock()
 
@@ -88,13 +92,13 @@ def check(fn: str, status: int) -> None:
 
 
 class on_device:
-    """``with on_device(dev):`` makes ``dev`` the current device for the launches inside (they go to
-    its current stream); costs nothing when it already is."""
+    """``with on_device(index):`` makes CUDA device ``index`` the current one for the launches inside (they
+    go to its current stream); costs next to nothing when it already is."""
 
     __slots__ = ("guard",)
 
-    def __init__(self, dev: torch.device):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    def __init__(self, index: int):
+        self.guard = None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -104,3 +108,23 @@ class on_device:
         if self.guard is not None:
             self.guard.__exit__(*exc)
         return False
+
+
+def same_device(name: str, first: torch.Tensor, *others) -> int:
+    """The CUDA device index of ``first``, which every other tensor (None: left out) has to share."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: every tensor must be on a CUDA device (got {first.device}); no CPU path exists")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if t.get_device() < 0:
+                raise ValueError(f"{name}: every tensor must be on a CUDA device (got {t.device}); no CPU path exists")
+            raise ValueError(f"{name}: tensors on different devices (cuda:{index} and {t.device})")
+    return index
+
+
+def stream_ptr(index: int) -> int:
+    """torch's current-stream handle of a device index."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream

@@ -24,103 +24,127 @@ There is no CPU path: CPU tensors are rejected.
 """
 from __future__ import annotations
 
-import ctypes as C
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import _lib as L
 from . import _lib_decoder as D
-from .ops import _check_dtype, _ptr, _require, _require_cuda, _stream_ptr
 
 Tensor = torch.Tensor
 
-_TYPES = (torch.bfloat16, torch.float16)
+_ZERO3 = (0, 0, 0)
 
 
-def _operand(t: Tensor) -> Tensor:
-    """``t [B, N, heads, dim]`` with strides the kernels read in place (unit stride along dim, the others
-    positive multiples of 8, 16-byte aligned); a contiguous copy otherwise (an expanded tensor, for
-    one)."""
-    s = t.stride()
-    if s[3] == 1 and t.data_ptr() % 16 == 0:
-        for i in (0, 1, 2):
-            if t.shape[i] > 1 and (s[i] <= 0 or s[i] % 8):
-                break
-        else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _operand(t: Tensor) -> Tuple[Tensor, Tuple[int, ...]]:
+    """``t [B, N, heads, dim]`` and its strides, such that the kernels can read it in place (unit stride along
+    dim, the others positive multiples of 8, 16-byte aligned); a contiguous copy where ``t`` is not
+    (an expanded tensor, for one)."""
+    sb, sn, sh, sd = t.stride()
+    b, n, h, _ = t.shape
+    if (sd == 1 and t.data_ptr() % 16 == 0 and (b <= 1 or (sb > 0 and sb % 8 == 0))
+            and (n <= 1 or (sn > 0 and sn % 8 == 0)) and (h <= 1 or (sh > 0 and sh % 8 == 0))):
+        return t, (sb, sn, sh)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()[:3]
 
 
-def _fill(name: str, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float], softcap: float,
-          slopes: Optional[Tensor], q_pos: Optional[Tensor], k_pos: Optional[Tensor], q_segment: Optional[Tensor],
-          k_segment: Optional[Tensor], k_len: Optional[Tensor], error_flag: Optional[Tensor]):
-    """The checked arguments of a call: ``(device, AttentionArgs)``; the tensors they point to are kept
-    in the struct's ``keep``."""
-    dev = _require_cuda(name, q, k, v, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
-    for what, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype not in _TYPES or t.dtype != q.dtype:
-            raise TypeError(f"{name}: q, k and v must share one of {list(_TYPES)}, {what} is {t.dtype}")
-        if t.dim() != 4:
-            raise ValueError(f"{name}: {what} must be [batch, rows, heads, dim], got {list(t.shape)}")
+class _Args(NamedTuple):
+    """The checked arguments of a call, in the order of ``s4d_attention_args``."""
+
+    index: int        # CUDA device
+    sizes: tuple      # batch, queries, keys, heads, kv_heads, dim, pos_dim
+    operands: tuple   # q, k, v pointers and strides
+    slopes: tuple     # pointer, strides
+    optional: tuple   # q_pos, k_pos, q_segment, k_segment, k_len
+    error_flag: int
+    scalars: tuple    # scale, softcap, dtype
+    keep: tuple       # the tensors pointed to that are copies
+
+
+def _checked(name: str, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float], softcap: float,
+             slopes: Optional[Tensor], q_pos: Optional[Tensor], k_pos: Optional[Tensor], q_segment: Optional[Tensor],
+             k_segment: Optional[Tensor], k_len: Optional[Tensor], error_flag: Optional[Tensor]) -> _Args:
+    index = D.same_device(name, q, k, v, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
+    dtype = q.dtype
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{name}: q, k and v must share one of [torch.bfloat16, torch.float16], got {dtype}, {k.dtype} "
+                        f"and {v.dtype}")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{name}: q, k and v must be [batch, rows, heads, dim], got {list(q.shape)}, {list(k.shape)} "
+                         f"and {list(v.shape)}")
     B, nq, H, dim = q.shape
-    nk, G = int(k.shape[1]), int(k.shape[2])
-    if k.shape != (B, nk, G, dim) or v.shape != k.shape:
+    kb, nk, G, kd = k.shape
+    if kb != B or kd != dim or v.shape != k.shape:
         raise ValueError(f"{name}: k and v must be [{B}, keys, kv_heads, {dim}], got {list(k.shape)} and "
                          f"{list(v.shape)}")
     if G == 0 or H % G:
         raise ValueError(f"{name}: the {H} heads must be a multiple of the {G} kv_heads")
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"{name}: dim must be a multiple of 8 from 8 to 128, got {dim}")
-    a = D.AttentionArgs()
-    a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim = B, nq, nk, H, G, dim
-    a.dtype = D.DTYPES[q.dtype]
-    q, k, v = _operand(q), _operand(k), _operand(v)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    a.scale = dim ** -0.5 if scale is None else float(scale)
-    a.softcap = float(softcap)
-    keep = [q, k, v]
-    if (slopes is None) != (q_pos is None) or (q_pos is None) != (k_pos is None):
-        raise ValueError(f"{name}: slopes, q_pos and k_pos go together")
+    (q, qs), (k, ks), (v, vs) = _operand(q), _operand(k), _operand(v)
+    keep = (q, k, v)
+    pos, slope, qp, kp = 0, (0, 0, 0, 0), 0, 0
     if slopes is not None:
-        _check_dtype(name, slopes, (torch.float32,), "slopes")
-        _check_dtype(name, q_pos, (torch.float32,), "q_pos")
-        _check_dtype(name, k_pos, (torch.float32,), "k_pos")
-        pos = int(q_pos.shape[-1]) if q_pos.dim() == 3 else 0
-        _require(pos in (1, 2) and tuple(q_pos.shape) == (B, nq, pos) and tuple(k_pos.shape) == (B, nk, pos),
-                 lambda: f"{name}: q_pos and k_pos must be [{B}, {nq} / {nk}, 1 or 2], got {list(q_pos.shape)} and "
-                         f"{list(k_pos.shape)}")
-        if tuple(slopes.shape) == (H,):
-            a.slope_stride[:] = (0, 0, slopes.stride(0))
+        if q_pos is None or k_pos is None:
+            raise ValueError(f"{name}: slopes, q_pos and k_pos go together")
+        if slopes.dtype != torch.float32 or q_pos.dtype != torch.float32 or k_pos.dtype != torch.float32:
+            raise TypeError(f"{name}: slopes, q_pos and k_pos must be torch.float32")
+        pos = q_pos.shape[-1] if q_pos.dim() == 3 else 0
+        if pos not in (1, 2) or q_pos.shape != (B, nq, pos) or k_pos.shape != (B, nk, pos):
+            raise ValueError(f"{name}: q_pos and k_pos must be [{B}, {nq} / {nk}, 1 or 2], got {list(q_pos.shape)} and "
+                             f"{list(k_pos.shape)}")
+        if slopes.shape == (H,):
+            slope = (slopes.data_ptr(), 0, 0, slopes.stride(0))
+        elif slopes.shape == (B, nq, H):
+            slope = (slopes.data_ptr(), *slopes.stride())
         else:
-            _require(tuple(slopes.shape) == (B, nq, H),
-                     lambda: f"{name}: slopes must be [{H}] or [{B}, {nq}, {H}], got {list(slopes.shape)}")
-            a.slope_stride[:] = slopes.stride()
-        q_pos, k_pos = q_pos.contiguous(), k_pos.contiguous()
-        a.pos_dim, a.slopes, a.q_pos, a.k_pos = pos, slopes.data_ptr(), q_pos.data_ptr(), k_pos.data_ptr()
-        keep += [slopes, q_pos, k_pos]
-    if (q_segment is None) != (k_segment is None):
+            raise ValueError(f"{name}: slopes must be [{H}] or [{B}, {nq}, {H}], got {list(slopes.shape)}")
+        if not (q_pos.is_contiguous() and k_pos.is_contiguous()):
+            q_pos, k_pos = q_pos.contiguous(), k_pos.contiguous()
+            keep += (q_pos, k_pos)
+        qp, kp = q_pos.data_ptr(), k_pos.data_ptr()
+    elif q_pos is not None or k_pos is not None:
+        raise ValueError(f"{name}: slopes, q_pos and k_pos go together")
+    qseg = kseg = 0
+    if q_segment is not None and k_segment is not None:
+        if q_segment.dtype != torch.int32 or k_segment.dtype != torch.int32:
+            raise TypeError(f"{name}: q_segment and k_segment must be torch.int32")
+        if q_segment.shape != (B, nq) or k_segment.shape != (B, nk):
+            raise ValueError(f"{name}: q_segment and k_segment must be [{B}, {nq}] and [{B}, {nk}]")
+        if not (q_segment.is_contiguous() and k_segment.is_contiguous()):
+            q_segment, k_segment = q_segment.contiguous(), k_segment.contiguous()
+            keep += (q_segment, k_segment)
+        qseg, kseg = q_segment.data_ptr(), k_segment.data_ptr()
+    elif q_segment is not None or k_segment is not None:
         raise ValueError(f"{name}: q_segment and k_segment go together")
-    if q_segment is not None:
-        _check_dtype(name, q_segment, (torch.int32,), "q_segment")
-        _check_dtype(name, k_segment, (torch.int32,), "k_segment")
-        _require(tuple(q_segment.shape) == (B, nq) and tuple(k_segment.shape) == (B, nk),
-                 lambda: f"{name}: q_segment and k_segment must be [{B}, {nq}] and [{B}, {nk}]")
-        q_segment, k_segment = q_segment.contiguous(), k_segment.contiguous()
-        a.q_segment, a.k_segment = q_segment.data_ptr(), k_segment.data_ptr()
-        keep += [q_segment, k_segment]
+    klen = 0
     if k_len is not None:
-        _check_dtype(name, k_len, (torch.int32,), "k_len")
-        _require(tuple(k_len.shape) == (B,), lambda: f"{name}: k_len must be [{B}], got {list(k_len.shape)}")
-        k_len = k_len.contiguous()
-        a.k_len = k_len.data_ptr()
-        keep.append(k_len)
+        if k_len.dtype != torch.int32:
+            raise TypeError(f"{name}: k_len must be torch.int32")
+        if k_len.shape != (B,):
+            raise ValueError(f"{name}: k_len must be [{B}], got {list(k_len.shape)}")
+        if not k_len.is_contiguous():
+            k_len = k_len.contiguous()
+            keep += (k_len,)
+        klen = k_len.data_ptr()
+    flag = 0
     if error_flag is not None:
-        _check_dtype(name, error_flag, (torch.int32,), "error_flag")
-        a.error_flag = error_flag.data_ptr()
-    a.keep = keep
-    return dev, a
+        if error_flag.dtype != torch.int32:
+            raise TypeError(f"{name}: error_flag must be torch.int32")
+        flag = error_flag.data_ptr()
+    return _Args(index, (B, nq, nk, H, G, dim, pos), (q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs), slope,
+                 (qp, kp, qseg, kseg, klen), flag, (dim ** -0.5 if scale is None else scale, softcap, D.DTYPES[dtype]),
+                 keep)
+
+
+def _pack(a: _Args, out: int, lse: int, workspace: int = 0, workspace_bytes: int = 0, per_row: int = 0, dout: int = 0,
+          dout_stride=_ZERO3, dq: int = 0, dk: int = 0, dv: int = 0, dslopes: int = 0) -> bytes:
+    return D.ATTENTION_ARGS.pack(*a.sizes, *a.operands, out, lse, *a.slopes, *a.optional, workspace, workspace_bytes,
+                                 a.error_flag, *a.scalars, per_row, dout, *dout_stride, dq, dk, dv, dslopes)
+
+
+def _address(t: Optional[Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None, softcap: float = 0.0,
@@ -136,25 +160,30 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
     ``slopes [H]`` or ``[B, Nq, H]`` fp32 with ``q_pos [B, Nq, 1 or 2]`` and ``k_pos [B, Nk, 1 or 2]``
     fp32 give the distance bias; ``q_segment [B, Nq]`` and ``k_segment [B, Nk]`` int32 the document
     mask; ``k_len [B]`` int32 the valid keys of each batch entry (read on the device, clamped to
-    0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into."""
+    0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into.  ``error_flag`` (int32) gets
+    ``S4D_FLAG_WAIT_TIMEOUT`` should a kernel give up waiting; the results are then not valid."""
     name = "decoder_attention_forward"
-    dev, a = _fill(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
+    a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
     else:
-        _require_cuda(name, q, out)
-        _check_dtype(name, out, (q.dtype,), "out")
-        _require(out.shape == q.shape and out.is_contiguous() and out.data_ptr() % 16 == 0,
-                 lambda: f"{name}: out must be a contiguous, 16-byte aligned {list(q.shape)} tensor")
-    lse = torch.empty(a.batch, a.heads, a.queries, dtype=torch.float32, device=dev)
-    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+        D.same_device(name, q, out)
+        if out.dtype != q.dtype:
+            raise TypeError(f"{name}: out must be {q.dtype}, got {out.dtype}")
+        if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"{name}: out must be a contiguous, 16-byte aligned {list(q.shape)} tensor")
+    B, nq, _, H = a.sizes[:4]
+    lse = q.new_empty((B, H, nq), dtype=torch.float32)
     lib = D.lib()
-    with D.on_device(dev):
-        need = lib.s4d_attention_forward_workspace_bytes(C.byref(a))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        a.workspace, a.workspace_bytes = _ptr(ws), need
-        st = lib.s4d_attention_forward(C.byref(a), _stream_ptr(dev))
-    D.check(name, st)
+    args = _pack(a, out.data_ptr(), lse.data_ptr())
+    with D.on_device(a.index):
+        need = lib.s4d_attention_forward_workspace_bytes(args)
+        if need:
+            ws = q.new_empty(need // 4, dtype=torch.float32)
+            args = _pack(a, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need)
+        st = lib.s4d_attention_forward(args, D.stream_ptr(a.index))
+    if st:
+        D.check(name, st)
     return out, lse
 
 
@@ -170,35 +199,37 @@ def decoder_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, ou
     ``need_dkv`` / ``need_dslopes`` False leave those out (None).  Positions have no gradient.  No
     atomics: equal calls give equal bits."""
     name = "decoder_attention_backward"
-    dev, a = _fill(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
-    _require_cuda(name, q, dout, out, lse)
-    _check_dtype(name, q, (torch.bfloat16,), "q")
-    for what, t in (("dout", dout), ("out", out)):
-        _check_dtype(name, t, (q.dtype,), what)
-        _require(t.shape == q.shape, lambda: f"{name}: {what} must be {list(q.shape)}, got {list(t.shape)}")
-    _require(out.is_contiguous() and out.data_ptr() % 16 == 0, lambda: f"{name}: out must be contiguous")
-    _check_dtype(name, lse, (torch.float32,), "lse")
-    _require(tuple(lse.shape) == (a.batch, a.heads, a.queries) and lse.is_contiguous(),
-             lambda: f"{name}: lse must be a contiguous [{a.batch}, {a.heads}, {a.queries}] tensor")
-    dout = _operand(dout)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=dev) if need_dkv else None for _ in range(2))
-    ds = torch.empty(slopes.shape, dtype=torch.float32, device=dev) if slopes is not None and need_dslopes else None
-    a.out, a.lse, a.dout, a.dq, a.dk, a.dv, a.dslopes = (out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(),
-                                                         _ptr(dk), _ptr(dv), _ptr(ds))
-    a.dout_stride[:] = dout.stride()[:3]
-    a.dslopes_per_row = int(ds is not None and ds.dim() == 3)
-    if a.batch == 0:
-        if ds is not None:
-            ds.zero_()
-        return dq, dk, dv, ds
+    a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
+    D.same_device(name, q, dout, out, lse)
+    B, nq, _, H = a.sizes[:4]
+    if q.dtype != torch.bfloat16 or dout.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: q, dout and out must be torch.bfloat16, got {q.dtype}, {dout.dtype} and {out.dtype}")
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"{name}: dout and out must be {list(q.shape)}, got {list(dout.shape)} and {list(out.shape)}")
+    if not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"{name}: out must be contiguous and 16-byte aligned")
+    if lse.dtype != torch.float32:
+        raise TypeError(f"{name}: lse must be torch.float32")
+    if lse.shape != (B, H, nq) or not lse.is_contiguous():
+        raise ValueError(f"{name}: lse must be a contiguous [{B}, {H}, {nq}] tensor")
+    dout, dstride = _operand(dout)
+    dq = q.new_empty(q.shape)
+    dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if need_dkv else (None, None)
+    ds = slopes.new_empty(slopes.shape) if slopes is not None and need_dslopes else None
+    if B == 0:
+        return dq, dk, dv, None if ds is None else ds.zero_()
+    rest = (int(ds is not None and ds.dim() == 3), dout.data_ptr(), dstride, dq.data_ptr(), _address(dk), _address(dv),
+            _address(ds))
     lib = D.lib()
-    with D.on_device(dev):
-        need = lib.s4d_attention_backward_workspace_bytes(C.byref(a))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        a.workspace, a.workspace_bytes = _ptr(ws), need
-        st = lib.s4d_attention_backward(C.byref(a), _stream_ptr(dev))
-    D.check(name, st)
+    args = _pack(a, out.data_ptr(), lse.data_ptr(), 0, 0, *rest)
+    with D.on_device(a.index):
+        need = lib.s4d_attention_backward_workspace_bytes(args)
+        if need:
+            ws = q.new_empty(need // 4, dtype=torch.float32)
+            args = _pack(a, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, *rest)
+        st = lib.s4d_attention_backward(args, D.stream_ptr(a.index))
+    if st:
+        D.check(name, st)
     return dq, dk, dv, ds
 
 
@@ -231,7 +262,8 @@ def decoder_attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = 
     name = "decoder_attention"
     if torch.is_grad_enabled():
         for what, t in (("q_pos", q_pos), ("k_pos", k_pos)):
-            _require(t is None or not t.requires_grad, lambda: f"{name}: {what} has no gradient; detach it")
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name}: {what} has no gradient; detach it")
         if q.dtype != torch.bfloat16 and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
             raise TypeError(f"{name}: gradients are implemented for torch.bfloat16, got {q.dtype}")
     return _DecoderAttention.apply(q, k, v, slopes, scale, softcap, q_pos, k_pos, q_segment, k_segment, k_len)

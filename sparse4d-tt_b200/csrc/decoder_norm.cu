@@ -13,6 +13,8 @@
 // The sums over rows for dw and db stay in registers: a block keeps its columns and walks the rows
 // with the stride of a grid that just fills the SMs, adds its row groups through shared memory
 // and writes one fp32 partial row per block; a second launch adds the partial rows in block order.
+// Small inputs (up to 2048 rows and 2^20 values, which stay in the L2 cache) need no second launch: more
+// blocks of the same one each read 8 columns of x and dy again and add them over all rows.
 // No atomics: the order of every addition depends on the sizes alone.
 #include "decoder_types.cuh"
 
@@ -27,7 +29,9 @@ struct NormParams {
   void* y;   // forward: y; backward: dx (may be null)
   float* mean;
   float* rstd;
-  float* partial;  // [gridDim.x, 2, width]: dw then db of each block, or null
+  float* partial;  // [row_blocks, 2, width]: dw then db of each block, or null
+  int row_blocks;  // blocks that walk rows; the ones behind them sum columns
+  void *dweight, *dbias;  // for those
   int64_t x_ld, dy_ld, y_ld;
   int64_t rows;
   int width;
@@ -151,8 +155,48 @@ __global__ void __launch_bounds__(Group<W>::kThreads) norm_forward_kernel(const 
   }
 }
 
+// dw and db of 8 columns: a thread adds one column over every (threads / 8)-th row, then the row lanes are
+// added by shuffles and through shared memory in a fixed order.
+template <typename T, int THREADS>
+__device__ __forceinline__ void sum_columns(const NormParams& p, int block) {
+  __shared__ float sums[2][THREADS / 32][8];
+  const int col = block * 8 + threadIdx.x % 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float a = 0.0f, b = 0.0f;
+  if (col < p.width) {
+    const T *x = static_cast<const T*>(p.x) + col, *dy = static_cast<const T*>(p.dy) + col;
+#pragma unroll 4
+    for (int64_t r = threadIdx.x / 8; r < p.rows; r += THREADS / 8) {
+      const float d = to_f32<T>(dy[r * p.dy_ld]);
+      a = fmaf(d, (to_f32<T>(x[r * p.x_ld]) - __ldg(p.mean + r)) * __ldg(p.rstd + r), a);
+      b += d;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 8; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if (lane < 8) sums[0][warp][lane] = a, sums[1][warp][lane] = b;
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  const int which = threadIdx.x / 8, c = block * 8 + threadIdx.x % 8;
+  void* out = which == 0 ? p.dweight : p.dbias;
+  if (out == nullptr || c >= p.width) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) v += sums[which][w][threadIdx.x % 8];
+  if (p.param_f32)
+    static_cast<float*>(out)[c] = v;
+  else
+    static_cast<T*>(out)[c] = from_f32<T>(v);
+}
+
 template <typename T, int W, int VEC, int K>
 __global__ void __launch_bounds__(Group<W>::kThreads) norm_backward_kernel(const NormParams p) {
+  if (int(blockIdx.x) >= p.row_blocks) {
+    sum_columns<T, Group<W>::kThreads>(p, int(blockIdx.x) - p.row_blocks);
+    return;
+  }
   constexpr int R = Group<W>::kRows;
   __shared__ float red[2][2][Group<W>::kWarps];  // two sums, two buffers: one barrier a row
   // partial sums of the block's other row groups, one 32-column-wide slice of a warp at a time
@@ -174,7 +218,7 @@ __global__ void __launch_bounds__(Group<W>::kThreads) norm_backward_kernel(const
   }
   const float inv = 1.0f / float(p.width);
   int buf = 0;
-  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += int64_t(gridDim.x) * R, buf ^= 1) {
+  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += int64_t(p.row_blocks) * R, buf ^= 1) {
     const int64_t row = base + group;
     const bool live = row < p.rows;
     const int64_t r = live ? row : 0;
@@ -310,6 +354,10 @@ int64_t backward_blocks(int64_t rows, int64_t width) {
   return need < fill ? need : fill;
 }
 
+// Whether dw and db are summed by the backward launch itself: while x and dy stay in the L2 cache and a
+// thread adds at most 64 rows.  900 x 256 f32: one launch of 4.9 us against 4.5 + 2.9 us.
+bool sums_in_one_launch(int64_t rows, int64_t width) { return rows <= 2048 && rows * width <= (1 << 20); }
+
 template <typename T, int W, int VEC, int K>
 int launch_norm(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
   const dim3 grid{static_cast<unsigned>(blocks)};
@@ -426,7 +474,7 @@ int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void* weight,
 }
 
 size_t s4d_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
-  if (rows <= 0 || width <= 0 || width > kNormMaxWidth || rows > 0x7fffffff) return 0;
+  if (rows <= 0 || width <= 0 || width > kNormMaxWidth || rows > 0x7fffffff || sums_in_one_launch(rows, width)) return 0;
   return size_t(backward_blocks(rows, width)) * 2 * size_t(width) * sizeof(float);
 }
 
@@ -444,7 +492,8 @@ int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
       !aligned_to(dweight, psize) || !aligned_to(dbias, psize) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
     return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: misaligned pointer");
   const int64_t blocks = rows > 0 ? backward_blocks(rows, width) : 0;
-  if (sums && rows > 0 &&
+  const bool one = sums_in_one_launch(rows, width);
+  if (sums && rows > 0 && !one &&
       (workspace == nullptr || !aligned_to(workspace, 16) ||
        workspace_bytes < s4d_norm_backward_workspace_bytes(rows, width)))
     return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: missing, misaligned or small workspace");
@@ -454,11 +503,12 @@ int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
     p.x = x, p.x_ld = x_ld, p.dy = dy, p.dy_ld = dy_ld, p.weight = weight, p.y = dx, p.y_ld = dx == nullptr ? 0 : dx_ld;
     p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd), p.rows = rows, p.width = int(width);
     p.param_f32 = param_dtype == S4D_DTYPE_F32;
-    p.partial = sums ? static_cast<float*>(workspace) : nullptr;
-    st = dispatch_type(true, dtype, p, blocks, stm);
+    p.partial = sums && !one ? static_cast<float*>(workspace) : nullptr;
+    p.row_blocks = int(blocks), p.dweight = dweight, p.dbias = dbias;
+    st = dispatch_type(true, dtype, p, blocks + (sums && one ? (width + 7) / 8 : 0), stm);
     if (st != S4D_OK) return st;
   }
-  if (!sums) return S4D_OK;
+  if (!sums || (one && rows > 0)) return S4D_OK;
   const dim3 grid(unsigned((width + 31) / 32), 2);
   const float* partial = static_cast<const float*>(workspace);
   cudaError_t e;

@@ -16,40 +16,41 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib_decoder as D
-from .ops import _check_dtype, _ptr, _require, _require_cuda, _stream_ptr
 
 Tensor = torch.Tensor
 
 MAX_WIDTH = 16384
-_TYPES = tuple(D.DTYPES)
 
 
-def _rows(t: Tensor, width: int) -> Tensor:
-    """``t [..., width]`` as ``[rows, width]`` with unit column stride: a view where the strides allow
-    one (rows may be strided, or one row broadcast), a contiguous copy otherwise."""
+def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
+    """``t [..., width]`` and the stride of its rows: ``t`` itself or a view where the strides allow it (rows
+    may be strided, or one row broadcast), a contiguous copy otherwise."""
+    if t.is_contiguous():
+        return t, width
     v = t if t.dim() == 2 else t.reshape(-1, width)
-    return v if (v.stride(1) == 1 or width == 1) and v.stride(0) >= 0 else v.contiguous()
+    if (v.stride(1) != 1 and width != 1) or v.stride(0) < 0:
+        v = v.contiguous()
+    return v, (v.stride(0) if v.shape[0] > 1 else width)
 
 
-def _params(name: str, dtype: torch.dtype, width: int, **ps: Optional[Tensor]) -> torch.dtype:
-    """The one type of the given ``[width]`` parameters (fp32 when there are none)."""
-    found = None
-    for k, t in ps.items():
-        if t is None:
-            continue
-        _require(tuple(t.shape) == (width,), lambda: f"{name}: {k} must be [{width}], got {list(t.shape)}")
-        _require(t.is_contiguous(), lambda: f"{name}: {k} must be contiguous")
-        _check_dtype(name, t, (torch.float32, dtype), k)
-        if found is not None and t.dtype != found:
-            raise TypeError(f"{name}: the parameters must share one type")
-        found = t.dtype
-    return torch.float32 if found is None else found
+def _param(name: str, what: str, t: Tensor, dtype: torch.dtype, width: int) -> torch.dtype:
+    if t.shape != (width,) or not t.is_contiguous():
+        raise ValueError(f"{name}: {what} must be a contiguous [{width}] tensor, got {list(t.shape)}")
+    if t.dtype != torch.float32 and t.dtype != dtype:
+        raise TypeError(f"{name}: {what} must be torch.float32 or {dtype}, got {t.dtype}")
+    return t.dtype
 
 
 def _width(name: str, x: Tensor) -> int:
-    _require(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_WIDTH,
-             lambda: f"{name}: the last dimension must be 1 to {MAX_WIDTH}, got {list(x.shape)}")
-    return int(x.shape[-1])
+    if x.dtype not in D.DTYPES:
+        raise TypeError(f"{name}: x must be one of {list(D.DTYPES)}, got {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"{name}: the last dimension must be 1 to {MAX_WIDTH}, got {list(x.shape)}")
+    return x.shape[-1]
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
@@ -58,25 +59,30 @@ def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optio
     ``x [..., width]``, ``mean`` and ``rstd`` (fp32, ``[...]``) as ``decoder_norm_backward`` takes
     them.  ``out``: a contiguous tensor like ``x`` to write ``y`` into (it may be ``x`` itself)."""
     name = "decoder_norm_forward"
-    dev = _require_cuda(name, x, weight, bias, out)
-    _check_dtype(name, x, _TYPES, "x")
-    width = _width(name, x)
-    pt = _params(name, x.dtype, width, weight=weight, bias=bias)
+    index = D.same_device(name, x, weight, bias, out)
+    width, dtype = _width(name, x), x.dtype
+    pt = torch.float32 if weight is None else _param(name, "weight", weight, dtype, width)
+    if bias is not None:
+        bt = _param(name, "bias", bias, dtype, width)
+        if weight is not None and bt != pt:
+            raise TypeError(f"{name}: weight and bias must share one type")
+        pt = bt
+    shape = x.shape
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    else:
-        _check_dtype(name, out, (x.dtype,), "out")
-        _require(out.shape == x.shape and out.is_contiguous(),
-                 lambda: f"{name}: out must be a contiguous {list(x.shape)} tensor")
-    v = _rows(x, width)
-    rows = int(v.shape[0])
-    stats = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
-    with D.on_device(dev):
-        st = D.lib().s4d_norm_forward(v.data_ptr(), v.stride(0) if rows > 1 else width, D.DTYPES[x.dtype],
-                                      _ptr(weight), _ptr(bias), D.DTYPES[pt], out.data_ptr(), width, mean.data_ptr(),
-                                      rstd.data_ptr(), rows, width, float(eps), _stream_ptr(dev))
-    D.check(name, st)
+        out = x.new_empty(shape)
+    elif out.dtype != dtype:
+        raise TypeError(f"{name}: out must be {dtype}, got {out.dtype}")
+    elif out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be a contiguous {list(shape)} tensor")
+    v, ld = _rows(x, width)
+    stats = shape[:-1]
+    mean, rstd = x.new_empty(stats, dtype=torch.float32), x.new_empty(stats, dtype=torch.float32)
+    with D.on_device(index):
+        st = D.lib().s4d_norm_forward(v.data_ptr(), ld, D.DTYPES[dtype], _ptr(weight), _ptr(bias), D.DTYPES[pt],
+                                      out.data_ptr(), width, mean.data_ptr(), rstd.data_ptr(), x.numel() // width,
+                                      width, eps, D.stream_ptr(index))
+    if st:
+        D.check(name, st)
     return out, mean, rstd
 
 
@@ -89,34 +95,36 @@ def decoder_norm_backward(dout: Tensor, x: Tensor, weight: Optional[Tensor], mea
     and ``dbias`` are ``[width]`` in ``param_dtype`` (the weight's type, or fp32 without a weight),
     summed over all rows in fp32 in an order that depends on the sizes alone."""
     name = "decoder_norm_backward"
-    dev = _require_cuda(name, dout, x, weight, mean, rstd)
-    _check_dtype(name, x, _TYPES, "x")
-    _check_dtype(name, dout, (x.dtype,), "dout")
-    width = _width(name, x)
-    _require(dout.shape == x.shape, lambda: f"{name}: dout must be {list(x.shape)}, got {list(dout.shape)}")
-    pt = _params(name, x.dtype, width, weight=weight)
+    index = D.same_device(name, x, dout, weight, mean, rstd)
+    width, dtype, shape = _width(name, x), x.dtype, x.shape
+    if dout.dtype != dtype:
+        raise TypeError(f"{name}: dout must be {dtype}, got {dout.dtype}")
+    if dout.shape != shape:
+        raise ValueError(f"{name}: dout must be {list(shape)}, got {list(dout.shape)}")
+    pt = torch.float32 if weight is None else _param(name, "weight", weight, dtype, width)
     if param_dtype is not None:
-        _require(param_dtype in (torch.float32, x.dtype) and (weight is None or param_dtype == weight.dtype),
-                 lambda: f"{name}: param_dtype must be the weight's type, torch.float32 or {x.dtype}")
+        if param_dtype not in (torch.float32, dtype) or (weight is not None and param_dtype != pt):
+            raise ValueError(f"{name}: param_dtype must be the weight's type, torch.float32 or {dtype}")
         pt = param_dtype
-    for k, t in (("mean", mean), ("rstd", rstd)):
-        _check_dtype(name, t, (torch.float32,), k)
-        _require(t.shape == x.shape[:-1] and t.is_contiguous(),
-                 lambda: f"{name}: {k} must be a contiguous {list(x.shape[:-1])} tensor")
-    v, g = _rows(x, width), _rows(dout, width)
-    rows = int(v.shape[0])
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_dx else None
-    dw = torch.empty(width, dtype=pt, device=dev) if need_dweight else None
-    db = torch.empty(width, dtype=pt, device=dev) if need_dbias else None
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise TypeError(f"{name}: mean and rstd must be torch.float32")
+    stats = shape[:-1]
+    if mean.shape != stats or rstd.shape != stats or not mean.is_contiguous() or not rstd.is_contiguous():
+        raise ValueError(f"{name}: mean and rstd must be contiguous {list(stats)} tensors")
+    (v, ld), (g, gld) = _rows(x, width), _rows(dout, width)
+    rows = x.numel() // width
+    dx = x.new_empty(shape) if need_dx else None
+    dw = x.new_empty(width, dtype=pt) if need_dweight else None
+    db = x.new_empty(width, dtype=pt) if need_dbias else None
     lib = D.lib()
-    with D.on_device(dev):
+    with D.on_device(index):
         need = lib.s4d_norm_backward_workspace_bytes(rows, width) if need_dweight or need_dbias else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        st = lib.s4d_norm_backward(g.data_ptr(), g.stride(0) if rows > 1 else width, v.data_ptr(),
-                                   v.stride(0) if rows > 1 else width, D.DTYPES[x.dtype], _ptr(weight), D.DTYPES[pt],
+        ws = x.new_empty(need // 4, dtype=torch.float32) if need else None
+        st = lib.s4d_norm_backward(g.data_ptr(), gld, v.data_ptr(), ld, D.DTYPES[dtype], _ptr(weight), D.DTYPES[pt],
                                    mean.data_ptr(), rstd.data_ptr(), _ptr(dx), width, _ptr(dw), _ptr(db), rows, width,
-                                   _ptr(ws), need, _stream_ptr(dev))
-    D.check(name, st)
+                                   _ptr(ws), need, D.stream_ptr(index))
+    if st:
+        D.check(name, st)
     return dx, dw, db
 
 

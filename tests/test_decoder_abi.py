@@ -38,6 +38,28 @@ def test_exports_are_the_header(lib):
     assert lib.s4d_decoder_abi_version() == D.ABI_VERSION
 
 
+def test_attention_args_format_is_the_struct(tmp_path):
+    """The packed arguments have the C struct's size and field offsets."""
+    import shutil
+    import struct
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    fields = ("batch q q_stride k_stride out lse slope_stride q_pos k_len workspace workspace_bytes error_flag scale dtype "
+              "dslopes_per_row dout dout_stride dq dslopes").split()
+    src = tmp_path / "o.c"
+    src.write_text('#include "s4d_decoder.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){'
+                   + "".join(f'printf("%zu ", offsetof(s4d_attention_args, {f}));' for f in fields)
+                   + 'printf("%zu", sizeof(s4d_attention_args));return 0;}')
+    subprocess.run([cc, "-I", os.path.join(REPO, "include"), str(src), "-o", str(tmp_path / "o")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "o")], capture_output=True, text=True).stdout.split()]
+    before = ("", "7q", "7q3P", "7q3P3q", "7q3P9q", "7q3P9qP", "7q3P9q3P", "7q3P9q3P3q", "7q3P9q3P3q4P", "7q3P9q3P3q5P",
+              "7q3P9q3P3q6P", "7q3P9q3P3q6PN", "7q3P9q3P3q6PNP", "7q3P9q3P3q6PNP2f", "7q3P9q3P3q6PNP2fi",
+              "7q3P9q3P3q6PNP2f2i", "7q3P9q3P3q6PNP2f2iP", "7q3P9q3P3q6PNP2f2iP3q", "7q3P9q3P3q6PNP2f2iP3q3P")
+    assert got == [struct.calcsize("@" + f) for f in before] + [D.ATTENTION_ARGS.size]
+
+
 def norm_fwd(lib, **kw):
     a = dict(x=P, ld=256, dtype=0, w=P, b=P, pt=0, y=P, yld=256, mean=P, rstd=P, rows=4, width=256, eps=1e-5)
     a.update(kw)
@@ -60,7 +82,7 @@ def test_norm_forward_rejects_on_host(lib, kw, status, text):
 
 
 def norm_bwd(lib, **kw):
-    a = dict(dy=P, dld=256, x=P, ld=256, dtype=1, w=P, pt=1, mean=P, rstd=P, dx=P, dxld=256, dw=P, db=P, rows=4,
+    a = dict(dy=P, dld=256, x=P, ld=256, dtype=1, w=P, pt=1, mean=P, rstd=P, dx=P, dxld=256, dw=P, db=P, rows=5000,
              width=256, ws=P, wsb=1 << 20)
     a.update(kw)
     st = lib.s4d_norm_backward(a["dy"], a["dld"], a["x"], a["ld"], a["dtype"], a["w"], a["pt"], a["mean"], a["rstd"],
@@ -82,7 +104,9 @@ def test_norm_backward_rejects_on_host(lib, kw, status, text):
 def test_norm_workspace(lib):
     assert lib.s4d_norm_backward_workspace_bytes(0, 256) == 0
     assert lib.s4d_norm_backward_workspace_bytes(5, 0) == 0
-    assert lib.s4d_norm_backward_workspace_bytes(8, 256) == 2 * 256 * 4
+    assert lib.s4d_norm_backward_workspace_bytes(8, 256) == 0  # summed by the one launch
+    assert lib.s4d_norm_backward_workspace_bytes(3000, 256) % (2 * 256 * 4) == 0
+    assert lib.s4d_norm_backward_workspace_bytes(3000, 256) > 0
     assert lib.s4d_norm_backward_workspace_bytes(1 << 40, 256) == 0
     assert lib.s4d_norm_backward_workspace_bytes(100000, 16384) >= 2 * 16384 * 4
 

@@ -137,6 +137,9 @@ def test_values_behind_masks_do_not_reach_out(cuda_device, bad, Nq):
     assert torch.equal(lse, clean_lse)
     sees = out[:, ~other]
     assert not torch.isfinite(sees).any()
+    for _ in range(60):  # the masked tiles' slow way runs beside the other stream of tiles: never another result
+        again, _ = decoder_attention_forward(q, k2, v2, **how2)
+        assert torch.equal(again[:, other], out[:, other]) and not torch.isfinite(again[:, ~other]).any()
 
 
 def test_rows_that_are_no_numbers_stay_alone(cuda_device):
@@ -329,6 +332,9 @@ def test_gradients_ignore_values_behind_masks(cuda_device, bad):
         assert not g[:, 300:].any(), n
     assert not got[1][1, 280:].any() and not got[2][1, 280:].any()
     assert not torch.isfinite(got[0][:, 160]).any()
+    for _ in range(40):
+        again = decoder_attention_backward(dout2, q2, k2, v2, out, lse, **how)
+        assert all(torch.equal(x[:, keep], y[:, keep]) for x, y in zip(again, got))
 
 
 def test_gradients_strides_expanded_and_parts(cuda_device):

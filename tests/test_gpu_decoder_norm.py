@@ -69,7 +69,7 @@ def check(x, dy, w, b, eps, y, dx, dw, db):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,width", [(1, 1), (1, 7), (3, 256), (900, 256), (17, 257), (64, 512), (33, 1000),
                                         (29, 1001), (40, 2048), (7, 2049), (9, 5000), (5, 8192), (3, 16384),
-                                        (2, 16383), (2801, 64)])
+                                        (2, 16383), (2801, 64), (2048, 512), (2049, 512), (300, 8192)])
 def test_forward_and_gradients(cuda_device, dtype, rows, width):
     x, dy, w, b = make(rows, width, dtype)
     y, mean, rstd = decoder_norm_forward(x, w, b, 1e-5)
