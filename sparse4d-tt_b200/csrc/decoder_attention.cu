@@ -71,7 +71,8 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t
 }
 
 constexpr int64_t kMaxRows = int64_t(1) << 31;
-constexpr int kKeyTile = 64;  // keys of a forward tile
+constexpr int kKeyTile = 64;       // keys of a forward tile
+constexpr int kBackwardTile = 32;  // queries or keys of a backward tile
 
 // Checks of sizes and of the arguments that forward and backward share; fn names the entry point.
 int check_args(const char* fn, const s4d_attention_args* a) {
@@ -166,10 +167,11 @@ int key_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, con
 }
 
 // A map of q or dout; without queries one of k's memory, which no kernel then reads.
-int query_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, const int64_t* stride, int box_rows) {
+int query_map(CUtensorMap* map, const s4d_attention_args& a, const void* base, const int64_t* stride, int box_rows,
+              int box_heads = 1) {
   if (a.queries == 0) return make_map(map, a.k, a.dtype, a.dim, 1, 1, 1, Strides(stride, 1, 1, 1), box_rows);
   return make_map(map, base, a.dtype, a.dim, a.heads, a.queries, a.batch, Strides(stride, a.batch, a.queries, a.heads),
-                  box_rows);
+                  box_rows, box_heads);
 }
 
 // dslopes of one slope per head: the sum of every row's ([B, H, Nq]), one head a block, its rows added
@@ -249,8 +251,7 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
   // that does not divide 128: the map is then not used)
   const bool whole = kAttnRows % p.rep == 0;
   if (st == S4D_OK)
-    st = make_map(&m.q, a.q, a.dtype, a.dim, a.heads, a.queries, a.batch, Strides(a.q_stride, a.batch, a.queries, a.heads),
-                  whole ? kAttnRows / p.rep : 1, whole ? p.rep : 1);
+    st = query_map(&m.q, a, a.q, a.q_stride, whole ? kAttnRows / p.rep : 1, whole ? p.rep : 1);
   if (st != S4D_OK) return st;
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   return a.dim <= 64 ? launch_attention_forward_d64(a.dtype, int(a.pos_dim), p, m, stm)
@@ -272,8 +273,8 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   if (st != S4D_OK) return st;
   const s4d_attention_args& a = *args;
   if (a.dtype != S4D_DTYPE_BF16) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for bf16");
-  if (ceil_div(a.queries, 64) > kAttnMaxTiles || ceil_div(a.keys, 64) > kAttnMaxTiles)
-    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 524288 queries and keys");
+  if (ceil_div(a.queries, kBackwardTile) > kAttnMaxTiles || ceil_div(a.keys, kBackwardTile) > kAttnMaxTiles)
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 262144 queries and keys");
   if (a.batch == 0) return S4D_OK;
   if ((a.dk == nullptr) != (a.dv == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "dk and dv go together");
   if (!aligned_to(a.dout, 16) || !aligned_to(a.dq, 16) || !aligned_to(a.dk, 16) || !aligned_to(a.dv, 16) ||
@@ -304,12 +305,17 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   if (a.queries > 0 || a.keys > 0) {
     AttnBackwardMaps m;
-    st = key_map(&m.k64, a, a.k, a.k_stride, 64);
-    if (st == S4D_OK) st = key_map(&m.v64, a, a.v, a.v_stride, 64);
-    if (st == S4D_OK) st = key_map(&m.k128, a, a.k, a.k_stride, 128);
-    if (st == S4D_OK) st = key_map(&m.v128, a, a.v, a.v_stride, 128);
-    if (st == S4D_OK) st = query_map(&m.q64, a, a.q, a.q_stride, 64);
-    if (st == S4D_OK) st = query_map(&m.do64, a, a.dout, a.dout_stride, 64);
+    st = key_map(&m.k_tile, a, a.k, a.k_stride, kBackwardTile);
+    if (st == S4D_OK) st = key_map(&m.v_tile, a, a.v, a.v_stride, kBackwardTile);
+    if (st == S4D_OK) st = key_map(&m.k_rows, a, a.k, a.k_stride, kAttnRows);
+    if (st == S4D_OK) st = key_map(&m.v_rows, a, a.v, a.v_stride, kAttnRows);
+    if (st == S4D_OK) st = query_map(&m.q_tile, a, a.q, a.q_stride, kBackwardTile);
+    if (st == S4D_OK) st = query_map(&m.do_tile, a, a.dout, a.dout_stride, kBackwardTile);
+    // as in the forward pass: not used for a rep that does not divide 128
+    const bool whole = kAttnRows % p.rep == 0;
+    const int own_rows = whole ? kAttnRows / p.rep : 1, own_heads = whole ? p.rep : 1;
+    if (st == S4D_OK) st = query_map(&m.q_rows, a, a.q, a.q_stride, own_rows, own_heads);
+    if (st == S4D_OK) st = query_map(&m.do_rows, a, a.dout, a.dout_stride, own_rows, own_heads);
     if (st == S4D_OK)
       st = a.dim <= 64 ? launch_attention_backward_d64(int(a.pos_dim), p, m, stm)
                        : launch_attention_backward_d128(int(a.pos_dim), p, m, stm);

@@ -220,6 +220,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory descriptors of a tile of 128-byte rows (64 16-bit elements) stored with the 128-byte
@@ -505,9 +510,10 @@ struct AttnForwardMaps {
 int launch_attention_forward_d64(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
 int launch_attention_forward_d128(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
 
-// Maps of the backward kernels, named by the rows of their boxes.
+// Maps of the backward kernels: boxes of 128 own rows (of the heads that share keys), and of 32 rows of a
+// walked tile.
 struct AttnBackwardMaps {
-  CUtensorMap k64, v64, k128, v128, q64, do64;
+  CUtensorMap q_rows, do_rows, k_rows, v_rows, q_tile, do_tile, k_tile, v_tile;
 };
 int launch_attention_backward_d64(int pos, const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st);
 int launch_attention_backward_d128(int pos, const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st);

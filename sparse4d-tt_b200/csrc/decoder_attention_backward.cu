@@ -18,28 +18,53 @@
 // fp16's subnormal range.
 //
 // What bounds it: as in the forward pass the work per score in registers (one exponential, one more
-// special-function instruction with a 2-D distance, two with a cap, and about twenty others), which
-// is why the tiles of the walked axis are 64 wide: two CTAs then share an SM at D <= 64.
+// special-function instruction with a 2-D distance, two with a cap, and about twenty others), so there
+// have to be row threads that are not waiting.  The walked axis goes in tiles of 32: S and dP then take
+// 64 tensor-memory columns, and two streams of four warps (four for dK and dV at D = 128, where one CTA
+// fills the SM's tensor memory) walk alternate tiles.  The sums dQ, dK and dV are linear in the tiles, so
+// the streams share them; the tensor cores take the tiles in order.
 #include "decoder_attention.cuh"
 
 namespace s4d {
 namespace {
 
 using T = __nv_bfloat16;
-constexpr int kCols = 64;  // rows of a walked tile
-constexpr int kAttnThreads = 192;  // warps 0-3: one score row a thread; 4: TMA; 5: tensor cores
+constexpr int kCols = 32;  // rows of a walked tile
+
+// Ring position of the n-th tile: stage and parity, advanced without a division.
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+};
+
+// Waits until the sums hold every tile before tile n, whose turn it is next: the last tile of each other
+// stream (the own stream's is done, its scores' buffer is in use again).  acc_done[s] counts the tiles
+// of stream s; none after n can be in, so a parity is enough.
+template <int STREAMS>
+__device__ __forceinline__ bool earlier_done(uint32_t acc_done, int n, volatile int* abort_flag, unsigned long long limit_ns) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 1; e < STREAMS; ++e)
+    if (n >= e) ok = ok && warp_wait(acc_done + 8 * ((n - e) % STREAMS), ((n - e) / STREAMS) & 1, abort_flag, limit_ns);
+  return ok;
+}
 
 template <int DP>
 struct Dq {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStages = DP == 64 ? 2 : 1;
-  static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kStages * kTile, kAux = kV + kStages * kTile;
-  static constexpr int kBars = kAux + 2 * 3 * kCols * 4;
-  static constexpr int kNumBars = 4 * kStages + 3;
-  static constexpr int kCtl = kBars + kNumBars * 8;
-  static constexpr int kKinds = kCtl + 16;
-  static constexpr uint32_t kTmem = 256;  // S / dS 64, dP 64, dQ DP
+  static constexpr int kStreams = 2, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  // a K tile is needed until its product with dS, a V tile only for dP
+  static constexpr int kKStages = DP == 64 ? 6 : 3, kVStages = DP == 64 ? 4 : 2;
+  static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
+  static constexpr int kBars = kAux + kWarps * 3 * kCols * 4;
+  static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kStreams + 2;
+  static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kKinds = kCtl + 32;
+  static constexpr uint32_t kTmem = 256;  // per stream S / dS 32, dP 32; dQ DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -47,13 +72,14 @@ template <int DP>
 struct Dkv {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStages = 2;  // of a Q and a dO tile
+  static constexpr int kStreams = DP == 64 ? 2 : 4, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStages = 6;  // of a Q and a dO tile
   static constexpr int kV = kOwn, kQ = kV + kOwn, kAux = kQ + kStages * 2 * kTile;
-  static constexpr int kBars = kAux + 2 * 6 * kCols * 4;
-  static constexpr int kNumBars = 2 * kStages + 4;
-  static constexpr int kCtl = kBars + kNumBars * 8;
-  static constexpr int kKinds = kCtl + 16;
-  static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;  // S / P 64, dP / dS 64, dV DP, dK DP
+  static constexpr int kBars = kAux + kWarps * 6 * kCols * 4;
+  static constexpr int kNumBars = 2 * kStages + 3 * kStreams + 2;
+  static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kKinds = kCtl + 32;
+  static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;  // per stream S / P 32, dP / dS 32; dV DP, dK DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -98,15 +124,15 @@ __device__ __forceinline__ uint32_t pack(F2 v) {
   return pack2<T>(a, b);
 }
 
-// One chunk of 32 keys of a query row.  aux arrays of a tile: -x, -y, segment.
+// One chunk of 16 keys of a query row.  aux arrays of a tile: -x, -y, segment.
 template <int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[32], const uint32_t (&pr)[32], uint32_t (&w)[16],
+__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[16], const uint32_t (&pr)[16], uint32_t (&w)[8],
                                          const ScoreConst& k, float slope2, float qx, float qy, int seg, float lse2,
                                          float delta, const float* aux, float (&sums)[3]) {
   F2 r0 = f2(0.0f), r1 = r0, e1 = r0;
   const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), nlse2 = f2(-lse2), ndelta = f2(-delta);
 #pragma unroll
-  for (int j4 = 0; j4 < 32; j4 += 4) {
+  for (int j4 = 0; j4 < 16; j4 += 4) {
     float4 x4, y4;
     int4 s4;
     if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(aux + j4);
@@ -141,140 +167,121 @@ __device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[32], const uint32_
   }
 }
 
+// Columns [col, col + 32) of a row from fp32 accumulators (zeros when nothing was accumulated).
+__device__ __forceinline__ void store_row32(T* row, int col, int dim, const uint32_t (&o)[32], bool any, float scale) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      w[x] = any ? pack2<T>(__uint_as_float(o[8 * e + 2 * x]) * scale, __uint_as_float(o[8 * e + 2 * x + 1]) * scale) : 0u;
+    if (col + e * 8 < dim) *reinterpret_cast<uint4*>(row + col + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 template <int DP, int POS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, 2)
-    attention_dq_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
+__global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
+    attention_dq_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
+                        const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                         const AttnParams p) {
   using S = Dq<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t k_full = sbase + S::kBars, k_empty = k_full + 8 * S::kStages, v_full = k_empty + 8 * S::kStages,
-                 v_empty = v_full + 8 * S::kStages, s_full = v_empty + 8 * S::kStages, ds_full = s_full + 8,
-                 o_full = ds_full + 8;
+  const uint32_t k_full = sbase + S::kBars, k_empty = k_full + 8 * S::kKStages, v_full = k_empty + 8 * S::kKStages,
+                 v_empty = v_full + 8 * S::kVStages, s_full = v_empty + 8 * S::kVStages,
+                 ds_full = s_full + 8 * S::kStreams, acc_done = ds_full + 8 * S::kStreams, o_full = acc_done + 8 * S::kStreams,
+                 own_full = o_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip = abort_flag + 1;
   unsigned char* kinds = smem + S::kKinds;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // blockIdx.x = (b G + g) row tiles + row tile; row r is query r / rep of head g rep + r % rep
   const uint32_t rep = uint32_t(p.rep);
-  const int64_t rows = p.nq * p.rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
-  int64_t u = blockIdx.x;
-  const int64_t row0 = u % row_tiles * kAttnRows;
+  const uint32_t rows = uint32_t(p.nq) * rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
+  uint32_t u = blockIdx.x;
+  const int64_t row0 = int64_t(u % row_tiles) * kAttnRows;
   u /= row_tiles;
-  const int g = int(u % p.kv_heads), b = int(u / p.kv_heads);
+  const int g = int(u % uint32_t(p.kv_heads)), b = int(u / uint32_t(p.kv_heads));
   int64_t valid = p.nk;
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
   const int tiles = int((valid + kCols - 1) / kCols);
+  const bool own_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+  if (warp == S::kWarps && lane == 0) {
+    for (int s = 0; s < S::kKStages; ++s) {
       mbar_init(k_full + 8 * s, 1);
       mbar_init(k_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < S::kVStages; ++s) {
       mbar_init(v_full + 8 * s, 1);
       mbar_init(v_empty + 8 * s, 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(ds_full, kAttnRows);
+    for (int s = 0; s < S::kStreams; ++s) {
+      mbar_init(s_full + 8 * s, 1);
+      mbar_init(ds_full + 8 * s, kAttnRows);
+      mbar_init(acc_done + 8 * s, 1);
+    }
     mbar_init(o_full, 1);
+    mbar_init(own_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (own_by_tma) {
+      mbar_expect_tx(own_full, 2 * S::kOwn);
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        tma_load_4d(sbase + c * S::kOwnBlock, &qm, own_full, c * 64, g * p.rep, int(uint32_t(row0) / rep), b);
+        tma_load_4d(sbase + S::kDo + c * S::kOwnBlock, &dom, own_full, c * 64, g * p.rep, int(uint32_t(row0) / rep), b);
+      }
+    }
   }
-  if (warp == 5) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
+  if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
   TileWalk walk{nullptr, tiles, int(valid / kCols)};
   if (p.q_seg != nullptr) {
-    const int64_t i0 = row0 / p.rep, i1 = (min(rows, row0 + kAttnRows) - 1) / p.rep;
+    const int64_t i0 = row0 / rep, i1 = (min(int64_t(rows), row0 + kAttnRows) - 1) / rep;
     const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
     classify_tiles(kinds, 0, tiles, kCols, valid, p.k_seg + b * p.nk, own, true);
     walk.kinds = kinds;
   }
-  for (int c = threadIdx.x; c < 2 * kAttnRows * (DP / 8); c += kAttnThreads) {
-    const bool is_do = c >= kAttnRows * (DP / 8);
-    const int e = is_do ? c - kAttnRows * (DP / 8) : c, r = e / (DP / 8), d = e % (DP / 8);
-    const int64_t row = row0 + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < rows && d * 8 < p.dim) {
-      const int64_t i = uint32_t(row) / rep, h = g * p.rep + uint32_t(row) % rep;
-      v = is_do ? ldg_nc_v4(static_cast<const T*>(p.dout) + b * p.do_sb + i * p.do_sn + h * p.do_sh + d * 8)
-                : ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_sn + h * p.q_sh + d * 8);
-    }
-    *reinterpret_cast<uint4*>(smem + (is_do ? S::kDo : 0) + (d / 8) * S::kOwnBlock + r * 128 +
-                              (((d & 7) ^ (r & 7)) << 4)) = v;
-  }
-  fence_proxy_async();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_dp = tmem + kCols, tmem_o = tmem + 2 * kCols;
-  const int t0 = walk.first();
 
-  if (warp == 4) {
-    if (lane == 0) {
-      int n = 0;
-      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
-        const int s = n % S::kStages;
-        const uint32_t parity = (n / S::kStages + 1) & 1;
-        // V first: its stage is free once dP is there, K's only after dQ
-        if (n >= S::kStages && !sleep_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        load_tile<DP, kCols>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, t * kCols, b);
-        if (n >= S::kStages && !sleep_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
-          mbar_wait(v_full + 8 * s, (n / S::kStages) & 1, nullptr);
-          break;
-        }
-        load_tile<DP, kCols>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, t * kCols, b);
-      }
-      for (int i = max(0, n - S::kStages); i < n; ++i) {
-        mbar_wait(k_full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
-        mbar_wait(v_full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
-      }
+  // The row threads' own values; their first tile's keys
+  const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
+  const int64_t row = row0 + tid;
+  const bool live = row < rows;
+  const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
+  const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
+  const int64_t out_row = (b * p.nq + i) * p.heads + h, lse_row = (int64_t(b) * p.heads + h) * p.nq + i;
+  float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
+  float lse2 = INFINITY, delta = 0.0f;  // a row without a key (or past the last): weights of 2^-inf
+  int seg = 0;
+  float nx = 0.0f, ny = 0.0f;  // a key of the next tile a lane, loaded one tile ahead
+  int ns = 0;
+  const int64_t at0 = b * p.nk;
+  auto fetch = [&](int t) {
+    if (t >= tiles) return;
+    const int64_t j = int64_t(t) * kCols + lane;
+    const bool in = j < valid;
+    if (p.k_seg != nullptr) ns = in ? __ldg(p.k_seg + at0 + j) : -1;
+    if constexpr (POS > 0) {
+      const float* kp = p.k_pos + (at0 + j) * POS;
+      nx = in ? -__ldg(kp) : 0.0f;
+      if constexpr (POS > 1) ny = in ? -__ldg(kp + 1) : 0.0f;
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      int n = 0;
-      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
-        const int s = n % S::kStages;
-        const uint32_t parity = (n / S::kStages) & 1;
-        const uint32_t kt = sbase + S::kK + s * S::kTile, vt = sbase + S::kV + s * S::kTile;
-        if (!sleep_wait(v_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        tc_fence_after();
-        mma_scores<T, DP>(tmem_dp, sbase + S::kDo, S::kOwnBlock, vt, S::kBlock, kCols);
-        mma_commit(v_empty + 8 * s);
-        if (!sleep_wait(k_full + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        tc_fence_after();
-        mma_scores<T, DP>(tmem, sbase, S::kOwnBlock, kt, S::kBlock, kCols);
-        mma_commit(s_full);
-        if (!sleep_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns)) break;
-        tc_fence_after();
-        if (!(walk.masked(t) && skip[n & 1])) mma_accumulate<T, DP, kCols>(tmem_o, tmem, kt, n > 0);
-        mma_commit(k_empty + 8 * s);
-      }
-      mma_commit(o_full);
-      mbar_wait(o_full, 0, nullptr);
-    }
-  } else {
-    const int tid = threadIdx.x;
-    const uint32_t lanes = uint32_t(warp * 32) << 16;
-    const int64_t row = row0 + tid;
-    const bool live = row < rows, warp_live = row0 + warp * 32 < rows;
-    const int64_t i = live ? uint32_t(row) / rep : 0;
-    const int h = g * p.rep + (live ? int(uint32_t(row) % rep) : 0);
-    const int64_t out_row = (b * p.nq + i) * p.heads + h, lse_row = (int64_t(b) * p.heads + h) * p.nq + i;
-    const ScoreConst k(p);
-    float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
+  };
+  if (warp < S::kWarps) {
     if constexpr (POS > 0) {
       slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
       qx = __ldg(p.q_pos + (b * p.nq + i) * POS);
       if constexpr (POS > 1) qy = __ldg(p.q_pos + (b * p.nq + i) * POS + 1);
     }
-    int seg = 0;
     if (p.q_seg != nullptr) {
       seg = __ldg(p.q_seg + b * p.nq + i);
       if (seg < 0) seg = -2;
+    } else {
+      fetch(stream);  // without segments stream s begins with tile s
     }
-    // a row without a key (and a row past the last) gets weights of 2^-inf
-    float lse2 = INFINITY, delta = 0.0f;
     if (live) {
       const float l = __ldg(p.lse + lse_row);
       if (l != -INFINITY) {
@@ -282,9 +289,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         const uint4* o4 = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + out_row * p.dim);
         const uint4* d4 = reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + b * p.do_sb + i * p.do_sn +
                                                          h * p.do_sh);
-#pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-          if (c * 8 >= p.dim) break;
+#pragma unroll 4
+        for (int c = 0; c < p.dim / 8; ++c) {
           float fo[8], fd[8];
           bf16x8_to_f32(ldg_nc_v4(o4 + c), fo);
           bf16x8_to_f32(ldg_nc_v4(d4 + c), fd);
@@ -292,111 +298,204 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           for (int e = 0; e < 8; ++e) delta = fmaf(fo[e], fd[e], delta);
         }
       }
-      p.delta[lse_row] = delta;
+      if (stream == 0) p.delta[lse_row] = delta;
     }
-    float* aux = reinterpret_cast<float*>(smem + S::kAux);  // [2][3][64]: -x, -y, segment of the keys
-    float nx = 0.0f, ny = 0.0f;
-    int ns = -1;
-    auto fetch = [&](int t) {
-      if (t >= tiles || tid >= kCols) return;
-      const int64_t j = int64_t(t) * kCols + tid;
-      const bool in = j < valid;
-      ns = in ? (p.k_seg != nullptr ? max(-1, __ldg(p.k_seg + b * p.nk + j)) : 0) : -1;
-      if constexpr (POS > 0) {
-        nx = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS) : 0.0f;
-        if constexpr (POS > 1) ny = in ? -__ldg(p.k_pos + (b * p.nk + j) * POS + 1) : 0.0f;
+  }
+  if (!own_by_tma) {
+    for (int c = threadIdx.x; c < 2 * kAttnRows * (DP / 8); c += S::kThreads) {
+      const bool is_do = c >= kAttnRows * (DP / 8);
+      const int e = is_do ? c - kAttnRows * (DP / 8) : c, r = e / (DP / 8), d = e % (DP / 8);
+      const uint32_t at = uint32_t(row0) + r;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (at < rows && d * 8 < p.dim) {
+        const int64_t qi = at / rep, hh = g * rep + at % rep;
+        v = is_do ? ldg_nc_v4(static_cast<const T*>(p.dout) + b * p.do_sb + qi * p.do_sn + hh * p.do_sh + d * 8)
+                  : ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + qi * p.q_sn + hh * p.q_sh + d * 8);
       }
+      *reinterpret_cast<uint4*>(smem + (is_do ? S::kDo : 0) + (d / 8) * S::kOwnBlock + r * 128 +
+                                (((d & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_proxy_async();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + S::kStreams * 2 * kCols;
+  const int t0 = walk.first();
+
+  if (warp == S::kWarps) {
+    if (lane == 0) {
+      int n = 0;
+      Ring kr, vr;
+      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
+        // V first: its stage is free once dP is there, K's only after dQ
+        if (n >= S::kVStages && !sleep_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+        load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, t * kCols, b);
+        if (n >= S::kKStages && !sleep_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) {
+          mbar_wait(v_full + 8 * vr.stage, vr.parity, nullptr);  // no copy may land in a CTA that is gone
+          break;
+        }
+        load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
+        kr.next(S::kKStages);
+        vr.next(S::kVStages);
+      }
+      if (own_by_tma) mbar_wait(own_full, 0, nullptr);
+      for (int e = max(0, n - S::kKStages); e < n; ++e)
+        mbar_wait(k_full + 8 * (e % S::kKStages), (e / S::kKStages) & 1, nullptr);
+      for (int e = max(0, n - S::kVStages); e < n; ++e)
+        mbar_wait(v_full + 8 * (e % S::kVStages), (e / S::kVStages) & 1, nullptr);
+    }
+  } else if (warp == S::kWarps + 1) {
+    const uint32_t leader = elect_one();
+    Ring ks, vs, ka;  // K and V of the next scores, K of the next product with dS
+    auto issue_scores = [&](int buf) {
+      if (!warp_wait(v_full + 8 * vs.stage, vs.parity, abort_flag, p.wait_limit_ns) ||
+          !warp_wait(k_full + 8 * ks.stage, ks.parity, abort_flag, p.wait_limit_ns))
+        return false;
+      if (leader) {
+        const uint32_t d = tmem + buf * 2 * kCols;
+        mma_scores<T, DP>(d + kCols, sbase + S::kDo, S::kOwnBlock, sbase + S::kV + vs.stage * S::kTile, S::kBlock, kCols);
+        mma_commit(v_empty + 8 * vs.stage);
+        mma_scores<T, DP>(d, sbase, S::kOwnBlock, sbase + S::kK + ks.stage * S::kTile, S::kBlock, kCols);
+        mma_commit(s_full + 8 * buf);
+      }
+      __syncwarp();
+      ks.next(S::kKStages);
+      vs.next(S::kVStages);
+      return true;
     };
-    fetch(t0);
+    bool ok = t0 >= tiles || !own_by_tma || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
+    int ahead = t0;
+    for (int e = 0; e < S::kStreams && ok && ahead < tiles; ++e, ahead = walk.next(ahead)) ok = issue_scores(e);
+    int n = 0;
+    for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
+      const int buf = n % S::kStreams;
+      if (!(ok = warp_wait(ds_full + 8 * buf, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns))) break;
+      if (leader) {
+        if (!(walk.masked(t) && skip[buf]))
+          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, n > 0);
+        mma_commit(k_empty + 8 * ka.stage);
+        mma_commit(acc_done + 8 * buf);
+      }
+      __syncwarp();
+      ka.next(S::kKStages);
+      if (ahead < tiles) {
+        ok = issue_scores(buf);
+        ahead = walk.next(ahead);
+      }
+    }
+    if (leader) {
+      mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
+      mbar_wait(o_full, 0, nullptr);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
+    const bool warp_live = row0 + warp % 4 * 32 < rows;
+    const ScoreConst k(p);
+    float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 3 * kCols;  // [3][32]: -x, -y, segment of the keys
+    const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
+    auto nth = [&](int t, int steps) {  // `steps` walked tiles on
+      for (int e = 0; e < steps && t < tiles; ++e) t = walk.next(t);
+      return t;
+    };
+    int t = nth(t0, stream), n = stream;
+    if (walk.kinds != nullptr) fetch(t);
     float sums[3] = {0.0f, 0.0f, 0.0f};  // sum dS, sum dS dist, sum P dist
     bool dead = false;
-    int n = 0;
-    for (int t = t0; t < tiles; ++n) {
-      const int next = walk.next(t);
+    for (; t < tiles; n += S::kStreams) {
+      const int next = nth(t, S::kStreams);
       const bool masked = walk.masked(t);
-      float* bx = aux + (n & 1) * 3 * kCols;
-      if (tid < kCols) {
-        bx[tid] = nx;
-        bx[kCols + tid] = ny;
-        reinterpret_cast<int*>(bx)[2 * kCols + tid] = ns;
+      if (POS > 0 || masked) {
+        __syncwarp();
+        if constexpr (POS > 0) aux[lane] = nx;
+        if constexpr (POS > 1) aux[kCols + lane] = ny;
+        if (masked)  // -1: a key that no row sees (rows have ids >= 0, or -2)
+          reinterpret_cast<int*>(aux)[2 * kCols + lane] = int64_t(t) * kCols + lane < valid ? max(-1, ns) : -1;
+        __syncwarp();
       }
-      barrier_sync(1, kAttnRows);
       fetch(next);
-      bool bad = false;
-      const unsigned char* kt = smem + S::kK + n % S::kStages * S::kTile;
+      bool bad = false;  // a masked tile whose K holds values that are no numbers
+      const unsigned char* kt = smem + S::kK + n % S::kKStages * S::kTile;
       if (masked) {
-        if (!dead) dead = !warp_wait(k_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
-        bad = barrier_any(2, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
+        if (!dead) dead = !warp_wait(k_full + 8 * (n % S::kKStages), (n / S::kKStages) & 1, abort_flag, p.wait_limit_ns);
+        bad = barrier_any(1 + stream, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
       }
-      if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
-      // only now: this tile's scores follow the products that read the flag's last value
-      if (masked && tid == 0) skip[n & 1] = bad;
+      if (!dead) dead = !warp_wait(s_full + 8 * stream, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns);
+      // only now: this tile's scores follow the product that read the flag's last value
+      if (masked && tid == 0) skip[stream] = bad;
       if (!dead && warp_live) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t sr[32], pr[32], w[16];
-          tmem_ld32_async(tmem + lanes + c * 32, sr);
-          tmem_ld32_async(tmem_dp + lanes + c * 32, pr);
+        for (int c = 0; c < kCols / 16; ++c) {
+          uint32_t sr[16], pr[16], w[8];
+          tmem_ld16_async(tmem_s + c * 16, sr);
+          tmem_ld16_async(tmem_s + kCols + c * 16, pr);
           tmem_ld_wait(sr);
           tmem_ld_wait(pr);
-          const float* cx = bx + c * 32;
           if (masked)
-            dq_chunk<POS, CAP, true>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, sums);
+            dq_chunk<POS, CAP, true>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, aux + c * 16, sums);
           else
-            dq_chunk<POS, CAP, false>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, cx, sums);
-          tmem_st16(tmem + lanes + c * 16, w);
+            dq_chunk<POS, CAP, false>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, aux + c * 16, sums);
+          tmem_st8(tmem_s + c * 8, w);
         }
         tmem_st_wait();
-        if (bad) accumulate_nonzero<T, DP, kCols>(tmem_o + lanes, tmem + lanes, kt, n == 0);
+        if (bad) {
+          // dQ is about to change outside the tensor cores
+          dead = !earlier_done<S::kStreams>(acc_done, n, abort_flag, p.wait_limit_ns);
+          if (!dead) accumulate_nonzero<T, DP, kCols>(tmem_o + lanes, tmem_s, kt, n == 0);
+        }
       }
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(ds_full + 8 * stream);
       t = next;
     }
-    if (!dead && n > 0) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
-    if (!dead && warp_live) {
-      if (POS > 0 && live && p.dslopes != nullptr) {
+    if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
+    if constexpr (POS > 0) {
+      // both streams' sums; o_full: no warp reads its keys' values any more
+      float* other = reinterpret_cast<float*>(smem + S::kAux);
+      if (stream == 1) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) other[e * kAttnRows + tid] = sums[e];
+      }
+      barrier_sync(3, S::kWarps * 32);
+      if (stream == 0 && live && p.dslopes != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) sums[e] += other[e * kAttnRows + tid];
         // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits, so
         // dS is off by P times that sum, and sum dS dist by that times sum P dist.
-        p.dslopes[p.dslopes_by_head ? lse_row : out_row] = -fmaf(-sums[0], sums[2], sums[1]);
+        p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
+            dead ? __int_as_float(0x7fc00000) : -fmaf(-sums[0], sums[2], sums[1]);
       }
+    }
+    if (!dead && warp_live) {
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
+      for (int c0 = 0; c0 < DP / 32 / S::kStreams; ++c0) {
+        const int c = c0 + stream * (DP / 32 / S::kStreams);
         if (c * 32 >= p.dim) break;
         uint32_t o[32];
         tmem_ld32_async(tmem_o + lanes + c * 32, o);
         tmem_ld_wait(o);
-        if (!live) continue;
-        T* dst = static_cast<T*>(p.dq) + out_row * p.dim + c * 32;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            w[x] = n > 0 ? pack2<T>(__uint_as_float(o[8 * e + 2 * x]) * p.scale, __uint_as_float(o[8 * e + 2 * x + 1]) * p.scale)
-                         : 0u;
-          if (c * 32 + e * 8 < p.dim) *reinterpret_cast<uint4*>(dst + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        if (live) store_row32(static_cast<T*>(p.dq) + out_row * p.dim, c * 32, p.dim, o, t0 < tiles, p.scale);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == S::kWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
   }
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
 }
 
-// One chunk of 32 query columns of a key's row.  aux arrays of a tile: -lse2, -delta, -x, -y, -slope2, segment.
+// One chunk of 16 query columns of a key's row.  aux arrays of a tile: -lse2, -delta, -x, -y, -slope2, segment.
 template <int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[32], const uint32_t (&pr)[32], uint32_t (&wp)[16],
-                                          uint32_t (&wd)[16], const ScoreConst& k, float kx, float ky, int seg,
+__device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[16], const uint32_t (&pr)[16], uint32_t (&wp)[8],
+                                          uint32_t (&wd)[8], const ScoreConst& k, float kx, float ky, int seg,
                                           const float* aux) {
   const F2 x2 = f2(kx), y2 = f2(ky);
 #pragma unroll
-  for (int j4 = 0; j4 < 32; j4 += 4) {
+  for (int j4 = 0; j4 < 16; j4 += 4) {
     const float4 l4 = *reinterpret_cast<const float4*>(aux + j4);
     const float4 d4 = *reinterpret_cast<const float4*>(aux + kCols + j4);
     float4 x4, y4, sl4;
@@ -423,7 +522,7 @@ __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[32], const uint32
 }
 
 template <int DP, int POS, bool CAP>
-__global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
+__global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                          const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
                          const AttnParams p) {
@@ -431,38 +530,50 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t full = sbase + S::kBars, empty = full + 8 * S::kStages, own_full = empty + 8 * S::kStages,
-                 s_full = own_full + 8, ds_full = s_full + 8, o_full = ds_full + 8;
+  const uint32_t full = sbase + S::kBars, empty = full + 8 * S::kStages, s_full = empty + 8 * S::kStages,
+                 ds_full = s_full + 8 * S::kStreams, own_full = ds_full + 8 * S::kStreams, acc_done = own_full + 8,
+                 o_full = acc_done + 8 * S::kStreams;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip = abort_flag + 1;
   unsigned char* kinds = smem + S::kKinds;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   // blockIdx.x = (b G + g) key tiles + key tile
-  const int64_t key_tiles = (p.nk + kAttnRows - 1) / kAttnRows;
-  int64_t u = blockIdx.x;
-  const int64_t key0 = u % key_tiles * kAttnRows;
+  const uint32_t key_tiles = uint32_t((p.nk + kAttnRows - 1) / kAttnRows);
+  uint32_t u = blockIdx.x;
+  const int64_t key0 = int64_t(u % key_tiles) * kAttnRows;
   u /= key_tiles;
-  const int g = int(u % p.kv_heads), b = int(u / p.kv_heads);
+  const int g = int(u % uint32_t(p.kv_heads)), b = int(u / uint32_t(p.kv_heads));
   int64_t valid = p.nk;
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
   // query tiles, walked once for every head that shares the keys; none when no key here is valid
   const int tiles = key0 < valid ? int((p.nq + kCols - 1) / kCols) : 0;
 
-  if (threadIdx.x == 0) {
+  if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, 1);
     }
+    for (int s = 0; s < S::kStreams; ++s) {
+      mbar_init(s_full + 8 * s, 1);
+      mbar_init(ds_full + 8 * s, kAttnRows);
+      mbar_init(acc_done + 8 * s, 1);
+    }
     mbar_init(own_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(ds_full, kAttnRows);
     mbar_init(o_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (tiles > 0) {
+      mbar_expect_tx(own_full, 2 * S::kOwn);
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        tma_load_4d(sbase + c * S::kOwnBlock, &km, own_full, c * 64, g, int(key0), b);
+        tma_load_4d(sbase + S::kV + c * S::kOwnBlock, &vm, own_full, c * 64, g, int(key0), b);
+      }
+    }
   }
-  if (warp == 5) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
+  if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
   const bool own_whole = key0 + kAttnRows <= valid;
   TileWalk walk{nullptr, tiles, own_whole ? int(p.nq / kCols) : 0};
   if (p.k_seg != nullptr) {
@@ -470,192 +581,211 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 2 : 1)
     classify_tiles(kinds, 0, tiles, kCols, p.nq, p.q_seg + b * p.nq, own, own_whole);
     walk.kinds = kinds;
   }
+
+  // The row threads' own key
+  const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the key, and the tensor-memory lane
+  const int64_t key = key0 + tid;
+  const bool live = key < p.nk;
+  float kx = 0.0f, ky = 0.0f;
+  // keys past the valid length match nothing (-2), nor do negative ids; without segments valid keys are 0
+  int seg = -2;
+  if (warp < S::kWarps && live) {
+    if (key < valid) seg = p.k_seg != nullptr ? __ldg(p.k_seg + b * p.nk + key) : 0;
+    if (seg < 0) seg = -2;
+    if constexpr (POS > 0) {
+      kx = __ldg(p.k_pos + (b * p.nk + key) * POS);
+      if constexpr (POS > 1) ky = __ldg(p.k_pos + (b * p.nk + key) * POS + 1);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_dp = tmem + kCols, tmem_dv = tmem + 2 * kCols, tmem_dk = tmem_dv + DP;
+  const uint32_t tmem = *tmem_slot, tmem_dv = tmem + S::kStreams * 2 * kCols, tmem_dk = tmem_dv + DP;
   const int t0 = walk.first();
   const bool work = t0 < tiles;
+  // the walk is repeated for every head: (head, tile) pairs in order
+  auto advance = [&](int& hh, int& t) {
+    t = walk.next(t);
+    if (t >= tiles) t = t0, ++hh;
+  };
 
-  if (warp == 4) {
-    if (lane == 0 && work) {
-      mbar_expect_tx(own_full, 2 * S::kOwn);
-      for (int c = 0; c < DP / 64; ++c) {
-        tma_load_4d(sbase + c * S::kOwnBlock, &km, own_full, c * 64, g, int(key0), b);
-        tma_load_4d(sbase + S::kV + c * S::kOwnBlock, &vm, own_full, c * 64, g, int(key0), b);
+  if (warp == S::kWarps) {
+    if (lane == 0 && tiles > 0) {
+      int n = 0, hh = 0, t = t0;
+      Ring r;
+      while (work && hh < p.rep) {
+        if (n >= S::kStages && !sleep_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+        const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile;
+        mbar_expect_tx(full + 8 * r.stage, 2 * S::kTile);
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          tma_load_4d(st + c * S::kBlock, &qm, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
+          tma_load_4d(st + S::kTile + c * S::kBlock, &dom, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
+        }
+        r.next(S::kStages);
+        advance(hh, t);
+        ++n;
       }
-      int n = 0;
-      bool ok = true;
-      for (int hh = 0; hh < p.rep && ok; ++hh)
-        for (int t = t0; t < tiles; t = walk.next(t), ++n) {
-          const int s = n % S::kStages;
-          if (n >= S::kStages && !sleep_wait(empty + 8 * s, (n / S::kStages + 1) & 1, abort_flag, p.wait_limit_ns)) {
-            ok = false;
-            break;
-          }
-          const uint32_t st = sbase + S::kQ + s * 2 * S::kTile;
-          mbar_expect_tx(full + 8 * s, 2 * S::kTile);
-          for (int c = 0; c < DP / 64; ++c) {
-            tma_load_4d(st + c * S::kBlock, &qm, full + 8 * s, c * 64, g * p.rep + hh, t * kCols, b);
-            tma_load_4d(st + S::kTile + c * S::kBlock, &dom, full + 8 * s, c * 64, g * p.rep + hh, t * kCols, b);
-          }
-        }
       mbar_wait(own_full, 0, nullptr);
-      for (int i = max(0, n - S::kStages); i < n; ++i)
-        mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, nullptr);
+      for (int e = max(0, n - S::kStages); e < n; ++e)
+        mbar_wait(full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      int n = 0;
-      bool ok = !work || sleep_wait(own_full, 0, abort_flag, p.wait_limit_ns);
-      for (int hh = 0; hh < p.rep && ok; ++hh)
-        for (int t = t0; t < tiles; t = walk.next(t), ++n) {
-          const int s = n % S::kStages;
-          const uint32_t qt = sbase + S::kQ + s * 2 * S::kTile, dot = qt + S::kTile;
-          if (!(ok = sleep_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns))) break;
-          tc_fence_after();
-          mma_scores<T, DP>(tmem, sbase, S::kOwnBlock, qt, S::kBlock, kCols);
-          mma_scores<T, DP>(tmem_dp, sbase + S::kV, S::kOwnBlock, dot, S::kBlock, kCols);
-          mma_commit(s_full);
-          if (!(ok = sleep_wait(ds_full, n & 1, abort_flag, p.wait_limit_ns))) break;
-          tc_fence_after();
-          if (!(walk.masked(t) && skip[n & 1])) {
-            mma_accumulate<T, DP, kCols>(tmem_dv, tmem, dot, n > 0);
-            mma_accumulate<T, DP, kCols>(tmem_dk, tmem_dp, qt, n > 0);
-          }
-          mma_commit(empty + 8 * s);
+  } else if (warp == S::kWarps + 1) {
+    const uint32_t leader = elect_one();
+    Ring rs, ra;  // the tile of the next scores, and of the next products with P and dS
+    auto issue_scores = [&](int buf) {
+      if (!warp_wait(full + 8 * rs.stage, rs.parity, abort_flag, p.wait_limit_ns)) return false;
+      if (leader) {
+        const uint32_t d = tmem + buf * 2 * kCols, qt = sbase + S::kQ + rs.stage * 2 * S::kTile;
+        mma_scores<T, DP>(d, sbase, S::kOwnBlock, qt, S::kBlock, kCols);
+        mma_scores<T, DP>(d + kCols, sbase + S::kV, S::kOwnBlock, qt + S::kTile, S::kBlock, kCols);
+        mma_commit(s_full + 8 * buf);
+      }
+      __syncwarp();
+      rs.next(S::kStages);
+      return true;
+    };
+    bool ok = !work || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
+    int ah = work ? 0 : p.rep, at = t0;
+    for (int e = 0; e < S::kStreams && ok && ah < p.rep; ++e) {
+      ok = issue_scores(e);
+      advance(ah, at);
+    }
+    int n = 0, hh = work ? 0 : p.rep, t = t0;
+    while (ok && hh < p.rep) {
+      const int buf = n % S::kStreams;
+      if (!(ok = warp_wait(ds_full + 8 * buf, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns))) break;
+      if (leader) {
+        if (!(walk.masked(t) && skip[buf])) {
+          const uint32_t d = tmem + buf * 2 * kCols, qt = sbase + S::kQ + ra.stage * 2 * S::kTile;
+          mma_accumulate<T, DP, kCols>(tmem_dv, d, qt + S::kTile, n > 0);
+          mma_accumulate<T, DP, kCols>(tmem_dk, d + kCols, qt, n > 0);
         }
-      mma_commit(o_full);
+        mma_commit(empty + 8 * ra.stage);
+        mma_commit(acc_done + 8 * buf);
+      }
+      __syncwarp();
+      ra.next(S::kStages);
+      if (ah < p.rep) {
+        ok = issue_scores(buf);
+        advance(ah, at);
+      }
+      advance(hh, t);
+      ++n;
+    }
+    if (leader) {
+      mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
       mbar_wait(o_full, 0, nullptr);
     }
+    __syncwarp();
   } else {
-    const int tid = threadIdx.x;
-    const uint32_t lanes = uint32_t(warp * 32) << 16;
-    const int64_t key = key0 + tid;
-    const bool live = key < p.nk;
+    const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const ScoreConst k(p);
-    float kx = 0.0f, ky = 0.0f;
-    // keys past the valid length match nothing (-2), nor do negative ids; without segments valid keys are 0
-    int seg = key < valid ? (p.k_seg != nullptr ? __ldg(p.k_seg + b * p.nk + key) : 0) : -2;
-    if (seg < 0) seg = -2;
-    if constexpr (POS > 0) {
-      if (live) {
-        kx = __ldg(p.k_pos + (b * p.nk + key) * POS);
-        if constexpr (POS > 1) ky = __ldg(p.k_pos + (b * p.nk + key) * POS + 1);
-      }
-    }
-    // [2][6][64]: -lse2, -delta, -x, -y, -slope2, segment of the queries; threads 0-63 carry the first two
-    // of their query one tile ahead, threads 64-127 the others
-    float* aux = reinterpret_cast<float*>(smem + S::kAux);
-    float c0 = 0.0f, c1 = 0.0f, c2 = 0.0f;
-    int c3 = -1;
-    const int e = tid & (kCols - 1);
+    // [6][32]: -lse2, -delta, -x, -y, -slope2, segment of the queries, one a lane, loaded one tile ahead
+    float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 6 * kCols;
+    const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
+    float c_lse = 0.0f, c_delta = 0.0f, c_x = 0.0f, c_y = 0.0f, c_slope = 0.0f;
+    int c_seg = 0;
     auto fetch = [&](int hh, int t) {
       if (hh >= p.rep) return;
-      const int64_t i = int64_t(t) * kCols + e;
+      const int64_t i = int64_t(t) * kCols + lane;
       const bool in = i < p.nq;
       const int h = g * p.rep + hh;
-      if (tid < kCols) {
-        const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
-        const float l = in ? __ldg(p.lse + r) : -INFINITY;
-        c0 = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
-        c1 = in ? -p.delta[r] : 0.0f;
-      } else {
-        if constexpr (POS > 0) {
-          c0 = in ? -__ldg(p.q_pos + (b * p.nq + i) * POS) : 0.0f;
-          if constexpr (POS > 1) c1 = in ? -__ldg(p.q_pos + (b * p.nq + i) * POS + 1) : 0.0f;
-          c2 = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
-        }
-        c3 = in ? (p.q_seg != nullptr ? max(-1, __ldg(p.q_seg + b * p.nq + i)) : 0) : -1;
+      const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
+      const float l = in ? __ldg(p.lse + r) : -INFINITY;
+      c_lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
+      c_delta = in ? -p.delta[r] : 0.0f;
+      if constexpr (POS > 0) {
+        const float* qp = p.q_pos + (b * p.nq + i) * POS;
+        c_x = in ? -__ldg(qp) : 0.0f;
+        if constexpr (POS > 1) c_y = in ? -__ldg(qp + 1) : 0.0f;
+        c_slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
       }
+      if (p.q_seg != nullptr) c_seg = in ? __ldg(p.q_seg + b * p.nq + i) : -1;
     };
-    int hh = 0, t = t0, n = 0;
+    auto skip_tiles = [&](int& hh, int& t, int steps) {
+      for (int e = 0; e < steps && hh < p.rep; ++e) advance(hh, t);
+    };
+    int hh = work ? 0 : p.rep, t = t0, n = stream;
+    skip_tiles(hh, t, stream);
+    fetch(hh, t);
     bool dead = false;
-    if (work) fetch(0, t0);
-    while (work && hh < p.rep) {
-      int next = walk.next(t), next_hh = hh;
-      if (next >= tiles) next = t0, ++next_hh;
+    for (; hh < p.rep; n += S::kStreams) {
+      int next_hh = hh, next = t;
+      skip_tiles(next_hh, next, S::kStreams);
       const bool masked = walk.masked(t);
-      float* bx = aux + (n & 1) * 6 * kCols;
-      if (tid < kCols) {
-        bx[e] = c0;
-        bx[kCols + e] = c1;
-      } else {
-        bx[2 * kCols + e] = c0;
-        bx[3 * kCols + e] = c1;
-        bx[4 * kCols + e] = c2;
-        reinterpret_cast<int*>(bx)[5 * kCols + e] = c3;
+      __syncwarp();
+      aux[lane] = c_lse;
+      aux[kCols + lane] = c_delta;
+      if constexpr (POS > 0) {
+        aux[2 * kCols + lane] = c_x;
+        if constexpr (POS > 1) aux[3 * kCols + lane] = c_y;
+        aux[4 * kCols + lane] = c_slope;
       }
-      barrier_sync(1, kAttnRows);
+      if (masked)  // -1: a query that sees no key here (keys have ids >= 0, or -2)
+        reinterpret_cast<int*>(aux)[5 * kCols + lane] = int64_t(t) * kCols + lane < p.nq ? max(-1, c_seg) : -1;
+      __syncwarp();
       fetch(next_hh, next);
-      bool bad = false;
+      bool bad = false;  // a masked tile whose Q or dO holds values that are no numbers
       const int s = n % S::kStages;
       const unsigned char *qt = smem + S::kQ + s * 2 * S::kTile, *dot = qt + S::kTile;
       if (masked) {
         if (!dead) dead = !warp_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
-        bad = barrier_any(2, kAttnRows, !dead && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, e));
+        bad = barrier_any(1 + stream, kAttnRows,
+                          !dead && tid < 2 * kCols && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, tid % kCols));
       }
-      if (!dead) dead = !warp_wait(s_full, n & 1, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * stream, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns);
       // only now: this tile's scores follow the products that read the flag's last value
-      if (masked && tid == 0) skip[n & 1] = bad;
+      if (masked && tid == 0) skip[stream] = bad;
       if (!dead) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t sr[32], pr[32], wp[16], wd[16];
-          tmem_ld32_async(tmem + lanes + c * 32, sr);
-          tmem_ld32_async(tmem_dp + lanes + c * 32, pr);
+        for (int c = 0; c < kCols / 16; ++c) {
+          uint32_t sr[16], pr[16], wp[8], wd[8];
+          tmem_ld16_async(tmem_s + c * 16, sr);
+          tmem_ld16_async(tmem_s + kCols + c * 16, pr);
           tmem_ld_wait(sr);
           tmem_ld_wait(pr);
           if (masked)
-            dkv_chunk<POS, CAP, true>(sr, pr, wp, wd, k, kx, ky, seg, bx + c * 32);
+            dkv_chunk<POS, CAP, true>(sr, pr, wp, wd, k, kx, ky, seg, aux + c * 16);
           else
-            dkv_chunk<POS, CAP, false>(sr, pr, wp, wd, k, kx, ky, seg, bx + c * 32);
-          tmem_st16(tmem + lanes + c * 16, wp);
-          tmem_st16(tmem_dp + lanes + c * 16, wd);
+            dkv_chunk<POS, CAP, false>(sr, pr, wp, wd, k, kx, ky, seg, aux + c * 16);
+          tmem_st8(tmem_s + c * 8, wp);
+          tmem_st8(tmem_s + kCols + c * 8, wd);
         }
         tmem_st_wait();
         if (bad) {
-          accumulate_nonzero<T, DP, kCols>(tmem_dv + lanes, tmem + lanes, dot, n == 0);
-          accumulate_nonzero<T, DP, kCols>(tmem_dk + lanes, tmem_dp + lanes, qt, n == 0);
+          // dV and dK are about to change outside the tensor cores
+          dead = !earlier_done<S::kStreams>(acc_done, n, abort_flag, p.wait_limit_ns);
+          if (!dead) {
+            accumulate_nonzero<T, DP, kCols>(tmem_dv + lanes, tmem_s, dot, n == 0);
+            accumulate_nonzero<T, DP, kCols>(tmem_dk + lanes, tmem_s + kCols, qt, n == 0);
+          }
         }
       }
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(ds_full + 8 * stream);
       t = next;
       hh = next_hh;
-      ++n;
     }
-    if (!dead && n > 0) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
+    if (!dead && work) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if (!dead) {
+      // dV's and dK's columns in 32s, shared out among the streams
       const int64_t off = ((b * p.nk + (live ? key : 0)) * p.kv_heads + g) * p.dim;
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const float scale = which == 0 ? 1.0f : p.scale;
-        T* base = static_cast<T*>(which == 0 ? p.dv : p.dk) + off;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          if (c * 32 >= p.dim) break;
-          uint32_t o[32];
-          tmem_ld32_async((which == 0 ? tmem_dv : tmem_dk) + lanes + c * 32, o);
-          tmem_ld_wait(o);
-          if (!live) continue;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t w[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              w[y] = n > 0 ? pack2<T>(__uint_as_float(o[8 * x + 2 * y]) * scale, __uint_as_float(o[8 * x + 2 * y + 1]) * scale)
-                           : 0u;
-            if (c * 32 + x * 8 < p.dim)
-              *reinterpret_cast<uint4*>(base + c * 32 + x * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
+      for (int c0 = 0; c0 < 2 * DP / 32 / S::kStreams; ++c0) {
+        const int c = c0 * S::kStreams + stream, col = c * 32 % DP;
+        const bool is_k = c * 32 >= DP;
+        if (col >= p.dim) continue;
+        uint32_t o[32];
+        tmem_ld32_async(tmem_dv + lanes + c * 32, o);
+        tmem_ld_wait(o);
+        if (live) store_row32(static_cast<T*>(is_k ? p.dk : p.dv) + off, col, p.dim, o, work, is_k ? p.scale : 1.0f);
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == S::kWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
   }
@@ -674,14 +804,16 @@ int launch(const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st) {
   const int64_t groups = int64_t(p.kv_heads) * p.batch;
   if (p.nq > 0) {
     const int64_t row_tiles = (p.nq * p.rep + kAttnRows - 1) / kAttnRows;
-    attention_dq_kernel<DP, POS, CAP><<<dim3(unsigned(row_tiles * groups)), kAttnThreads,
-                                        Dq<DP>::smem(p.q_seg != nullptr ? (p.nk + kCols - 1) / kCols : 0), st>>>(m.k64, m.v64, p);
+    attention_dq_kernel<DP, POS, CAP><<<dim3(unsigned(row_tiles * groups)), Dq<DP>::kThreads,
+                                        Dq<DP>::smem(p.q_seg != nullptr ? (p.nk + kCols - 1) / kCols : 0), st>>>(
+        m.q_rows, m.do_rows, m.k_tile, m.v_tile, p);
     rc = cuda_check(cudaGetLastError(), "attention_dq_kernel launch");
   }
   if (rc == S4D_OK && p.nk > 0 && p.dk != nullptr) {
     const int64_t key_tiles = (p.nk + kAttnRows - 1) / kAttnRows;
-    attention_dkv_kernel<DP, POS, CAP><<<dim3(unsigned(key_tiles * groups)), kAttnThreads,
-                                         Dkv<DP>::smem(p.q_seg != nullptr ? (p.nq + kCols - 1) / kCols : 0), st>>>(m.k128, m.v128, m.q64, m.do64, p);
+    attention_dkv_kernel<DP, POS, CAP><<<dim3(unsigned(key_tiles * groups)), Dkv<DP>::kThreads,
+                                         Dkv<DP>::smem(p.q_seg != nullptr ? (p.nq + kCols - 1) / kCols : 0), st>>>(
+        m.k_rows, m.v_rows, m.q_tile, m.do_tile, p);
     rc = cuda_check(cudaGetLastError(), "attention_dkv_kernel launch");
   }
   return rc;

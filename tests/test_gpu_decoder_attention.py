@@ -114,12 +114,13 @@ def test_no_keys_no_queries_no_batch(cuda_device):
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("Nq", [2, 300])
-def test_values_behind_masks_do_not_reach_out(cuda_device, bad, Nq):
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_behind_masks_do_not_reach_out(cuda_device, D, Nq, bad):
     """Keys past the valid length, padding and another document hold infinities and NaNs: the rows that do
     not see them are bit-equal to the ones without; the rows that do are not numbers."""
     sizes = ids(150, 60, 90, -20)
     qid = [sizes[i * len(sizes) // Nq] for i in range(Nq)]
-    q, k, v, how = make(2, Nq, len(sizes), 4, 2, 64, segments=(qid, sizes), k_len=[320, 280], pos=2, cap=20.0)
+    q, k, v, how = make(2, Nq, len(sizes), 4, 2, D, segments=(qid, sizes), k_len=[320, 280], pos=2, cap=20.0)
     clean, clean_lse = decoder_attention_forward(q, k, v, **how)
     k2, v2 = k.clone(), v.clone()
     how2 = dict(how, k_pos=how["k_pos"].clone())
@@ -303,11 +304,12 @@ def test_gradients_without_keys_queries_or_batch(cuda_device):
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_gradients_ignore_values_behind_masks(cuda_device, bad):
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_ignore_values_behind_masks(cuda_device, D, bad):
     """Infinities and NaNs in padding, past the valid length and in another document, in keys, values,
     queries and the output's gradient."""
     sizes = ids(150, 60, 90, -20)
-    q, k, v, how = make(2, 320, 320, 4, 2, 64, segments=(sizes, sizes), k_len=[320, 280], pos=2, slopes="row", cap=20.0)
+    q, k, v, how = make(2, 320, 320, 4, 2, D, segments=(sizes, sizes), k_len=[320, 280], pos=2, slopes="row", cap=20.0)
     dout, clean = gradients(q, k, v, how)
     t = [x.clone() for x in (q, k, v, dout)]
     how = dict(how, q_pos=how["q_pos"].clone(), k_pos=how["k_pos"].clone())
