@@ -461,6 +461,15 @@ __device__ __forceinline__ void classify_tiles(unsigned char* kinds, int64_t fir
   }
 }
 
+// Ring position of a tile: stage and parity, advanced without a division.
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+};
+
 // The tiles a CTA walks: by the table of kinds, or without segments all of them, the first `whole` of
 // them full and the others masked (the axis ends in the last one, or the own tile is not whole).
 struct TileWalk {

@@ -31,15 +31,6 @@ namespace {
 using T = __nv_bfloat16;
 constexpr int kCols = 32;  // rows of a walked tile
 
-// Ring position of the n-th tile: stage and parity, advanced without a division.
-struct Ring {
-  int stage = 0;
-  uint32_t parity = 0;
-  __device__ __forceinline__ void next(int stages) {
-    if (++stage == stages) stage = 0, parity ^= 1;
-  }
-};
-
 // Waits until the sums hold every tile before tile n, whose turn it is next: the last tile of each other
 // stream (the own stream's is done, its scores' buffer is in use again).  acc_done[s] counts the tiles
 // of stream s; none after n can be in, so a parity is enough.
@@ -60,7 +51,9 @@ struct Dq {
   // a K tile is needed until its product with dS, a V tile only for dP
   static constexpr int kKStages = DP == 64 ? 6 : 3, kVStages = DP == 64 ? 4 : 2;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
-  static constexpr int kBars = kAux + kWarps * 3 * kCols * 4;
+  // with each K tile: -x, -y and segment of its keys
+  static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > 3 * kAttnRows * 4 ? kKStages * 3 * kCols * 4 : 3 * kAttnRows * 4;
+  static constexpr int kBars = kAux + kAuxBytes;
   static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kStreams + 2;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
@@ -75,7 +68,8 @@ struct Dkv {
   static constexpr int kStreams = DP == 64 ? 2 : 4, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
   static constexpr int kStages = 6;  // of a Q and a dO tile
   static constexpr int kV = kOwn, kQ = kV + kOwn, kAux = kQ + kStages * 2 * kTile;
-  static constexpr int kBars = kAux + kWarps * 6 * kCols * 4;
+  // with each stage: -lse2, -delta, -x, -y, -slope2 and segment of its queries
+  static constexpr int kBars = kAux + kStages * 6 * kCols * 4;
   static constexpr int kNumBars = 2 * kStages + 3 * kStreams + 2;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
@@ -212,7 +206,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kKStages; ++s) {
-      mbar_init(k_full + 8 * s, 1);
+      mbar_init(k_full + 8 * s, 33);  // the copy, and the lanes that write the keys' values
       mbar_init(k_empty + 8 * s, 1);
     }
     for (int s = 0; s < S::kVStages; ++s) {
@@ -220,7 +214,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
       mbar_init(v_empty + 8 * s, 1);
     }
     for (int s = 0; s < S::kStreams; ++s) {
-      mbar_init(s_full + 8 * s, 1);
+      mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
       mbar_init(ds_full + 8 * s, kAttnRows);
       mbar_init(acc_done + 8 * s, 1);
     }
@@ -246,7 +240,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
     walk.kinds = kinds;
   }
 
-  // The row threads' own values; their first tile's keys
+  // The row threads' own values
   const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
   const int64_t row = row0 + tid;
   const bool live = row < rows;
@@ -256,20 +250,6 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
   float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
   float lse2 = INFINITY, delta = 0.0f;  // a row without a key (or past the last): weights of 2^-inf
   int seg = 0;
-  float nx = 0.0f, ny = 0.0f;  // a key of the next tile a lane, loaded one tile ahead
-  int ns = 0;
-  const int64_t at0 = b * p.nk;
-  auto fetch = [&](int t) {
-    if (t >= tiles) return;
-    const int64_t j = int64_t(t) * kCols + lane;
-    const bool in = j < valid;
-    if (p.k_seg != nullptr) ns = in ? __ldg(p.k_seg + at0 + j) : -1;
-    if constexpr (POS > 0) {
-      const float* kp = p.k_pos + (at0 + j) * POS;
-      nx = in ? -__ldg(kp) : 0.0f;
-      if constexpr (POS > 1) ny = in ? -__ldg(kp + 1) : 0.0f;
-    }
-  };
   if (warp < S::kWarps) {
     if constexpr (POS > 0) {
       slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
@@ -279,8 +259,6 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
     if (p.q_seg != nullptr) {
       seg = __ldg(p.q_seg + b * p.nq + i);
       if (seg < 0) seg = -2;
-    } else {
-      fetch(stream);  // without segments stream s begins with tile s
     }
     if (live) {
       const float l = __ldg(p.lse + lse_row);
@@ -324,27 +302,47 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
   const int t0 = walk.first();
 
   if (warp == S::kWarps) {
-    if (lane == 0) {
-      int n = 0;
-      Ring kr, vr;
-      for (int t = t0; t < tiles; t = walk.next(t), ++n) {
-        // V first: its stage is free once dP is there, K's only after dQ
-        if (n >= S::kVStages && !sleep_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
-        load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, t * kCols, b);
-        if (n >= S::kKStages && !sleep_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) {
-          mbar_wait(v_full + 8 * vr.stage, vr.parity, nullptr);  // no copy may land in a CTA that is gone
-          break;
-        }
-        load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
-        kr.next(S::kKStages);
-        vr.next(S::kVStages);
+    // a key of the next tile a lane, loaded one tile ahead and written beside its K tile
+    float nx = 0.0f, ny = 0.0f;
+    int ns = 0;
+    auto fetch = [&](int t) {
+      if (t >= tiles) return;
+      const int64_t j = int64_t(t) * kCols + lane, at = b * p.nk + j;
+      const bool in = j < valid;
+      ns = in ? 0 : -1;  // -1: a key that no row sees (rows have ids >= 0, or -2)
+      if (p.k_seg != nullptr && in) ns = max(-1, __ldg(p.k_seg + at));
+      if constexpr (POS > 0) {
+        nx = in ? -__ldg(p.k_pos + at * POS) : 0.0f;
+        if constexpr (POS > 1) ny = in ? -__ldg(p.k_pos + at * POS + 1) : 0.0f;
       }
-      if (own_by_tma) mbar_wait(own_full, 0, nullptr);
-      for (int e = max(0, n - S::kKStages); e < n; ++e)
-        mbar_wait(k_full + 8 * (e % S::kKStages), (e / S::kKStages) & 1, nullptr);
-      for (int e = max(0, n - S::kVStages); e < n; ++e)
-        mbar_wait(v_full + 8 * (e % S::kVStages), (e / S::kVStages) & 1, nullptr);
+    };
+    int n = 0;
+    Ring kr, vr;
+    fetch(t0);
+    for (int t = t0; t < tiles; ++n) {
+      // V first: its stage is free once dP is there, K's only after dQ
+      if (n >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+      if (lane == 0) load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, t * kCols, b);
+      if (n >= S::kKStages && !warp_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) {
+        mbar_wait(v_full + 8 * vr.stage, vr.parity, nullptr);  // no copy may land in a CTA that is gone
+        break;
+      }
+      if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
+      float* aux = reinterpret_cast<float*>(smem + S::kAux) + kr.stage * 3 * kCols + lane;
+      if constexpr (POS > 0) aux[0] = nx;
+      if constexpr (POS > 1) aux[kCols] = ny;
+      reinterpret_cast<int*>(aux)[2 * kCols] = ns;
+      mbar_arrive(k_full + 8 * kr.stage);
+      kr.next(S::kKStages);
+      vr.next(S::kVStages);
+      t = walk.next(t);
+      fetch(t);
     }
+    if (own_by_tma) mbar_wait(own_full, 0, nullptr);
+    for (int e = max(0, n - S::kKStages); e < n; ++e)
+      mbar_wait(k_full + 8 * (e % S::kKStages), (e / S::kKStages) & 1, nullptr);
+    for (int e = max(0, n - S::kVStages); e < n; ++e)
+      mbar_wait(v_full + 8 * (e % S::kVStages), (e / S::kVStages) & 1, nullptr);
   } else if (warp == S::kWarps + 1) {
     const uint32_t leader = elect_one();
     Ring ks, vs, ka;  // K and V of the next scores, K of the next product with dS
@@ -358,6 +356,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
         mma_commit(v_empty + 8 * vs.stage);
         mma_scores<T, DP>(d, sbase, S::kOwnBlock, sbase + S::kK + ks.stage * S::kTile, S::kBlock, kCols);
         mma_commit(s_full + 8 * buf);
+        mbar_arrive(s_full + 8 * buf);
       }
       __syncwarp();
       ks.next(S::kKStages);
@@ -393,35 +392,27 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool warp_live = row0 + warp % 4 * 32 < rows;
     const ScoreConst k(p);
-    float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 3 * kCols;  // [3][32]: -x, -y, segment of the keys
     const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
     auto nth = [&](int t, int steps) {  // `steps` walked tiles on
       for (int e = 0; e < steps && t < tiles; ++e) t = walk.next(t);
       return t;
     };
     int t = nth(t0, stream), n = stream;
-    if (walk.kinds != nullptr) fetch(t);
     float sums[3] = {0.0f, 0.0f, 0.0f};  // sum dS, sum dS dist, sum P dist
     bool dead = false;
-    for (; t < tiles; n += S::kStreams) {
+    uint32_t turn = 0;  // parity of this stream's tiles
+    Ring r{stream, 0};  // stages of their K tiles
+    for (; t < tiles; n += S::kStreams, turn ^= 1) {
       const int next = nth(t, S::kStreams);
       const bool masked = walk.masked(t);
-      if (POS > 0 || masked) {
-        __syncwarp();
-        if constexpr (POS > 0) aux[lane] = nx;
-        if constexpr (POS > 1) aux[kCols + lane] = ny;
-        if (masked)  // -1: a key that no row sees (rows have ids >= 0, or -2)
-          reinterpret_cast<int*>(aux)[2 * kCols + lane] = int64_t(t) * kCols + lane < valid ? max(-1, ns) : -1;
-        __syncwarp();
-      }
-      fetch(next);
       bool bad = false;  // a masked tile whose K holds values that are no numbers
-      const unsigned char* kt = smem + S::kK + n % S::kKStages * S::kTile;
+      const unsigned char* kt = smem + S::kK + r.stage * S::kTile;
+      const float* aux = reinterpret_cast<const float*>(smem + S::kAux) + r.stage * 3 * kCols;
       if (masked) {
-        if (!dead) dead = !warp_wait(k_full + 8 * (n % S::kKStages), (n / S::kKStages) & 1, abort_flag, p.wait_limit_ns);
+        if (!dead) dead = !warp_wait(k_full + 8 * r.stage, r.parity, abort_flag, p.wait_limit_ns);
         bad = barrier_any(1 + stream, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
       }
-      if (!dead) dead = !warp_wait(s_full + 8 * stream, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * stream, turn, abort_flag, p.wait_limit_ns);
       // only now: this tile's scores follow the product that read the flag's last value
       if (masked && tid == 0) skip[stream] = bad;
       if (!dead && warp_live) {
@@ -448,6 +439,8 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
       tc_fence_before();
       mbar_arrive(ds_full + 8 * stream);
       t = next;
+#pragma unroll
+      for (int e = 0; e < S::kStreams; ++e) r.next(S::kKStages);
     }
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if constexpr (POS > 0) {
@@ -552,11 +545,11 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(full + 8 * s, 1);
+      mbar_init(full + 8 * s, 33);  // the copies, and the lanes that write the queries' values
       mbar_init(empty + 8 * s, 1);
     }
     for (int s = 0; s < S::kStreams; ++s) {
-      mbar_init(s_full + 8 * s, 1);
+      mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
       mbar_init(ds_full + 8 * s, kAttnRows);
       mbar_init(acc_done + 8 * s, 1);
     }
@@ -610,11 +603,33 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
   };
 
   if (warp == S::kWarps) {
-    if (lane == 0 && tiles > 0) {
-      int n = 0, hh = 0, t = t0;
-      Ring r;
-      while (work && hh < p.rep) {
-        if (n >= S::kStages && !sleep_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+    // a query of the next tile a lane, loaded one tile ahead and written beside its Q and dO tiles
+    float c_lse = 0.0f, c_delta = 0.0f, c_x = 0.0f, c_y = 0.0f, c_slope = 0.0f;
+    int c_seg = 0;
+    auto fetch = [&](int hh, int t) {
+      if (hh >= p.rep) return;
+      const int64_t i = int64_t(t) * kCols + lane;
+      const bool in = i < p.nq;
+      const int h = g * p.rep + hh;
+      const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
+      const float l = in ? __ldg(p.lse + r) : -INFINITY;
+      c_lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
+      c_delta = in ? -p.delta[r] : 0.0f;
+      if constexpr (POS > 0) {
+        const float* qp = p.q_pos + (b * p.nq + i) * POS;
+        c_x = in ? -__ldg(qp) : 0.0f;
+        if constexpr (POS > 1) c_y = in ? -__ldg(qp + 1) : 0.0f;
+        c_slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
+      }
+      c_seg = in ? 0 : -1;  // -1: a query that sees no key here (keys have ids >= 0, or -2)
+      if (p.q_seg != nullptr && in) c_seg = max(-1, __ldg(p.q_seg + b * p.nq + i));
+    };
+    int n = 0, hh = work ? 0 : p.rep, t = t0;
+    Ring r;
+    fetch(hh, t);
+    while (hh < p.rep) {
+      if (n >= S::kStages && !warp_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+      if (lane == 0) {
         const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile;
         mbar_expect_tx(full + 8 * r.stage, 2 * S::kTile);
 #pragma unroll
@@ -622,14 +637,25 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
           tma_load_4d(st + c * S::kBlock, &qm, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
           tma_load_4d(st + S::kTile + c * S::kBlock, &dom, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
         }
-        r.next(S::kStages);
-        advance(hh, t);
-        ++n;
       }
-      mbar_wait(own_full, 0, nullptr);
-      for (int e = max(0, n - S::kStages); e < n; ++e)
-        mbar_wait(full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
+      float* aux = reinterpret_cast<float*>(smem + S::kAux) + r.stage * 6 * kCols + lane;
+      aux[0] = c_lse;
+      aux[kCols] = c_delta;
+      if constexpr (POS > 0) {
+        aux[2 * kCols] = c_x;
+        if constexpr (POS > 1) aux[3 * kCols] = c_y;
+        aux[4 * kCols] = c_slope;
+      }
+      reinterpret_cast<int*>(aux)[5 * kCols] = c_seg;
+      mbar_arrive(full + 8 * r.stage);
+      r.next(S::kStages);
+      advance(hh, t);
+      fetch(hh, t);
+      ++n;
     }
+    if (tiles > 0) mbar_wait(own_full, 0, nullptr);
+    for (int e = max(0, n - S::kStages); e < n; ++e)
+      mbar_wait(full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
   } else if (warp == S::kWarps + 1) {
     const uint32_t leader = elect_one();
     Ring rs, ra;  // the tile of the next scores, and of the next products with P and dS
@@ -640,6 +666,7 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
         mma_scores<T, DP>(d, sbase, S::kOwnBlock, qt, S::kBlock, kCols);
         mma_scores<T, DP>(d + kCols, sbase + S::kV, S::kOwnBlock, qt + S::kTile, S::kBlock, kCols);
         mma_commit(s_full + 8 * buf);
+        mbar_arrive(s_full + 8 * buf);
       }
       __syncwarp();
       rs.next(S::kStages);
@@ -681,60 +708,26 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
   } else {
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const ScoreConst k(p);
-    // [6][32]: -lse2, -delta, -x, -y, -slope2, segment of the queries, one a lane, loaded one tile ahead
-    float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 6 * kCols;
     const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
-    float c_lse = 0.0f, c_delta = 0.0f, c_x = 0.0f, c_y = 0.0f, c_slope = 0.0f;
-    int c_seg = 0;
-    auto fetch = [&](int hh, int t) {
-      if (hh >= p.rep) return;
-      const int64_t i = int64_t(t) * kCols + lane;
-      const bool in = i < p.nq;
-      const int h = g * p.rep + hh;
-      const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
-      const float l = in ? __ldg(p.lse + r) : -INFINITY;
-      c_lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
-      c_delta = in ? -p.delta[r] : 0.0f;
-      if constexpr (POS > 0) {
-        const float* qp = p.q_pos + (b * p.nq + i) * POS;
-        c_x = in ? -__ldg(qp) : 0.0f;
-        if constexpr (POS > 1) c_y = in ? -__ldg(qp + 1) : 0.0f;
-        c_slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
-      }
-      if (p.q_seg != nullptr) c_seg = in ? __ldg(p.q_seg + b * p.nq + i) : -1;
-    };
     auto skip_tiles = [&](int& hh, int& t, int steps) {
       for (int e = 0; e < steps && hh < p.rep; ++e) advance(hh, t);
     };
     int hh = work ? 0 : p.rep, t = t0, n = stream;
     skip_tiles(hh, t, stream);
-    fetch(hh, t);
     bool dead = false;
-    for (; hh < p.rep; n += S::kStreams) {
-      int next_hh = hh, next = t;
-      skip_tiles(next_hh, next, S::kStreams);
+    uint32_t turn = 0;  // parity of this stream's tiles
+    Ring r{stream, 0};  // their stages
+    for (; hh < p.rep; n += S::kStreams, turn ^= 1) {
       const bool masked = walk.masked(t);
-      __syncwarp();
-      aux[lane] = c_lse;
-      aux[kCols + lane] = c_delta;
-      if constexpr (POS > 0) {
-        aux[2 * kCols + lane] = c_x;
-        if constexpr (POS > 1) aux[3 * kCols + lane] = c_y;
-        aux[4 * kCols + lane] = c_slope;
-      }
-      if (masked)  // -1: a query that sees no key here (keys have ids >= 0, or -2)
-        reinterpret_cast<int*>(aux)[5 * kCols + lane] = int64_t(t) * kCols + lane < p.nq ? max(-1, c_seg) : -1;
-      __syncwarp();
-      fetch(next_hh, next);
       bool bad = false;  // a masked tile whose Q or dO holds values that are no numbers
-      const int s = n % S::kStages;
-      const unsigned char *qt = smem + S::kQ + s * 2 * S::kTile, *dot = qt + S::kTile;
+      const unsigned char *qt = smem + S::kQ + r.stage * 2 * S::kTile, *dot = qt + S::kTile;
+      const float* aux = reinterpret_cast<const float*>(smem + S::kAux) + r.stage * 6 * kCols;
       if (masked) {
-        if (!dead) dead = !warp_wait(full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
+        if (!dead) dead = !warp_wait(full + 8 * r.stage, r.parity, abort_flag, p.wait_limit_ns);
         bad = barrier_any(1 + stream, kAttnRows,
                           !dead && tid < 2 * kCols && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, tid % kCols));
       }
-      if (!dead) dead = !warp_wait(s_full + 8 * stream, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * stream, turn, abort_flag, p.wait_limit_ns);
       // only now: this tile's scores follow the products that read the flag's last value
       if (masked && tid == 0) skip[stream] = bad;
       if (!dead) {
@@ -764,8 +757,9 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
       }
       tc_fence_before();
       mbar_arrive(ds_full + 8 * stream);
-      t = next;
-      hh = next_hh;
+      skip_tiles(hh, t, S::kStreams);
+#pragma unroll
+      for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages);
     }
     if (!dead && work) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if (!dead) {

@@ -3,7 +3,8 @@
 //
 // One CTA owns 128 rows of one shared head: row r is query r / rep of head g rep + r % rep, so that
 // the rep heads that share keys read them once.  It walks the keys in tiles of 64:
-//   one warp    loads K and V tiles by TMA into rings of shared memory;
+//   one warp    loads K and V tiles by TMA into rings of shared memory, and writes the keys' positions and
+//               segments beside them;
 //   one warp    issues S = Q K^T for the next tile into one of two score buffers in tensor memory (64
 //               columns each), and once P of this tile is there O += P V, with P read from tensor
 //               memory and V as an MN-major operand;
@@ -41,9 +42,11 @@ struct Fwd {
   static constexpr int kWarps = 4 * kStreams;          // row threads; then the TMA and the tensor-core warp
   static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kK = kQ, kV = kK + kStages * kTile, kAux = kV + kStages * kTile;
-  // per row warp: negated x, y of the keys and their segments (after the last tile: m and l of its
-  // rows); barriers; tensor-memory slot, abort, skip[2]
-  static constexpr int kBars = kAux + kWarps * 3 * kKeys * 4;
+  // negated x, y and segment of a tile's keys (after the last tile: m and l of the rows).  A slot is read
+  // until the tile's P is there, so it is free for tile n once V of tile n - 1 has found a free stage: one
+  // slot more than stages.  Then barriers; tensor-memory slot, abort, skip[2]
+  static constexpr int kSlots = kStages + 1;
+  static constexpr int kBars = kAux + kSlots * 3 * kKeys * 4;
   static constexpr int kNumBars = 4 * kStages + 8;
   static constexpr int kCtl = kBars + kNumBars * 8;
   static constexpr int kKinds = kCtl + 16;
@@ -129,13 +132,13 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(k_full + 8 * s, 1);
+      mbar_init(k_full + 8 * s, 33);  // the copy, and the lanes that write the keys' values
       mbar_init(k_empty + 8 * s, 1);
       mbar_init(v_full + 8 * s, 1);
       mbar_init(v_empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(s_full + 8 * s, 1);
+      mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the keys' values
       mbar_init(p_full + 8 * s, kAttnRows);
       mbar_init(pv_done + 8 * s, 1);
     }
@@ -151,51 +154,22 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   const int tiles = int(max(int64_t(0), min(p.tiles_per_split, (valid + kKeys - 1) / kKeys - first)));
   TileWalk walk{nullptr, tiles, int(max(int64_t(0), min(int64_t(tiles), valid / kKeys - first)))};
   const bool q_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
-  int loaded = 0;                                // tiles already asked for (the TMA thread)
-  if (warp == S::kWarps && lane == 0) {
-    if (q_by_tma) {
-      mbar_expect_tx(q_full, S::kQ);
-#pragma unroll
-      for (int c = 0; c < DP / 64; ++c)
-        tma_load_4d(sbase + c * S::kOwnBlock, &qm, q_full, c * 64, g * p.rep, int(uint32_t(row0) / rep), b);
-    }
-    // without segments every tile is walked: the first loads need not wait for the other warps
-    if (p.q_seg == nullptr)
-      for (; loaded < min(S::kStages, tiles); ++loaded) {
-        const int key = int((first + loaded) * kKeys);
-        load_tile<DP, kKeys>(sbase + S::kK + loaded * S::kTile, &km, k_full + 8 * loaded, g, key, b);
-        load_tile<DP, kKeys>(sbase + S::kV + loaded * S::kTile, &vm, v_full + 8 * loaded, g, key, b);
-      }
-  }
-  if (p.q_seg != nullptr) {
-    const int64_t i0 = row0 / rep, i1 = (min(int64_t(rows), row0 + kAttnRows) - 1) / rep;
-    const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
-    classify_tiles(kinds, first, tiles, kKeys, valid, p.k_seg + b * p.nk, own, true);
-    walk.kinds = kinds;
-  }
-  // The row threads' own values and their first tile's keys
-  const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
-  const int64_t row = row0 + tid;
-  const bool live = row < rows;
-  const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
-  const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
   const int64_t left = valid - first * kKeys;  // keys of this part and after it
-  const int64_t at0 = b * p.nk + first * kKeys;
-  float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
-  int seg = 0;  // own segment: -2 (matches nothing) or >= 0; without segments 0
-  // two keys of the next tile a lane, loaded one tile ahead
+  // The TMA warp's lanes: two keys of a tile each, into registers (one tile ahead) and then into a
+  // slot beside the tiles
   float2 nx = make_float2(0.0f, 0.0f), ny = nx;
   int2 ns = make_int2(0, 0);
   auto fetch = [&](int t) {
     if (t >= tiles) return;
-    const int64_t j = int64_t(t) * kKeys + 2 * lane;
+    const int64_t j = int64_t(t) * kKeys + 2 * lane, at = b * p.nk + first * kKeys + j;
     const bool in0 = j < left, in1 = j + 1 < left;
+    ns = make_int2(in0 ? 0 : -1, in1 ? 0 : -1);  // -1: a key that no row sees (rows have ids >= 0, or -2)
     if (p.k_seg != nullptr) {
-      ns.x = in0 ? __ldg(p.k_seg + at0 + j) : -1;
-      ns.y = in1 ? __ldg(p.k_seg + at0 + j + 1) : -1;
+      if (in0) ns.x = max(-1, __ldg(p.k_seg + at));
+      if (in1) ns.y = max(-1, __ldg(p.k_seg + at + 1));
     }
     if constexpr (POS > 0) {
-      const float* kp = p.k_pos + (at0 + j) * POS;
+      const float* kp = p.k_pos + at * POS;
       nx.x = in0 ? -__ldg(kp) : 0.0f;
       nx.y = in1 ? -__ldg(kp + POS) : 0.0f;
       if constexpr (POS > 1) {
@@ -204,6 +178,50 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       }
     }
   };
+  auto load_k = [&](int s, int slot, int t) {
+    if (lane == 0) load_tile<DP, kKeys>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, int((first + t) * kKeys), b);
+    float* aux = reinterpret_cast<float*>(smem + S::kAux) + slot * 3 * kKeys + 2 * lane;
+    if constexpr (POS > 0) *reinterpret_cast<float2*>(aux) = nx;
+    if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kKeys) = ny;
+    *reinterpret_cast<int2*>(aux + 2 * kKeys) = ns;
+    mbar_arrive(k_full + 8 * s);
+  };
+  auto load_v = [&](int s, int t) {
+    if (lane == 0) load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, int((first + t) * kKeys), b);
+  };
+  int loaded = 0;  // tiles already asked for (the TMA warp)
+  if (warp == S::kWarps) {
+    __syncwarp();  // lane 0's barriers
+    if (q_by_tma && lane == 0) {
+      mbar_expect_tx(q_full, S::kQ);
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c)
+        tma_load_4d(sbase + c * S::kOwnBlock, &qm, q_full, c * 64, g * p.rep, int(uint32_t(row0) / rep), b);
+    }
+    // without segments every tile is walked: the first loads need not wait for the other warps
+    if (p.q_seg == nullptr) {
+      fetch(0);
+      for (; loaded < min(S::kStages, tiles); ++loaded) {
+        load_v(loaded, loaded);
+        load_k(loaded, loaded, loaded);
+        fetch(loaded + 1);
+      }
+    }
+  }
+  if (p.q_seg != nullptr) {
+    const int64_t i0 = row0 / rep, i1 = (min(int64_t(rows), row0 + kAttnRows) - 1) / rep;
+    const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
+    classify_tiles(kinds, first, tiles, kKeys, valid, p.k_seg + b * p.nk, own, true);
+    walk.kinds = kinds;
+  }
+  // The row threads' own values
+  const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
+  const int64_t row = row0 + tid;
+  const bool live = row < rows;
+  const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
+  const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
+  float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
+  int seg = 0;  // own segment: -2 (matches nothing) or >= 0; without segments 0
   if (warp < S::kWarps) {
     if constexpr (POS > 0) {
       slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
@@ -213,8 +231,6 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     if (p.q_seg != nullptr) {
       seg = __ldg(p.q_seg + b * p.nq + i);
       if (seg < 0) seg = -2;
-    } else {
-      fetch(stream);  // without segments stream s begins with tile s
     }
   }
   // Q where TMA cannot gather it: 16-byte pieces, zero past the last row and column, in the swizzled
@@ -239,41 +255,46 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   const int t0 = walk.first();
 
   if (warp == S::kWarps) {
-    if (lane == 0) {
-      int n = loaded;
-      for (int t = loaded > 0 ? loaded : t0; t < tiles; t = walk.next(t), ++n) {
-        const int s = n % S::kStages;
-        const uint32_t parity = (n / S::kStages + 1) & 1;
-        const int key = int((first + t) * kKeys);
-        if (n >= S::kStages && !sleep_wait(k_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) break;
-        load_tile<DP, kKeys>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, key, b);
-        if (n >= S::kStages && !sleep_wait(v_empty + 8 * s, parity, abort_flag, p.wait_limit_ns)) {
-          // the K load is out: it may not land in the memory of a CTA that is gone
-          mbar_wait(k_full + 8 * s, (n / S::kStages) & 1, nullptr);
-          break;
-        }
-        load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, key, b);
+    int n = loaded, t = loaded > 0 ? loaded : t0;
+    Ring r{loaded % S::kStages, uint32_t(loaded / S::kStages) & 1}, slot{loaded, 0};
+    if (loaded == 0) fetch(t);
+    for (; t < tiles; ++n) {
+      const bool again = n >= S::kStages;
+      if (again && !warp_wait(k_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+      load_k(r.stage, slot.stage, t);
+      if (again && !warp_wait(v_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) {
+        // the K load is out: it may not land in the memory of a CTA that is gone
+        mbar_wait(k_full + 8 * r.stage, r.parity, nullptr);
+        break;
       }
-      if (q_by_tma) mbar_wait(q_full, 0, nullptr);
-      for (int e = max(0, n - S::kStages); e < n; ++e) {
-        mbar_wait(k_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
-        mbar_wait(v_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
-      }
+      load_v(r.stage, t);
+      r.next(S::kStages);
+      slot.next(S::kSlots);
+      t = walk.next(t);
+      fetch(t);
+    }
+    if (q_by_tma) mbar_wait(q_full, 0, nullptr);
+    for (int e = max(0, n - S::kStages); e < n; ++e) {
+      mbar_wait(k_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
+      mbar_wait(v_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
     }
   } else if (warp == S::kWarps + 1) {
     // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one
     // lane issues.
     const uint32_t leader = elect_one();
     // S of tile n, n counting the walked tiles
+    Ring kr, vr;
     auto issue_scores = [&](int n) {
-      const int s = n % S::kStages;
-      if (!warp_wait(k_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns)) return false;
+      if (!warp_wait(k_full + 8 * kr.stage, kr.parity, abort_flag, p.wait_limit_ns)) return false;
       if (leader) {
-        mma_scores<T, DP>(tmem + (n & 1) * kKeys, sbase, S::kOwnBlock, sbase + S::kK + s * S::kTile, S::kBlock, kKeys);
-        mma_commit(k_empty + 8 * s);
+        mma_scores<T, DP>(tmem + (n & 1) * kKeys, sbase, S::kOwnBlock, sbase + S::kK + kr.stage * S::kTile, S::kBlock,
+                          kKeys);
+        mma_commit(k_empty + 8 * kr.stage);
         mma_commit(s_full + 8 * (n & 1));
+        mbar_arrive(s_full + 8 * (n & 1));
       }
       __syncwarp();
+      kr.next(S::kStages);
       return true;
     };
     // the scores of two tiles are out before the first P is waited for, and tile n + 2's follow the
@@ -283,8 +304,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
                               (t1 >= tiles || issue_scores(1)));
     int n = 0, ahead = t1 < tiles ? walk.next(t1) : tiles;
     for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
-      const int s = n % S::kStages;
-      ok = warp_wait(v_full + 8 * s, (n / S::kStages) & 1, abort_flag, p.wait_limit_ns) &&
+      const int s = vr.stage;
+      ok = warp_wait(v_full + 8 * s, vr.parity, abort_flag, p.wait_limit_ns) &&
            warp_wait(p_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
       if (!ok) break;
       if (leader) {
@@ -295,6 +316,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         mma_commit(pv_done + 8 * (n % S::kStreams));
       }
       __syncwarp();
+      vr.next(S::kStages);
       if (ahead < tiles) {
         ok = issue_scores(n + 2);
         ahead = walk.next(ahead);
@@ -309,36 +331,24 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool warp_live = row0 + warp % 4 * 32 < rows;
     const ScoreConst k(p);
-    float* aux = reinterpret_cast<float*>(smem + S::kAux) + warp * 3 * kKeys;  // [3][64]: -x, -y, segment
     auto nth = [&](int t, int steps) {  // `steps` walked tiles on
       for (int e = 0; e < steps && t < tiles; ++e) t = walk.next(t);
       return t;
     };
     int t = nth(t0, stream);
-    if (walk.kinds != nullptr) fetch(t);
     float m = -INFINITY, l = 0.0f;
     bool dead = false;
     int n = stream;
+    Ring r{stream, 0}, slot{stream, 0};  // of this stream's tiles
     for (; t < tiles; n += S::kStreams) {
       const int next = nth(t, S::kStreams);
       const bool masked = walk.masked(t), first_tile = n == stream;
-      if (POS > 0 || masked) {
-        __syncwarp();
-        if constexpr (POS > 0) *reinterpret_cast<float2*>(aux + 2 * lane) = nx;
-        if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kKeys + 2 * lane) = ny;
-        if (masked) {  // -1: a key that no row sees (rows have ids >= 0, or -2)
-          const int64_t j = int64_t(t) * kKeys + 2 * lane;
-          *reinterpret_cast<int2*>(aux + 2 * kKeys + 2 * lane) =
-              make_int2(j < left ? max(-1, ns.x) : -1, j + 1 < left ? max(-1, ns.y) : -1);
-        }
-        __syncwarp();
-      }
-      fetch(next);
       bool bad = false;  // a masked tile whose V holds values that are no numbers
-      const unsigned char* vt = smem + S::kV + n % S::kStages * S::kTile;
+      const unsigned char* vt = smem + S::kV + r.stage * S::kTile;
+      const float* aux = reinterpret_cast<const float*>(smem + S::kAux) + slot.stage * 3 * kKeys;
       const uint32_t tmem_s = tmem + lanes + (n & 1) * kKeys, tmem_acc = tmem_o + lanes + stream * DP;
       if (masked) {
-        if (!dead) dead = !warp_wait(v_full + 8 * (n % S::kStages), (n / S::kStages) & 1, abort_flag, p.wait_limit_ns);
+        if (!dead) dead = !warp_wait(v_full + 8 * r.stage, r.parity, abort_flag, p.wait_limit_ns);
         bad = barrier_any(1 + stream, kAttnRows, !dead && tid < kKeys && row_not_finite<T, DP>(vt, S::kBlock, tid));
       }
       if (!dead) dead = !warp_wait(s_full + 8 * (n & 1), (n >> 1) & 1, abort_flag, p.wait_limit_ns);
@@ -412,6 +422,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       tc_fence_before();
       mbar_arrive(p_full + 8 * (n & 1));
       t = next;
+#pragma unroll
+      for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages), slot.next(S::kSlots);
     }
     // With two streams each takes half of the columns and adds what both have there.
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
