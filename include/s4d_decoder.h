@@ -114,7 +114,7 @@ S4D_API int s4d_attention_forward(const s4d_attention_args* args, void* stream);
  *   workspace  s4d_attention_backward_workspace_bytes(args) bytes, 16-byte aligned
  * No atomics: equal calls give equal bits.  Pairs that are not seen take no part, whatever q, k, v,
  * dout and the positions hold there; gradients of rows that see nothing or are seen by nothing are 0.
- * At most 262144 queries and keys. */
+ * At most 524288 queries and keys. */
 S4D_API size_t s4d_attention_backward_workspace_bytes(const s4d_attention_args* args);
 S4D_API int s4d_attention_backward(const s4d_attention_args* args, void* stream);
 

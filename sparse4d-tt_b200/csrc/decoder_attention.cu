@@ -72,7 +72,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t
 
 constexpr int64_t kMaxRows = int64_t(1) << 31;
 constexpr int kKeyTile = 64;       // keys of a forward tile
-constexpr int kBackwardTile = 32;  // queries or keys of a backward tile
+constexpr int kBackwardTile = 64;  // queries or keys of a backward tile
 
 // Checks of sizes and of the arguments that forward and backward share; fn names the entry point.
 int check_args(const char* fn, const s4d_attention_args* a) {
@@ -274,7 +274,7 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   const s4d_attention_args& a = *args;
   if (a.dtype != S4D_DTYPE_BF16) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for bf16");
   if (ceil_div(a.queries, kBackwardTile) > kAttnMaxTiles || ceil_div(a.keys, kBackwardTile) > kAttnMaxTiles)
-    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 262144 queries and keys");
+    S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 524288 queries and keys");
   if (a.batch == 0) return S4D_OK;
   if ((a.dk == nullptr) != (a.dv == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "dk and dv go together");
   if (!aligned_to(a.dout, 16) || !aligned_to(a.dq, 16) || !aligned_to(a.dk, 16) || !aligned_to(a.dv, 16) ||

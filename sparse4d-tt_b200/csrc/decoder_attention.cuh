@@ -519,7 +519,7 @@ struct AttnForwardMaps {
 int launch_attention_forward_d64(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
 int launch_attention_forward_d128(int dtype, int pos, const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st);
 
-// Maps of the backward kernels: boxes of 128 own rows (of the heads that share keys), and of 32 rows of a
+// Maps of the backward kernels: boxes of 128 own rows (of the heads that share keys), and of 64 rows of a
 // walked tile.
 struct AttnBackwardMaps {
   CUtensorMap q_rows, do_rows, k_rows, v_rows, q_tile, do_tile, k_tile, v_tile;

@@ -18,18 +18,21 @@
 // fp16's subnormal range.
 //
 // What bounds it: as in the forward pass the work per score in registers (one exponential, one more
-// special-function instruction with a 2-D distance, two with a cap, and about twenty others), so there
-// have to be row threads that are not waiting.  The walked axis goes in tiles of 32: S and dP then take
-// 64 tensor-memory columns, and two streams of four warps (four for dK and dV at D = 128, where one CTA
-// fills the SM's tensor memory) walk alternate tiles.  The sums dQ, dK and dV are linear in the tiles, so
-// the streams share them; the tensor cores take the tiles in order.
+// special-function instruction with a 2-D distance, two with a cap, and about twenty others), and the
+// turn-round of a tile: its dS has to be multiplied before the next scores can go over it, about 1,800
+// clocks in which its row threads wait.  So one CTA takes the SM's whole tensor memory: S and dP of a
+// tile of 64 (128 columns) for each of three streams of four row warps (two for dK and dV at D = 128),
+// which walk every third tile.  The sums dQ, dK and dV are linear in the tiles, so the streams share
+// them; the tensor cores take the tiles in order.  Tiles of 32 with two CTAs of two streams on an SM
+// measured 930 us for dQ and 1,180 us for dK and dV at 8,192 tokens, 16 heads (8 shared), D = 64: the
+// 128-row operand is read from shared memory once for each product, however few columns that has.
 #include "decoder_attention.cuh"
 
 namespace s4d {
 namespace {
 
 using T = __nv_bfloat16;
-constexpr int kCols = 32;  // rows of a walked tile
+constexpr int kCols = 64;  // rows of a walked tile
 
 // Waits until the sums hold every tile before tile n, whose turn it is next: the last tile of each other
 // stream (the own stream's is done, its scores' buffer is in use again).  acc_done[s] counts the tiles
@@ -47,17 +50,19 @@ template <int DP>
 struct Dq {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = 2, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStreams = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
   // a K tile is needed until its product with dS, a V tile only for dP
-  static constexpr int kKStages = DP == 64 ? 6 : 3, kVStages = DP == 64 ? 4 : 2;
+  static constexpr int kKStages = DP == 64 ? 6 : 5, kVStages = DP == 64 ? 4 : 3;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
   // with each K tile: -x, -y and segment of its keys
-  static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > 3 * kAttnRows * 4 ? kKStages * 3 * kCols * 4 : 3 * kAttnRows * 4;
+  // (at the end: the other streams' sums)
+  static constexpr int kSums = (kStreams - 1) * 3 * kAttnRows * 4;
+  static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > kSums ? kKStages * 3 * kCols * 4 : kSums;
   static constexpr int kBars = kAux + kAuxBytes;
   static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kStreams + 2;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
-  static constexpr uint32_t kTmem = 256;  // per stream S / dS 32, dP 32; dQ DP
+  static constexpr uint32_t kTmem = 512;  // per stream S / dS 64, dP 64; dQ DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -65,15 +70,15 @@ template <int DP>
 struct Dkv {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = DP == 64 ? 2 : 4, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
-  static constexpr int kStages = 6;  // of a Q and a dO tile
+  static constexpr int kStreams = DP == 64 ? 3 : 2, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStages = DP == 64 ? 6 : 4;  // of a Q and a dO tile
   static constexpr int kV = kOwn, kQ = kV + kOwn, kAux = kQ + kStages * 2 * kTile;
   // with each stage: -lse2, -delta, -x, -y, -slope2 and segment of its queries
   static constexpr int kBars = kAux + kStages * 6 * kCols * 4;
   static constexpr int kNumBars = 2 * kStages + 3 * kStreams + 2;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
-  static constexpr uint32_t kTmem = DP == 64 ? 256 : 512;  // per stream S / P 32, dP / dS 32; dV DP, dK DP
+  static constexpr uint32_t kTmem = 512;  // per stream S / P 64, dP / dS 64; dV DP, dK DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -174,7 +179,7 @@ __device__ __forceinline__ void store_row32(T* row, int col, int dim, const uint
 }
 
 template <int DP, int POS, bool CAP>
-__global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
+__global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
                         const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                         const AttnParams p) {
@@ -302,18 +307,26 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
   const int t0 = walk.first();
 
   if (warp == S::kWarps) {
-    // a key of the next tile a lane, loaded one tile ahead and written beside its K tile
-    float nx = 0.0f, ny = 0.0f;
-    int ns = 0;
+    // two keys of the next tile a lane, loaded one tile ahead and written beside its K tile
+    float2 nx = make_float2(0.0f, 0.0f), ny = nx;
+    int2 ns = make_int2(0, 0);
     auto fetch = [&](int t) {
       if (t >= tiles) return;
-      const int64_t j = int64_t(t) * kCols + lane, at = b * p.nk + j;
-      const bool in = j < valid;
-      ns = in ? 0 : -1;  // -1: a key that no row sees (rows have ids >= 0, or -2)
-      if (p.k_seg != nullptr && in) ns = max(-1, __ldg(p.k_seg + at));
+      const int64_t j = int64_t(t) * kCols + 2 * lane, at = b * p.nk + j;
+      const bool in0 = j < valid, in1 = j + 1 < valid;
+      ns = make_int2(in0 ? 0 : -1, in1 ? 0 : -1);  // -1: a key that no row sees (rows have ids >= 0, or -2)
+      if (p.k_seg != nullptr) {
+        if (in0) ns.x = max(-1, __ldg(p.k_seg + at));
+        if (in1) ns.y = max(-1, __ldg(p.k_seg + at + 1));
+      }
       if constexpr (POS > 0) {
-        nx = in ? -__ldg(p.k_pos + at * POS) : 0.0f;
-        if constexpr (POS > 1) ny = in ? -__ldg(p.k_pos + at * POS + 1) : 0.0f;
+        const float* kp = p.k_pos + at * POS;
+        nx.x = in0 ? -__ldg(kp) : 0.0f;
+        nx.y = in1 ? -__ldg(kp + POS) : 0.0f;
+        if constexpr (POS > 1) {
+          ny.x = in0 ? -__ldg(kp + 1) : 0.0f;
+          ny.y = in1 ? -__ldg(kp + POS + 1) : 0.0f;
+        }
       }
     };
     int n = 0;
@@ -328,10 +341,10 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
         break;
       }
       if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
-      float* aux = reinterpret_cast<float*>(smem + S::kAux) + kr.stage * 3 * kCols + lane;
-      if constexpr (POS > 0) aux[0] = nx;
-      if constexpr (POS > 1) aux[kCols] = ny;
-      reinterpret_cast<int*>(aux)[2 * kCols] = ns;
+      float* aux = reinterpret_cast<float*>(smem + S::kAux) + kr.stage * 3 * kCols + 2 * lane;
+      if constexpr (POS > 0) *reinterpret_cast<float2*>(aux) = nx;
+      if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kCols) = ny;
+      *reinterpret_cast<int2*>(aux + 2 * kCols) = ns;
       mbar_arrive(k_full + 8 * kr.stage);
       kr.next(S::kKStages);
       vr.next(S::kVStages);
@@ -366,13 +379,14 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
     bool ok = t0 >= tiles || !own_by_tma || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
     int ahead = t0;
     for (int e = 0; e < S::kStreams && ok && ahead < tiles; ++e, ahead = walk.next(ahead)) ok = issue_scores(e);
-    int n = 0;
-    for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
-      const int buf = n % S::kStreams;
-      if (!(ok = warp_wait(ds_full + 8 * buf, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns))) break;
+    bool any = false;
+    Ring turn;  // the stream whose tile is next
+    for (int t = t0; ok && t < tiles; t = walk.next(t), any = true, turn.next(S::kStreams)) {
+      const int buf = turn.stage;
+      if (!(ok = warp_wait(ds_full + 8 * buf, turn.parity, abort_flag, p.wait_limit_ns))) break;
       if (leader) {
         if (!(walk.masked(t) && skip[buf]))
-          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, n > 0);
+          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, any);
         mma_commit(k_empty + 8 * ka.stage);
         mma_commit(acc_done + 8 * buf);
       }
@@ -444,16 +458,18 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
     }
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if constexpr (POS > 0) {
-      // both streams' sums; o_full: no warp reads its keys' values any more
+      // all streams' sums; o_full: no warp reads its keys' values any more
       float* other = reinterpret_cast<float*>(smem + S::kAux);
-      if (stream == 1) {
+      if (stream > 0) {
 #pragma unroll
-        for (int e = 0; e < 3; ++e) other[e * kAttnRows + tid] = sums[e];
+        for (int e = 0; e < 3; ++e) other[((stream - 1) * 3 + e) * kAttnRows + tid] = sums[e];
       }
-      barrier_sync(3, S::kWarps * 32);
+      barrier_sync(1 + S::kStreams, S::kWarps * 32);
       if (stream == 0 && live && p.dslopes != nullptr) {
 #pragma unroll
-        for (int e = 0; e < 3; ++e) sums[e] += other[e * kAttnRows + tid];
+        for (int s = 0; s < S::kStreams - 1; ++s)
+#pragma unroll
+          for (int e = 0; e < 3; ++e) sums[e] += other[(s * 3 + e) * kAttnRows + tid];
         // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits, so
         // dS is off by P times that sum, and sum dS dist by that times sum P dist.
         p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
@@ -461,10 +477,8 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 2)
       }
     }
     if (!dead && warp_live) {
-#pragma unroll
-      for (int c0 = 0; c0 < DP / 32 / S::kStreams; ++c0) {
-        const int c = c0 + stream * (DP / 32 / S::kStreams);
-        if (c * 32 >= p.dim) break;
+      // dQ's columns in 32s, shared out among the streams
+      for (int c = stream; c * 32 < p.dim; c += S::kStreams) {
         uint32_t o[32];
         tmem_ld32_async(tmem_o + lanes + c * 32, o);
         tmem_ld_wait(o);
@@ -515,7 +529,7 @@ __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[16], const uint32
 }
 
 template <int DP, int POS, bool CAP>
-__global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
+__global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                          const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
                          const AttnParams p) {
@@ -603,26 +617,30 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
   };
 
   if (warp == S::kWarps) {
-    // a query of the next tile a lane, loaded one tile ahead and written beside its Q and dO tiles
-    float c_lse = 0.0f, c_delta = 0.0f, c_x = 0.0f, c_y = 0.0f, c_slope = 0.0f;
-    int c_seg = 0;
+    // two queries of the next tile a lane, loaded one tile ahead and written beside its Q and dO tiles
+    float2 c_lse, c_delta, c_x = make_float2(0.0f, 0.0f), c_y = c_x, c_slope = c_x;
+    int2 c_seg;
     auto fetch = [&](int hh, int t) {
       if (hh >= p.rep) return;
-      const int64_t i = int64_t(t) * kCols + lane;
-      const bool in = i < p.nq;
       const int h = g * p.rep + hh;
-      const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
-      const float l = in ? __ldg(p.lse + r) : -INFINITY;
-      c_lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
-      c_delta = in ? -p.delta[r] : 0.0f;
-      if constexpr (POS > 0) {
-        const float* qp = p.q_pos + (b * p.nq + i) * POS;
-        c_x = in ? -__ldg(qp) : 0.0f;
-        if constexpr (POS > 1) c_y = in ? -__ldg(qp + 1) : 0.0f;
-        c_slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
-      }
-      c_seg = in ? 0 : -1;  // -1: a query that sees no key here (keys have ids >= 0, or -2)
-      if (p.q_seg != nullptr && in) c_seg = max(-1, __ldg(p.q_seg + b * p.nq + i));
+      auto one = [&](int64_t i, float& lse, float& delta, float& x, float& y, float& slope, int& sg) {
+        const bool in = i < p.nq;
+        const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
+        const float l = in ? __ldg(p.lse + r) : -INFINITY;
+        lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
+        delta = in ? -p.delta[r] : 0.0f;
+        if constexpr (POS > 0) {
+          const float* qp = p.q_pos + (b * p.nq + i) * POS;
+          x = in ? -__ldg(qp) : 0.0f;
+          if constexpr (POS > 1) y = in ? -__ldg(qp + 1) : 0.0f;
+          slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
+        }
+        sg = in ? 0 : -1;  // -1: a query that sees no key here (keys have ids >= 0, or -2)
+        if (p.q_seg != nullptr && in) sg = max(-1, __ldg(p.q_seg + b * p.nq + i));
+      };
+      const int64_t i = int64_t(t) * kCols + 2 * lane;
+      one(i, c_lse.x, c_delta.x, c_x.x, c_y.x, c_slope.x, c_seg.x);
+      one(i + 1, c_lse.y, c_delta.y, c_x.y, c_y.y, c_slope.y, c_seg.y);
     };
     int n = 0, hh = work ? 0 : p.rep, t = t0;
     Ring r;
@@ -638,15 +656,15 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
           tma_load_4d(st + S::kTile + c * S::kBlock, &dom, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
         }
       }
-      float* aux = reinterpret_cast<float*>(smem + S::kAux) + r.stage * 6 * kCols + lane;
-      aux[0] = c_lse;
-      aux[kCols] = c_delta;
+      float* aux = reinterpret_cast<float*>(smem + S::kAux) + r.stage * 6 * kCols + 2 * lane;
+      *reinterpret_cast<float2*>(aux) = c_lse;
+      *reinterpret_cast<float2*>(aux + kCols) = c_delta;
       if constexpr (POS > 0) {
-        aux[2 * kCols] = c_x;
-        if constexpr (POS > 1) aux[3 * kCols] = c_y;
-        aux[4 * kCols] = c_slope;
+        *reinterpret_cast<float2*>(aux + 2 * kCols) = c_x;
+        if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + 3 * kCols) = c_y;
+        *reinterpret_cast<float2*>(aux + 4 * kCols) = c_slope;
       }
-      reinterpret_cast<int*>(aux)[5 * kCols] = c_seg;
+      *reinterpret_cast<int2*>(aux + 5 * kCols) = c_seg;
       mbar_arrive(full + 8 * r.stage);
       r.next(S::kStages);
       advance(hh, t);
@@ -678,15 +696,17 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
       ok = issue_scores(e);
       advance(ah, at);
     }
-    int n = 0, hh = work ? 0 : p.rep, t = t0;
+    int hh = work ? 0 : p.rep, t = t0;
+    bool any = false;
+    Ring turn;  // the stream whose tile is next
     while (ok && hh < p.rep) {
-      const int buf = n % S::kStreams;
-      if (!(ok = warp_wait(ds_full + 8 * buf, (n / S::kStreams) & 1, abort_flag, p.wait_limit_ns))) break;
+      const int buf = turn.stage;
+      if (!(ok = warp_wait(ds_full + 8 * buf, turn.parity, abort_flag, p.wait_limit_ns))) break;
       if (leader) {
         if (!(walk.masked(t) && skip[buf])) {
           const uint32_t d = tmem + buf * 2 * kCols, qt = sbase + S::kQ + ra.stage * 2 * S::kTile;
-          mma_accumulate<T, DP, kCols>(tmem_dv, d, qt + S::kTile, n > 0);
-          mma_accumulate<T, DP, kCols>(tmem_dk, d + kCols, qt, n > 0);
+          mma_accumulate<T, DP, kCols>(tmem_dv, d, qt + S::kTile, any);
+          mma_accumulate<T, DP, kCols>(tmem_dk, d + kCols, qt, any);
         }
         mma_commit(empty + 8 * ra.stage);
         mma_commit(acc_done + 8 * buf);
@@ -698,7 +718,8 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
         advance(ah, at);
       }
       advance(hh, t);
-      ++n;
+      any = true;
+      turn.next(S::kStreams);
     }
     if (leader) {
       mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
@@ -765,9 +786,8 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, DP == 64 ? 2 : 1)
     if (!dead) {
       // dV's and dK's columns in 32s, shared out among the streams
       const int64_t off = ((b * p.nk + (live ? key : 0)) * p.kv_heads + g) * p.dim;
-#pragma unroll
-      for (int c0 = 0; c0 < 2 * DP / 32 / S::kStreams; ++c0) {
-        const int c = c0 * S::kStreams + stream, col = c * 32 % DP;
+      for (int c = stream; c < 2 * DP / 32; c += S::kStreams) {
+        const int col = c * 32 % DP;
         const bool is_k = c * 32 >= DP;
         if (col >= p.dim) continue;
         uint32_t o[32];
