@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(1024) slope_sum_kernel(const float* rows, int 
 }
 
 size_t backward_workspace(const s4d_attention_args& a) {
-  const size_t rows = size_t(a.batch) * size_t(a.queries) * size_t(a.heads) * sizeof(float);
+  const size_t rows = size_t(a.batch) * size_t(a.heads);
   const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
-  return rows + (sum ? rows : 0);
+  return rows * size_t(ceil_div(a.queries, kRecordTile)) * kRecordBytes + (sum ? rows * size_t(a.queries) * sizeof(float) : 0);
 }
 
 }  // namespace
@@ -297,10 +297,9 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   p.dout = a.dout, p.do_sb = d.b, p.do_sn = d.n, p.do_sh = d.h;
   p.dq = a.dq, p.dk = a.dk, p.dv = a.dv;
   p.splits = 1;
-  p.delta = static_cast<float*>(a.workspace);
-  const int64_t rows = a.batch * a.queries;
+  p.records = static_cast<float*>(a.workspace);
   const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
-  p.dslopes = sum ? p.delta + rows * a.heads : a.dslopes;
+  p.dslopes = sum ? p.records + a.batch * a.heads * ceil_div(a.queries, kRecordTile) * (kRecordBytes / 4) : a.dslopes;
   p.dslopes_by_head = sum;
   cudaStream_t stm = static_cast<cudaStream_t>(stream);
   if (a.queries > 0 || a.keys > 0) {

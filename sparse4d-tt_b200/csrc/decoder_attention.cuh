@@ -48,12 +48,18 @@ struct AttnParams {
   float* part_lse;  // [splits, B, H, Nq]
   // backward
   void *dq, *dk, *dv;
-  float* delta;    // [B, H, Nq]
+  float* records;  // [B, H, query tiles of 64][6][64]: what dK and dV need of each query (see below)
   float* dslopes;  // [B, Nq, H], by head [B, H, Nq], or null
   int dslopes_by_head;
   int32_t* error_flag;
   unsigned long long wait_limit_ns;
 };
+
+// Query values of one head, written by the dQ kernel and copied a tile at a time by the dK, dV kernel:
+// -log2e lse (-inf: the query sees no key, or does not exist), -delta, x, y, -log2e slope, segment
+// (-1: sees nothing).
+constexpr int kRecordTile = 64, kRecordFields = 6;
+constexpr int kRecordBytes = kRecordTile * kRecordFields * 4;
 
 // ---- arithmetic ---------------------------------------------------------------------------------
 
@@ -152,9 +158,9 @@ __device__ __forceinline__ F2 tanh_rest(F2 acc, float k1) {
   return mul2(f2(rcp(a), rcp(b)), f2(2.0f));
 }
 
-// Distances of one point (x, y) to two points given by their negated coordinates.
+// Distances of one point, given by its negated coordinates (nx, ny), to two points.
 template <int POS>
-__device__ __forceinline__ F2 distance(F2 x, F2 y, F2 nx, F2 ny) {
+__device__ __forceinline__ F2 distance(F2 nx, F2 ny, F2 x, F2 y) {
   const F2 dx = add2(x, nx);
   float a, b;
   if constexpr (POS == 1) {
@@ -226,6 +232,22 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// N consecutive columns of this thread's lane.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
+  static_assert(N == 8 || N == 16 || N == 32, "one load");
+  if constexpr (N == 8) tmem_ld8_async(taddr, r);
+  if constexpr (N == 16) tmem_ld16_async(taddr, r);
+  if constexpr (N == 32) tmem_ld32_async(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[N]) {
+  static_assert(N == 8 || N == 16 || N == 32, "one store");
+  if constexpr (N == 8) tmem_st8(taddr, r);
+  if constexpr (N == 16) tmem_st16(taddr, r);
+  if constexpr (N == 32) tmem_st32(taddr, r);
+}
 
 // Shared-memory descriptors of a tile of 128-byte rows (64 16-bit elements) stored with the 128-byte
 // swizzle from a 1024-byte aligned base: start >> 4 in bits 0-13, descriptor version 1 in bits
@@ -352,6 +374,56 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   const bool ok = __all_sync(0xffffffffu, sleep_wait(bar, parity, abort_flag, limit_ns));
   tc_fence_after();
   return ok;
+}
+
+// ---- asynchronous copies of a walked tile's small values ----------------------------------------------
+
+// 4 bytes from global to shared memory without a register; copy_arrive arrives on `bar` once this
+// thread's copies so far have landed (an arrival that the barrier's count includes).
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void store4(uint32_t dst, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+}
+// `bytes` (a multiple of 16) between 16-byte aligned addresses, counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// The values of 64 keys of a tile, x[64], y[64] (POS) and segment[64] at shared-memory address dst, two
+// keys a lane of one warp: asynchronous, so that a warp may be several tiles ahead.  Key j of the tile
+// exists when j < left; what is past that is masked by segment -1 (rows have ids >= 0).  `bar`
+// counts two arrivals of every lane for them.
+constexpr uint32_t kKeyValueArrivals = 64;
+template <int POS>
+__device__ __forceinline__ void load_key_values(uint32_t dst, uint32_t bar, const float* k_pos, const int32_t* k_seg,
+                                                int64_t left) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = 2 * int(threadIdx.x & 31) + u;
+    const bool in = j < left;
+    if constexpr (POS > 0) {
+      if (in) {
+        copy4(dst + j * 4, k_pos + j * POS);
+        if constexpr (POS > 1) copy4(dst + 256 + j * 4, k_pos + j * POS + 1);
+      } else {
+        store4(dst + j * 4, 0u);
+        store4(dst + 256 + j * 4, 0u);
+      }
+    }
+    if (in && k_seg != nullptr)
+      copy4(dst + 512 + j * 4, k_seg + j);
+    else
+      store4(dst + 512 + j * 4, in ? 0u : 0xffffffffu);
+  }
+  copy_arrive(bar);
+  mbar_arrive(bar);  // for the plain stores
 }
 
 // ---- values that are no numbers behind a mask --------------------------------------------------------

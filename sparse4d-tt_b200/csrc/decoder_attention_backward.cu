@@ -5,7 +5,8 @@
 //   dQ = scale dX K,  dK = scale dX^T Q,  dV = P^T dO.
 //
 // Two kernels, so that nothing is added by atomics and equal calls give equal bits: one owns 128
-// query rows and walks the keys (dQ, dslopes and delta, which the second needs), one owns 128 keys of
+// query rows and walks the keys (dQ, dslopes, and a record of each query for
+// the second), one owns 128 keys of
 // a shared head and walks the query rows of every head that shares them (dK and dV).  That costs the
 // two score products and the exponential a second time (7 products instead of 5), and saves a pass
 // of fp32 additions over dQ in memory.  Both have the forward kernel's roles: one score row a thread, S and
@@ -20,29 +21,35 @@
 // What bounds it: as in the forward pass the work per score in registers (one exponential, one more
 // special-function instruction with a 2-D distance, two with a cap, and about twenty others), and the
 // turn-round of a tile: its dS has to be multiplied before the next scores can go over it, about 1,800
-// clocks in which its row threads wait.  So one CTA takes the SM's whole tensor memory: S and dP of a
-// tile of 64 (128 columns) for each of three streams of four row warps (two for dK and dV at D = 128),
-// which walk every third tile.  The sums dQ, dK and dV are linear in the tiles, so the streams share
-// them; the tensor cores take the tiles in order.  Tiles of 32 with two CTAs of two streams on an SM
-// measured 930 us for dQ and 1,180 us for dK and dV at 8,192 tokens, 16 heads (8 shared), D = 64: the
-// 128-row operand is read from shared memory once for each product, however few columns that has.
+// clocks.  So one CTA takes the SM's whole tensor memory: S and dP of three tiles of 64 (128 columns
+// each) for two streams of four row warps that walk alternate tiles, so that the next tile's scores are
+// there when a stream comes to it (two tiles for dK and dV at D = 128, whose sums take the other half).
+// The sums dQ, dK and dV are linear in the tiles, so the streams share them; the tensor cores take the
+// tiles in order.  KERNEL_VARIANTS
 #include "decoder_attention.cuh"
 
 namespace s4d {
 namespace {
 
 using T = __nv_bfloat16;
+#ifndef CHK
+#define CHK 16
+#endif
+#ifndef NST
+#define NST 3
+#endif
 constexpr int kCols = 64;  // rows of a walked tile
+constexpr int kChunk = CHK;  // of them a row thread holds in registers at a time (twice)
 
 // Waits until the sums hold every tile before tile n, whose turn it is next: the last tile of each other
-// stream (the own stream's is done, its scores' buffer is in use again).  acc_done[s] counts the tiles
-// of stream s; none after n can be in, so a parity is enough.
-template <int STREAMS>
+// score buffer (the own buffer's is done, it is in use again).  acc_done[s] counts the tiles of buffer
+// s; none after n can be in, so a parity is enough.
+template <int BUFFERS>
 __device__ __forceinline__ bool earlier_done(uint32_t acc_done, int n, volatile int* abort_flag, unsigned long long limit_ns) {
   bool ok = true;
 #pragma unroll
-  for (int e = 1; e < STREAMS; ++e)
-    if (n >= e) ok = ok && warp_wait(acc_done + 8 * ((n - e) % STREAMS), ((n - e) / STREAMS) & 1, abort_flag, limit_ns);
+  for (int e = 1; e < BUFFERS; ++e)
+    if (n >= e) ok = ok && warp_wait(acc_done + 8 * ((n - e) % BUFFERS), ((n - e) / BUFFERS) & 1, abort_flag, limit_ns);
   return ok;
 }
 
@@ -50,19 +57,19 @@ template <int DP>
 struct Dq {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStreams = NST, kBuffers = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
   // a K tile is needed until its product with dS, a V tile only for dP
   static constexpr int kKStages = DP == 64 ? 6 : 5, kVStages = DP == 64 ? 4 : 3;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
-  // with each K tile: -x, -y and segment of its keys
+  // with each K tile: x, y and segment of its keys
   // (at the end: the other streams' sums)
   static constexpr int kSums = (kStreams - 1) * 3 * kAttnRows * 4;
   static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > kSums ? kKStages * 3 * kCols * 4 : kSums;
   static constexpr int kBars = kAux + kAuxBytes;
-  static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kStreams + 2;
+  static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kBuffers + 3;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
-  static constexpr uint32_t kTmem = 512;  // per stream S / dS 64, dP 64; dQ DP
+  static constexpr uint32_t kTmem = 512;  // per buffer S / dS 64, dP 64; dQ DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -70,15 +77,15 @@ template <int DP>
 struct Dkv {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = DP == 64 ? 3 : 2, kWarps = 4 * kStreams, kThreads = (kWarps + 2) * 32;
+  static constexpr int kStreams = DP == 64 ? NST : 2, kBuffers = DP == 64 ? 3 : 2, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
   static constexpr int kStages = DP == 64 ? 6 : 4;  // of a Q and a dO tile
   static constexpr int kV = kOwn, kQ = kV + kOwn, kAux = kQ + kStages * 2 * kTile;
-  // with each stage: -lse2, -delta, -x, -y, -slope2 and segment of its queries
+  // with each stage: its queries' record
   static constexpr int kBars = kAux + kStages * 6 * kCols * 4;
-  static constexpr int kNumBars = 2 * kStages + 3 * kStreams + 2;
+  static constexpr int kNumBars = 2 * kStages + 3 * kBuffers + 3;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
-  static constexpr uint32_t kTmem = 512;  // per stream S / P 64, dP / dS 64; dV DP, dK DP
+  static constexpr uint32_t kTmem = 512;  // per buffer S / P 64, dP / dS 64; dV DP, dK DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -123,15 +130,15 @@ __device__ __forceinline__ uint32_t pack(F2 v) {
   return pack2<T>(a, b);
 }
 
-// One chunk of 16 keys of a query row.  aux arrays of a tile: -x, -y, segment.
-template <int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[16], const uint32_t (&pr)[16], uint32_t (&w)[8],
-                                         const ScoreConst& k, float slope2, float qx, float qy, int seg, float lse2,
+// One chunk of CH keys of a query row (qx, qy negated).  aux arrays of a tile: x, y, segment.
+template <int POS, bool CAP, bool MASKED, int CH>
+__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[CH], const uint32_t (&pr)[CH], uint32_t (&w)[CH / 2],
+                                         const ScoreConst& k, float slope2, float qx, float qy, int seg, bool sees, float lse2,
                                          float delta, const float* aux, float (&sums)[3]) {
   F2 r0 = f2(0.0f), r1 = r0, e1 = r0;
   const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), nlse2 = f2(-lse2), ndelta = f2(-delta);
 #pragma unroll
-  for (int j4 = 0; j4 < 16; j4 += 4) {
+  for (int j4 = 0; j4 < CH; j4 += 4) {
     float4 x4, y4;
     int4 s4;
     if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(aux + j4);
@@ -140,7 +147,7 @@ __device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[16], const uint32_
 #pragma unroll
     for (int u = 0; u < 4; u += 2) {
       bool seen0 = true, seen1 = true;
-      if constexpr (MASKED) seen0 = (u == 0 ? s4.x : s4.z) == seg, seen1 = (u == 0 ? s4.y : s4.w) == seg;
+      if constexpr (MASKED) seen0 = sees && (u == 0 ? s4.x : s4.z) == seg, seen1 = sees && (u == 0 ? s4.y : s4.w) == seg;
       F2 dist = f2(0.0f);
       if constexpr (POS > 0) dist = distance<POS>(x2, y2, half_of(x4, u), POS > 1 ? half_of(y4, u) : x2);
       const Terms t = score_terms<POS, CAP, MASKED>(pair_of(sr + j4 + u), k, nslope, dist, nlse2, pair_of(pr + j4 + u),
@@ -178,6 +185,22 @@ __device__ __forceinline__ void store_row32(T* row, int col, int dim, const uint
   }
 }
 
+template <int POS>
+__device__ __forceinline__ void write_record(const AttnParams& p, int b, int h, int64_t i, float nlse2, float ndelta, float x,
+                                             float y, float nslope2, int seg) {
+  const int64_t tiles = (p.nq + kRecordTile - 1) / kRecordTile;
+  float* r = p.records + ((int64_t(b) * p.heads + h) * tiles + i / kRecordTile) * (kRecordTile * kRecordFields) +
+             i % kRecordTile;
+  r[0] = nlse2;
+  r[kRecordTile] = ndelta;
+  if constexpr (POS > 0) {
+    r[2 * kRecordTile] = x;
+    r[3 * kRecordTile] = y;
+    r[4 * kRecordTile] = nslope2;
+  }
+  reinterpret_cast<int*>(r)[5 * kRecordTile] = seg;
+}
+
 template <int DP, int POS, bool CAP>
 __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
@@ -189,8 +212,8 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   const uint32_t k_full = sbase + S::kBars, k_empty = k_full + 8 * S::kKStages, v_full = k_empty + 8 * S::kKStages,
                  v_empty = v_full + 8 * S::kVStages, s_full = v_empty + 8 * S::kVStages,
-                 ds_full = s_full + 8 * S::kStreams, acc_done = ds_full + 8 * S::kStreams, o_full = acc_done + 8 * S::kStreams,
-                 own_full = o_full + 8;
+                 ds_full = s_full + 8 * S::kBuffers, acc_done = ds_full + 8 * S::kBuffers, o_full = acc_done + 8 * S::kBuffers,
+                 own_full = o_full + 8, scores_out = own_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip = abort_flag + 1;
@@ -211,19 +234,20 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kKStages; ++s) {
-      mbar_init(k_full + 8 * s, 33);  // the copy, and the lanes that write the keys' values
+      mbar_init(k_full + 8 * s, 1 + kKeyValueArrivals);  // the K tile, and the keys' values
       mbar_init(k_empty + 8 * s, 1);
     }
     for (int s = 0; s < S::kVStages; ++s) {
       mbar_init(v_full + 8 * s, 1);
       mbar_init(v_empty + 8 * s, 1);
     }
-    for (int s = 0; s < S::kStreams; ++s) {
+    for (int s = 0; s < S::kBuffers; ++s) {
       mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
       mbar_init(ds_full + 8 * s, kAttnRows);
       mbar_init(acc_done + 8 * s, 1);
     }
     mbar_init(o_full, 1);
+    mbar_init(scores_out, 1);
     mbar_init(own_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -254,16 +278,17 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   const int64_t out_row = (b * p.nq + i) * p.heads + h, lse_row = (int64_t(b) * p.heads + h) * p.nq + i;
   float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
   float lse2 = INFINITY, delta = 0.0f;  // a row without a key (or past the last): weights of 2^-inf
-  int seg = 0;
+  int seg = 0;       // without segments 0
+  bool sees = true;  // false: a negative id, which sees nothing
   if (warp < S::kWarps) {
     if constexpr (POS > 0) {
       slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
-      qx = __ldg(p.q_pos + (b * p.nq + i) * POS);
-      if constexpr (POS > 1) qy = __ldg(p.q_pos + (b * p.nq + i) * POS + 1);
+      qx = -__ldg(p.q_pos + (b * p.nq + i) * POS);  // negated: differences are sums
+      if constexpr (POS > 1) qy = -__ldg(p.q_pos + (b * p.nq + i) * POS + 1);
     }
     if (p.q_seg != nullptr) {
       seg = __ldg(p.q_seg + b * p.nq + i);
-      if (seg < 0) seg = -2;
+      sees = seg >= 0;
     }
     if (live) {
       const float l = __ldg(p.lse + lse_row);
@@ -281,7 +306,13 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
           for (int e = 0; e < 8; ++e) delta = fmaf(fo[e], fd[e], delta);
         }
       }
-      if (stream == 0) p.delta[lse_row] = delta;
+      if (stream == 0) write_record<POS>(p, b, h, i, -lse2, -delta, -qx, -qy, -slope2, sees ? seg : -1);
+    }
+    // queries that fill up the last tile of records
+    if (row0 + kAttnRows >= rows) {
+      const int64_t end = (p.nq + kRecordTile - 1) / kRecordTile * kRecordTile;
+      for (int64_t e = p.nq * rep + threadIdx.x; e < end * rep; e += S::kWarps * 32)
+        write_record<POS>(p, b, int(g * rep + e % rep), e / rep, -INFINITY, 0.0f, 0.0f, 0.0f, 0.0f, -1);
     }
   }
   if (!own_by_tma) {
@@ -303,35 +334,12 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_o = tmem + S::kStreams * 2 * kCols;
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + S::kBuffers * 2 * kCols;
   const int t0 = walk.first();
 
   if (warp == S::kWarps) {
-    // two keys of the next tile a lane, loaded one tile ahead and written beside its K tile
-    float2 nx = make_float2(0.0f, 0.0f), ny = nx;
-    int2 ns = make_int2(0, 0);
-    auto fetch = [&](int t) {
-      if (t >= tiles) return;
-      const int64_t j = int64_t(t) * kCols + 2 * lane, at = b * p.nk + j;
-      const bool in0 = j < valid, in1 = j + 1 < valid;
-      ns = make_int2(in0 ? 0 : -1, in1 ? 0 : -1);  // -1: a key that no row sees (rows have ids >= 0, or -2)
-      if (p.k_seg != nullptr) {
-        if (in0) ns.x = max(-1, __ldg(p.k_seg + at));
-        if (in1) ns.y = max(-1, __ldg(p.k_seg + at + 1));
-      }
-      if constexpr (POS > 0) {
-        const float* kp = p.k_pos + at * POS;
-        nx.x = in0 ? -__ldg(kp) : 0.0f;
-        nx.y = in1 ? -__ldg(kp + POS) : 0.0f;
-        if constexpr (POS > 1) {
-          ny.x = in0 ? -__ldg(kp + 1) : 0.0f;
-          ny.y = in1 ? -__ldg(kp + POS + 1) : 0.0f;
-        }
-      }
-    };
     int n = 0;
     Ring kr, vr;
-    fetch(t0);
     for (int t = t0; t < tiles; ++n) {
       // V first: its stage is free once dP is there, K's only after dQ
       if (n >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
@@ -341,15 +349,12 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
         break;
       }
       if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
-      float* aux = reinterpret_cast<float*>(smem + S::kAux) + kr.stage * 3 * kCols + 2 * lane;
-      if constexpr (POS > 0) *reinterpret_cast<float2*>(aux) = nx;
-      if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kCols) = ny;
-      *reinterpret_cast<int2*>(aux + 2 * kCols) = ns;
-      mbar_arrive(k_full + 8 * kr.stage);
+      const int64_t key = int64_t(t) * kCols, at = b * p.nk + key;
+      load_key_values<POS>(sbase + S::kAux + kr.stage * 3 * kCols * 4, k_full + 8 * kr.stage, p.k_pos + at * POS,
+                           p.k_seg != nullptr ? p.k_seg + at : nullptr, valid - key);
       kr.next(S::kKStages);
       vr.next(S::kVStages);
       t = walk.next(t);
-      fetch(t);
     }
     if (own_by_tma) mbar_wait(own_full, 0, nullptr);
     for (int e = max(0, n - S::kKStages); e < n; ++e)
@@ -358,47 +363,51 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
       mbar_wait(v_full + 8 * (e % S::kVStages), (e / S::kVStages) & 1, nullptr);
   } else if (warp == S::kWarps + 1) {
     const uint32_t leader = elect_one();
-    Ring ks, vs, ka;  // K and V of the next scores, K of the next product with dS
-    auto issue_scores = [&](int buf) {
-      if (!warp_wait(v_full + 8 * vs.stage, vs.parity, abort_flag, p.wait_limit_ns) ||
-          !warp_wait(k_full + 8 * ks.stage, ks.parity, abort_flag, p.wait_limit_ns))
-        return false;
+    Ring ks, vs, buf;
+    bool ok = t0 >= tiles || !own_by_tma || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
+    int n = 0;
+    for (int t = t0; ok && t < tiles; t = walk.next(t), ++n) {
+      // the buffer's last dS is multiplied (its parity is the one before this tile's)
+      ok = warp_wait(v_full + 8 * vs.stage, vs.parity, abort_flag, p.wait_limit_ns) &&
+           warp_wait(k_full + 8 * ks.stage, ks.parity, abort_flag, p.wait_limit_ns) &&
+           (n < S::kBuffers || warp_wait(acc_done + 8 * buf.stage, buf.parity ^ 1, abort_flag, p.wait_limit_ns));
+      if (!ok) break;
       if (leader) {
-        const uint32_t d = tmem + buf * 2 * kCols;
+        const uint32_t d = tmem + buf.stage * 2 * kCols;
         mma_scores<T, DP>(d + kCols, sbase + S::kDo, S::kOwnBlock, sbase + S::kV + vs.stage * S::kTile, S::kBlock, kCols);
         mma_commit(v_empty + 8 * vs.stage);
         mma_scores<T, DP>(d, sbase, S::kOwnBlock, sbase + S::kK + ks.stage * S::kTile, S::kBlock, kCols);
-        mma_commit(s_full + 8 * buf);
-        mbar_arrive(s_full + 8 * buf);
+        mma_commit(s_full + 8 * buf.stage);
+        mbar_arrive(s_full + 8 * buf.stage);
       }
       __syncwarp();
       ks.next(S::kKStages);
       vs.next(S::kVStages);
-      return true;
-    };
-    bool ok = t0 >= tiles || !own_by_tma || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
-    int ahead = t0;
-    for (int e = 0; e < S::kStreams && ok && ahead < tiles; ++e, ahead = walk.next(ahead)) ok = issue_scores(e);
-    bool any = false;
-    Ring turn;  // the stream whose tile is next
-    for (int t = t0; ok && t < tiles; t = walk.next(t), any = true, turn.next(S::kStreams)) {
-      const int buf = turn.stage;
-      if (!(ok = warp_wait(ds_full + 8 * buf, turn.parity, abort_flag, p.wait_limit_ns))) break;
+      buf.next(S::kBuffers);
+    }
+    if (leader) {
+      mma_commit(scores_out);  // also on the abort path: nothing may run once tensor memory is freed
+      mbar_wait(scores_out, 0, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == S::kWarps + 2) {
+    const uint32_t leader = elect_one();
+    Ring ka, buf;
+    bool ok = true, any = false;
+    for (int t = t0; ok && t < tiles; t = walk.next(t), any = true) {
+      if (!(ok = warp_wait(ds_full + 8 * buf.stage, buf.parity, abort_flag, p.wait_limit_ns))) break;
       if (leader) {
-        if (!(walk.masked(t) && skip[buf]))
-          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, any);
+        if (!(walk.masked(t) && skip[buf.stage]))
+          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf.stage * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, any);
+        mma_commit(acc_done + 8 * buf.stage);
         mma_commit(k_empty + 8 * ka.stage);
-        mma_commit(acc_done + 8 * buf);
       }
       __syncwarp();
       ka.next(S::kKStages);
-      if (ahead < tiles) {
-        ok = issue_scores(buf);
-        ahead = walk.next(ahead);
-      }
+      buf.next(S::kBuffers);
     }
     if (leader) {
-      mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
+      mma_commit(o_full);
       mbar_wait(o_full, 0, nullptr);
     }
     __syncwarp();
@@ -406,7 +415,6 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const bool warp_live = row0 + warp % 4 * 32 < rows;
     const ScoreConst k(p);
-    const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
     auto nth = [&](int t, int steps) {  // `steps` walked tiles on
       for (int e = 0; e < steps && t < tiles; ++e) t = walk.next(t);
       return t;
@@ -414,9 +422,9 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     int t = nth(t0, stream), n = stream;
     float sums[3] = {0.0f, 0.0f, 0.0f};  // sum dS, sum dS dist, sum P dist
     bool dead = false;
-    uint32_t turn = 0;  // parity of this stream's tiles
-    Ring r{stream, 0};  // stages of their K tiles
-    for (; t < tiles; n += S::kStreams, turn ^= 1) {
+    Ring r{stream, 0}, buf{stream, 0};  // K stages and score buffers of this stream's tiles
+    for (; t < tiles; n += S::kStreams) {
+      const uint32_t tmem_s = tmem + lanes + buf.stage * 2 * kCols;
       const int next = nth(t, S::kStreams);
       const bool masked = walk.masked(t);
       bool bad = false;  // a masked tile whose K holds values that are no numbers
@@ -426,35 +434,42 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
         if (!dead) dead = !warp_wait(k_full + 8 * r.stage, r.parity, abort_flag, p.wait_limit_ns);
         bad = barrier_any(1 + stream, kAttnRows, !dead && tid < kCols && row_not_finite<T, DP>(kt, S::kBlock, tid));
       }
-      if (!dead) dead = !warp_wait(s_full + 8 * stream, turn, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * buf.stage, buf.parity, abort_flag, p.wait_limit_ns);
       // only now: this tile's scores follow the product that read the flag's last value
-      if (masked && tid == 0) skip[stream] = bad;
+      if (masked && tid == 0) skip[buf.stage] = bad;
       if (!dead && warp_live) {
+        // the next chunk's loads are under way while one is computed
+        uint32_t sr[2][kChunk], pr[2][kChunk];
+        tmem_ld<kChunk>(tmem_s, sr[0]);
+        tmem_ld<kChunk>(tmem_s + kCols, pr[0]);
 #pragma unroll
-        for (int c = 0; c < kCols / 16; ++c) {
-          uint32_t sr[16], pr[16], w[8];
-          tmem_ld16_async(tmem_s + c * 16, sr);
-          tmem_ld16_async(tmem_s + kCols + c * 16, pr);
-          tmem_ld_wait(sr);
-          tmem_ld_wait(pr);
+        for (int c = 0; c < kCols / kChunk; ++c) {
+          uint32_t w[kChunk / 2];
+          tmem_ld_wait(sr[c & 1]);
+          tmem_ld_wait(pr[c & 1]);
+          if (c + 1 < kCols / kChunk) {
+            tmem_ld<kChunk>(tmem_s + (c + 1) * kChunk, sr[(c + 1) & 1]);
+            tmem_ld<kChunk>(tmem_s + kCols + (c + 1) * kChunk, pr[(c + 1) & 1]);
+          }
+          const float* cx = aux + c * kChunk;
           if (masked)
-            dq_chunk<POS, CAP, true>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, aux + c * 16, sums);
+            dq_chunk<POS, CAP, true>(sr[c & 1], pr[c & 1], w, k, slope2, qx, qy, seg, sees, lse2, delta, cx, sums);
           else
-            dq_chunk<POS, CAP, false>(sr, pr, w, k, slope2, qx, qy, seg, lse2, delta, aux + c * 16, sums);
-          tmem_st8(tmem_s + c * 8, w);
+            dq_chunk<POS, CAP, false>(sr[c & 1], pr[c & 1], w, k, slope2, qx, qy, seg, sees, lse2, delta, cx, sums);
+          tmem_st<kChunk / 2>(tmem_s + c * (kChunk / 2), w);
         }
         tmem_st_wait();
         if (bad) {
           // dQ is about to change outside the tensor cores
-          dead = !earlier_done<S::kStreams>(acc_done, n, abort_flag, p.wait_limit_ns);
+          dead = !earlier_done<S::kBuffers>(acc_done, n, abort_flag, p.wait_limit_ns);
           if (!dead) accumulate_nonzero<T, DP, kCols>(tmem_o + lanes, tmem_s, kt, n == 0);
         }
       }
       tc_fence_before();
-      mbar_arrive(ds_full + 8 * stream);
+      mbar_arrive(ds_full + 8 * buf.stage);
       t = next;
 #pragma unroll
-      for (int e = 0; e < S::kStreams; ++e) r.next(S::kKStages);
+      for (int e = 0; e < S::kStreams; ++e) r.next(S::kKStages), buf.next(S::kBuffers);
     }
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if constexpr (POS > 0) {
@@ -495,14 +510,14 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
 }
 
-// One chunk of 16 query columns of a key's row.  aux arrays of a tile: -lse2, -delta, -x, -y, -slope2, segment.
-template <int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[16], const uint32_t (&pr)[16], uint32_t (&wp)[8],
-                                          uint32_t (&wd)[8], const ScoreConst& k, float kx, float ky, int seg,
+// One chunk of CH query columns of a key's row (kx, ky negated).  aux: the queries' record.
+template <int POS, bool CAP, bool MASKED, int CH>
+__device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[CH], const uint32_t (&pr)[CH], uint32_t (&wp)[CH / 2],
+                                          uint32_t (&wd)[CH / 2], const ScoreConst& k, float kx, float ky, int seg, bool sees,
                                           const float* aux) {
   const F2 x2 = f2(kx), y2 = f2(ky);
 #pragma unroll
-  for (int j4 = 0; j4 < 16; j4 += 4) {
+  for (int j4 = 0; j4 < CH; j4 += 4) {
     const float4 l4 = *reinterpret_cast<const float4*>(aux + j4);
     const float4 d4 = *reinterpret_cast<const float4*>(aux + kCols + j4);
     float4 x4, y4, sl4;
@@ -514,7 +529,7 @@ __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[16], const uint32
 #pragma unroll
     for (int u = 0; u < 4; u += 2) {
       bool seen0 = true, seen1 = true;
-      if constexpr (MASKED) seen0 = (u == 0 ? s4.x : s4.z) == seg, seen1 = (u == 0 ? s4.y : s4.w) == seg;
+      if constexpr (MASKED) seen0 = sees && (u == 0 ? s4.x : s4.z) == seg, seen1 = sees && (u == 0 ? s4.y : s4.w) == seg;
       F2 dist = f2(0.0f), nslope = dist;
       if constexpr (POS > 0) {
         dist = distance<POS>(x2, y2, half_of(x4, u), POS > 1 ? half_of(y4, u) : x2);
@@ -538,8 +553,8 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   const uint32_t full = sbase + S::kBars, empty = full + 8 * S::kStages, s_full = empty + 8 * S::kStages,
-                 ds_full = s_full + 8 * S::kStreams, own_full = ds_full + 8 * S::kStreams, acc_done = own_full + 8,
-                 o_full = acc_done + 8 * S::kStreams;
+                 ds_full = s_full + 8 * S::kBuffers, own_full = ds_full + 8 * S::kBuffers, acc_done = own_full + 8,
+                 o_full = acc_done + 8 * S::kBuffers, scores_out = o_full + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kCtl);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip = abort_flag + 1;
@@ -559,16 +574,17 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(full + 8 * s, 33);  // the copies, and the lanes that write the queries' values
+      mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, 1);
     }
-    for (int s = 0; s < S::kStreams; ++s) {
+    for (int s = 0; s < S::kBuffers; ++s) {
       mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
       mbar_init(ds_full + 8 * s, kAttnRows);
       mbar_init(acc_done + 8 * s, 1);
     }
     mbar_init(own_full, 1);
     mbar_init(o_full, 1);
+    mbar_init(scores_out, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (tiles > 0) {
@@ -594,20 +610,22 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   const int64_t key = key0 + tid;
   const bool live = key < p.nk;
   float kx = 0.0f, ky = 0.0f;
-  // keys past the valid length match nothing (-2), nor do negative ids; without segments valid keys are 0
-  int seg = -2;
+  int seg = 0;                // without segments 0
+  bool sees = key < valid;  // false: past the valid length, or a negative id: seen by nothing
   if (warp < S::kWarps && live) {
-    if (key < valid) seg = p.k_seg != nullptr ? __ldg(p.k_seg + b * p.nk + key) : 0;
-    if (seg < 0) seg = -2;
+    if (p.k_seg != nullptr) {
+      seg = __ldg(p.k_seg + b * p.nk + key);
+      sees = sees && seg >= 0;
+    }
     if constexpr (POS > 0) {
-      kx = __ldg(p.k_pos + (b * p.nk + key) * POS);
-      if constexpr (POS > 1) ky = __ldg(p.k_pos + (b * p.nk + key) * POS + 1);
+      kx = -__ldg(p.k_pos + (b * p.nk + key) * POS);  // negated: differences are sums
+      if constexpr (POS > 1) ky = -__ldg(p.k_pos + (b * p.nk + key) * POS + 1);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_dv = tmem + S::kStreams * 2 * kCols, tmem_dk = tmem_dv + DP;
+  const uint32_t tmem = *tmem_slot, tmem_dv = tmem + S::kBuffers * 2 * kCols, tmem_dk = tmem_dv + DP;
   const int t0 = walk.first();
   const bool work = t0 < tiles;
   // the walk is repeated for every head: (head, tile) pairs in order
@@ -617,128 +635,92 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   };
 
   if (warp == S::kWarps) {
-    // two queries of the next tile a lane, loaded one tile ahead and written beside its Q and dO tiles
-    float2 c_lse, c_delta, c_x = make_float2(0.0f, 0.0f), c_y = c_x, c_slope = c_x;
-    int2 c_seg;
-    auto fetch = [&](int hh, int t) {
-      if (hh >= p.rep) return;
-      const int h = g * p.rep + hh;
-      auto one = [&](int64_t i, float& lse, float& delta, float& x, float& y, float& slope, int& sg) {
-        const bool in = i < p.nq;
-        const int64_t r = (int64_t(b) * p.heads + h) * p.nq + i;
-        const float l = in ? __ldg(p.lse + r) : -INFINITY;
-        lse = l == -INFINITY ? -INFINITY : -l * kLog2e;  // no key seen: weights of 2^-inf
-        delta = in ? -p.delta[r] : 0.0f;
-        if constexpr (POS > 0) {
-          const float* qp = p.q_pos + (b * p.nq + i) * POS;
-          x = in ? -__ldg(qp) : 0.0f;
-          if constexpr (POS > 1) y = in ? -__ldg(qp + 1) : 0.0f;
-          slope = in ? -__ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e : 0.0f;
-        }
-        sg = in ? 0 : -1;  // -1: a query that sees no key here (keys have ids >= 0, or -2)
-        if (p.q_seg != nullptr && in) sg = max(-1, __ldg(p.q_seg + b * p.nq + i));
-      };
-      const int64_t i = int64_t(t) * kCols + 2 * lane;
-      one(i, c_lse.x, c_delta.x, c_x.x, c_y.x, c_slope.x, c_seg.x);
-      one(i + 1, c_lse.y, c_delta.y, c_x.y, c_y.y, c_slope.y, c_seg.y);
-    };
-    int n = 0, hh = work ? 0 : p.rep, t = t0;
-    Ring r;
-    fetch(hh, t);
-    while (hh < p.rep) {
-      if (n >= S::kStages && !warp_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
-      if (lane == 0) {
-        const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile;
-        mbar_expect_tx(full + 8 * r.stage, 2 * S::kTile);
+    if (lane == 0) {
+      int n = 0, hh = work ? 0 : p.rep, t = t0;
+      Ring r;
+      const int64_t query_tiles = (p.nq + kRecordTile - 1) / kRecordTile;
+      for (; hh < p.rep; advance(hh, t), ++n) {
+        if (n >= S::kStages && !sleep_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+        const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile, bar = full + 8 * r.stage;
+        const int h = g * p.rep + hh;
+        mbar_expect_tx(bar, 2 * S::kTile + kRecordBytes);
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-          tma_load_4d(st + c * S::kBlock, &qm, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
-          tma_load_4d(st + S::kTile + c * S::kBlock, &dom, full + 8 * r.stage, c * 64, g * p.rep + hh, t * kCols, b);
+          tma_load_4d(st + c * S::kBlock, &qm, bar, c * 64, h, t * kCols, b);
+          tma_load_4d(st + S::kTile + c * S::kBlock, &dom, bar, c * 64, h, t * kCols, b);
         }
+        bulk_load(sbase + S::kAux + r.stage * kRecordBytes,
+                  p.records + ((int64_t(b) * p.heads + h) * query_tiles + t) * (kRecordTile * kRecordFields), kRecordBytes,
+                  bar);
+        r.next(S::kStages);
       }
-      float* aux = reinterpret_cast<float*>(smem + S::kAux) + r.stage * 6 * kCols + 2 * lane;
-      *reinterpret_cast<float2*>(aux) = c_lse;
-      *reinterpret_cast<float2*>(aux + kCols) = c_delta;
-      if constexpr (POS > 0) {
-        *reinterpret_cast<float2*>(aux + 2 * kCols) = c_x;
-        if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + 3 * kCols) = c_y;
-        *reinterpret_cast<float2*>(aux + 4 * kCols) = c_slope;
-      }
-      *reinterpret_cast<int2*>(aux + 5 * kCols) = c_seg;
-      mbar_arrive(full + 8 * r.stage);
-      r.next(S::kStages);
-      advance(hh, t);
-      fetch(hh, t);
-      ++n;
+      if (tiles > 0) mbar_wait(own_full, 0, nullptr);
+      for (int e = max(0, n - S::kStages); e < n; ++e)
+        mbar_wait(full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
     }
-    if (tiles > 0) mbar_wait(own_full, 0, nullptr);
-    for (int e = max(0, n - S::kStages); e < n; ++e)
-      mbar_wait(full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
   } else if (warp == S::kWarps + 1) {
     const uint32_t leader = elect_one();
-    Ring rs, ra;  // the tile of the next scores, and of the next products with P and dS
-    auto issue_scores = [&](int buf) {
-      if (!warp_wait(full + 8 * rs.stage, rs.parity, abort_flag, p.wait_limit_ns)) return false;
+    Ring r, buf;
+    bool ok = !work || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
+    int n = 0, hh = work ? 0 : p.rep, t = t0;
+    for (; ok && hh < p.rep; advance(hh, t), ++n) {
+      // the buffer's last P and dS are multiplied (its parity is the one before this tile's)
+      ok = warp_wait(full + 8 * r.stage, r.parity, abort_flag, p.wait_limit_ns) &&
+           (n < S::kBuffers || warp_wait(acc_done + 8 * buf.stage, buf.parity ^ 1, abort_flag, p.wait_limit_ns));
+      if (!ok) break;
       if (leader) {
-        const uint32_t d = tmem + buf * 2 * kCols, qt = sbase + S::kQ + rs.stage * 2 * S::kTile;
+        const uint32_t d = tmem + buf.stage * 2 * kCols, qt = sbase + S::kQ + r.stage * 2 * S::kTile;
         mma_scores<T, DP>(d, sbase, S::kOwnBlock, qt, S::kBlock, kCols);
         mma_scores<T, DP>(d + kCols, sbase + S::kV, S::kOwnBlock, qt + S::kTile, S::kBlock, kCols);
-        mma_commit(s_full + 8 * buf);
-        mbar_arrive(s_full + 8 * buf);
+        mma_commit(s_full + 8 * buf.stage);
+        mbar_arrive(s_full + 8 * buf.stage);
       }
       __syncwarp();
-      rs.next(S::kStages);
-      return true;
-    };
-    bool ok = !work || warp_wait(own_full, 0, abort_flag, p.wait_limit_ns);
-    int ah = work ? 0 : p.rep, at = t0;
-    for (int e = 0; e < S::kStreams && ok && ah < p.rep; ++e) {
-      ok = issue_scores(e);
-      advance(ah, at);
+      r.next(S::kStages);
+      buf.next(S::kBuffers);
     }
+    if (leader) {
+      mma_commit(scores_out);  // also on the abort path: nothing may run once tensor memory is freed
+      mbar_wait(scores_out, 0, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == S::kWarps + 2) {
+    const uint32_t leader = elect_one();
+    Ring r, buf;
+    bool ok = true, any = false;
     int hh = work ? 0 : p.rep, t = t0;
-    bool any = false;
-    Ring turn;  // the stream whose tile is next
-    while (ok && hh < p.rep) {
-      const int buf = turn.stage;
-      if (!(ok = warp_wait(ds_full + 8 * buf, turn.parity, abort_flag, p.wait_limit_ns))) break;
+    for (; ok && hh < p.rep; advance(hh, t), any = true) {
+      if (!(ok = warp_wait(ds_full + 8 * buf.stage, buf.parity, abort_flag, p.wait_limit_ns))) break;
       if (leader) {
-        if (!(walk.masked(t) && skip[buf])) {
-          const uint32_t d = tmem + buf * 2 * kCols, qt = sbase + S::kQ + ra.stage * 2 * S::kTile;
+        if (!(walk.masked(t) && skip[buf.stage])) {
+          const uint32_t d = tmem + buf.stage * 2 * kCols, qt = sbase + S::kQ + r.stage * 2 * S::kTile;
           mma_accumulate<T, DP, kCols>(tmem_dv, d, qt + S::kTile, any);
           mma_accumulate<T, DP, kCols>(tmem_dk, d + kCols, qt, any);
         }
-        mma_commit(empty + 8 * ra.stage);
-        mma_commit(acc_done + 8 * buf);
+        mma_commit(acc_done + 8 * buf.stage);
+        mma_commit(empty + 8 * r.stage);
       }
       __syncwarp();
-      ra.next(S::kStages);
-      if (ah < p.rep) {
-        ok = issue_scores(buf);
-        advance(ah, at);
-      }
-      advance(hh, t);
-      any = true;
-      turn.next(S::kStreams);
+      r.next(S::kStages);
+      buf.next(S::kBuffers);
     }
     if (leader) {
-      mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
+      mma_commit(o_full);
       mbar_wait(o_full, 0, nullptr);
     }
     __syncwarp();
   } else {
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
     const ScoreConst k(p);
-    const uint32_t tmem_s = tmem + lanes + stream * 2 * kCols;
     auto skip_tiles = [&](int& hh, int& t, int steps) {
       for (int e = 0; e < steps && hh < p.rep; ++e) advance(hh, t);
     };
     int hh = work ? 0 : p.rep, t = t0, n = stream;
     skip_tiles(hh, t, stream);
     bool dead = false;
-    uint32_t turn = 0;  // parity of this stream's tiles
-    Ring r{stream, 0};  // their stages
-    for (; hh < p.rep; n += S::kStreams, turn ^= 1) {
+    Ring r{stream, 0}, buf{stream, 0};  // stages and score buffers of this stream's tiles
+    for (; hh < p.rep; n += S::kStreams) {
+      const uint32_t tmem_s = tmem + lanes + buf.stage * 2 * kCols;
       const bool masked = walk.masked(t);
       bool bad = false;  // a masked tile whose Q or dO holds values that are no numbers
       const unsigned char *qt = smem + S::kQ + r.stage * 2 * S::kTile, *dot = qt + S::kTile;
@@ -748,28 +730,33 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
         bad = barrier_any(1 + stream, kAttnRows,
                           !dead && tid < 2 * kCols && row_not_finite<T, DP>(tid < kCols ? qt : dot, S::kBlock, tid % kCols));
       }
-      if (!dead) dead = !warp_wait(s_full + 8 * stream, turn, abort_flag, p.wait_limit_ns);
+      if (!dead) dead = !warp_wait(s_full + 8 * buf.stage, buf.parity, abort_flag, p.wait_limit_ns);
       // only now: this tile's scores follow the products that read the flag's last value
-      if (masked && tid == 0) skip[stream] = bad;
+      if (masked && tid == 0) skip[buf.stage] = bad;
       if (!dead) {
+        uint32_t sr[2][kChunk], pr[2][kChunk];
+        tmem_ld<kChunk>(tmem_s, sr[0]);
+        tmem_ld<kChunk>(tmem_s + kCols, pr[0]);
 #pragma unroll
-        for (int c = 0; c < kCols / 16; ++c) {
-          uint32_t sr[16], pr[16], wp[8], wd[8];
-          tmem_ld16_async(tmem_s + c * 16, sr);
-          tmem_ld16_async(tmem_s + kCols + c * 16, pr);
-          tmem_ld_wait(sr);
-          tmem_ld_wait(pr);
+        for (int c = 0; c < kCols / kChunk; ++c) {
+          uint32_t wp[kChunk / 2], wd[kChunk / 2];
+          tmem_ld_wait(sr[c & 1]);
+          tmem_ld_wait(pr[c & 1]);
+          if (c + 1 < kCols / kChunk) {
+            tmem_ld<kChunk>(tmem_s + (c + 1) * kChunk, sr[(c + 1) & 1]);
+            tmem_ld<kChunk>(tmem_s + kCols + (c + 1) * kChunk, pr[(c + 1) & 1]);
+          }
           if (masked)
-            dkv_chunk<POS, CAP, true>(sr, pr, wp, wd, k, kx, ky, seg, aux + c * 16);
+            dkv_chunk<POS, CAP, true>(sr[c & 1], pr[c & 1], wp, wd, k, kx, ky, seg, sees, aux + c * kChunk);
           else
-            dkv_chunk<POS, CAP, false>(sr, pr, wp, wd, k, kx, ky, seg, aux + c * 16);
-          tmem_st8(tmem_s + c * 8, wp);
-          tmem_st8(tmem_s + kCols + c * 8, wd);
+            dkv_chunk<POS, CAP, false>(sr[c & 1], pr[c & 1], wp, wd, k, kx, ky, seg, sees, aux + c * kChunk);
+          tmem_st<kChunk / 2>(tmem_s + c * (kChunk / 2), wp);
+          tmem_st<kChunk / 2>(tmem_s + kCols + c * (kChunk / 2), wd);
         }
         tmem_st_wait();
         if (bad) {
           // dV and dK are about to change outside the tensor cores
-          dead = !earlier_done<S::kStreams>(acc_done, n, abort_flag, p.wait_limit_ns);
+          dead = !earlier_done<S::kBuffers>(acc_done, n, abort_flag, p.wait_limit_ns);
           if (!dead) {
             accumulate_nonzero<T, DP, kCols>(tmem_dv + lanes, tmem_s, dot, n == 0);
             accumulate_nonzero<T, DP, kCols>(tmem_dk + lanes, tmem_s + kCols, qt, n == 0);
@@ -777,10 +764,10 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
         }
       }
       tc_fence_before();
-      mbar_arrive(ds_full + 8 * stream);
+      mbar_arrive(ds_full + 8 * buf.stage);
       skip_tiles(hh, t, S::kStreams);
 #pragma unroll
-      for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages);
+      for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages), buf.next(S::kBuffers);
     }
     if (!dead && work) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if (!dead) {

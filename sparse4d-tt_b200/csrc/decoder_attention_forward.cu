@@ -42,7 +42,7 @@ struct Fwd {
   static constexpr int kWarps = 4 * kStreams;          // row threads; then the TMA and the tensor-core warp
   static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kK = kQ, kV = kK + kStages * kTile, kAux = kV + kStages * kTile;
-  // negated x, y and segment of a tile's keys (after the last tile: m and l of the rows).  A slot is read
+  // x, y and segment of a tile's keys (after the last tile: m and l of the rows).  A slot is read
   // until the tile's P is there, so it is free for tile n once V of tile n - 1 has found a free stage: one
   // slot more than stages.  Then barriers; tensor-memory slot, abort, skip[2]
   static constexpr int kSlots = kStages + 1;
@@ -57,7 +57,7 @@ struct Fwd {
 // 32 scores of a row, in base 2, and their maximum.
 template <int POS, bool CAP, bool MASKED>
 __device__ __forceinline__ void scores(uint32_t (&r)[32], const ScoreConst& k, float slope2, float qx, float qy,
-                                       int seg, const float* aux, float& mx) {
+                                       int seg, bool sees, const float* aux, float& mx) {
   const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), k1 = f2(k.k1), c = f2(k.c), nc = f2(-k.c);
 #pragma unroll
   for (int j4 = 0; j4 < 32; j4 += 4) {
@@ -71,16 +71,16 @@ __device__ __forceinline__ void scores(uint32_t (&r)[32], const ScoreConst& k, f
       const F2 acc = f2(__uint_as_float(r[j4 + u]), __uint_as_float(r[j4 + u + 1]));
       F2 s = CAP ? fma2(nc, tanh_rest(acc, k.k1), c) : mul2(acc, k1);
       if constexpr (POS > 0) {
-        const F2 nx = u == 0 ? f2(x4.x, x4.y) : f2(x4.z, x4.w);
-        F2 ny = nx;
-        if constexpr (POS > 1) ny = u == 0 ? f2(y4.x, y4.y) : f2(y4.z, y4.w);
-        s = fma2(nslope, distance<POS>(x2, y2, nx, ny), s);
+        const F2 kx = u == 0 ? f2(x4.x, x4.y) : f2(x4.z, x4.w);
+        F2 ky = kx;
+        if constexpr (POS > 1) ky = u == 0 ? f2(y4.x, y4.y) : f2(y4.z, y4.w);
+        s = fma2(nslope, distance<POS>(x2, y2, kx, ky), s);
       }
       float a, b;
       split(s, a, b);
       if constexpr (MASKED) {
-        a = (u == 0 ? s4.x : s4.z) == seg ? a : -INFINITY;
-        b = (u == 0 ? s4.y : s4.w) == seg ? b : -INFINITY;
+        a = sees && (u == 0 ? s4.x : s4.z) == seg ? a : -INFINITY;
+        b = sees && (u == 0 ? s4.y : s4.w) == seg ? b : -INFINITY;
       }
       mx = max3(mx, a, b);
       r[j4 + u] = __float_as_uint(a);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(k_full + 8 * s, 33);  // the copy, and the lanes that write the keys' values
+      mbar_init(k_full + 8 * s, 1 + kKeyValueArrivals);  // the K tile, and the keys' values
       mbar_init(k_empty + 8 * s, 1);
       mbar_init(v_full + 8 * s, 1);
       mbar_init(v_empty + 8 * s, 1);
@@ -155,36 +155,11 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   TileWalk walk{nullptr, tiles, int(max(int64_t(0), min(int64_t(tiles), valid / kKeys - first)))};
   const bool q_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
   const int64_t left = valid - first * kKeys;  // keys of this part and after it
-  // The TMA warp's lanes: two keys of a tile each, into registers (one tile ahead) and then into a
-  // slot beside the tiles
-  float2 nx = make_float2(0.0f, 0.0f), ny = nx;
-  int2 ns = make_int2(0, 0);
-  auto fetch = [&](int t) {
-    if (t >= tiles) return;
-    const int64_t j = int64_t(t) * kKeys + 2 * lane, at = b * p.nk + first * kKeys + j;
-    const bool in0 = j < left, in1 = j + 1 < left;
-    ns = make_int2(in0 ? 0 : -1, in1 ? 0 : -1);  // -1: a key that no row sees (rows have ids >= 0, or -2)
-    if (p.k_seg != nullptr) {
-      if (in0) ns.x = max(-1, __ldg(p.k_seg + at));
-      if (in1) ns.y = max(-1, __ldg(p.k_seg + at + 1));
-    }
-    if constexpr (POS > 0) {
-      const float* kp = p.k_pos + at * POS;
-      nx.x = in0 ? -__ldg(kp) : 0.0f;
-      nx.y = in1 ? -__ldg(kp + POS) : 0.0f;
-      if constexpr (POS > 1) {
-        ny.x = in0 ? -__ldg(kp + 1) : 0.0f;
-        ny.y = in1 ? -__ldg(kp + POS + 1) : 0.0f;
-      }
-    }
-  };
   auto load_k = [&](int s, int slot, int t) {
     if (lane == 0) load_tile<DP, kKeys>(sbase + S::kK + s * S::kTile, &km, k_full + 8 * s, g, int((first + t) * kKeys), b);
-    float* aux = reinterpret_cast<float*>(smem + S::kAux) + slot * 3 * kKeys + 2 * lane;
-    if constexpr (POS > 0) *reinterpret_cast<float2*>(aux) = nx;
-    if constexpr (POS > 1) *reinterpret_cast<float2*>(aux + kKeys) = ny;
-    *reinterpret_cast<int2*>(aux + 2 * kKeys) = ns;
-    mbar_arrive(k_full + 8 * s);
+    const int64_t key = int64_t(t) * kKeys, at = b * p.nk + first * kKeys + key;
+    load_key_values<POS>(sbase + S::kAux + slot * 3 * kKeys * 4, k_full + 8 * s, p.k_pos + at * POS,
+                         p.k_seg != nullptr ? p.k_seg + at : nullptr, left - key);
   };
   auto load_v = [&](int s, int t) {
     if (lane == 0) load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, int((first + t) * kKeys), b);
@@ -200,11 +175,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     }
     // without segments every tile is walked: the first loads need not wait for the other warps
     if (p.q_seg == nullptr) {
-      fetch(0);
       for (; loaded < min(S::kStages, tiles); ++loaded) {
-        load_v(loaded, loaded);
         load_k(loaded, loaded, loaded);
-        fetch(loaded + 1);
+        load_v(loaded, loaded);
       }
     }
   }
@@ -221,16 +194,17 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
   const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
   float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
-  int seg = 0;  // own segment: -2 (matches nothing) or >= 0; without segments 0
+  int seg = 0;  // own segment; without segments 0
+  bool sees = true;  // false: a negative id, which sees nothing
   if (warp < S::kWarps) {
     if constexpr (POS > 0) {
       slope2 = __ldg(p.slopes + b * p.sl_b + i * p.sl_n + h * p.sl_h) * kLog2e;
-      qx = __ldg(p.q_pos + (b * p.nq + i) * POS);
-      if constexpr (POS > 1) qy = __ldg(p.q_pos + (b * p.nq + i) * POS + 1);
+      qx = -__ldg(p.q_pos + (b * p.nq + i) * POS);  // negated: differences are sums
+      if constexpr (POS > 1) qy = -__ldg(p.q_pos + (b * p.nq + i) * POS + 1);
     }
     if (p.q_seg != nullptr) {
       seg = __ldg(p.q_seg + b * p.nq + i);
-      if (seg < 0) seg = -2;
+      sees = seg >= 0;
     }
   }
   // Q where TMA cannot gather it: 16-byte pieces, zero past the last row and column, in the swizzled
@@ -257,7 +231,6 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   if (warp == S::kWarps) {
     int n = loaded, t = loaded > 0 ? loaded : t0;
     Ring r{loaded % S::kStages, uint32_t(loaded / S::kStages) & 1}, slot{loaded, 0};
-    if (loaded == 0) fetch(t);
     for (; t < tiles; ++n) {
       const bool again = n >= S::kStages;
       if (again && !warp_wait(k_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
@@ -271,7 +244,6 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       r.next(S::kStages);
       slot.next(S::kSlots);
       t = walk.next(t);
-      fetch(t);
     }
     if (q_by_tma) mbar_wait(q_full, 0, nullptr);
     for (int e = max(0, n - S::kStages); e < n; ++e) {
@@ -362,9 +334,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
           tmem_ld32_async(tmem_s, r0);
           tmem_ld_wait(r0);
           if (masked)
-            scores<POS, CAP, true>(r0, k, slope2, qx, qy, seg, aux, mx);
+            scores<POS, CAP, true>(r0, k, slope2, qx, qy, seg, sees, aux, mx);
           else
-            scores<POS, CAP, false>(r0, k, slope2, qx, qy, seg, aux, mx);
+            scores<POS, CAP, false>(r0, k, slope2, qx, qy, seg, sees, aux, mx);
           tmem_st32(tmem_s, r0);
           tmem_ld32_async(tmem_s + 32, r1);
           tmem_ld_wait(r1);
@@ -374,14 +346,14 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
           tmem_ld_wait(r0);
           tmem_ld_wait(r1);
           if (masked)
-            scores<POS, CAP, true>(r0, k, slope2, qx, qy, seg, aux, mx);
+            scores<POS, CAP, true>(r0, k, slope2, qx, qy, seg, sees, aux, mx);
           else
-            scores<POS, CAP, false>(r0, k, slope2, qx, qy, seg, aux, mx);
+            scores<POS, CAP, false>(r0, k, slope2, qx, qy, seg, sees, aux, mx);
         }
         if (masked)
-          scores<POS, CAP, true>(r1, k, slope2, qx, qy, seg, aux + 32, mx);
+          scores<POS, CAP, true>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
         else
-          scores<POS, CAP, false>(r1, k, slope2, qx, qy, seg, aux + 32, mx);
+          scores<POS, CAP, false>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
         const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
         const bool any_grow = __any_sync(0xffffffffu, grow);
         if (!first_tile && (any_grow || bad))  // O is about to change outside the tensor cores
