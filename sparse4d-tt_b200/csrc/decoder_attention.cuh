@@ -376,6 +376,15 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return ok;
 }
 
+// One arrival for a whole (converged) warp, after its tensor-memory stores: a barrier takes arrivals one
+// at a time, and 128 of them are a visible part of a tile's turn-round.
+constexpr uint32_t kRowWarps = kAttnRows / 32;  // arrivals of a stream's row threads
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // ---- asynchronous copies of a walked tile's small values ----------------------------------------------
 
 // 4 bytes from global to shared memory without a register; copy_arrive arrives on `bar` once this
@@ -399,8 +408,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // The values of 64 keys of a tile, x[64], y[64] (POS) and segment[64] at shared-memory address dst, two
 // keys a lane of one warp: asynchronous, so that a warp may be several tiles ahead.  Key j of the tile
 // exists when j < left; what is past that is masked by segment -1 (rows have ids >= 0).  `bar`
-// counts two arrivals of every lane for them.
-constexpr uint32_t kKeyValueArrivals = 64;
+// counts kKeyValueArrivals arrivals for them.
+constexpr uint32_t kKeyValueArrivals = 33;
 template <int POS>
 __device__ __forceinline__ void load_key_values(uint32_t dst, uint32_t bar, const float* k_pos, const int32_t* k_seg,
                                                 int64_t left) {
@@ -423,7 +432,8 @@ __device__ __forceinline__ void load_key_values(uint32_t dst, uint32_t bar, cons
       store4(dst + 512 + j * 4, in ? 0u : 0xffffffffu);
   }
   copy_arrive(bar);
-  mbar_arrive(bar);  // for the plain stores
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);  // for the plain stores
 }
 
 // ---- values that are no numbers behind a mask --------------------------------------------------------

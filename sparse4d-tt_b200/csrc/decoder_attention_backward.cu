@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     }
     for (int s = 0; s < S::kBuffers; ++s) {
       mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
-      mbar_init(ds_full + 8 * s, kAttnRows);
+      mbar_init(ds_full + 8 * s, kRowWarps);
       mbar_init(acc_done + 8 * s, 1);
     }
     mbar_init(o_full, 1);
@@ -465,8 +465,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
           if (!dead) accumulate_nonzero<T, DP, kCols>(tmem_o + lanes, tmem_s, kt, n == 0);
         }
       }
-      tc_fence_before();
-      mbar_arrive(ds_full + 8 * buf.stage);
+      warp_arrive(ds_full + 8 * buf.stage);
       t = next;
 #pragma unroll
       for (int e = 0; e < S::kStreams; ++e) r.next(S::kKStages), buf.next(S::kBuffers);
@@ -579,7 +578,7 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     }
     for (int s = 0; s < S::kBuffers; ++s) {
       mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the tile's values
-      mbar_init(ds_full + 8 * s, kAttnRows);
+      mbar_init(ds_full + 8 * s, kRowWarps);
       mbar_init(acc_done + 8 * s, 1);
     }
     mbar_init(own_full, 1);
@@ -763,8 +762,7 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
           }
         }
       }
-      tc_fence_before();
-      mbar_arrive(ds_full + 8 * buf.stage);
+      warp_arrive(ds_full + 8 * buf.stage);
       skip_tiles(hh, t, S::kStreams);
 #pragma unroll
       for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages), buf.next(S::kBuffers);

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full + 8 * s, 2);  // the products, and the warp that saw the keys' values
-      mbar_init(p_full + 8 * s, kAttnRows);
+      mbar_init(p_full + 8 * s, kRowWarps);
       mbar_init(pv_done + 8 * s, 1);
     }
     mbar_init(o_full, 1);
@@ -391,8 +391,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         tmem_st_wait();
         if (bad && !dead) accumulate_nonzero<T, DP, kKeys>(tmem_acc, tmem_s, vt, first_tile);
       }
-      tc_fence_before();
-      mbar_arrive(p_full + 8 * (n & 1));
+      warp_arrive(p_full + 8 * (n & 1));
       t = next;
 #pragma unroll
       for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages), slot.next(S::kSlots);
