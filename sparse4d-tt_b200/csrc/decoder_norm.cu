@@ -10,12 +10,18 @@
 // the deviations from it (no cancellation for rows far from zero) are reduced by shuffles and,
 // for W > 1, through shared memory.
 //
-// The sums over rows for dw and db stay in registers: a block keeps its columns and walks the rows
-// with the stride of a grid that just fills the SMs, adds its row groups through shared memory
+// A block keeps the weight and bias of its columns in registers and walks the rows with the stride of a grid
+// that just fills the SMs, the next row's loads under way during one row's sums (not in the backward
+// pass of f32 rows, where registers are short).  Reading the parameters again for every row costs more
+// than the rows: 16,384 x 4,096 bf16 forward 69 us against 49 us.
+//
+// The sums over rows for dw and db stay in registers: a block adds its row groups through shared memory
 // and writes one fp32 partial row per block; a second launch adds the partial rows in block order.
 // Small inputs (up to 2048 rows and 2^20 values, which stay in the L2 cache) need no second launch: more
 // blocks of the same one each read 8 columns of x and dy again and add them over all rows.
 // No atomics: the order of every addition depends on the sizes alone.
+#include <algorithm>
+
 #include "decoder_types.cuh"
 
 namespace s4d {
@@ -89,69 +95,81 @@ __device__ __forceinline__ void load_param(const void* p, bool f32, int col, flo
 
 // Chunk k of a thread covers columns [col, col + VEC), col = (k * 32 W + thread of the group) VEC.
 template <typename T, int W, int VEC, int K>
-__global__ void __launch_bounds__(Group<W>::kThreads) norm_forward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(Group<W>::kThreads, 1) norm_forward_kernel(const NormParams p) {
+  constexpr int R = Group<W>::kRows;
   __shared__ float red[2][Group<W>::kWarps];
-  const int gt = threadIdx.x % (32 * W);
-  const int64_t row = int64_t(blockIdx.x) * Group<W>::kRows + threadIdx.x / (32 * W);
-  const bool live = row < p.rows;
-  if (W == 1 && !live) return;  // whole warps: no block barrier below
-  const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.x_ld;
-  float v[K][VEC];
-  float s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
+  const int group = threadIdx.x / (32 * W), gt = threadIdx.x % (32 * W);
+  constexpr bool kHold = W < 32;  // 1024 threads have 64 registers: they read the parameters again
+  float w[K][VEC], b[K][VEC];
+  auto load_params = [&](int k) {
     const int col = (k * 32 * W + gt) * VEC;
-    if (live && col < p.width) {
-      load_vec<T, VEC>(xr + col, v[k]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[k][i] = 0.0f;
-    }
+    for (int i = 0; i < VEC; ++i) w[k][i] = 1.0f, b[k][i] = 0.0f;
+    if (col < p.width && p.weight != nullptr) load_param<T, VEC>(p.weight, p.param_f32, col, w[k]);
+    if (col < p.width && p.bias != nullptr) load_param<T, VEC>(p.bias, p.param_f32, col, b[k]);
+  };
+  if (kHold) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_params(k);
   }
+  RawVec<T, VEC> raw[K];
+  auto load_row = [&](int64_t row) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.x_ld;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s += v[k][i];
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * 32 * W + gt) * VEC;
+      if (row < p.rows && col < p.width)
+        raw[k].load(xr + col);
+      else
+        raw[k].clear();
+    }
+  };
   const float inv = 1.0f / float(p.width);
-  const float mean = group_sum<W>(s, red[0]) * inv;
-  float q = 0.0f;
+  const int64_t step = int64_t(gridDim.x) * R;
+  if (kHold) load_row(int64_t(blockIdx.x) * R + group);
+  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += step) {
+    const int64_t row = base + group;
+    const bool live = row < p.rows;
+    if (!kHold) load_row(row);
+    float v[K][VEC];
+    float s = 0.0f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if ((k * 32 * W + gt) * VEC < p.width) {
+    for (int k = 0; k < K; ++k) {
+      raw[k].widen(v[k]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = v[k][i] - mean;
-        q = fmaf(d, d, q);
+      for (int i = 0; i < VEC; ++i) s += v[k][i];
+    }
+    if (kHold && base + step < p.rows) load_row(row + step);
+    const float mean = group_sum<W>(s, red[0]) * inv;
+    float q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if ((k * 32 * W + gt) * VEC < p.width) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float d = v[k][i] - mean;
+          q = fmaf(d, d, q);
+        }
       }
     }
-  }
-  const float rstd = 1.0f / sqrtf(group_sum<W>(q, red[1]) * inv + p.eps);
-  if (!live) return;
-  if (gt == 0 && p.mean != nullptr) {
-    p.mean[row] = mean;
-    p.rstd[row] = rstd;
-  }
-  T* yr = static_cast<T*>(p.y) + row * p.y_ld;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (k * 32 * W + gt) * VEC;
-    if (col >= p.width) break;
-    float o[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = (v[k][i] - mean) * rstd;
-    if (p.weight != nullptr) {
-      float w[VEC];
-      load_param<T, VEC>(p.weight, p.param_f32, col, w);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] *= w[i];
+    // red[0] is free again behind this sum's barrier, red[1] behind the next row's first
+    const float rstd = 1.0f / sqrtf(group_sum<W>(q, red[1]) * inv + p.eps);
+    if (!live) continue;
+    if (gt == 0 && p.mean != nullptr) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
     }
-    if (p.bias != nullptr) {
-      float b[VEC];
-      load_param<T, VEC>(p.bias, p.param_f32, col, b);
+    T* yr = static_cast<T*>(p.y) + row * p.y_ld;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i] += b[i];
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * 32 * W + gt) * VEC;
+      if (col >= p.width) break;
+      if (!kHold) load_params(k);
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = fmaf((v[k][i] - mean) * rstd, w[k][i], b[k][i]);
+      store_vec<T, VEC>(yr + col, o);
     }
-    store_vec<T, VEC>(yr + col, o);
   }
 }
 
@@ -192,52 +210,90 @@ __device__ __forceinline__ void sum_columns(const NormParams& p, int block) {
 }
 
 template <typename T, int W, int VEC, int K>
-__global__ void __launch_bounds__(Group<W>::kThreads) norm_backward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(Group<W>::kThreads, 1) norm_backward_kernel(const NormParams p) {
   if (int(blockIdx.x) >= p.row_blocks) {
     sum_columns<T, Group<W>::kThreads>(p, int(blockIdx.x) - p.row_blocks);
     return;
   }
   constexpr int R = Group<W>::kRows;
   __shared__ float red[2][2][Group<W>::kWarps];  // two sums, two buffers: one barrier a row
-  // partial sums of the block's other row groups, one 32-column-wide slice of a warp at a time
+  // at the end: partial sums of the block's row groups, a chunk at a time
   __shared__ float join[R > 1 ? 2 * R * 32 * W * VEC : 1];
   const int group = threadIdx.x / (32 * W), gt = threadIdx.x % (32 * W);
   griddep_launch_dependents();  // the reduction waits for this whole launch before it reads
   float w[K][VEC], aw[K][VEC], ab[K][VEC];
+  auto load_weight = [&](int k) {
+    const int col = (k * 32 * W + gt) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) w[k][i] = 1.0f;
+    if (p.weight != nullptr && col < p.width) load_param<T, VEC>(p.weight, p.param_f32, col, w[k]);
+  };
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int col = (k * 32 * W + gt) * VEC;
-    if (p.weight != nullptr && col < p.width) {
-      load_param<T, VEC>(p.weight, p.param_f32, col, w[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) w[k][i] = 1.0f;
-    }
+    if (W < 32) load_weight(k);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) aw[k][i] = 0.0f, ab[k][i] = 0.0f;
   }
   const float inv = 1.0f / float(p.width);
   int buf = 0;
-  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += int64_t(p.row_blocks) * R, buf ^= 1) {
-    const int64_t row = base + group;
-    const bool live = row < p.rows;
-    const int64_t r = live ? row : 0;
-    const T* xr = static_cast<const T*>(p.x) + r * p.x_ld;
-    const T* dyr = static_cast<const T*>(p.dy) + r * p.dy_ld;
-    float n[K][VEC], g[K][VEC];
+  // the next row's loads under way during this row's sums, where the registers allow it
+  constexpr bool kAhead = sizeof(T) == 2 && W < 16 && (VEC == 8 || K == 8);
+  RawVec<T, VEC> rx[K], rd[K];
+  auto load_row = [&](int64_t row) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.x_ld;
+    const T* dyr = static_cast<const T*>(p.dy) + row * p.dy_ld;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int col = (k * 32 * W + gt) * VEC;
-      if (live && col < p.width) {
-        load_vec<T, VEC>(xr + col, n[k]);
-        load_vec<T, VEC>(dyr + col, g[k]);
+      if (row < p.rows && col < p.width) {
+        rx[k].load(xr + col);
+        rd[k].load(dyr + col);
+      } else {
+        rx[k].clear();
+        rd[k].clear();
       }
     }
-    const float mean = __ldg(p.mean + r), rstd = __ldg(p.rstd + r);
+  };
+  const int64_t step = int64_t(p.row_blocks) * R;
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto load_stats = [&](int64_t row) {
+    if (row >= p.rows) return;
+    next_mean = __ldg(p.mean + row);
+    next_rstd = __ldg(p.rstd + row);
+  };
+  load_stats(int64_t(blockIdx.x) * R + group);
+  if (kAhead) load_row(int64_t(blockIdx.x) * R + group);
+  for (int64_t base = int64_t(blockIdx.x) * R; base < p.rows; base += step, buf ^= 1) {
+    const int64_t row = base + group;
+    const bool live = row < p.rows;
+    const int64_t r = live ? row : 0;
+    float n[K][VEC], g[K][VEC];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        rx[k].widen(n[k]);
+        rd[k].widen(g[k]);
+      }
+      if (base + step < p.rows) load_row(row + step);
+    } else {
+      const T* xr = static_cast<const T*>(p.x) + r * p.x_ld;
+      const T* dyr = static_cast<const T*>(p.dy) + r * p.dy_ld;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int col = (k * 32 * W + gt) * VEC;
+        if (live && col < p.width) {
+          load_vec<T, VEC>(xr + col, n[k]);
+          load_vec<T, VEC>(dyr + col, g[k]);
+        }
+      }
+    }
+    const float mean = next_mean, rstd = next_rstd;
+    load_stats(row + step);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const bool in = live && (k * 32 * W + gt) * VEC < p.width;
+      if (W == 32) load_weight(k);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float nn = in ? (n[k][i] - mean) * rstd : 0.0f, d = in ? g[k][i] : 0.0f;
@@ -345,45 +401,80 @@ int warps_for(int64_t width) {
 
 int rows_per_block(int w) { return w < 8 ? 8 / w : 1; }
 
-// Blocks of the backward launch: enough to fill the SMs at the registers its threads need (16
-// warps an SM: two blocks of 256 threads, one of 512 or 1024), fewer when there are fewer rows.
-int64_t backward_blocks(int64_t rows, int64_t width) {
+// Partial rows of dw and db at most: the blocks of a backward launch that fills the SMs (at most four of 256
+// threads an SM, one of 512 or 1024).
+int64_t most_row_blocks(int64_t rows, int64_t width) {
   const int w = warps_for(width), r = rows_per_block(w);
-  const int64_t need = (rows + r - 1) / r;
-  const int64_t fill = int64_t(device_sms()) * (w <= 8 ? 2 : 1);
+  const int64_t need = (rows + r - 1) / r, fill = int64_t(device_sms()) * (w <= 8 ? 4 : 1);
   return need < fill ? need : fill;
 }
 
+// Blocks of `kernel` that fill the device at once; the SMs' share is asked once per device and kernel.
+template <typename Kern>
+int64_t filling_blocks(Kern kernel, int threads, int (&cache)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  int each = dev >= 0 && dev < 64 ? cache[dev] : 0;
+  if (each == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, threads, 0) != cudaSuccess || each < 1) {
+      cudaGetLastError();
+      each = 1;
+    }
+    if (dev >= 0 && dev < 64) cache[dev] = each;
+  }
+  return int64_t(device_sms()) * each;
+}
+
 // Whether dw and db are summed by the backward launch itself: while x and dy stay in the L2 cache and a
-// thread adds at most 64 rows.  900 x 256 f32: one launch of 4.9 us against 4.5 + 2.9 us.
+// thread adds at most 64 rows.  900 x 256 f32: one launch of 6.0 us against 4.5 + 4.7 us.
 bool sums_in_one_launch(int64_t rows, int64_t width) { return rows <= 2048 && rows * width <= (1 << 20); }
 
+// The forward launch; the backward launch, and into p.row_blocks how many partial rows it writes (with
+// `columns` more blocks that sum columns).
 template <typename T, int W, int VEC, int K>
-int launch_norm(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
-  const dim3 grid{static_cast<unsigned>(blocks)};
+int launch_norm(bool backward, NormParams& p, int64_t columns, cudaStream_t st) {
+  static int cache[2][64] = {};
+  constexpr int kThreads = Group<W>::kThreads;
+  const int64_t need = (p.rows + Group<W>::kRows - 1) / Group<W>::kRows;
   if (backward) {
-    norm_backward_kernel<T, W, VEC, K><<<grid, Group<W>::kThreads, 0, st>>>(p);
+    const int64_t fill = filling_blocks(norm_backward_kernel<T, W, VEC, K>, kThreads, cache[1]);
+    p.row_blocks = int(std::min(std::min(need, fill), most_row_blocks(p.rows, p.width)));
+    norm_backward_kernel<T, W, VEC, K><<<dim3(unsigned(p.row_blocks + columns)), kThreads, 0, st>>>(p);
     return cuda_check(cudaGetLastError(), "norm_backward_kernel launch");
   }
-  norm_forward_kernel<T, W, VEC, K><<<grid, Group<W>::kThreads, 0, st>>>(p);
+  const int64_t fill = filling_blocks(norm_forward_kernel<T, W, VEC, K>, kThreads, cache[0]);
+  norm_forward_kernel<T, W, VEC, K><<<dim3(unsigned(std::min(need, fill))), kThreads, 0, st>>>(p);
   return cuda_check(cudaGetLastError(), "norm_forward_kernel launch");
 }
 
 template <typename T, int VEC>
-int dispatch_width(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
+int dispatch_width(bool backward, NormParams& p, int64_t columns, cudaStream_t st) {
   constexpr int K = kEpt / VEC;
-  switch (warps_for(p.width)) {
-    case 1:
-      // narrow rows: only as many chunks as the width needs (a decoder row of 256 is half of 512)
-      if constexpr (K > 1) {
-        if (p.width <= 32 * kEpt / 2) return launch_norm<T, 1, VEC, K / 2>(backward, p, blocks, st);
-      }
-      return launch_norm<T, 1, VEC, K>(backward, p, blocks, st);
-    case 2: return launch_norm<T, 2, VEC, K>(backward, p, blocks, st);
-    case 4: return launch_norm<T, 4, VEC, K>(backward, p, blocks, st);
-    case 8: return launch_norm<T, 8, VEC, K>(backward, p, blocks, st);
-    case 16: return launch_norm<T, 16, VEC, K>(backward, p, blocks, st);
-    default: return launch_norm<T, 32, VEC, K>(backward, p, blocks, st);
+  if constexpr (VEC == 1) {
+    // Rows that cannot be read as vectors are read an element at a time: half as many a thread and twice the
+    // warps keep more of them under way (7,213 x 1,001 f16 forward 13.7 against 12.4 us, backward
+    // 26.9 against 17.5 us).
+    if (p.width <= 256) return launch_norm<T, 1, 1, 8>(backward, p, columns, st);
+    switch (warps_for(p.width)) {
+      case 1: return launch_norm<T, 2, 1, 8>(backward, p, columns, st);
+      case 2: return launch_norm<T, 4, 1, 8>(backward, p, columns, st);
+      case 4: return launch_norm<T, 8, 1, 8>(backward, p, columns, st);
+      case 8: return launch_norm<T, 16, 1, 8>(backward, p, columns, st);
+      case 16: return launch_norm<T, 32, 1, 8>(backward, p, columns, st);
+      default: return launch_norm<T, 32, 1, 16>(backward, p, columns, st);
+    }
+  } else {
+    switch (warps_for(p.width)) {
+      case 1:
+        // narrow rows: only as many chunks as the width needs (a decoder row of 256 is half of 512)
+        if (p.width <= 32 * kEpt / 2) return launch_norm<T, 1, VEC, K / 2>(backward, p, columns, st);
+        return launch_norm<T, 1, VEC, K>(backward, p, columns, st);
+      case 2: return launch_norm<T, 2, VEC, K>(backward, p, columns, st);
+      case 4: return launch_norm<T, 4, VEC, K>(backward, p, columns, st);
+      case 8: return launch_norm<T, 8, VEC, K>(backward, p, columns, st);
+      case 16: return launch_norm<T, 16, VEC, K>(backward, p, columns, st);
+      default: return launch_norm<T, 32, VEC, K>(backward, p, columns, st);
+    }
   }
 }
 
@@ -392,18 +483,18 @@ bool vector_rows(const void* p, int64_t ld, int size) {
 }
 
 template <typename T>
-int dispatch_vector(bool backward, const NormParams& p, int64_t blocks, cudaStream_t st) {
+int dispatch_vector(bool backward, NormParams& p, int64_t columns, cudaStream_t st) {
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = p.width % VEC == 0 && vector_rows(p.x, p.x_ld, sizeof(T)) && vector_rows(p.y, p.y_ld, sizeof(T)) &&
                    vector_rows(p.dy, p.dy_ld, sizeof(T)) && vector_rows(p.weight, 0, 4) && vector_rows(p.bias, 0, 4);
-  return vec ? dispatch_width<T, VEC>(backward, p, blocks, st) : dispatch_width<T, 1>(backward, p, blocks, st);
+  return vec ? dispatch_width<T, VEC>(backward, p, columns, st) : dispatch_width<T, 1>(backward, p, columns, st);
 }
 
-int dispatch_type(bool backward, int dtype, const NormParams& p, int64_t blocks, cudaStream_t st) {
+int dispatch_type(bool backward, int dtype, NormParams& p, int64_t columns, cudaStream_t st) {
   switch (dtype) {
-    case S4D_DTYPE_F32: return dispatch_vector<float>(backward, p, blocks, st);
-    case S4D_DTYPE_BF16: return dispatch_vector<__nv_bfloat16>(backward, p, blocks, st);
-    default: return dispatch_vector<__half>(backward, p, blocks, st);
+    case S4D_DTYPE_F32: return dispatch_vector<float>(backward, p, columns, st);
+    case S4D_DTYPE_BF16: return dispatch_vector<__nv_bfloat16>(backward, p, columns, st);
+    default: return dispatch_vector<__half>(backward, p, columns, st);
   }
 }
 
@@ -469,13 +560,12 @@ int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void* weight,
   p.x = x, p.x_ld = x_ld, p.weight = weight, p.bias = bias, p.y = y, p.y_ld = y_ld;
   p.mean = mean, p.rstd = rstd, p.rows = rows, p.width = int(width), p.eps = eps;
   p.param_f32 = param_dtype == S4D_DTYPE_F32;
-  const int r = rows_per_block(warps_for(width));
-  return dispatch_type(false, dtype, p, (rows + r - 1) / r, static_cast<cudaStream_t>(stream));
+  return dispatch_type(false, dtype, p, 0, static_cast<cudaStream_t>(stream));
 }
 
 size_t s4d_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
   if (rows <= 0 || width <= 0 || width > kNormMaxWidth || rows > 0x7fffffff || sums_in_one_launch(rows, width)) return 0;
-  return size_t(backward_blocks(rows, width)) * 2 * size_t(width) * sizeof(float);
+  return size_t(most_row_blocks(rows, width)) * 2 * size_t(width) * sizeof(float);
 }
 
 int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype, const void* weight,
@@ -491,7 +581,7 @@ int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
   if (!aligned_to(dy, size) || !aligned_to(x, size) || !aligned_to(dx, size) || !aligned_to(weight, psize) ||
       !aligned_to(dweight, psize) || !aligned_to(dbias, psize) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
     return fail(S4D_ERR_INVALID_ARG, "s4d_norm_backward: misaligned pointer");
-  const int64_t blocks = rows > 0 ? backward_blocks(rows, width) : 0;
+  int blocks = 0;  // partial rows
   const bool one = sums_in_one_launch(rows, width);
   if (sums && rows > 0 && !one &&
       (workspace == nullptr || !aligned_to(workspace, 16) ||
@@ -504,22 +594,23 @@ int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld
     p.mean = const_cast<float*>(mean), p.rstd = const_cast<float*>(rstd), p.rows = rows, p.width = int(width);
     p.param_f32 = param_dtype == S4D_DTYPE_F32;
     p.partial = sums && !one ? static_cast<float*>(workspace) : nullptr;
-    p.row_blocks = int(blocks), p.dweight = dweight, p.dbias = dbias;
-    st = dispatch_type(true, dtype, p, blocks + (sums && one ? (width + 7) / 8 : 0), stm);
+    p.dweight = dweight, p.dbias = dbias;
+    st = dispatch_type(true, dtype, p, sums && one ? (width + 7) / 8 : 0, stm);
     if (st != S4D_OK) return st;
+    blocks = p.row_blocks;
   }
   if (!sums || (one && rows > 0)) return S4D_OK;
   const dim3 grid(unsigned((width + 31) / 32), 2);
   const float* partial = static_cast<const float*>(workspace);
   cudaError_t e;
   if (param_dtype == S4D_DTYPE_F32)
-    e = launch_pdl(blocks > 0, norm_reduce_kernel<float>, grid, dim3(1024), 0, stm, partial, int(blocks), int(width),
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<float>, grid, dim3(1024), 0, stm, partial, blocks, int(width),
                    static_cast<float*>(dweight), static_cast<float*>(dbias));
   else if (param_dtype == S4D_DTYPE_BF16)
-    e = launch_pdl(blocks > 0, norm_reduce_kernel<__nv_bfloat16>, grid, dim3(1024), 0, stm, partial, int(blocks),
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<__nv_bfloat16>, grid, dim3(1024), 0, stm, partial, blocks,
                    int(width), static_cast<__nv_bfloat16*>(dweight), static_cast<__nv_bfloat16*>(dbias));
   else
-    e = launch_pdl(blocks > 0, norm_reduce_kernel<__half>, grid, dim3(1024), 0, stm, partial, int(blocks), int(width),
+    e = launch_pdl(blocks > 0, norm_reduce_kernel<__half>, grid, dim3(1024), 0, stm, partial, blocks, int(width),
                    static_cast<__half*>(dweight), static_cast<__half*>(dbias));
   return cuda_check(e, "norm_reduce_kernel launch");
 }

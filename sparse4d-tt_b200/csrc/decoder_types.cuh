@@ -41,6 +41,26 @@ __device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
   }
 }
 
+// The same in two steps, for loads that are to be under way while something else is computed.
+template <typename T, int VEC>
+struct RawVec {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void widen(float (&f)[VEC]) const {
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_f32<T>(e[i]);
+  }
+};
+template <typename T>
+struct RawVec<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void clear() { v = from_f32<T>(0.0f); }
+  __device__ __forceinline__ void widen(float (&f)[1]) const { f[0] = to_f32<T>(v); }
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
   if constexpr (VEC == 1) {
