@@ -119,22 +119,27 @@ int check_args(const char* fn, const s4d_attention_args* a) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Parts of the keys.  A tile of 128 rows and one shared head is one CTA, and two of them share an SM:
-// with fewer CTAs than that the keys are cut until the SMs are full, but not below two tiles of 64
-// keys a part (one for each stream of row warps).  Up to 11 parts become at most 8, which one cluster
-// joins in shared memory: a second launch and its pass over memory cost more than a quarter of the
-// CTAs brings.
+// Parts of the keys.  A tile of 128 rows and one shared head is one CTA.  With fewer CTAs than SMs the keys
+// are cut until every SM has one, or two when a part then still has 16 tiles of 64 keys: the two on an
+// SM keep more loads under way, but each of its tiles takes longer, and more parts take longer to join.
+// (2 x 16 queries over 30,000 keys, 2 shared heads of 64: 35.6 us with one CTA an SM, 42.0 with two; one
+// query over 4 x 65,536 keys, 8 shared heads of 128: 349 us with one, 175 with two.)  A part is not
+// cut below two tiles, one for each stream of row warps.  Up to 11 parts become at most 8, which
+// one cluster joins in shared memory: a second launch and its pass over memory cost more than a quarter
+// of the CTAs brings.
 int64_t key_splits(const s4d_attention_args& a) {
   const int64_t ctas = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), kAttnRows);
-  const int64_t tiles = ceil_div(a.keys, kKeyTile), most = 2 * device_sms();
+  const int64_t tiles = ceil_div(a.keys, kKeyTile), sms = device_sms();
   const int64_t least = ceil_div(tiles, kAttnMaxTiles);
-  int64_t splits = ctas > 0 ? most / ctas : 1;
+  if (ctas == 0 || tiles == 0) return 1;
+  int64_t splits = sms / ctas > 1 ? sms / ctas : 1;
+  if (tiles / splits >= 16 && 2 * sms / ctas > splits) splits = 2 * sms / ctas;
   if (splits > tiles / 2) splits = tiles / 2;
   if (splits > 8 && splits < 12) splits = 8;
   if (splits < least) splits = least;
   if (splits < 1) splits = 1;
   // as many parts as there are after each got the same number of tiles
-  return tiles == 0 ? 1 : ceil_div(tiles, ceil_div(tiles, splits));
+  return ceil_div(tiles, ceil_div(tiles, splits));
 }
 
 int cluster_of(int64_t splits) { return splits <= 8 ? int(splits) : 1; }
@@ -241,7 +246,7 @@ int s4d_attention_forward(const s4d_attention_args* args, void* stream) {
     S4D_BAD(S4D_ERR_INVALID_ARG, "missing, misaligned or small workspace");
   p.splits = int(splits);
   p.cluster = cluster_of(splits);
-  p.tiles_per_split = ceil_div(tiles, splits);
+  p.tiles_per_split = tiles > 0 ? ceil_div(tiles, splits) : 0;
   p.part_o = static_cast<float*>(a.workspace);
   p.part_lse = p.part_o + (need > 0 ? splits * a.batch * a.queries * a.heads * a.dim : 0);
   AttnForwardMaps m;
