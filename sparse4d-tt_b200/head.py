@@ -11,7 +11,9 @@ package's ``DeformableFeatureAggregation`` (the hand-written kernels); the dense
 them -- decoupled multi-head attention (``model/multihead_attention.py``), the asymmetric FFN
 (``model/asymmetric_ffn.py``), LayerNorm, the refinement MLPs (``model/refinement_module.py``) and
 the anchor encoder (``model/sparse_box3d_encoder.py``) -- are torch operations (cuBLAS, SDPA),
-as the reference runs them through TT-NN matmuls.
+as the reference runs them through TT-NN matmuls; the attention can run on this library's own kernel
+instead (``ATTENTION_KERNEL``), which also takes a distance bias, capped scores and groups of
+instances that do not see one another.
 
 ``Sparse4DHead.forward`` launches only device work (no host synchronisation), so
 ``graph.capture`` records a whole decoder pass; ``HeadGraph`` does that over static inputs.
@@ -25,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .attention import decoder_attention_forward
 from .dfa import MATMUL_PRECISIONS, DeformableFeatureAggregation, _matmul_precision, preprocess_dfa_parameters
 from .graph import capture, chained_camera_terms
 
@@ -122,7 +125,14 @@ class Sparse4DHead:
     (``torch.float32`` by default, or ``torch.bfloat16``) is the type the attention's softmax(QK^T)V
     runs in: bf16 (the reference's TT-NN attention runs in bf16) uses the flash kernels, about 9x
     faster than the fp32 kernel at 900 tokens, with q, k, v rounded to bf16 and the result
-    returned as fp32."""
+    returned as fp32.
+
+    ``model_config["ATTENTION_KERNEL"]``: ``"sdpa"`` (default, torch's) or ``"decoder"``
+    (``attention.decoder_attention_forward``, for bf16 and fp16).  With ``"decoder"``,
+    ``ATTENTION_DISTANCE_SLOPES`` (one number a head) subtracts slope times the distance of two
+    instances in the ground plane from their score, with the anchors as they are refined from
+    layer to layer; ``ATTENTION_SOFTCAP`` caps the scores; and ``forward(..., instance_group=)`` keeps
+    groups of instances (denoising groups) from seeing one another."""
 
     def __init__(self, device, parameters: Dict, model_config: Optional[Dict] = None, embed_dims: int = 256,
                  num_groups: int = 8, num_levels: int = 4, num_cams: int = 6, num_learnable_pts: int = 6):
@@ -135,8 +145,19 @@ class Sparse4DHead:
         self.attention_dtype = cfg.get("ATTENTION_DTYPE", torch.float32)
         if self.attention_dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise ValueError("ATTENTION_DTYPE must be torch.float32, torch.bfloat16 or torch.float16")
-        cfg.pop("ATTENTION_DTYPE", None)  # a head option, not a DFA one
+        self.attention_kernel = cfg.get("ATTENTION_KERNEL", "sdpa")
+        if self.attention_kernel not in ("sdpa", "decoder"):
+            raise ValueError('ATTENTION_KERNEL must be "sdpa" or "decoder"')
+        if self.attention_kernel == "decoder" and self.attention_dtype == torch.float32:
+            raise ValueError('ATTENTION_KERNEL "decoder" needs ATTENTION_DTYPE torch.bfloat16 or torch.float16')
+        slopes = cfg.get("ATTENTION_DISTANCE_SLOPES")
+        self.attention_softcap = float(cfg.get("ATTENTION_SOFTCAP", 0.0))
+        if self.attention_kernel != "decoder" and (slopes is not None or self.attention_softcap):
+            raise ValueError('ATTENTION_DISTANCE_SLOPES and ATTENTION_SOFTCAP need ATTENTION_KERNEL "decoder"')
         dev = self.device
+        self.attention_slopes = None if slopes is None else _to(dev, torch.as_tensor(slopes, dtype=torch.float32))
+        for k in ("ATTENTION_DTYPE", "ATTENTION_KERNEL", "ATTENTION_DISTANCE_SLOPES", "ATTENTION_SOFTCAP"):
+            cfg.pop(k, None)  # head options, not DFA ones
         self.layers = []
         for op, p in zip(self.operation_order, parameters["layers"]):
             if op == "deformable":
@@ -168,24 +189,34 @@ class Sparse4DHead:
                           _run_mlp(anchor[..., SIN_YAW:COS_YAW + 1], e["yaw_fc"]),
                           _run_mlp(anchor[..., VX:VX + 3], e["vel_fc"])], dim=-1)
 
-    def _attention(self, p, query: Tensor, value: Optional[Tensor]) -> Tensor:
+    def _attention(self, p, query: Tensor, value: Optional[Tensor], anchor: Tensor,
+                   group: Optional[Tensor]) -> Tensor:
         """Decoupled self-attention (``model/sparse4d_head.py:_graph_model``): query and key are
         ``[inst, anchor_embed]`` (2C), the value ``fc_before(inst)`` (``gnn``) or the query
-        itself (``temp_gnn`` without temporal instances); identity shortcut, then ``fc_after``."""
+        itself (``temp_gnn`` without temporal instances); identity shortcut, then ``fc_after``.
+        ``anchor`` and ``group`` are the decoder kernel's positions and segments."""
         bs, n, e = query.shape
         heads = p["num_heads"]
         wq, wk, wv = p["in_proj_weight"].chunk(3, dim=0)
         bq, bk, bv = p["in_proj_bias"].chunk(3, dim=0)
         v_in = query if value is None else value
-        q = F.linear(query, wq, bq).view(bs, n, heads, e // heads).transpose(1, 2)
-        k = F.linear(query, wk, bk).view(bs, n, heads, e // heads).transpose(1, 2)
-        v = F.linear(v_in, wv, bv).view(bs, n, heads, e // heads).transpose(1, 2)
+        q = F.linear(query, wq, bq).view(bs, n, heads, e // heads)
+        k = F.linear(query, wk, bk).view(bs, n, heads, e // heads)
+        v = F.linear(v_in, wv, bv).view(bs, n, heads, e // heads)
         dt = self.attention_dtype
-        if dt == torch.float32:
-            o = F.scaled_dot_product_attention(q, k, v)
+        if self.attention_kernel == "decoder":
+            xy = None if self.attention_slopes is None else anchor[..., X:Z].contiguous()
+            o, _ = decoder_attention_forward(q.to(dt), k.to(dt), v.to(dt), softcap=self.attention_softcap,
+                                             slopes=self.attention_slopes, q_pos=xy, k_pos=xy, q_segment=group,
+                                             k_segment=group)
+            o = o.reshape(bs, n, e).float()
         else:
-            o = F.scaled_dot_product_attention(q.to(dt), k.to(dt), v.to(dt)).float()
-        o = o.transpose(1, 2).reshape(bs, n, e)
+            q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+            if dt == torch.float32:
+                o = F.scaled_dot_product_attention(q, k, v)
+            else:
+                o = F.scaled_dot_product_attention(q.to(dt), k.to(dt), v.to(dt)).float()
+            o = o.transpose(1, 2).reshape(bs, n, e)
         out = query + F.linear(o, p["out_proj_weight"], p["out_proj_bias"])
         return F.linear(out, self.fc_after)
 
@@ -209,13 +240,18 @@ class Sparse4DHead:
     # ---- forward ---------------------------------------------------------------------------------
     def forward(self, feature_maps, projection_mat: Tensor, image_wh: Tensor, spatial_shapes: Sequence[Tuple[int, int]],
                 bs: int, anchor: Optional[Tensor] = None, instance_feature: Optional[Tensor] = None,
-                time_interval: Optional[Tensor] = None) -> Dict[str, List[Optional[Tensor]]]:
+                time_interval: Optional[Tensor] = None,
+                instance_group: Optional[Tensor] = None) -> Dict[str, List[Optional[Tensor]]]:
         """One decoder pass: per decoder the refined anchors ``[bs, A, 11]`` (``prediction``),
         and for the first and last decoders the class scores ``[bs, A, num_cls]`` and quality
         ``[bs, A, 2]``.  ``feature_maps`` as ``DeformableFeatureAggregation.run`` takes them
         (packed once here when given as per-level maps).  ``anchor`` / ``instance_feature``
-        default to the instance bank's (expanded over ``bs``); ``time_interval [bs]`` to 0.5."""
+        default to the instance bank's (expanded over ``bs``); ``time_interval [bs]`` to 0.5.
+        ``instance_group [bs, A]`` (int32, with ``ATTENTION_KERNEL = "decoder"``): instances attend only to
+        their own group, a negative group to nothing."""
         dev = self.device
+        if instance_group is not None and self.attention_kernel != "decoder":
+            raise ValueError('instance_group needs ATTENTION_KERNEL "decoder"')
         A = self.anchor.shape[0]
         if anchor is None:
             anchor = self.anchor[None].expand(bs, -1, -1)
@@ -238,9 +274,10 @@ class Sparse4DHead:
             embed = self.anchor_embed(anchor)
             for i, (op, p) in enumerate(zip(self.operation_order, self.layers)):
                 if op == "temp_gnn":
-                    inst = self._attention(p, torch.cat([inst, embed], dim=-1), None)
+                    inst = self._attention(p, torch.cat([inst, embed], dim=-1), None, anchor, instance_group)
                 elif op == "gnn":
-                    inst = self._attention(p, torch.cat([inst, embed], dim=-1), F.linear(inst, self.fc_before))
+                    inst = self._attention(p, torch.cat([inst, embed], dim=-1), F.linear(inst, self.fc_before), anchor,
+                                           instance_group)
                 elif op == "norm":
                     inst = _layer_norm(inst, p[0], p[1])
                 elif op == "ffn":
@@ -263,11 +300,13 @@ class Sparse4DHead:
 class HeadGraph:
     """A whole decoder pass of ``Sparse4DHead`` over ``bs`` frames as one CUDA graph.  Static
     inputs: the packed maps ``mc_ms_feat [bs, num_feat, C]``, ``projection_mat [bs, Ncam, 4, 4]``,
-    ``image_wh [bs, Ncam, 2]`` and the initial ``anchor [bs, A, 11]`` (the instance bank's by
-    default); ``run(...)`` copies new ones in and replays, ``output`` is the replay's result dict."""
+    ``image_wh [bs, Ncam, 2]``, the initial ``anchor [bs, A, 11]`` (the instance bank's by
+    default) and, when one is given, ``instance_group [bs, A]``; ``run(...)`` copies new ones in and
+    replays, ``output`` is the replay's result dict."""
 
     def __init__(self, head: Sparse4DHead, bs: int, spatial_shapes: Sequence[Tuple[int, int]],
-                 feature_dtype: torch.dtype = torch.bfloat16, warmup: int = 2):
+                 feature_dtype: torch.dtype = torch.bfloat16, warmup: int = 2,
+                 instance_group: Optional[Tensor] = None):
         dev = head.device
         nc = 6
         self.head, self.bs, self.spatial_shapes = head, bs, [tuple(s) for s in spatial_shapes]
@@ -278,12 +317,13 @@ class HeadGraph:
         self.projection_mat[..., 3, 3] = 1.0
         self.image_wh = torch.ones(bs, nc, 2, device=dev)
         self.anchor = head.anchor[None].expand(bs, -1, -1).contiguous()
+        self.instance_group = None if instance_group is None else instance_group.to(dev).clone()
         self._call = capture(self._forward, warmup=warmup)
 
     def _forward(self):
         packed = (self.mc_ms_feat, self.spatial_shape, self.scale_start_index)
         return self.head.forward(packed, self.projection_mat, self.image_wh, self.spatial_shapes, self.bs,
-                                 anchor=self.anchor)
+                                 anchor=self.anchor, instance_group=self.instance_group)
 
     @property
     def output(self):
@@ -293,9 +333,12 @@ class HeadGraph:
         return self._call.replay()
 
     def run(self, mc_ms_feat: Optional[Tensor] = None, projection_mat: Optional[Tensor] = None,
-            image_wh: Optional[Tensor] = None, anchor: Optional[Tensor] = None):
+            image_wh: Optional[Tensor] = None, anchor: Optional[Tensor] = None,
+            instance_group: Optional[Tensor] = None):
+        if instance_group is not None and self.instance_group is None:
+            raise ValueError("this graph was captured without instance_group")
         for dst, src in ((self.mc_ms_feat, mc_ms_feat), (self.projection_mat, projection_mat),
-                         (self.image_wh, image_wh), (self.anchor, anchor)):
+                         (self.image_wh, image_wh), (self.anchor, anchor), (self.instance_group, instance_group)):
             if src is not None:
                 dst.copy_(src, non_blocking=True)
         return self.replay()

@@ -119,3 +119,103 @@ def test_norm_rejects_cpu_tensors_and_bad_arguments():
         s4d.decoder_norm(x, torch.ones(8), torch.zeros(8))
     with pytest.raises(ValueError, match="CUDA"):
         s4d.decoder_norm_backward(x, x, None, torch.zeros(4), torch.zeros(4))
+
+
+# ---- attention ------------------------------------------------------------------------------------------
+
+
+def attention_args(**kw):
+    a = dict(batch=2, queries=10, keys=20, heads=4, kv_heads=2, dim=64, pos_dim=0, q=P, k=P, v=P,
+             q_stride=(2560, 256, 64), k_stride=(2560, 128, 64), v_stride=(2560, 128, 64), out=P, lse=P, slopes=0,
+             slope_stride=(0, 0, 1), q_pos=0, k_pos=0, q_segment=0, k_segment=0, k_len=0, ws=0, wsb=0, flag=0,
+             scale=0.125, softcap=0.0, dtype=1, per_row=0, dout=P, dout_stride=(2560, 256, 64), dq=P, dk=P, dv=P,
+             dslopes=0)
+    a.update(kw)
+    return D.ATTENTION_ARGS.pack(
+        a["batch"], a["queries"], a["keys"], a["heads"], a["kv_heads"], a["dim"], a["pos_dim"], a["q"], a["k"], a["v"],
+        *a["q_stride"], *a["k_stride"], *a["v_stride"], a["out"], a["lse"], a["slopes"], *a["slope_stride"], a["q_pos"],
+        a["k_pos"], a["q_segment"], a["k_segment"], a["k_len"], a["ws"], a["wsb"], a["flag"], a["scale"], a["softcap"],
+        a["dtype"], a["per_row"], a["dout"], *a["dout_stride"], a["dq"], a["dk"], a["dv"], a["dslopes"])
+
+
+SHARED = [
+    (dict(dtype=0), INVALID, "bf16 or f16"), (dict(batch=-1), INVALID, "sizes"), (dict(heads=3), INVALID, "multiple"),
+    (dict(kv_heads=0), INVALID, "sizes"), (dict(dim=60), UNSUPPORTED, "dim"), (dict(dim=136), UNSUPPORTED, "dim"),
+    (dict(dim=0), UNSUPPORTED, "dim"), (dict(pos_dim=3), UNSUPPORTED, "pos_dim"),
+    (dict(scale=float("inf")), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale"),
+    (dict(softcap=-1.0), INVALID, "softcap"), (dict(softcap=float("nan")), INVALID, "softcap"),
+    (dict(queries=1 << 31), UNSUPPORTED, "too many"), (dict(keys=1 << 31), UNSUPPORTED, "too many"),
+    (dict(batch=1 << 20, queries=1 << 20), UNSUPPORTED, "too many"), (dict(q_segment=P), INVALID, "together"),
+    (dict(q=P + 8), INVALID, "misaligned"), (dict(k_len=P + 2), INVALID, "misaligned"), (dict(q=0), INVALID, "null q"),
+    (dict(v=0), INVALID, "null k or v"), (dict(out=0), INVALID, "null q or out"),
+    (dict(pos_dim=1), INVALID, "null slopes"), (dict(pos_dim=1, slopes=P, q_pos=P), INVALID, "null slopes"),
+    (dict(q_stride=(2560, 256, 60)), INVALID, "strides"), (dict(k_stride=(2560, 0, 64)), INVALID, "strides"),
+    (dict(v_stride=(-8, 128, 64)), INVALID, "strides"), (dict(v_stride=(1 << 40, 128, 64)), INVALID, "strides"),
+]
+
+
+@pytest.mark.parametrize("kw,status,text", SHARED)
+def test_attention_rejects_on_host(lib, kw, status, text):
+    for fn in (lib.s4d_attention_forward, lib.s4d_attention_backward):
+        st = fn(attention_args(ws=P, wsb=1 << 30, **kw), None)
+        msg = lib.s4d_decoder_last_error().decode()
+        assert st == status and text in msg, (st, msg)
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(dtype=2), UNSUPPORTED, "bf16"), (dict(keys=(1 << 19) + 1), UNSUPPORTED, "524288"), (dict(dk=0), INVALID, "together"),
+    (dict(dout=0), INVALID, "null dout"), (dict(dq=0), INVALID, "null dout"), (dict(lse=0), INVALID, "null dout"),
+    (dict(dslopes=P), INVALID, "without a distance bias"), (dict(dout_stride=(2560, 256, 4)), INVALID, "strides of dout"),
+    (dict(dq=P + 8), INVALID, "misaligned"), (dict(wsb=64), INVALID, "workspace"), (dict(ws=0), INVALID, "workspace"),
+    (dict(batch=0, q=0, k=0, v=0, out=0, dout=0, dq=0, dk=0, dv=0), OK, ""),
+])
+def test_attention_backward_rejects_on_host(lib, kw, status, text):
+    st = lib.s4d_attention_backward(attention_args(**dict(dict(ws=P, wsb=1 << 30), **kw)), None)
+    assert st == status and text in lib.s4d_decoder_last_error().decode()
+
+
+def test_attention_forward_empty_and_workspace(lib):
+    assert lib.s4d_attention_forward(attention_args(batch=0, q=0, k=0, v=0, out=0), None) == OK
+    assert lib.s4d_attention_forward(attention_args(queries=0, q=0, out=0), None) == OK
+    need = lib.s4d_attention_forward_workspace_bytes
+    assert need(attention_args()) == 0                                       # short keys: one part
+    assert need(attention_args(batch=64, queries=900, keys=900)) == 0        # rows enough
+    long = dict(batch=1, queries=1, keys=1 << 20, heads=1, kv_heads=1, k_stride=(64, 64, 64), v_stride=(64, 64, 64))
+    assert need(attention_args(**long)) % (65 * 4) == 0 and need(attention_args(**long)) > 0
+    st = lib.s4d_attention_forward(attention_args(**long), None)
+    assert st == INVALID and "workspace" in lib.s4d_decoder_last_error().decode()
+    assert need(attention_args(heads=3)) == 0 and need(attention_args(batch=-2)) == 0
+    assert lib.s4d_attention_forward(None, None) == INVALID
+    assert need(None) == 0 and lib.s4d_attention_backward_workspace_bytes(None) == 0
+
+
+def test_attention_rejects_cpu_tensors():
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: s4d.decoder_attention_forward(q, q, q), lambda: s4d.decoder_attention(q, q, q),
+                 lambda: s4d.decoder_attention_backward(q, q, q, q, q, torch.zeros(1, 2, 4))):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    """A guard is entered only when the tensors' device is not the current one."""
+    entered = []
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *exc):
+            entered.append("out")
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    with D.on_device(0):
+        pass
+    assert not entered
+    with D.on_device(3):
+        entered.append("in")
+    assert entered == [3, "in", "out"]

@@ -418,3 +418,51 @@ def test_gradient_against_differences(cuda_device):
         want = (loss(up) - loss(down)) / 2e-5
         have = (got.double() * d).sum().item()
         assert abs(want - have) <= 0.03 * got.double().abs().sum().item(), (name, want, have)
+
+
+def test_python_refusals(cuda_device):
+    q, k, v, how = make(2, 20, 30, 4, 2, 64, pos=2)
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    f = decoder_attention_forward
+    for bad in (lambda: f(q.float(), k.float(), v.float()), lambda: f(q, k.half(), v), lambda: f(q, k, v, k_len=torch.ones(2).cuda()),
+                lambda: f(q, k, v, q_segment=torch.ones(2, 20).cuda(), k_segment=torch.ones(2, 30).cuda()),
+                lambda: f(q, k, v, **dict(how, slopes=how["slopes"].double())), lambda: f(q, k, v, out=out.half()),
+                lambda: f(q, k, v, error_flag=torch.zeros(1, device="cuda"))):
+        with pytest.raises(TypeError):
+            bad()
+    seg = torch.zeros(2, 20, dtype=torch.int32, device="cuda")
+    for bad in (lambda: f(q[0], k, v), lambda: f(q, k[:1], v[:1]), lambda: f(q, k, v[:, :5]), lambda: f(q[:, :, :3], k, v),
+                lambda: f(q[..., :60], k[..., :60], v[..., :60]), lambda: f(q, k, v, slopes=how["slopes"]),
+                lambda: f(q, k, v, q_pos=how["q_pos"]), lambda: f(q, k, v, **dict(how, slopes=how["slopes"][:3])),
+                lambda: f(q, k, v, **dict(how, k_pos=how["q_pos"])), lambda: f(q, k, v, q_segment=seg),
+                lambda: f(q, k, v, q_segment=seg, k_segment=seg), lambda: f(q, k, v, k_len=seg[0]),
+                lambda: f(q, k, v, out=out[:, :, :2]), lambda: f(q, k, v, softcap=-1.0), lambda: f(q, k, v, scale=math.inf),
+                lambda: f(q, k.cpu(), v)):
+        with pytest.raises(ValueError):
+            bad()
+    b = decoder_attention_backward
+    for bad in (lambda: b(out.half(), q, k, v, out, lse, **how), lambda: b(out, q, k, v, out, lse.double(), **how)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: b(out[:, :5], q, k, v, out, lse, **how), lambda: b(out, q, k, v, out, lse[:, :1], **how),
+                lambda: b(out, q, k, v, out.transpose(1, 2).contiguous().transpose(1, 2), lse, **how)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_wait_limit_flag_stays_clear_and_step_counts(cuda_device):
+    """The error flag is only ever set by a wait that gave up."""
+    q, k, v, how = make(3, 500, 700, 4, 2, 128, pos=1, k_len=[700, 0, 333])
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = decoder_attention_forward(q, k, v, **how, error_flag=flag)
+    decoder_attention_backward(torch.randn_like(out), q, k, v, out, lse, **how, error_flag=flag)
+    assert flag.item() == 0
+
+
+@pytest.mark.parametrize("rep", [1, 2, 3, 5, 8, 16, 128, 130])
+def test_shared_heads_of_every_kind(cuda_device, rep):
+    """Heads a key that divide the 128 rows of a tile and ones that do not, more heads than rows."""
+    q, k, v, how = make(1, 9, 140, rep, 1, 64, pos=1, slopes="row")
+    check_forward(q, k, v, how, *decoder_attention_forward(q, k, v, **how))
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)

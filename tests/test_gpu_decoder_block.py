@@ -1,0 +1,183 @@
+"""The decoder operators together: a training block (norm, attention with a learned distance bias over
+groups, residual, norm) against the same block in 64 bits, as an eager step and as a captured one; and
+the decoder head with its attention on decoder_attention_forward."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from helpers import pcc
+from oracle import head_torch as oh
+from sparse4d_tt_b200 import decoder_attention, decoder_norm, ops
+from sparse4d_tt_b200 import synthetic as syn
+from sparse4d_tt_b200.graph import capture
+from sparse4d_tt_b200.head import HeadGraph, Sparse4DHead, preprocess_head_parameters
+
+pytestmark = pytest.mark.gpu
+
+B, N, H, D = 2, 230, 4, 64
+E = H * D
+
+
+def block_inputs():
+    g = torch.Generator().manual_seed(11)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    p = {"w1": 1 + 0.2 * r(E), "b1": 0.1 * r(E), "wqkv": r(3 * E, E) / math.sqrt(E), "wo": r(E, E) / math.sqrt(E),
+         "slopes": 0.05 + 0.1 * torch.rand(H, generator=g), "w2": 1 + 0.2 * r(E), "b2": 0.1 * r(E)}
+    x, dy = r(B, N, E), r(B, N, E)
+    pos = torch.rand(B, N, 2, generator=g) * 40
+    group = torch.tensor([0] * 150 + [1] * 40 + [2] * 30 + [-1] * 10, dtype=torch.int32).expand(B, -1).contiguous()
+    return {k: v.cuda() for k, v in p.items()}, x.cuda(), dy.cuda(), pos.cuda(), group.cuda()
+
+
+def block(p, x, pos, group):
+    y = decoder_norm(x, p["w1"], p["b1"])
+    q, k, v = F.linear(y, p["wqkv"]).bfloat16().view(B, N, 3, H, D).unbind(2)
+    o = decoder_attention(q, k, v, softcap=15.0, slopes=p["slopes"], q_pos=pos, k_pos=pos, q_segment=group,
+                          k_segment=group)
+    return decoder_norm(x + F.linear(o.float().reshape(B, N, E), p["wo"]), p["w2"], p["b2"])
+
+
+def block64(p, x, pos, group):
+    y = F.layer_norm(x, (E,), p["w1"], p["b1"], 1e-5)
+    q, k, v = (t.transpose(1, 2) for t in F.linear(y, p["wqkv"]).view(B, N, 3, H, D).unbind(2))
+    s = 15.0 * torch.tanh(q @ k.transpose(-1, -2) / math.sqrt(D) / 15.0)
+    # positions have no gradient, and a root's derivative at 0 is none either
+    dist = (pos[:, :, None] - pos[:, None]).square().sum(-1).sqrt()
+    s = s - p["slopes"][None, :, None, None] * dist[:, None]
+    ok = ((group[:, :, None] == group[:, None]) & (group[:, :, None] >= 0))[:, None]
+    w = torch.where(ok.any(-1, keepdim=True), torch.softmax(s.masked_fill(~ok, -1e300), -1), torch.zeros_like(s))
+    o = (w @ v).transpose(1, 2).reshape(B, N, E)
+    return F.layer_norm(x + F.linear(o, p["wo"]), (E,), p["w2"], p["b2"], 1e-5)
+
+
+def test_block_trains_like_its_64_bit_form(cuda_device):
+    """Up to six bf16 roundings (q, k, v, P, out, dS) of at most 2^-8 of a norm each lie behind every
+    gradient: 2.4e-2 relative in the 2-norm."""
+    p, x, dy, pos, group = block_inputs()
+    leaves = {k: v.clone().requires_grad_() for k, v in p.items()}
+    xl = x.clone().requires_grad_()
+    out = block(leaves, xl, pos, group)
+    out.backward(dy)
+    l64 = {k: v.double().requires_grad_() for k, v in p.items()}
+    x64 = x.double().requires_grad_()
+    ref = block64(l64, x64, pos.double(), group)
+    ref.backward(dy.double())
+    err = lambda a, b: ((a.double() - b).norm() / b.norm()).item()  # noqa: E731
+    assert err(out.detach(), ref.detach()) <= 2.4e-2
+    assert err(xl.grad, x64.grad) <= 2.4e-2
+    for k in p:
+        assert err(leaves[k].grad, l64[k].grad) <= 2.4e-2, (k, err(leaves[k].grad, l64[k].grad))
+
+
+def test_block_step_captured(cuda_device):
+    """A whole step (forward and gradients) in a CUDA graph equals the eager one bit for bit, replay after
+    replay, with new data in its inputs.  No eager graph of the same leaves is alive while it is captured."""
+    p, x, dy, pos, group = block_inputs()
+
+    def step():
+        leaves = {k: v.detach().requires_grad_() for k, v in p.items()}
+        xl = x.detach().requires_grad_()
+        out = block(leaves, xl, pos, group)
+        return (out.detach(), *torch.autograd.grad(out, [xl, *leaves.values()], dy))
+
+    call = capture(step)
+    for _ in range(2):
+        want = [t.clone() for t in step()]
+        got = call.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        x.copy_(x.flip(1))
+        dy.neg_()
+
+
+# ---- the head ------------------------------------------------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def head_case():
+    head = oh.build_head(42)
+    cfg = syn.DFAConfig(bs=2)
+    ins = syn.make_inputs(cfg, 9, feature_dtype=torch.bfloat16)
+    d = torch.device("cuda:0")
+    packed = ops.pack_feature_maps([m.to(d) for m in ins.feature_maps], dtype=torch.bfloat16)
+    return preprocess_head_parameters(head), cfg, ins, packed
+
+
+BASE = {"FEATURE_DTYPE": torch.bfloat16, "MATMUL_PRECISION": "tf32", "ATTENTION_DTYPE": torch.bfloat16}
+
+
+def run(gh, case, **kw):
+    _, cfg, ins, packed = case
+    d = torch.device("cuda:0")
+    anchor = kw.pop("anchor", ins.anchor.to(d))
+    return gh.forward(packed, ins.projection_mat.to(d), ins.image_wh.to(d), cfg.spatial_shapes, cfg.bs, anchor=anchor,
+                      **kw)["prediction"]
+
+
+def steps_agree(a, b, anchor, least):
+    prev_a, prev_b = anchor, anchor
+    for x, y in zip(a, b):
+        assert pcc((x - prev_a).cpu(), (y - prev_b).cpu()) >= least
+        prev_a, prev_b = x, y
+
+
+def test_head_on_the_decoder_kernel_follows_sdpa(cuda_device, head_case):
+    """Without bias and masks the two kernels compute the same attention up to bf16 roundings: the decoders'
+    refinement steps agree as the bf16 head does with the fp32 oracle."""
+    params = head_case[0]
+    a = run(Sparse4DHead("cuda:0", params, BASE), head_case)
+    b = run(Sparse4DHead("cuda:0", params, dict(BASE, ATTENTION_KERNEL="decoder")), head_case)
+    steps_agree(a, b, head_case[2].anchor.cuda(), 0.999)
+
+
+class PlainHead(Sparse4DHead):
+    """The head with its attention written out in fp32 on the same rounded q, k and v."""
+
+    def _attention(self, p, query, value, anchor, group):
+        bs, n, e = query.shape
+        heads = p["num_heads"]
+        v_in = query if value is None else value
+        w, b = p["in_proj_weight"].chunk(3, dim=0), p["in_proj_bias"].chunk(3, dim=0)
+        q, k, v = (F.linear(t, w[i], b[i]).view(bs, n, heads, -1).transpose(1, 2).bfloat16().float()
+                   for i, t in enumerate((query, query, v_in)))
+        s = q @ k.transpose(-1, -2) * (e // heads) ** -0.5
+        s = self.attention_softcap * torch.tanh(s / self.attention_softcap)
+        xy = anchor[..., :2]
+        s = s - self.attention_slopes[None, :, None, None] * (xy[:, :, None] - xy[:, None]).norm(dim=-1)[:, None]
+        ok = (group[:, :, None] == group[:, None])[:, None]
+        o = (torch.softmax(s.masked_fill(~ok, -math.inf), -1) @ v).transpose(1, 2).reshape(bs, n, e)
+        return F.linear(query + F.linear(o, p["out_proj_weight"], p["out_proj_bias"]), self.fc_after)
+
+
+def test_head_with_bias_cap_and_groups(cuda_device, head_case):
+    params, cfg, ins, packed = head_case
+    d = torch.device("cuda:0")
+    conf = dict(BASE, ATTENTION_KERNEL="decoder", ATTENTION_DISTANCE_SLOPES=[0.2 * 2.0 ** -i for i in range(8)],
+                ATTENTION_SOFTCAP=20.0)
+    group = (torch.arange(900) >= 700).int().expand(cfg.bs, -1).contiguous().cuda()
+    gh = Sparse4DHead("cuda:0", params, conf)
+    a = [t.clone() for t in run(gh, head_case, instance_group=group)]
+    steps_agree(a, run(PlainHead("cuda:0", params, conf), head_case, instance_group=group), ins.anchor.cuda(), 0.999)
+    # one group's anchors do not reach the other's predictions, and do reach their own
+    moved = ins.anchor.cuda().clone()
+    moved[:, 700:, :3] += 3.0
+    b = run(gh, head_case, instance_group=group, anchor=moved)
+    assert all(torch.equal(x[:, :700], y[:, :700]) for x, y in zip(a, b))
+    assert not torch.equal(a[-1][:, 700:], b[-1][:, 700:])
+    graph = HeadGraph(gh, cfg.bs, cfg.spatial_shapes, instance_group=group)
+    out = graph.run(packed[0], ins.projection_mat.to(d), ins.image_wh.to(d), ins.anchor.to(d), group)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(out["prediction"], a))
+
+
+def test_head_option_checks(cuda_device, head_case):
+    params = head_case[0]
+    for bad in ({"ATTENTION_KERNEL": "flash"}, {"ATTENTION_KERNEL": "decoder", "ATTENTION_DTYPE": torch.float32},
+                {"ATTENTION_SOFTCAP": 5.0}, {"ATTENTION_DISTANCE_SLOPES": [0.1] * 8}):
+        with pytest.raises(ValueError):
+            Sparse4DHead("cuda:0", params, dict(BASE, **bad))
+    with pytest.raises(ValueError, match="instance_group"):
+        run(Sparse4DHead("cuda:0", params, BASE), head_case,
+            instance_group=torch.zeros(2, 900, dtype=torch.int32, device="cuda"))
