@@ -5,14 +5,14 @@
 //   dQ = scale dX K,  dK = scale dX^T Q,  dV = P^T dO.
 //
 // Two kernels, so that nothing is added by atomics and equal calls give equal bits: one owns 128
-// query rows and walks the keys (dQ, dslopes, and a record of each query for
-// the second), one owns 128 keys of
-// a shared head and walks the query rows of every head that shares them (dK and dV).  That costs the
-// two score products and the exponential a second time (7 products instead of 5), and saves a pass
-// of fp32 additions over dQ in memory.  Both have the forward kernel's roles: one score row a thread, S and
-// dP side by side in tensor memory (64 columns each), the 16-bit P and dS written back over them as
-// the tensor-memory operand of the next products, the other operand read MN-major from the same
-// shared-memory tile that served the scores.
+// query rows and walks the keys (dQ, dslopes, and a record of each query for the second), one owns 128
+// keys of a shared head and walks the query rows of every head that shares them (dK and dV).  That
+// costs the two score products and the exponential a second time (7 products instead of 5), and
+// saves a pass of fp32 additions over dQ in memory.  Both have the forward kernel's roles: one score
+// row a thread, S and dP side by side in tensor memory (64 columns each), the 16-bit P and dS
+// written back over them as the tensor-memory operand of the next products, the other operand read
+// MN-major from the same shared-memory tile that served the scores.  The products of the scores and
+// the ones that add to the sums are issued by two warps, so that neither waits for the other's turn.
 //
 // P and dS are rounded to bf16 because the tensor cores multiply them with bf16 operands; the bias's
 // gradient is summed from the unrounded fp32 values.  fp16 is not offered: dS of a long row lies in
@@ -22,24 +22,23 @@
 // special-function instruction with a 2-D distance, two with a cap, and about twenty others), and the
 // turn-round of a tile: its dS has to be multiplied before the next scores can go over it, about 1,800
 // clocks.  So one CTA takes the SM's whole tensor memory: S and dP of three tiles of 64 (128 columns
-// each) for two streams of four row warps that walk alternate tiles, so that the next tile's scores are
-// there when a stream comes to it (two tiles for dK and dV at D = 128, whose sums take the other half).
-// The sums dQ, dK and dV are linear in the tiles, so the streams share them; the tensor cores take the
-// tiles in order.  KERNEL_VARIANTS
+// each), a stream of four row warps for each, so that two streams compute while the third waits (two
+// tiles and streams for dK and dV at D = 128, whose sums take the other half).  The sums dQ, dK and dV
+// are linear in the tiles, so the streams share them; the tensor cores take the tiles in order.  Twelve
+// row warps leave a thread 128 registers: it holds 16 scores and 16 dP at a time.
+//
+// Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance: dq 756, dk and dv 862 us; with two streams
+// and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with two CTAs an SM, two
+// streams and tiles of 32 each 930 and 1180.  Without the arithmetic of the scores dk and dv take 574 us,
+// without the products too 337; its 512 CTAs on 148 SMs leave 14 % of the slots empty.
 #include "decoder_attention.cuh"
 
 namespace s4d {
 namespace {
 
 using T = __nv_bfloat16;
-#ifndef CHK
-#define CHK 16
-#endif
-#ifndef NST
-#define NST 3
-#endif
-constexpr int kCols = 64;  // rows of a walked tile
-constexpr int kChunk = CHK;  // of them a row thread holds in registers at a time (twice)
+constexpr int kCols = 64;   // rows of a walked tile
+constexpr int kChunk = 16;  // of them a row thread holds in registers at a time (twice)
 
 // Waits until the sums hold every tile before tile n, whose turn it is next: the last tile of each other
 // score buffer (the own buffer's is done, it is in use again).  acc_done[s] counts the tiles of buffer
@@ -57,12 +56,11 @@ template <int DP>
 struct Dq {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = NST, kBuffers = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
+  static constexpr int kStreams = 3, kBuffers = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
   // a K tile is needed until its product with dS, a V tile only for dP
   static constexpr int kKStages = DP == 64 ? 6 : 5, kVStages = DP == 64 ? 4 : 3;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
-  // with each K tile: x, y and segment of its keys
-  // (at the end: the other streams' sums)
+  // with each K tile: x, y and segment of its keys (at the end: the other streams' sums)
   static constexpr int kSums = (kStreams - 1) * 3 * kAttnRows * 4;
   static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > kSums ? kKStages * 3 * kCols * 4 : kSums;
   static constexpr int kBars = kAux + kAuxBytes;
@@ -77,7 +75,8 @@ template <int DP>
 struct Dkv {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = DP == 64 ? NST : 2, kBuffers = DP == 64 ? 3 : 2, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
+  static constexpr int kStreams = DP == 64 ? 3 : 2, kBuffers = kStreams, kWarps = 4 * kStreams;
+  static constexpr int kThreads = (kWarps + 3) * 32;
   static constexpr int kStages = DP == 64 ? 6 : 4;  // of a Q and a dO tile
   static constexpr int kV = kOwn, kQ = kV + kOwn, kAux = kQ + kStages * 2 * kTile;
   // with each stage: its queries' record
