@@ -34,7 +34,8 @@ S4D_API const char* s4d_decoder_last_error(void);
  *               x_ld may be 0 for one broadcast row, y_ld >= width)
  *   weight/bias [width] of `param_dtype` (S4D_DTYPE_F32 or `dtype`), or NULL
  *   mean, rstd  [rows] f32, written for the backward pass; both or neither may be NULL
- * 1 <= width <= 16384.  Statistics and arithmetic are f32, rounded once into y. */
+ * 1 <= width <= 16384.  Statistics and arithmetic are f32, rounded once into y.  y may be x (the same rows
+ * at the same places); otherwise no result overlaps an argument. */
 S4D_API int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void* weight, const void* bias,
                              int param_dtype, void* y, int64_t y_ld, float* mean, float* rstd, int64_t rows,
                              int64_t width, float eps, void* stream);
@@ -45,7 +46,7 @@ S4D_API int s4d_norm_forward(const void* x, int64_t x_ld, int dtype, const void*
  * sizes alone, so that equal calls give equal bits.  rows = 0 writes zeros to them.
  * workspace: s4d_norm_backward_workspace_bytes(rows, width) bytes, 16-byte aligned, read and
  * written by this call only while it runs (may be NULL when that is 0 or neither dweight nor dbias is
- * wanted). */
+ * wanted).  No result overlaps an argument. */
 S4D_API size_t s4d_norm_backward_workspace_bytes(int64_t rows, int64_t width);
 S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype,
                               const void* weight, int param_dtype, const float* mean, const float* rstd, void* dx,
@@ -60,7 +61,8 @@ S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int6
  *   out_i = sum_j softmax_j(s) v_j over the seen keys, 0 for a query that sees none;
  *   lse_i = log sum_j exp(s), -inf for such a query.
  * What q, k, v and the positions hold at pairs that are not seen never reaches out: an infinity or
- * a NaN there changes nothing.
+ * a NaN there changes nothing.  Distances of two coordinates are roots of an f32 sum of squares, so
+ * differences of positions stay below 2^63.  No result overlaps an argument.
  *
  *   dtype         S4D_DTYPE_BF16 or S4D_DTYPE_F16, of q, k, v and out
  *   q             [batch, queries, heads, dim], k and v [batch, keys, kv_heads, dim]: unit stride along
@@ -76,6 +78,7 @@ S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int6
  *   workspace     s4d_attention_forward_workspace_bytes(args) bytes, 16-byte aligned, used by this call
  *                 only while it runs (0 bytes: may be NULL)
  *   error_flag    int32 or NULL: S4D_FLAG_WAIT_TIMEOUT as in s4d_dfa.h
+ *   softcap       0 (none), or up to 1024: a capped score is off by a few 2^-23 softcap
  * P is rounded to `dtype` for its product with v; sums and softmax statistics are f32.  Equal calls
  * give equal bits.  batch and the axes may be 0; rows of one shared head (queries * heads /
  * kv_heads) and keys must stay below 2^31.

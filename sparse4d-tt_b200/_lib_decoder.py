@@ -123,6 +123,17 @@ def same_device(name: str, first: torch.Tensor, *others) -> int:
     return index
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from one tensor's first to its last element meets the other's."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    lo, hi = [], []
+    for t in (a, b):
+        lo.append(t.data_ptr())
+        hi.append(t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))
+    return lo[0] < hi[1] and lo[1] < hi[0]
+
+
 def stream_ptr(index: int) -> int:
     """torch's current-stream handle of a device index."""
     if _raw_stream is not None:

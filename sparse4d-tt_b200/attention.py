@@ -4,9 +4,9 @@
 For head h, query i and key j::
 
     x = scale q_i.k_j                     scale = dim ** -0.5 unless given
-    z = softcap tanh(x / softcap)         (x when softcap is 0)
-    s = z - slopes_h |q_pos_i - k_pos_j|  positions in 1 or 2 coordinates; slopes per head, or per
-                                          query and head
+    z = softcap tanh(x / softcap)         (x when softcap is 0; at most 1024)
+    s = z - slopes_h |q_pos_i - k_pos_j|  positions in 1 or 2 coordinates (with 2, differences below 2^63);
+                                          slopes per head, or per query and head
     seen: j < k_len[b]  and  q_segment_i == k_segment_j >= 0
     out_i = sum over the seen keys of softmax(s)_j v_j; 0 for a query that sees none
 
@@ -139,8 +139,11 @@ def _checked(name: str, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float],
 
 def _pack(a: _Args, out: int, lse: int, workspace: int = 0, workspace_bytes: int = 0, per_row: int = 0, dout: int = 0,
           dout_stride=_ZERO3, dq: int = 0, dk: int = 0, dv: int = 0, dslopes: int = 0) -> bytes:
-    return D.ATTENTION_ARGS.pack(*a.sizes, *a.operands, out, lse, *a.slopes, *a.optional, workspace, workspace_bytes,
-                                 a.error_flag, *a.scalars, per_row, dout, *dout_stride, dq, dk, dv, dslopes)
+    try:
+        return D.ATTENTION_ARGS.pack(*a.sizes, *a.operands, out, lse, *a.slopes, *a.optional, workspace, workspace_bytes,
+                                     a.error_flag, *a.scalars, per_row, dout, *dout_stride, dq, dk, dv, dslopes)
+    except OverflowError:
+        raise ValueError(f"scale and softcap must fit in fp32, got {a.scalars[:2]}") from None
 
 
 def _address(t: Optional[Tensor]) -> int:
@@ -160,7 +163,7 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
     ``slopes [H]`` or ``[B, Nq, H]`` fp32 with ``q_pos [B, Nq, 1 or 2]`` and ``k_pos [B, Nk, 1 or 2]``
     fp32 give the distance bias; ``q_segment [B, Nq]`` and ``k_segment [B, Nk]`` int32 the document
     mask; ``k_len [B]`` int32 the valid keys of each batch entry (read on the device, clamped to
-    0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into.  ``error_flag`` (int32) gets
+    0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into (not one of the arguments).  ``error_flag`` (int32) gets
     ``S4D_FLAG_WAIT_TIMEOUT`` should a kernel give up waiting; the results are then not valid."""
     name = "decoder_attention_forward"
     a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
@@ -172,6 +175,8 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
             raise TypeError(f"{name}: out must be {q.dtype}, got {out.dtype}")
         if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError(f"{name}: out must be a contiguous, 16-byte aligned {list(q.shape)} tensor")
+        if any(t is not None and D.overlap(out, t) for t in (q, k, v, slopes, q_pos, k_pos, q_segment, k_segment, k_len)):
+            raise ValueError(f"{name}: out must not share memory with the arguments")
     B, nq, _, H = a.sizes[:4]
     lse = q.new_empty((B, H, nq), dtype=torch.float32)
     lib = D.lib()

@@ -1,5 +1,6 @@
 // extern "C" entry points of the decoder's attention (include/s4d_decoder.h): argument validation on
 // the host, tensor maps and the choice of launches.
+#include <cmath>
 #include <mutex>
 
 #include "decoder_attention.cuh"
@@ -71,6 +72,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t dim, int64_t
 }
 
 constexpr int64_t kMaxRows = int64_t(1) << 31;
+constexpr float kMaxSoftcap = 1024.0f;
 constexpr int kKeyTile = 64;       // keys of a forward tile
 constexpr int kBackwardTile = 64;  // queries or keys of a backward tile
 
@@ -90,7 +92,12 @@ int check_args(const char* fn, const s4d_attention_args* a) {
     S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "dim must be a multiple of 8 from 8 to 128");
   if (a->pos_dim < 0 || a->pos_dim > 2) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "pos_dim must be 0, 1 or 2");
   if (!(a->scale > -INFINITY && a->scale < INFINITY)) S4D_BAD(S4D_ERR_INVALID_ARG, "scale must be finite");
-  if (!(a->softcap >= 0.0f && a->softcap < INFINITY)) S4D_BAD(S4D_ERR_INVALID_ARG, "softcap must be finite and >= 0");
+  // a capped score is cap - cap * (1 - tanh), off by a few 2^-23 cap: above the limit that is no longer small
+  // beside the rounding of the weights to 16 bits
+  if (!(a->softcap >= 0.0f && a->softcap <= kMaxSoftcap))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "softcap must be 0 (none) or at most 1024");
+  if (!std::isfinite(ScoreConst(a->scale, a->softcap).k1))
+    S4D_BAD(S4D_ERR_INVALID_ARG, "scale, or scale / softcap, is too large for fp32");
   int64_t n = 0;
   if (!size_product({a->queries, a->heads / a->kv_heads}, kMaxRows, &n) || a->keys >= kMaxRows ||
       a->batch >= kMaxRows || a->heads >= (1 << 20) ||

@@ -146,8 +146,9 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 struct ScoreConst {
   float k1;   // scale log2e, or 2 scale / cap log2e
   float c;    // cap log2e
-  __device__ explicit ScoreConst(const AttnParams& p)
-      : k1(p.cap > 0.0f ? 2.0f * p.scale / p.cap * kLog2e : p.scale * kLog2e), c(p.cap * kLog2e) {}
+  __host__ __device__ ScoreConst(float scale, float cap)
+      : k1(cap > 0.0f ? 2.0f * scale / cap * kLog2e : scale * kLog2e), c(cap * kLog2e) {}
+  __device__ explicit ScoreConst(const AttnParams& p) : ScoreConst(p.scale, p.cap) {}
 };
 
 // 2 / (1 + e^2y): tanh(y) = 1 - that

@@ -74,6 +74,9 @@ def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optio
         raise TypeError(f"{name}: out must be {dtype}, got {out.dtype}")
     elif out.shape != shape or not out.is_contiguous():
         raise ValueError(f"{name}: out must be a contiguous {list(shape)} tensor")
+    elif (D.overlap(out, x) and (out.data_ptr() != x.data_ptr() or not x.is_contiguous())) or any(
+            t is not None and D.overlap(out, t) for t in (weight, bias)):
+        raise ValueError(f"{name}: out must be x itself or share no memory with the arguments")
     v, ld = _rows(x, width)
     stats = shape[:-1]
     mean, rstd = x.new_empty(stats, dtype=torch.float32), x.new_empty(stats, dtype=torch.float32)

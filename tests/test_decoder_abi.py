@@ -162,6 +162,17 @@ def test_attention_rejects_on_host(lib, kw, status, text):
         assert st == status and text in msg, (st, msg)
 
 
+@pytest.mark.parametrize("kw,text", [
+    (dict(softcap=1025.0), "1024"), (dict(softcap=float("inf")), "1024"), (dict(softcap=1e-38, scale=100.0), "too large"),
+    (dict(scale=3e38), "too large"), (dict(scale=-3e38), "too large"),
+])
+def test_attention_rejects_scales_without_an_fp32_score(lib, kw, text):
+    for fn in (lib.s4d_attention_forward, lib.s4d_attention_backward):
+        st = fn(attention_args(ws=P, wsb=1 << 30, **kw), None)
+        msg = lib.s4d_decoder_last_error().decode()
+        assert st == INVALID and text in msg, (st, msg)
+
+
 @pytest.mark.parametrize("kw,status,text", [
     (dict(dtype=2), UNSUPPORTED, "bf16"), (dict(keys=(1 << 19) + 1), UNSUPPORTED, "524288"), (dict(dk=0), INVALID, "together"),
     (dict(dout=0), INVALID, "null dout"), (dict(dq=0), INVALID, "null dout"), (dict(lse=0), INVALID, "null dout"),
@@ -219,3 +230,12 @@ def test_launches_go_to_the_tensors_device(monkeypatch):
     with D.on_device(3):
         entered.append("in")
     assert entered == [3, "in", "out"]
+
+
+def test_overlap():
+    x = torch.zeros(100, 64)
+    a, b = x[:, :32], x[:, 32:]
+    assert D.overlap(x, a) and D.overlap(a, b)          # a and b interleave: their ranges meet
+    assert not D.overlap(x[:50], x[50:]) and D.overlap(x[:51], x[50:])
+    assert not D.overlap(x[:0], x) and not D.overlap(x, torch.zeros(3))
+    assert D.overlap(x[0].expand(5, 64), x[0]) and not D.overlap(x[0].expand(5, 64), x[1])

@@ -466,3 +466,21 @@ def test_shared_heads_of_every_kind(cuda_device, rep):
     check_forward(q, k, v, how, *decoder_attention_forward(q, k, v, **how))
     dout, grads = gradients(q, k, v, how)
     check_backward(q, k, v, how, dout, grads)
+
+
+def test_out_that_shares_memory_and_scales_beyond_fp32_are_rejected(cuda_device):
+    buf = torch.randn(3, 2, 64, 4, 64, device="cuda").bfloat16()
+    q, k, v = buf
+    for bad in (lambda: decoder_attention_forward(q, k, v, out=q), lambda: decoder_attention_forward(q, k, v, out=v),
+                lambda: decoder_attention_forward(q, k, v, out=buf.view(-1)[64:64 + q.numel()].view(q.shape)),
+                lambda: decoder_attention_forward(q, k, v, scale=1e39), lambda: decoder_attention_forward(q, k, v, softcap=2e3)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.parametrize("cap", [1024.0, 1e-3])
+def test_largest_and_small_caps(cuda_device, cap):
+    q, k, v, how = make(1, 100, 150, 2, 2, 64, cap=cap)
+    check_forward(q, k, v, how, *decoder_attention_forward(q, k, v, **how))
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)

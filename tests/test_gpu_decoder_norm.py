@@ -206,3 +206,13 @@ def test_gradient_against_differences(cuda_device):
         d = torch.zeros_like(W)
         d[j] = 1e-6
         assert abs((loss(X, W + d) - loss(X, W - d)).item() / 2e-6 - dw[j].item()) < 1e-4
+
+
+def test_out_that_shares_memory_is_rejected(cuda_device):
+    buf = torch.randn(64, 64, device="cuda")
+    w = buf[3]
+    for bad in (lambda: decoder_norm_forward(buf[1:], out=buf[:-1]), lambda: decoder_norm_forward(buf[:1].expand(8, 64), out=buf[:8]),
+                lambda: decoder_norm_forward(buf[8:], w, out=buf[:56]), lambda: decoder_norm_forward(buf[:, :32], out=buf[:32].view(64, 32))):
+        with pytest.raises(ValueError):
+            bad()
+    decoder_norm_forward(buf[32:], w, out=buf[32:])  # x itself
