@@ -309,12 +309,13 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t a_bl
            idesc_f16<T>(n, false), k != 0);
 }
 
-// D[128, DP] (+)= A B with A [128, ROWS] in tensor memory and B [ROWS, DP] in shared memory.
-template <typename T, int DP, int ROWS>
+// D[128, DP] (+)= A B with A [128, ROWS] in tensor memory (16 values of a row every STEP columns) and B
+// [ROWS, DP] in shared memory.
+template <typename T, int DP, int ROWS, int STEP = 8>
 __device__ __forceinline__ void mma_accumulate(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
 #pragma unroll
   for (int k = 0; k < ROWS / 16; ++k)
-    mma_ts(d, a + 8 * k, desc_sw128(b, DP > 64 ? ROWS * 128 : 1024) + 128 * k, idesc_f16<T>(DP, true), accumulate || k != 0);
+    mma_ts(d, a + STEP * k, desc_sw128(b, DP > 64 ? ROWS * 128 : 1024) + 128 * k, idesc_f16<T>(DP, true), accumulate || k != 0);
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int h, int n,
@@ -460,7 +461,7 @@ __device__ __forceinline__ bool row_not_finite(const unsigned char* tile, int bl
 // acc[lane, :] (+)= sum over the ROWS rows j of a tile with a[lane, j] != 0 of a[lane, j] tile[j, :]:
 // what mma_accumulate computes, except that a zero weight hides the row's infinities and NaNs
 // instead of turning them into NaN.  For tiles that are masked in part and hold such values.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int STEP = 8>
 __device__ __noinline__ void accumulate_nonzero(uint32_t acc, uint32_t a, const unsigned char* tile, bool init) {
   for (int c = 0; c < DP / 16; ++c) {
     float o[16];
@@ -472,7 +473,7 @@ __device__ __noinline__ void accumulate_nonzero(uint32_t acc, uint32_t a, const 
     const unsigned char* block = tile + (c / 4) * (ROWS * 128);
     for (int j0 = 0; j0 < ROWS; j0 += 16) {
       uint32_t w[8];
-      tmem_ld8_async(a + j0 / 2, w);
+      tmem_ld8_async(a + j0 / 16 * STEP, w);
       tmem_ld_wait(w);
 #pragma unroll
       for (int jj = 0; jj < 16; ++jj) {

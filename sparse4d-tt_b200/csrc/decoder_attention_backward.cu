@@ -14,23 +14,27 @@
 // MN-major from the same shared-memory tile that served the scores.  The products of the scores and
 // the ones that add to the sums are issued by two warps, so that neither waits for the other's turn.
 //
-// P and dS are rounded to bf16 because the tensor cores multiply them with bf16 operands; the bias's
-// gradient is summed from the unrounded fp32 values.  fp16 is not offered: dS of a long row lies in
-// fp16's subnormal range.
+// P and dS are rounded to bf16 because the tensor cores multiply them with bf16 operands (dQ and dK then
+// are off by 0.0017 of their size from this, as much again from their own rounding); the bias's gradient
+// is summed from the unrounded fp32 values.  fp16 is not offered: dS of a long row lies in fp16's
+// subnormal range.  delta comes from an O that is rounded too, which would weigh as much as dP itself where
+// a row's weight lies on few keys.  So the first kernel also adds R_i = sum_j dS_ij, which an exact delta
+// makes 0, and the product P K: the second kernel gets delta + R, dQ loses R P K, dslope R sum P dist
+// (8192 tokens: dq 755 us without the product, 803 with it).
 //
 // What bounds it: as in the forward pass the work per score in registers (one exponential, one more
 // special-function instruction with a 2-D distance, two with a cap, and about twenty others), and the
 // turn-round of a tile: its dS has to be multiplied before the next scores can go over it, about 1,800
 // clocks.  So one CTA takes the SM's whole tensor memory: S and dP of three tiles of 64 (128 columns
 // each), a stream of four row warps for each, so that two streams compute while the third waits (two
-// tiles and streams for dK and dV at D = 128, whose sums take the other half).  The sums dQ, dK and dV
+// tiles and streams at D = 128, whose two sums take the other half).  The sums dQ, dK and dV
 // are linear in the tiles, so the streams share them; the tensor cores take the tiles in order.  Twelve
 // row warps leave a thread 128 registers: it holds 16 scores and 16 dP at a time.
 //
-// Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance: dq 756, dk and dv 862 us; with two streams
-// and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with two CTAs an SM, two
-// streams and tiles of 32 each 930 and 1180.  Without the arithmetic of the scores dk and dv take 574 us,
-// without the products too 337; its 512 CTAs on 148 SMs leave 14 % of the slots empty.
+// Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance, before P K was added: dq 756, dk and dv
+// 862 us; with two streams and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with
+// two CTAs an SM, two streams and tiles of 32 each 930 and 1180.  Without the arithmetic of the scores dk
+// and dv take 574 us, without the products too 337; its 512 CTAs on 148 SMs leave 14 % of the slots empty.
 #include "decoder_attention.cuh"
 
 namespace s4d {
@@ -56,18 +60,19 @@ template <int DP>
 struct Dq {
   static constexpr int kOwnBlock = kAttnRows * 128, kBlock = kCols * 128;
   static constexpr int kOwn = DP / 64 * kOwnBlock, kTile = DP / 64 * kBlock;
-  static constexpr int kStreams = 3, kBuffers = 3, kWarps = 4 * kStreams, kThreads = (kWarps + 3) * 32;
+  static constexpr int kStreams = DP == 64 ? 3 : 2, kBuffers = kStreams, kWarps = 4 * kStreams;
+  static constexpr int kThreads = (kWarps + 3) * 32;
   // a K tile is needed until its product with dS, a V tile only for dP
   static constexpr int kKStages = DP == 64 ? 6 : 5, kVStages = DP == 64 ? 4 : 3;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
-  // with each K tile: x, y and segment of its keys (at the end: the other streams' sums)
-  static constexpr int kSums = (kStreams - 1) * 3 * kAttnRows * 4;
+  // with each K tile: x, y and segment of its keys (at the end: the streams' sums)
+  static constexpr int kSums = kStreams * 3 * kAttnRows * 4;
   static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > kSums ? kKStages * 3 * kCols * 4 : kSums;
   static constexpr int kBars = kAux + kAuxBytes;
   static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kBuffers + 3;
   static constexpr int kCtl = kBars + (kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kKinds = kCtl + 32;
-  static constexpr uint32_t kTmem = 512;  // per buffer S / dS 64, dP 64; dQ DP
+  static constexpr uint32_t kTmem = 512;  // per buffer S / dS and P 64, dP 64; dQ DP, P K DP
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
@@ -88,9 +93,10 @@ struct Dkv {
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
-// Two scores: their weights, gradients dS and (CAP) the cap's derivative 1 - tanh^2 = rest (2 - rest).
+// Two scores: their weights P, gradients dS, and both times (CAP) the cap's derivative 1 - tanh^2 =
+// rest (2 - rest).
 struct Terms {
-  F2 p, ds, dx;
+  F2 p, ds, px, dx;
 };
 template <int POS, bool CAP, bool MASKED>
 __device__ __forceinline__ Terms score_terms(F2 acc, const ScoreConst& k, F2 nslope, F2 dist, F2 nlse2, F2 dp,
@@ -111,12 +117,17 @@ __device__ __forceinline__ Terms score_terms(F2 acc, const ScoreConst& k, F2 nsl
   Terms r;
   r.p = f2(a, b);
   r.ds = mul2(r.p, add2(dp, ndelta));
+  r.px = CAP ? mul2(r.p, deriv) : r.p;
   r.dx = CAP ? mul2(r.ds, deriv) : r.ds;
   if constexpr (MASKED) {  // dP and the derivative of a masked pair may be no numbers
     split(r.ds, a, b);
     r.ds = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
     split(r.dx, a, b);
     r.dx = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
+    if constexpr (CAP) {
+      split(r.px, a, b);
+      r.px = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
+    }
   }
   return r;
 }
@@ -131,7 +142,7 @@ __device__ __forceinline__ uint32_t pack(F2 v) {
 
 // One chunk of CH keys of a query row (qx, qy negated).  aux arrays of a tile: x, y, segment.
 template <int POS, bool CAP, bool MASKED, int CH>
-__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[CH], const uint32_t (&pr)[CH], uint32_t (&w)[CH / 2],
+__device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[CH], const uint32_t (&pr)[CH], uint32_t (&w)[CH],
                                          const ScoreConst& k, float slope2, float qx, float qy, int seg, bool sees, float lse2,
                                          float delta, const float* aux, float (&sums)[3]) {
   F2 r0 = f2(0.0f), r1 = r0, e1 = r0;
@@ -151,22 +162,23 @@ __device__ __forceinline__ void dq_chunk(const uint32_t (&sr)[CH], const uint32_
       if constexpr (POS > 0) dist = distance<POS>(x2, y2, half_of(x4, u), POS > 1 ? half_of(y4, u) : x2);
       const Terms t = score_terms<POS, CAP, MASKED>(pair_of(sr + j4 + u), k, nslope, dist, nlse2, pair_of(pr + j4 + u),
                                                     ndelta, seen0, seen1);
+      r0 = add2(r0, t.ds);
       if constexpr (POS > 0) {
         if constexpr (MASKED) {
           float a, b;
           split(dist, a, b);
           dist = f2(seen0 ? a : 0.0f, seen1 ? b : 0.0f);
         }
-        r0 = add2(r0, t.ds);
         r1 = fma2(t.ds, dist, r1);
         e1 = fma2(t.p, dist, e1);
       }
       w[(j4 + u) / 2] = pack(t.dx);
+      w[CH / 2 + (j4 + u) / 2] = pack(t.px);
     }
   }
+  float a, b;
+  split(r0, a, b), sums[0] += a + b;
   if constexpr (POS > 0) {
-    float a, b;
-    split(r0, a, b), sums[0] += a + b;
     split(r1, a, b), sums[1] += a + b;
     split(e1, a, b), sums[2] += a + b;
   }
@@ -305,7 +317,6 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
           for (int e = 0; e < 8; ++e) delta = fmaf(fo[e], fd[e], delta);
         }
       }
-      if (stream == 0) write_record<POS>(p, b, h, i, -lse2, -delta, -qx, -qy, -slope2, sees ? seg : -1);
     }
     // queries that fill up the last tile of records
     if (row0 + kAttnRows >= rows) {
@@ -396,8 +407,11 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     for (int t = t0; ok && t < tiles; t = walk.next(t), any = true) {
       if (!(ok = warp_wait(ds_full + 8 * buf.stage, buf.parity, abort_flag, p.wait_limit_ns))) break;
       if (leader) {
-        if (!(walk.masked(t) && skip[buf.stage]))
-          mma_accumulate<T, DP, kCols>(tmem_o, tmem + buf.stage * 2 * kCols, sbase + S::kK + ka.stage * S::kTile, any);
+        if (!(walk.masked(t) && skip[buf.stage])) {
+          const uint32_t a = tmem + buf.stage * 2 * kCols, kt = sbase + S::kK + ka.stage * S::kTile;
+          mma_accumulate<T, DP, kCols, 16>(tmem_o, a, kt, any);
+          mma_accumulate<T, DP, kCols, 16>(tmem_o + DP, a + 8, kt, any);
+        }
         mma_commit(acc_done + 8 * buf.stage);
         mma_commit(k_empty + 8 * ka.stage);
       }
@@ -443,7 +457,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
         tmem_ld<kChunk>(tmem_s + kCols, pr[0]);
 #pragma unroll
         for (int c = 0; c < kCols / kChunk; ++c) {
-          uint32_t w[kChunk / 2];
+          uint32_t w[kChunk];  // dS, then P
           tmem_ld_wait(sr[c & 1]);
           tmem_ld_wait(pr[c & 1]);
           if (c + 1 < kCols / kChunk) {
@@ -455,13 +469,14 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
             dq_chunk<POS, CAP, true>(sr[c & 1], pr[c & 1], w, k, slope2, qx, qy, seg, sees, lse2, delta, cx, sums);
           else
             dq_chunk<POS, CAP, false>(sr[c & 1], pr[c & 1], w, k, slope2, qx, qy, seg, sees, lse2, delta, cx, sums);
-          tmem_st<kChunk / 2>(tmem_s + c * (kChunk / 2), w);
+          tmem_st<kChunk>(tmem_s + c * kChunk, w);
         }
         tmem_st_wait();
         if (bad) {
           // dQ is about to change outside the tensor cores
           dead = !earlier_done<S::kBuffers>(acc_done, n, abort_flag, p.wait_limit_ns);
-          if (!dead) accumulate_nonzero<T, DP, kCols>(tmem_o + lanes, tmem_s, kt, n == 0);
+          if (!dead) accumulate_nonzero<T, DP, kCols, 16>(tmem_o + lanes, tmem_s, kt, n == 0);
+          if (!dead) accumulate_nonzero<T, DP, kCols, 16>(tmem_o + DP + lanes, tmem_s + 8, kt, n == 0);
         }
       }
       warp_arrive(ds_full + 8 * buf.stage);
@@ -470,31 +485,36 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
       for (int e = 0; e < S::kStreams; ++e) r.next(S::kKStages), buf.next(S::kBuffers);
     }
     if (!dead && t0 < tiles) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
-    if constexpr (POS > 0) {
-      // all streams' sums; o_full: no warp reads its keys' values any more
-      float* other = reinterpret_cast<float*>(smem + S::kAux);
-      if (stream > 0) {
+    // The streams' sums; o_full: no warp reads its keys' values any more.
+    float* all = reinterpret_cast<float*>(smem + S::kAux);
 #pragma unroll
-        for (int e = 0; e < 3; ++e) other[((stream - 1) * 3 + e) * kAttnRows + tid] = sums[e];
-      }
-      barrier_sync(1 + S::kStreams, S::kWarps * 32);
-      if (stream == 0 && live && p.dslopes != nullptr) {
+    for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) all[(stream * 3 + e) * kAttnRows + tid] = sums[e], sums[e] = 0.0f;
+    barrier_sync(1 + S::kStreams, S::kWarps * 32);
 #pragma unroll
-        for (int s = 0; s < S::kStreams - 1; ++s)
+    for (int s = 0; s < S::kStreams; ++s)
 #pragma unroll
-          for (int e = 0; e < 3; ++e) sums[e] += other[(s * 3 + e) * kAttnRows + tid];
-        // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits, so
-        // dS is off by P times that sum, and sum dS dist by that times sum P dist.
-        p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
-            dead ? __int_as_float(0x7fc00000) : -fmaf(-sums[0], sums[2], sums[1]);
-      }
+      for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) sums[e] += all[(s * 3 + e) * kAttnRows + tid];
+    // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits (and made
+    // from 16-bit P), so delta is short of that sum, sum dS dist is off by it times sum P dist, and dQ by
+    // it times P K.
+    if (live && stream == 0) {
+      write_record<POS>(p, b, h, i, -lse2, -(delta + sums[0]), -qx, -qy, -slope2, sees ? seg : -1);
+      if constexpr (POS > 0)
+        if (p.dslopes != nullptr)
+          p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
+              dead ? __int_as_float(0x7fc00000) : -fmaf(-sums[0], sums[2], sums[1]);
     }
     if (!dead && warp_live) {
       // dQ's columns in 32s, shared out among the streams
       for (int c = stream; c * 32 < p.dim; c += S::kStreams) {
-        uint32_t o[32];
+        uint32_t o[32], pk[32];
         tmem_ld32_async(tmem_o + lanes + c * 32, o);
+        tmem_ld32_async(tmem_o + DP + lanes + c * 32, pk);
         tmem_ld_wait(o);
+        tmem_ld_wait(pk);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          o[e] = __float_as_uint(fmaf(-sums[0], __uint_as_float(pk[e]), __uint_as_float(o[e])));
         if (live) store_row32(static_cast<T*>(p.dq) + out_row * p.dim, c * 32, p.dim, o, t0 < tiles, p.scale);
       }
     }

@@ -484,3 +484,40 @@ def test_largest_and_small_caps(cuda_device, cap):
     check_forward(q, k, v, how, *decoder_attention_forward(q, k, v, **how))
     dout, grads = gradients(q, k, v, how)
     check_backward(q, k, v, how, dout, grads)
+
+
+@pytest.mark.parametrize("D,pos,cap", [(64, 2, 0.0), (64, 0, 20.0), (128, 1, 0.0)])
+def test_gradients_do_not_see_the_rounding_of_out(cuda_device, D, pos, cap):
+    """delta_i = dO_i . O_i is made from a rounded O.  What it is short of, at most r = (h + h) |dO| P |V| (O
+    rounded, and made from rounded P), is taken out of dQ and dK again; left over is r times the
+    relative error of the correction: P's rounding h, the scores' 2 e and the sums' N u.  Weights that lie on
+    few keys, where dS is small beside r."""
+    B, Nq, Nk, H, G = 1, 200, 260, 4, 2
+    q, k, v, how = make(B, Nq, Nk, H, G, D, pos=pos, cap=cap)
+    q = q * 4
+    dout, (dq, dk, dv, ds) = gradients(q, k, v, how)
+    r = reference(q, k, v, dout=dout, **how)
+    h, n = half_step(q.dtype), max(Nq, Nk) * U
+    e = score_error(q, k, None, cap, how.get("slopes"), how.get("q_pos"), how.get("k_pos"))
+    scale = D ** -0.5
+    tol_q, tol_k = torch.zeros_like(r["dq"]), torch.zeros_like(r["dk"])
+    for hd in range(H):
+        Q, K, V, dO = q[0, :, hd].double(), k[0, :, hd // 2].double(), v[0, :, hd // 2].double(), dout[0, :, hd].double()
+        x = scale * Q @ K.T
+        t = torch.tanh(x / cap) if cap else 0 * x
+        s = cap * t if cap else x
+        if pos:
+            dist = (how["q_pos"][0].double()[:, None] - how["k_pos"][0].double()[None]).square().sum(-1).sqrt()
+            s = s - how["slopes"][hd].double() * dist
+        p = torch.softmax(s, 1)
+        dp = dO @ V.T
+        dS = p * (dp - (p * dp).sum(1, keepdim=True))
+        mag = p * (dO.abs() @ V.abs().T)
+        short = p * (2 * h * mag.sum(1, keepdim=True))  # before the correction
+        off = (h + 2 * e + (D + 16) * U + n) * dS.abs() + (2 * e + (D + 16) * U + n) * mag + (h + 2 * e + n + 16 * U) * short \
+            + p * ((2 * e + n + (D + 16) * U) * mag.sum(1, keepdim=True))
+        tol_q[0, :, hd] = scale * off @ K.abs()
+        tol_k[0, :, hd // 2] += scale * off.T @ Q.abs()
+    for got, name, tol in ((dq, "dq", tol_q), (dk, "dk", tol_k)):
+        tol = tol + h * (r[name].abs() + tol) + 1e-30
+        assert ((got.double() - r[name]).abs() <= tol).all(), name
