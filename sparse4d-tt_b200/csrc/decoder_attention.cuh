@@ -40,10 +40,13 @@ struct AttnParams {
   int64_t nq, nk;
   int batch, heads, kv_heads, rep, dim;
   float scale, cap;
-  // forward over parts of the keys
+  // A CTA takes tile first_tile + blockIdx.x / splits and one of the parts of the other axis.
+  int64_t first_tile;
   int splits;   // parts
-  int cluster;  // CTAs that join their parts in shared memory: splits, or 1 (joined by a second launch)
+  int cluster;  // CTAs that join their parts in shared memory: splits, or 1 (forward: joined by a second launch)
   int64_t tiles_per_split;
+  // A launch over the first tiles, and one over the rest (from first_tile) beside the end of it.
+  int ahead, behind;
   float* part_o;    // [splits, B, Nq, H, D]
   float* part_lse;  // [splits, B, H, Nq]
   // backward
@@ -592,6 +595,27 @@ __device__ __forceinline__ float4 peer_f4(uint32_t addr) {
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(addr));
   return v;
+}
+
+// Four of the fp32 values at `addr` of every CTA of the cluster, added in the order of the ranks.
+__device__ __forceinline__ float4 cluster_sum(uint32_t addr, int cluster) {
+  float4 v[8], sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int s = 0; s < 8; ++s)
+    if (s < cluster) v[s] = peer_f4(peer_addr(addr, s));
+#pragma unroll
+  for (int s = 0; s < 8; ++s)
+    if (s < cluster) sum.x += v[s].x, sum.y += v[s].y, sum.z += v[s].z, sum.w += v[s].w;
+  return sum;
+}
+__device__ __forceinline__ float cluster_sum1(uint32_t addr, int cluster) {
+  float sum = 0.0f;
+  for (int s = 0; s < cluster; ++s) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(addr, s)));
+    sum += v;
+  }
+  return sum;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------

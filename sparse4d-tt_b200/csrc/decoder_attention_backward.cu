@@ -34,7 +34,8 @@
 // Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance, before P K was added: dq 756, dk and dv
 // 862 us; with two streams and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with
 // two CTAs an SM, two streams and tiles of 32 each 930 and 1180.  Without the arithmetic of the scores dk
-// and dv take 574 us, without the products too 337; its 512 CTAs on 148 SMs leave 14 % of the slots empty.
+// and dv take 574 us, without the products too 337; its 512 tiles of keys on 148 SMs left
+// 14 % of the slots empty until the last ones were cut (launch_tiles below).
 #include "decoder_attention.cuh"
 
 namespace s4d {
@@ -65,8 +66,8 @@ struct Dq {
   // a K tile is needed until its product with dS, a V tile only for dP
   static constexpr int kKStages = DP == 64 ? 6 : 5, kVStages = DP == 64 ? 4 : 3;
   static constexpr int kDo = kOwn, kK = kDo + kOwn, kV = kK + kKStages * kTile, kAux = kV + kVStages * kTile;
-  // with each K tile: x, y and segment of its keys (at the end: the streams' sums)
-  static constexpr int kSums = kStreams * 3 * kAttnRows * 4;
+  // with each K tile: x, y and segment of its keys (at the end: each stream's sums and all's)
+  static constexpr int kSums = (kStreams + 1) * 3 * kAttnRows * 4;
   static constexpr int kAuxBytes = kKStages * 3 * kCols * 4 > kSums ? kKStages * 3 * kCols * 4 : kSums;
   static constexpr int kBars = kAux + kAuxBytes;
   static constexpr int kNumBars = 2 * kKStages + 2 * kVStages + 3 * kBuffers + 3;
@@ -196,6 +197,50 @@ __device__ __forceinline__ void store_row32(T* row, int col, int dim, const uint
   }
 }
 
+// A row's fp32 sums for the other CTAs of a cluster: N values in pieces of four, piece j of row r at
+// j ^ (r & 7), from the start of the tiles in shared memory, which nothing reads any more.
+template <int N>
+__device__ __forceinline__ uint32_t shared_piece(uint32_t base, int r, int j) {
+  return base + r * (N * 4) + ((j ^ (r & 7)) << 4);
+}
+// ... from the accumulators (zeros when nothing was accumulated, NaN from a CTA that gave up).
+template <int N, int STREAMS>
+__device__ __forceinline__ void share_rows(unsigned char* smem, uint32_t acc, int row, int stream, bool any, bool dead) {
+  for (int c = stream; c < N / 32; c += STREAMS) {
+    uint32_t o[32];
+    tmem_ld32_async(acc + c * 32, o);
+    tmem_ld_wait(o);
+    const uint32_t none = dead ? 0x7fc00000u : 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<uint4*>(smem + row * (N * 4) + (((c * 8 + e) ^ (row & 7)) << 4)) =
+          any && !dead ? make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_uint4(none, none, none, none);
+  }
+}
+
+// The CTA's part of an own tile of 128 rows (dq) or keys (dkv) of a shared head: blockIdx.x, divided by the
+// parts, counts (b G + g) tiles + tile from first_tile.
+struct OwnTile {
+  int part, g, b;
+  uint32_t row0;
+};
+template <bool PARTS>
+__device__ __forceinline__ OwnTile own_tile(const AttnParams& p, uint32_t rows) {
+  uint32_t u = blockIdx.x;
+  const uint32_t tiles = (rows + kAttnRows - 1) / kAttnRows;
+  OwnTile o;
+  o.part = 0;
+  if constexpr (PARTS) {
+    o.part = int(u % uint32_t(p.cluster));
+    u = uint32_t(p.first_tile) + u / uint32_t(p.cluster);
+  }
+  o.row0 = u % tiles * kAttnRows;
+  u /= tiles;
+  o.g = int(u % uint32_t(p.kv_heads));
+  o.b = int(u / uint32_t(p.kv_heads));
+  return o;
+}
+
 template <int POS>
 __device__ __forceinline__ void write_record(const AttnParams& p, int b, int h, int64_t i, float nlse2, float ndelta, float x,
                                              float y, float nslope2, int seg) {
@@ -212,7 +257,7 @@ __device__ __forceinline__ void write_record(const AttnParams& p, int b, int h, 
   reinterpret_cast<int*>(r)[5 * kRecordTile] = seg;
 }
 
-template <int DP, int POS, bool CAP>
+template <int DP, int POS, bool CAP, bool PARTS>
 __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
                         const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
@@ -231,16 +276,15 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   unsigned char* kinds = smem + S::kKinds;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  // blockIdx.x = (b G + g) row tiles + row tile; row r is query r / rep of head g rep + r % rep
-  const uint32_t rep = uint32_t(p.rep);
-  const uint32_t rows = uint32_t(p.nq) * rep, row_tiles = (rows + kAttnRows - 1) / kAttnRows;
-  uint32_t u = blockIdx.x;
-  const int64_t row0 = int64_t(u % row_tiles) * kAttnRows;
-  u /= row_tiles;
-  const int g = int(u % uint32_t(p.kv_heads)), b = int(u / uint32_t(p.kv_heads));
+  // row r is query r / rep of head g rep + r % rep
+  const uint32_t rep = uint32_t(p.rep), rows = uint32_t(p.nq) * rep;
+  const OwnTile own = own_tile<PARTS>(p, rows);
+  const int64_t row0 = own.row0;
+  const int g = own.g, b = own.b;
   int64_t valid = p.nk;
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
-  const int tiles = int((valid + kCols - 1) / kCols);
+  const int first = PARTS ? own.part * int(p.tiles_per_split) : 0;  // the part's first tile of keys
+  const int tiles = max(0, min(int(p.tiles_per_split), int((valid + kCols - 1) / kCols) - first));
   const bool own_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
 
   if (warp == S::kWarps && lane == 0) {
@@ -272,11 +316,11 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     }
   }
   if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
-  TileWalk walk{nullptr, tiles, int(valid / kCols)};
-  if (p.q_seg != nullptr) {
+  TileWalk walk{nullptr, tiles, max(0, min(tiles, int(valid / kCols) - first))};
+  if (!PARTS && p.q_seg != nullptr) {
     const int64_t i0 = row0 / rep, i1 = (min(int64_t(rows), row0 + kAttnRows) - 1) / rep;
-    const SegRange own = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
-    classify_tiles(kinds, 0, tiles, kCols, valid, p.k_seg + b * p.nk, own, true);
+    const SegRange ids = seg_range(p.q_seg + b * p.nq + i0, int(i1 - i0 + 1));
+    classify_tiles(kinds, 0, tiles, kCols, valid, p.k_seg + b * p.nk, ids, true);
     walk.kinds = kinds;
   }
 
@@ -344,6 +388,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (!PARTS && p.ahead) griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + S::kBuffers * 2 * kCols;
   const int t0 = walk.first();
 
@@ -353,13 +398,13 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     for (int t = t0; t < tiles; ++n) {
       // V first: its stage is free once dP is there, K's only after dQ
       if (n >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
-      if (lane == 0) load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, t * kCols, b);
+      if (lane == 0) load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, (first + t) * kCols, b);
       if (n >= S::kKStages && !warp_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) {
         mbar_wait(v_full + 8 * vr.stage, vr.parity, nullptr);  // no copy may land in a CTA that is gone
         break;
       }
-      if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, t * kCols, b);
-      const int64_t key = int64_t(t) * kCols, at = b * p.nk + key;
+      if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, (first + t) * kCols, b);
+      const int64_t key = int64_t(first + t) * kCols, at = b * p.nk + key;
       load_key_values<POS>(sbase + S::kAux + kr.stage * 3 * kCols * 4, k_full + 8 * kr.stage, p.k_pos + at * POS,
                            p.k_seg != nullptr ? p.k_seg + at : nullptr, valid - key);
       kr.next(S::kKStages);
@@ -494,30 +539,70 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     for (int s = 0; s < S::kStreams; ++s)
 #pragma unroll
       for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) sums[e] += all[(s * 3 + e) * kAttnRows + tid];
-    // With an exact delta sum dS would be 0; the O that delta was made from is rounded to 16 bits (and made
-    // from 16-bit P), so delta is short of that sum, sum dS dist is off by it times sum P dist, and dQ by
-    // it times P K.
-    if (live && stream == 0) {
-      write_record<POS>(p, b, h, i, -lse2, -(delta + sums[0]), -qx, -qy, -slope2, sees ? seg : -1);
+    // What a row's sums and products give.  With an exact delta sum dS would be 0; the O that delta was made
+    // from is rounded to 16 bits (and made from 16-bit P), so delta is short of that sum, sum dS dist is off
+    // by it times sum P dist, and dQ by it times P K.
+    auto finish_row = [&](const float (&total)[3]) {
+      write_record<POS>(p, b, h, i, -lse2, -(delta + total[0]), -qx, -qy, -slope2, sees ? seg : -1);
       if constexpr (POS > 0)
         if (p.dslopes != nullptr)
           p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
-              dead ? __int_as_float(0x7fc00000) : -fmaf(-sums[0], sums[2], sums[1]);
-    }
-    if (!dead && warp_live) {
-      // dQ's columns in 32s, shared out among the streams
-      for (int c = stream; c * 32 < p.dim; c += S::kStreams) {
-        uint32_t o[32], pk[32];
-        tmem_ld32_async(tmem_o + lanes + c * 32, o);
-        tmem_ld32_async(tmem_o + DP + lanes + c * 32, pk);
-        tmem_ld_wait(o);
-        tmem_ld_wait(pk);
+              dead ? __int_as_float(0x7fc00000) : -fmaf(-total[0], total[2], total[1]);
+    };
+    if constexpr (!PARTS) {
+      if (live && stream == 0) finish_row(sums);
+      if (!dead && warp_live) {
+        // dQ's columns in 32s, shared out among the streams
+        for (int c = stream; c * 32 < p.dim; c += S::kStreams) {
+          uint32_t o[32], pk[32];
+          tmem_ld32_async(tmem_o + lanes + c * 32, o);
+          tmem_ld32_async(tmem_o + DP + lanes + c * 32, pk);
+          tmem_ld_wait(o);
+          tmem_ld_wait(pk);
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          o[e] = __float_as_uint(fmaf(-sums[0], __uint_as_float(pk[e]), __uint_as_float(o[e])));
-        if (live) store_row32(static_cast<T*>(p.dq) + out_row * p.dim, c * 32, p.dim, o, t0 < tiles, p.scale);
+          for (int e = 0; e < 32; ++e)
+            o[e] = __float_as_uint(fmaf(-sums[0], __uint_as_float(pk[e]), __uint_as_float(o[e])));
+          if (live) store_row32(static_cast<T*>(p.dq) + out_row * p.dim, c * 32, p.dim, o, t0 < tiles, p.scale);
+        }
       }
+    } else {
+      // dQ, P K and the sums of this part of the keys, for the cluster
+      float* total = all + S::kStreams * 3 * kAttnRows;
+      if (stream == 0)
+#pragma unroll
+        for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) total[e * kAttnRows + tid] = sums[e];
+      share_rows<2 * DP, S::kStreams>(smem, tmem_o + lanes, tid, stream, t0 < tiles, dead);
+      cluster_sync();
+      if (live && stream == 0 && tid % p.cluster == own.part) {
+        float v[3] = {};
+#pragma unroll
+        for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) v[e] = cluster_sum1(smem_u32(total + e * kAttnRows + tid), p.cluster);
+        finish_row(v);
+      }
+      constexpr int kLanes = DP / 8, kRowsPerWarp = 32 / kLanes;
+      const int col = lane % kLanes * 8;
+      for (int r = own.part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && row0 + r < rows;
+           r += p.cluster * kRowsPerWarp * S::kWarps) {
+        const float short_of = cluster_sum1(smem_u32(total + r), p.cluster);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 o = cluster_sum(shared_piece<2 * DP>(sbase, r, col / 4 + e), p.cluster);
+          const float4 pk = cluster_sum(shared_piece<2 * DP>(sbase, r, (DP + col) / 4 + e), p.cluster);
+          w[2 * e] = pack2<T>(fmaf(-short_of, pk.x, o.x) * p.scale, fmaf(-short_of, pk.y, o.y) * p.scale);
+          w[2 * e + 1] = pack2<T>(fmaf(-short_of, pk.z, o.z) * p.scale, fmaf(-short_of, pk.w, o.w) * p.scale);
+        }
+        const uint32_t at = uint32_t(row0) + r, qi = at / rep, hh = g * rep + (at - qi * rep);
+        if (col < p.dim)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.dq) + ((b * p.nq + qi) * p.heads + hh) * p.dim + col) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      cluster_sync();  // the peers still read this CTA's shared memory
     }
+  }
+  if (PARTS && warp >= S::kWarps) {
+    cluster_sync();
+    cluster_sync();
   }
   tc_fence_before();
   __syncthreads();
@@ -526,6 +611,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     tmem_dealloc(tmem, S::kTmem);
   }
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  if (PARTS && p.behind) griddep_wait();  // what follows this launch follows the one ahead too
 }
 
 // One chunk of CH query columns of a key's row (kx, ky negated).  aux: the queries' record.
@@ -561,7 +647,7 @@ __device__ __forceinline__ void dkv_chunk(const uint32_t (&sr)[CH], const uint32
   }
 }
 
-template <int DP, int POS, bool CAP>
+template <int DP, int POS, bool CAP, bool PARTS>
 __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
                          const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap dom,
@@ -579,16 +665,14 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   unsigned char* kinds = smem + S::kKinds;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  // blockIdx.x = (b G + g) key tiles + key tile
-  const uint32_t key_tiles = uint32_t((p.nk + kAttnRows - 1) / kAttnRows);
-  uint32_t u = blockIdx.x;
-  const int64_t key0 = int64_t(u % key_tiles) * kAttnRows;
-  u /= key_tiles;
-  const int g = int(u % uint32_t(p.kv_heads)), b = int(u / uint32_t(p.kv_heads));
+  const OwnTile own = own_tile<PARTS>(p, uint32_t(p.nk));
+  const int64_t key0 = own.row0;
+  const int g = own.g, b = own.b;
   int64_t valid = p.nk;
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
-  // query tiles, walked once for every head that shares the keys; none when no key here is valid
-  const int tiles = key0 < valid ? int((p.nq + kCols - 1) / kCols) : 0;
+  // the part's query tiles, walked once for every head that shares the keys; none when no key here is valid
+  const int first = PARTS ? own.part * int(p.tiles_per_split) : 0, query_tiles = int((p.nq + kCols - 1) / kCols);
+  const int tiles = key0 < valid ? max(0, min(int(p.tiles_per_split), query_tiles - first)) : 0;
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -616,10 +700,10 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   }
   if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
   const bool own_whole = key0 + kAttnRows <= valid;
-  TileWalk walk{nullptr, tiles, own_whole ? int(p.nq / kCols) : 0};
-  if (p.k_seg != nullptr) {
-    const SegRange own = seg_range(p.k_seg + b * p.nk + key0, int(min(valid - key0, int64_t(kAttnRows))));
-    classify_tiles(kinds, 0, tiles, kCols, p.nq, p.q_seg + b * p.nq, own, own_whole);
+  TileWalk walk{nullptr, tiles, own_whole ? max(0, min(tiles, int(p.nq / kCols) - first)) : 0};
+  if (!PARTS && p.k_seg != nullptr) {
+    const SegRange ids = seg_range(p.k_seg + b * p.nk + key0, int(min(valid - key0, int64_t(kAttnRows))));
+    classify_tiles(kinds, 0, tiles, kCols, p.nq, p.q_seg + b * p.nq, ids, own_whole);
     walk.kinds = kinds;
   }
 
@@ -643,6 +727,7 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (!PARTS && p.ahead) griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot, tmem_dv = tmem + S::kBuffers * 2 * kCols, tmem_dk = tmem_dv + DP;
   const int t0 = walk.first();
   const bool work = t0 < tiles;
@@ -656,7 +741,6 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     if (lane == 0) {
       int n = 0, hh = work ? 0 : p.rep, t = t0;
       Ring r;
-      const int64_t query_tiles = (p.nq + kRecordTile - 1) / kRecordTile;
       for (; hh < p.rep; advance(hh, t), ++n) {
         if (n >= S::kStages && !sleep_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
         const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile, bar = full + 8 * r.stage;
@@ -664,11 +748,11 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
         mbar_expect_tx(bar, 2 * S::kTile + kRecordBytes);
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-          tma_load_4d(st + c * S::kBlock, &qm, bar, c * 64, h, t * kCols, b);
-          tma_load_4d(st + S::kTile + c * S::kBlock, &dom, bar, c * 64, h, t * kCols, b);
+          tma_load_4d(st + c * S::kBlock, &qm, bar, c * 64, h, (first + t) * kCols, b);
+          tma_load_4d(st + S::kTile + c * S::kBlock, &dom, bar, c * 64, h, (first + t) * kCols, b);
         }
         bulk_load(sbase + S::kAux + r.stage * kRecordBytes,
-                  p.records + ((int64_t(b) * p.heads + h) * query_tiles + t) * (kRecordTile * kRecordFields), kRecordBytes,
+                  p.records + ((int64_t(b) * p.heads + h) * query_tiles + first + t) * (kRecordTile * kRecordFields), kRecordBytes,
                   bar);
         r.next(S::kStages);
       }
@@ -787,7 +871,25 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
       for (int e = 0; e < S::kStreams; ++e) r.next(S::kStages), buf.next(S::kBuffers);
     }
     if (!dead && work) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
-    if (!dead) {
+    if constexpr (PARTS) {
+      // dV and dK of this part of the queries, for the cluster
+      share_rows<2 * DP, S::kStreams>(smem, tmem_dv + lanes, tid, stream, work, dead);
+      cluster_sync();
+      constexpr int kLanes = 2 * DP / 8, kRowsPerWarp = 32 / kLanes;
+      const int at = lane % kLanes * 8, col = at % DP;
+      for (int r = own.part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && key0 + r < p.nk;
+           r += p.cluster * kRowsPerWarp * S::kWarps) {
+        const float4 x = cluster_sum(shared_piece<2 * DP>(sbase, r, at / 4), p.cluster);
+        const float4 y = cluster_sum(shared_piece<2 * DP>(sbase, r, at / 4 + 1), p.cluster);
+        const float f = at >= DP ? p.scale : 1.0f;
+        if (col < p.dim)
+          *reinterpret_cast<uint4*>(static_cast<T*>(at >= DP ? p.dk : p.dv) +
+                                    ((b * p.nk + key0 + r) * p.kv_heads + g) * p.dim + col) =
+              make_uint4(pack2<T>(x.x * f, x.y * f), pack2<T>(x.z * f, x.w * f), pack2<T>(y.x * f, y.y * f),
+                         pack2<T>(y.z * f, y.w * f));
+      }
+      cluster_sync();  // the peers still read this CTA's shared memory
+    } else if (!dead) {
       // dV's and dK's columns in 32s, shared out among the streams
       const int64_t off = ((b * p.nk + (live ? key : 0)) * p.kv_heads + g) * p.dim;
       for (int c = stream; c < 2 * DP / 32; c += S::kStreams) {
@@ -801,6 +903,10 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
       }
     }
   }
+  if (PARTS && warp >= S::kWarps) {
+    cluster_sync();
+    cluster_sync();
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == S::kWarps + 1) {
@@ -808,32 +914,93 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     tmem_dealloc(tmem, S::kTmem);
   }
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  if (PARTS && p.behind) griddep_wait();  // what follows this launch follows the one ahead too
+}
+
+// `tiles` own tiles (a CTA an SM) with `walked` tiles of the other axis each, `weight` times.  The tiles that
+// fill the SMs are one launch of `whole_kernel`.  The rest, which would leave SMs idle for as long as a whole
+// tile takes, are one of `kernel` beside the end of the first, cut into as many parts of the other axis as
+// there is room for clusters of that many CTAs, up to eight: each keeps its sums in shared memory and
+// joins a share of the rows.  A part keeps six tiles or more, since its start and the join take as long as
+// two.  (4 x 1800 tokens, 8 heads, 480 own tiles: forward and backward pass 406 us without, 376 us with
+// it; 8192 tokens, 512 tiles of keys: 2090 and 1988 us; 900 tokens, 64 tiles, all cut: 69 and 58.5 us.)
+// Tiles with segments differ in length and fill the SMs as they come, and are short: those are not cut (8 x
+// 1437 tokens in groups, 768 tiles: 251 us, cut 256; 900 in three groups, 64 tiles: 55.0 and 55.2 us).
+template <typename S, typename K, typename... Maps>
+int launch_tiles(K whole_kernel, K kernel, const char* what, bool (&smem_set)[2][64], int (&fits)[64][9], AttnParams p,
+                 int64_t tiles, int64_t walked, int64_t weight, cudaStream_t st, const Maps&... maps) {
+  int rc = set_kernel_smem(whole_kernel, S::smem(kAttnMaxTiles), what, smem_set[0]);
+  if (rc == S4D_OK) rc = set_kernel_smem(kernel, S::smem(kAttnMaxTiles), what, smem_set[1]);
+  if (rc != S4D_OK) return rc;
+  const int64_t sms = device_sms(), rest = tiles % sms;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {1, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int dev = 0, parts = 1;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  for (int c = 8; c > 1 && rest > 0 && p.q_seg == nullptr && parts == 1; --c) {
+    if (rest * c > sms || walked * weight < 6 * c || walked < c) continue;
+    int fit = dev >= 0 && dev < 64 ? fits[dev][c] : 0;
+    if (fit == 0) {
+      attr[0].val.clusterDim.x = unsigned(c);
+      cfg.gridDim = dim3(unsigned(c));
+      cfg.dynamicSmemBytes = S::smem(0);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        fit = 0;
+      }
+      if (dev >= 0 && dev < 64) fits[dev][c] = fit > 0 ? fit : -1;
+    }
+    if (rest <= fit) parts = c;
+  }
+  const int64_t whole = parts > 1 ? tiles - rest : tiles;
+  p.splits = p.cluster = 1;
+  p.first_tile = 0;
+  p.ahead = parts > 1;
+  p.behind = 0;
+  p.tiles_per_split = walked;
+  if (whole > 0) {
+    cfg.gridDim = dim3(unsigned(whole));
+    cfg.dynamicSmemBytes = S::smem(p.q_seg != nullptr ? walked : 0);
+    cfg.numAttrs = 0;
+    rc = cuda_check(cudaLaunchKernelEx(&cfg, whole_kernel, maps..., p), what);
+  }
+  if (rc != S4D_OK || parts == 1) return rc;
+  p.tiles_per_split = (walked + parts - 1) / parts;
+  p.splits = p.cluster = parts;
+  p.first_tile = whole;
+  p.behind = whole > 0;
+  attr[0].val.clusterDim.x = unsigned(parts);
+  cfg.gridDim = dim3(unsigned(rest * parts));
+  cfg.dynamicSmemBytes = S::smem(0);
+  cfg.numAttrs = whole > 0 ? 2 : 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, maps..., p), what);
 }
 
 template <int DP, int POS, bool CAP>
 int launch(const AttnParams& p, const AttnBackwardMaps& m, cudaStream_t st) {
-  static bool dq_set[64] = {}, dkv_set[64] = {};
-  int rc = set_kernel_smem(attention_dq_kernel<DP, POS, CAP>, Dq<DP>::smem(kAttnMaxTiles),
-                           "cudaFuncSetAttribute(attention_dq_kernel)", dq_set);
-  if (rc == S4D_OK)
-    rc = set_kernel_smem(attention_dkv_kernel<DP, POS, CAP>, Dkv<DP>::smem(kAttnMaxTiles),
-                         "cudaFuncSetAttribute(attention_dkv_kernel)", dkv_set);
-  if (rc != S4D_OK) return rc;
+  static bool dq_set[2][64] = {}, dkv_set[2][64] = {};
+  static int dq_fits[64][9] = {}, dkv_fits[64][9] = {};
   const int64_t groups = int64_t(p.kv_heads) * p.batch;
-  if (p.nq > 0) {
-    const int64_t row_tiles = (p.nq * p.rep + kAttnRows - 1) / kAttnRows;
-    attention_dq_kernel<DP, POS, CAP><<<dim3(unsigned(row_tiles * groups)), Dq<DP>::kThreads,
-                                        Dq<DP>::smem(p.q_seg != nullptr ? (p.nk + kCols - 1) / kCols : 0), st>>>(
-        m.q_rows, m.do_rows, m.k_tile, m.v_tile, p);
-    rc = cuda_check(cudaGetLastError(), "attention_dq_kernel launch");
-  }
-  if (rc == S4D_OK && p.nk > 0 && p.dk != nullptr) {
-    const int64_t key_tiles = (p.nk + kAttnRows - 1) / kAttnRows;
-    attention_dkv_kernel<DP, POS, CAP><<<dim3(unsigned(key_tiles * groups)), Dkv<DP>::kThreads,
-                                         Dkv<DP>::smem(p.q_seg != nullptr ? (p.nq + kCols - 1) / kCols : 0), st>>>(
-        m.k_rows, m.v_rows, m.q_tile, m.do_tile, p);
-    rc = cuda_check(cudaGetLastError(), "attention_dkv_kernel launch");
-  }
+  const int64_t query_tiles = (p.nq + kCols - 1) / kCols, key_tiles = (p.nk + kCols - 1) / kCols;
+  int rc = S4D_OK;
+  if (p.nq > 0)
+    rc = launch_tiles<Dq<DP>>(attention_dq_kernel<DP, POS, CAP, false>, attention_dq_kernel<DP, POS, CAP, true>,
+                              "attention_dq_kernel launch", dq_set, dq_fits, p,
+                              (p.nq * p.rep + kAttnRows - 1) / kAttnRows * groups, key_tiles, 1, st, m.q_rows, m.do_rows,
+                              m.k_tile, m.v_tile);
+  if (rc == S4D_OK && p.nk > 0 && p.dk != nullptr)
+    rc = launch_tiles<Dkv<DP>>(attention_dkv_kernel<DP, POS, CAP, false>, attention_dkv_kernel<DP, POS, CAP, true>,
+                               "attention_dkv_kernel launch", dkv_set, dkv_fits, p,
+                               (p.nk + kAttnRows - 1) / kAttnRows * groups, query_tiles, p.rep, st, m.k_rows, m.v_rows,
+                               m.q_tile, m.do_tile);
   return rc;
 }
 

@@ -521,3 +521,44 @@ def test_gradients_do_not_see_the_rounding_of_out(cuda_device, D, pos, cap):
     for got, name, tol in ((dq, "dq", tol_q), (dk, "dk", tol_k)):
         tol = tol + h * (r[name].abs() + tol) + 1e-30
         assert ((got.double() - r[name]).abs() <= tol).all(), name
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D,how", [
+    (5, 900, 900, 4, 4, 64, dict(pos=2)),                    # 160 tiles of either kind: twelve are cut in two
+    (2, 1700, 1600, 6, 6, 128, dict(cap=20.0)),              # 168 and 156: in four
+    (3, 1500, 1500, 16, 4, 64, dict(pos=1, slopes="row", k_len=[1500, 700, 0])),
+    (1, 2100, 5, 3, 1, 64, dict(pos=2)),                     # nothing to cut for dq, one tile for dk and dv
+    (1, 1024, 1100, 2, 2, 64, dict()),                       # fewer tiles than SMs: all are cut
+])
+def test_gradients_of_tiles_cut_into_parts(cuda_device, B, Nq, Nk, H, G, D, how):
+    """The tiles that do not fill the SMs are cut along the other axis and joined."""
+    q, k, v, how = make(B, Nq, Nk, H, G, D, **how)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+    for _ in range(20):
+        again = gradients(q, k, v, how)[1]
+        assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize("D,B,groups", [(64, 1, False), (128, 1, False), (64, 3, False), (64, 3, True)])
+def test_gradients_of_parts_with_masked_values_that_are_no_numbers(cuda_device, D, B, groups):
+    """Valid keys that end inside a tile of some part (without groups), groups (tiles then stay whole), keys and
+    queries that nothing sees and hold NaN and infinity, in a captured graph too."""
+    N, H = 1200, 6
+    ids = torch.arange(N) // 170
+    ids[1100:] = -1
+    q, k, v, how = make(B, N, N, H, H, D, pos=2, segments=(ids, ids) if groups else None, k_len=[950, 1100, 1000][:B])
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+    q2, k2, v2, dout2 = (t.clone() for t in (q, k, v, dout))
+    for t in (q2, k2, v2, dout2) if groups else (k2, v2):
+        t[:, 1100:] = float("nan")
+    k2[0, 950:], v2[0, 960:] = float("inf"), float("nan")
+    out, lse = decoder_attention_forward(q2, k2, v2, **how)
+    run = lambda: decoder_attention_backward(dout2, q2, k2, v2, out, lse, **how)  # noqa: E731
+    first = [t.clone() for t in run()]
+    check_backward(q, k, v, how, dout, first)
+    graph = capture(run)
+    for grads in [run() for _ in range(10)] + [graph.replay()]:
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, first))
