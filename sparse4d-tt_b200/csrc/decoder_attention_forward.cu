@@ -30,9 +30,9 @@
 // Measured (kernel alone, bf16 unless said): 32 x 900 tokens, 8 heads of 64, 2-D distance 213 us (212 M
 // exponentials and as many square roots: 119 us at 16 a clock); 8 x 1437, 8 heads of 64, segments 68 us;
 // 2 x 4096, 16 heads of 128 on 4, capped, f16 420 us (270 us for its three special-function instructions
-// a score); 8192 tokens, 16 heads of 64 on 8, 1-D distance 585 us.  What is left over is not one
-// unit: with the square root taken out the first takes 167 us, without exponentials 212, without products 197,
-// and an empty tile loop with all its hand-overs 105.
+// a score); 8192 tokens, 16 heads of 64 on 8, 1-D distance 585 us.  What is left over is not one unit:
+// when the first took 229, it took 167 with the square root taken out, 212 without exponentials, 197 without
+// products, and 105 with an empty tile loop and all its hand-overs.
 #include "decoder_attention.cuh"
 
 namespace s4d {
