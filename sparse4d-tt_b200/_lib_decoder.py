@@ -1,4 +1,5 @@
-"""ctypes binding of ``lib/libs4d_decoder.so`` (the C ABI declared in ``include/s4d_decoder.h``).
+"""ctypes binding of ``lib/libs4d_decoder.so`` (the C ABI declared in ``include/s4d_decoder.h``), and
+the module that takes the calls which need nothing but a launch (``csrc/decoder_calls.cpp``).
 
 The library is loaded on first use.  If it is missing, every operator of it raises instead of
 falling back to another implementation.
@@ -6,6 +7,8 @@ falling back to another implementation.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import struct
 import threading
@@ -17,6 +20,8 @@ from . import _lib as L
 # The in-tree build; S4D_DECODER_LIB may point at another build of the same ABI.
 LIB_PATH = os.environ.get("S4D_DECODER_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib",
                                                              "libs4d_decoder.so")
+
+CALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "s4d_decoder_calls.so")
 
 S4D_DTYPE_F16 = 2
 DTYPES = {torch.float32: L.S4D_DTYPE_F32, torch.bfloat16: L.S4D_DTYPE_BF16, torch.float16: S4D_DTYPE_F16}
@@ -81,6 +86,30 @@ def lib():
                                        f"{ABI_VERSION}; rebuild it (python sparse4d-tt_b200/build.py)")
                 _lib = handle
     return _lib
+
+
+_calls = None
+
+
+def calls():
+    """The module of csrc/decoder_calls.cpp, over the functions of ``lib()``.  Each of its calls answers None
+    for what is not its to take."""
+    global _calls
+    if _calls is None:
+        handle = lib()
+        with _lock:
+            if _calls is None:
+                if not os.path.exists(CALLS_PATH):
+                    raise RuntimeError(f"{CALLS_PATH} is not built; run `python __graft_entry__.py build` "
+                                       "(or python sparse4d-tt_b200/build.py).")
+                loader = importlib.machinery.ExtensionFileLoader("s4d_decoder_calls", CALLS_PATH)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+                loader.exec_module(module)
+                module.init(*(C.cast(getattr(handle, n), C.c_void_p).value for n in (
+                    "s4d_norm_forward", "s4d_norm_backward_workspace_bytes", "s4d_norm_backward",
+                    "s4d_attention_forward_workspace_bytes", "s4d_attention_forward")))
+                _calls = module
+    return _calls
 
 
 def check(fn: str, status: int) -> None:

@@ -166,6 +166,10 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
     0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into (not one of the arguments).  ``error_flag`` (int32) gets
     ``S4D_FLAG_WAIT_TIMEOUT`` should a kernel give up waiting; the results are then not valid."""
     name = "decoder_attention_forward"
+    if out is None and error_flag is None:
+        done = D.calls().attention_forward(q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len)
+        if done is not None:
+            return done
     a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
     if out is None:
         out = q.new_empty(q.shape)

@@ -1,5 +1,5 @@
 """Build ``lib/libs4d_dfa.so`` (the C ABI of ``include/s4d_dfa.h``) and ``lib/libs4d_decoder.so``
-(``include/s4d_decoder.h``) for sm_100a with nvcc.
+(``include/s4d_decoder.h``) for sm_100a with nvcc, and the Python module of the latter's calls with g++.
 
     python sparse4d-tt_b200/build.py [--verbose-ptxas]
 
@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
@@ -24,6 +25,7 @@ SOURCES = ["capi.cu", "kps_project.cu", "dfa_gather.cu", "kps_noalloc.cu", "line
            "instance_bank.cu", "peer.cu", "layer_norm.cu"]
 # The decoder's operators: each (source, defines) is compiled by itself, several at a time.
 DECODER_LIB_PATH = os.path.join(LIB_DIR, "libs4d_decoder.so")
+CALLS_PATH = os.path.join(LIB_DIR, "s4d_decoder_calls.so")
 DECODER_SOURCES = [("decoder_capi.cu",), ("decoder_norm.cu",), ("decoder_attention.cu",),
                    ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=64"),
                    ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=128"),
@@ -45,13 +47,13 @@ def _run(cmd, what: str, verbose_ptxas: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError(f"nvcc failed building {what}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed building {what}")
     if verbose_ptxas:
         sys.stdout.write(res.stderr)
 
 
 def build_decoder(verbose_ptxas: bool = False, force: bool = False) -> str:
-    """``libs4d_decoder.so``: objects newer than their source and every header are kept."""
+    """``libs4d_decoder.so`` and the module of its calls; objects newer than their source and every header are kept."""
     obj_dir = os.path.join(LIB_DIR, "obj")
     headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".cuh")]
     headers += [os.path.join(INCLUDE, h) for h in os.listdir(INCLUDE)] + [os.path.abspath(__file__)]
@@ -76,7 +78,28 @@ def build_decoder(verbose_ptxas: bool = False, force: bool = False) -> str:
         _run([nvcc_path(), *ARCH_FLAGS, "--shared", "-o", DECODER_LIB_PATH + ".tmp", *objs, "-lcudart"],
              "libs4d_decoder.so", False)
         os.replace(DECODER_LIB_PATH + ".tmp", DECODER_LIB_PATH)
+    build_calls(force)
     return DECODER_LIB_PATH
+
+
+def build_calls(force: bool = False) -> str:
+    """The Python module of csrc/decoder_calls.cpp (host code against torch's headers; it needs no nvcc)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    src = os.path.join(CSRC, "decoder_calls.cpp")
+    deps = [src, os.path.join(INCLUDE, "s4d_dfa.h"), os.path.join(INCLUDE, "s4d_decoder.h")]
+    if not force and os.path.exists(CALLS_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(CALLS_PATH) for d in deps):
+        return CALLS_PATH
+    os.makedirs(LIB_DIR, exist_ok=True)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    dirs = [INCLUDE, *include_paths(), sysconfig.get_paths()["include"], cuda]
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(a for d in dirs for a in ("-I", d)),
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", CALLS_PATH + ".tmp", src, "-L",
+          os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
+         "s4d_decoder_calls.so", False)
+    os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
+    return CALLS_PATH
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:

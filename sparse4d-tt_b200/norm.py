@@ -59,6 +59,10 @@ def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optio
     ``x [..., width]``, ``mean`` and ``rstd`` (fp32, ``[...]``) as ``decoder_norm_backward`` takes
     them.  ``out``: a contiguous tensor like ``x`` to write ``y`` into (it may be ``x`` itself)."""
     name = "decoder_norm_forward"
+    if out is None:
+        done = D.calls().norm_forward(x, weight, bias, eps)
+        if done is not None:
+            return done
     index = D.same_device(name, x, weight, bias, out)
     width, dtype = _width(name, x), x.dtype
     pt = torch.float32 if weight is None else _param(name, "weight", weight, dtype, width)
@@ -98,6 +102,10 @@ def decoder_norm_backward(dout: Tensor, x: Tensor, weight: Optional[Tensor], mea
     and ``dbias`` are ``[width]`` in ``param_dtype`` (the weight's type, or fp32 without a weight),
     summed over all rows in fp32 in an order that depends on the sizes alone."""
     name = "decoder_norm_backward"
+    if param_dtype is None or (weight is not None and param_dtype == weight.dtype):
+        done = D.calls().norm_backward(dout, x, weight, mean, rstd, need_dx, need_dweight, need_dbias)
+        if done is not None:
+            return done
     index = D.same_device(name, x, dout, weight, mean, rstd)
     width, dtype, shape = _width(name, x), x.dtype, x.shape
     if dout.dtype != dtype:

@@ -239,3 +239,16 @@ def test_overlap():
     assert not D.overlap(x[:50], x[50:]) and D.overlap(x[:51], x[50:])
     assert not D.overlap(x[:0], x) and not D.overlap(x, torch.zeros(3))
     assert D.overlap(x[0].expand(5, 64), x[0]) and not D.overlap(x[0].expand(5, 64), x[1])
+
+
+def test_calls_module_leaves_what_is_not_its_to_take():
+    """Tensors off the current CUDA device, wrong counts and wrong kinds of arguments answer None."""
+    c = D.calls()
+    x, s = torch.zeros(4, 8), torch.zeros(4)
+    assert c.norm_forward(x, None, None, 1e-5) is None
+    assert c.norm_forward(x, None, None) is None and c.norm_forward(None, None, None, 1e-5) is None
+    assert c.norm_forward(3, None, None, 1e-5) is None
+    assert c.norm_backward(x, x, None, s, s, True, True, True) is None
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    assert c.attention_forward(q, q, q, None, 0.0, *[None] * 6) is None
+    assert c.attention_forward(None, None, None, None, 0.0, *[None] * 6) is None

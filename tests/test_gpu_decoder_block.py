@@ -9,7 +9,9 @@ import torch.nn.functional as F
 
 from helpers import pcc
 from oracle import head_torch as oh
-from sparse4d_tt_b200 import decoder_attention, decoder_norm, ops
+from sparse4d_tt_b200 import _lib_decoder as lib_decoder
+from sparse4d_tt_b200 import (decoder_attention, decoder_attention_forward, decoder_norm, decoder_norm_backward,
+                              decoder_norm_forward, ops)
 from sparse4d_tt_b200 import synthetic as syn
 from sparse4d_tt_b200.graph import capture
 from sparse4d_tt_b200.head import HeadGraph, Sparse4DHead, preprocess_head_parameters
@@ -181,3 +183,71 @@ def test_head_option_checks(cuda_device, head_case):
     with pytest.raises(ValueError, match="instance_group"):
         run(Sparse4DHead("cuda:0", params, BASE), head_case,
             instance_group=torch.zeros(2, 900, dtype=torch.int32, device="cuda"))
+
+
+def test_calls_module_and_python_path_agree(cuda_device, monkeypatch):
+    """What the calls module takes, and what it leaves to the Python path, gives the same bits; what it cannot
+    take it leaves."""
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    x, dy, w, b = r(3, 40, 96), r(3, 40, 96), r(96), r(96)
+    q, k, v = r(2, 30, 4, 64).bfloat16(), r(2, 90, 2, 64).bfloat16(), r(2, 90, 2, 64).bfloat16()
+    how = dict(softcap=9.0, slopes=torch.rand(4, generator=g).cuda(), q_pos=r(2, 30, 2), k_pos=r(2, 90, 2),
+               q_segment=torch.randint(-1, 3, (2, 30), generator=g).int().cuda(),
+               k_segment=torch.randint(-1, 3, (2, 90), generator=g).int().cuda(),
+               k_len=torch.tensor([90, 50], dtype=torch.int32).cuda())
+    long = r(1, 1, 8, 128).bfloat16(), r(1, 20000, 1, 128).bfloat16(), r(1, 20000, 1, 128).bfloat16()
+    row = dict(how, slopes=torch.rand(2, 30, 4, generator=g).cuda())
+
+    def everything():
+        out = []
+        for t, p in ((x, (w, b)), (x.half(), (w, None)), (x.bfloat16(), (w.bfloat16(), b.bfloat16())), (x, (None, None)),
+                     (x[:, :0], (w, b)), (x[0, 0], (w, b))):
+            y, mean, rstd = decoder_norm_forward(t, *p)
+            d = dy.to(t.dtype)[:, :t.shape[1]] if t.dim() == 3 else dy[0, 0]
+            out += [y, mean, rstd, *decoder_norm_backward(d.contiguous(), t, p[0], mean, rstd),
+                    *decoder_norm_backward(d.contiguous(), t, p[0], mean, rstd, need_dx=False, need_dbias=False)]
+        for a in ((q, k, v), long, (q[:0], k[:0], v[:0]), (q.half(), k.half(), v.half())):
+            out += decoder_attention_forward(*a)
+        out += [*decoder_attention_forward(q, k, v, **how), *decoder_attention_forward(q, k, v, scale=0.5, **row)]
+        return out
+
+    class Leaves:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    taken = []
+
+    class Counts:
+        def __getattr__(self, name):
+            def call(*a):
+                done = getattr(calls, name)(*a)
+                taken.append(done is not None)
+                return done
+            return call
+
+    calls = lib_decoder.calls()
+    monkeypatch.setattr(lib_decoder, "_calls", Counts())
+    first = everything()
+    assert all(taken) and len(taken) == 24
+    monkeypatch.setattr(lib_decoder, "_calls", Leaves())
+    for a, b_ in zip(first, everything(), strict=True):
+        assert (a is None) == (b_ is None)
+        if a is not None:
+            assert a.shape == b_.shape and a.dtype == b_.dtype and a.is_contiguous() and torch.equal(a, b_)
+    monkeypatch.setattr(lib_decoder, "_calls", calls)
+    c = calls
+    for bad in (lambda: c.norm_forward(x.transpose(0, 1), w, b, 1e-5), lambda: c.norm_forward(x, w[:5], b, 1e-5),
+                lambda: c.norm_forward(x, w, b.half(), 1e-5), lambda: c.norm_forward(x.double(), None, None, 1e-5),
+                lambda: c.norm_forward(x, w.cpu(), b, 1e-5), lambda: c.norm_forward(x, w, b, float("nan")),
+                lambda: c.norm_backward(dy[:, :5], x, w, x[..., 0].contiguous(), x[..., 0].contiguous(), True, True, True),
+                lambda: c.norm_backward(dy, x, w, x[..., 0], x[..., 0], True, True, True),
+                lambda: c.attention_forward(q, k, v.half(), None, 0.0, *[None] * 6),
+                lambda: c.attention_forward(q[..., ::2], k[..., ::2], v[..., ::2], None, 0.0, *[None] * 6),
+                lambda: c.attention_forward(q, k, v, None, 0.0, how["slopes"], *[None] * 5),
+                lambda: c.attention_forward(q, k, v, None, 0.0, None, how["q_pos"], *[None] * 4),
+                lambda: c.attention_forward(q, k, v, None, 0.0, how["slopes"], how["q_pos"], how["q_pos"], *[None] * 3),
+                lambda: c.attention_forward(q, k, v, None, 0.0, None, None, None, how["q_segment"], None, None),
+                lambda: c.attention_forward(q, k, v, None, 5e3, *[None] * 6),
+                lambda: c.attention_forward(q, k, v, q, 0.0, *[None] * 6)):
+        assert bad() is None
