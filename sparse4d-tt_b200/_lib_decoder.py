@@ -1,5 +1,5 @@
 """ctypes binding of ``lib/libs4d_decoder.so`` (the C ABI declared in ``include/s4d_decoder.h``), and
-the module that takes the calls which need nothing but a launch (``csrc/decoder_calls.cpp``).
+the module that takes the calls which need nothing but launches (``csrc/decoder_calls.cpp``).
 
 The library is loaded on first use.  If it is missing, every operator of it raises instead of
 falling back to another implementation.
@@ -107,7 +107,8 @@ def calls():
                 loader.exec_module(module)
                 module.init(*(C.cast(getattr(handle, n), C.c_void_p).value for n in (
                     "s4d_norm_forward", "s4d_norm_backward_workspace_bytes", "s4d_norm_backward",
-                    "s4d_attention_forward_workspace_bytes", "s4d_attention_forward")))
+                    "s4d_attention_forward_workspace_bytes", "s4d_attention_forward",
+                    "s4d_attention_backward_workspace_bytes", "s4d_attention_backward")))
                 _calls = module
     return _calls
 

@@ -208,6 +208,11 @@ def decoder_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, ou
     ``need_dkv`` / ``need_dslopes`` False leave those out (None).  Positions have no gradient.  No
     atomics: equal calls give equal bits."""
     name = "decoder_attention_backward"
+    if error_flag is None:
+        done = D.calls().attention_backward(dout, q, k, v, out, lse, scale, softcap, slopes, q_pos, k_pos, q_segment,
+                                            k_segment, k_len, need_dkv, need_dslopes)
+        if done is not None:
+            return done
     a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
     D.same_device(name, q, dout, out, lse)
     B, nq, _, H = a.sizes[:4]

@@ -96,7 +96,7 @@ def build_calls(force: bool = False) -> str:
     dirs = [INCLUDE, *include_paths(), sysconfig.get_paths()["include"], cuda]
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(a for d in dirs for a in ("-I", d)),
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", CALLS_PATH + ".tmp", src, "-L",
-          os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
+          os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"],
          "s4d_decoder_calls.so", False)
     os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
     return CALLS_PATH

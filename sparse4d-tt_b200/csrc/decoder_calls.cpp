@@ -1,17 +1,17 @@
-// The decoder's forward passes and the norm's backward pass as calls from Python, for the calls that need
-// nothing but a launch: every tensor on the current CUDA device, in place as the kernels read it.  Checks,
+// The decoder's attention and norm, forward and backward, as calls from Python, for the calls that need
+// nothing but launches: every tensor on the current CUDA device, in place as the kernels read it.  Checks,
 // results, workspace and launch are one call here; anything else (another device, a layout that needs
 // a copy, an argument that is to be refused) returns None, and attention.py and norm.py take the call
 // from its start, with the copies and the messages.
 //
-// A small call is bound by the host: forward and backward norm of 900 x 256 take 5.4 us on the GPU, and
-// took 34 us of calls from Python.
+// A small call is bound by the host: forward and backward norm of 900 x 256 take 5.4 us on the GPU, 34 us of
+// calls from Python and 16.5 from here; attention of 13 queries over 600 keys 8.7, 17.8 and 7.
 //
 // The C ABI's functions come as addresses (init), so that the library that lib() loaded is the one called.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -29,6 +29,8 @@ decltype(&s4d_norm_backward_workspace_bytes) norm_backward_ws_fn;
 decltype(&s4d_norm_backward) norm_backward_fn;
 decltype(&s4d_attention_forward_workspace_bytes) attention_forward_ws_fn;
 decltype(&s4d_attention_forward) attention_forward_fn;
+decltype(&s4d_attention_backward_workspace_bytes) attention_backward_ws_fn;
+decltype(&s4d_attention_backward) attention_backward_fn;
 
 // The arguments of one call.  ok() is false from the first that does not fit on.
 class Args {
@@ -81,7 +83,7 @@ int dtype_of(at::ScalarType t) {
 }
 
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int device) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, c10::DeviceIndex(device)));
+  return at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, c10::DeviceIndex(device)), std::nullopt);
 }
 
 void* address(const at::Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
@@ -176,48 +178,55 @@ bool operand(Args& a, const at::Tensor* t, int64_t* stride) {
   return a.ok();
 }
 
-// (q, k, v, scale or None, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len; the last six or None)
-// -> (out, lse) or None
-PyObject* attention_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  Args a(args, n, 11);
-  const at::Tensor *q = a.tensor(0), *k = a.tensor(1), *v = a.tensor(2);
-  if (!a.ok() || q->dim() != 4 || k->dim() != 4) Py_RETURN_NONE;
+// q, k, v, scale or None, softcap, slopes, q_pos, k_pos, q_segment, k_segment and k_len (the last six or None),
+// from argument `at` on.
+bool attention_args(Args& a, int at, s4d_attention_args& c) {
+  const at::Tensor *q = a.tensor(at), *k = a.tensor(at + 1), *v = a.tensor(at + 2);
+  if (!a.ok() || q->dim() != 4 || k->dim() != 4) return false;
   const at::ScalarType type = q->scalar_type();
-  s4d_attention_args c = {};
   c.batch = q->size(0), c.queries = q->size(1), c.heads = q->size(2), c.dim = q->size(3);
   c.keys = k->size(1), c.kv_heads = k->size(2);
   a.need((type == at::kBFloat16 || type == at::kHalf) && k->scalar_type() == type && v->scalar_type() == type &&
          k->size(0) == c.batch && k->size(3) == c.dim && v->sizes() == k->sizes());
-  if (!a.ok() || !operand(a, q, c.q_stride) || !operand(a, k, c.k_stride) || !operand(a, v, c.v_stride)) Py_RETURN_NONE;
+  if (!a.ok() || !operand(a, q, c.q_stride) || !operand(a, k, c.k_stride) || !operand(a, v, c.v_stride)) return false;
   c.q = q->data_ptr(), c.k = k->data_ptr(), c.v = v->data_ptr();
   c.dtype = dtype_of(type);
-  c.scale = a.none(3) ? float(std::pow(double(c.dim), -0.5)) : a.number(3);
-  c.softcap = a.number(4);
-  const at::Tensor* slopes = a.tensor(5, true);
+  c.scale = a.none(at + 3) ? float(std::pow(double(c.dim), -0.5)) : a.number(at + 3);
+  c.softcap = a.number(at + 4);
+  const at::Tensor* slopes = a.tensor(at + 5, true);
   if (slopes != nullptr) {
-    const at::Tensor* qp = a.tensor(6);
-    if (!a.need(slopes->scalar_type() == at::kFloat && qp != nullptr && qp->dim() == 3)) Py_RETURN_NONE;
+    const at::Tensor* qp = a.tensor(at + 6);
+    if (!a.need(slopes->scalar_type() == at::kFloat && qp != nullptr && qp->dim() == 3)) return false;
     c.pos_dim = qp->size(2);
-    qp = a.tensor(6, at::kFloat, {c.batch, c.queries, c.pos_dim});
-    const at::Tensor* kp = a.tensor(7, at::kFloat, {c.batch, c.keys, c.pos_dim});
+    qp = a.tensor(at + 6, at::kFloat, {c.batch, c.queries, c.pos_dim});
+    const at::Tensor* kp = a.tensor(at + 7, at::kFloat, {c.batch, c.keys, c.pos_dim});
     a.need(c.pos_dim == 1 || c.pos_dim == 2);
     if (slopes->dim() == 1)
       a.need(slopes->size(0) == c.heads), c.slope_stride[2] = slopes->stride(0);
     else if (a.need(slopes->sizes() == at::IntArrayRef({c.batch, c.queries, c.heads})))
       for (int i = 0; i < 3; ++i) c.slope_stride[i] = slopes->stride(i);
-    if (!a.ok()) Py_RETURN_NONE;
+    if (!a.ok()) return false;
     c.slopes = slopes->data_ptr<float>(), c.q_pos = qp->data_ptr<float>(), c.k_pos = kp->data_ptr<float>();
-  } else {
-    a.need(a.none(6) && a.none(7));
+    c.dslopes_per_row = slopes->dim() == 3;
+  } else if (!a.need(a.none(at + 6) && a.none(at + 7))) {
+    return false;
   }
-  a.need(a.none(8) == a.none(9));
-  const at::Tensor *qs = a.tensor(8, at::kInt, {c.batch, c.queries}, true), *ks = a.tensor(9, at::kInt, {c.batch, c.keys}, true);
-  const at::Tensor* kl = a.tensor(10, at::kInt, {c.batch}, true);
-  if (!a.ok()) Py_RETURN_NONE;
-  c.q_segment = static_cast<const int32_t*>(address(qs)), c.k_segment = static_cast<const int32_t*>(address(ks));
-  c.k_len = static_cast<const int32_t*>(address(kl));
-  at::Tensor out = empty(q->sizes(), type, a.device()), lse = empty({c.batch, c.heads, c.queries}, at::kFloat, a.device()), ws;
+  a.need(a.none(at + 8) == a.none(at + 9));
+  c.q_segment = static_cast<const int32_t*>(address(a.tensor(at + 8, at::kInt, {c.batch, c.queries}, true)));
+  c.k_segment = static_cast<const int32_t*>(address(a.tensor(at + 9, at::kInt, {c.batch, c.keys}, true)));
+  c.k_len = static_cast<const int32_t*>(address(a.tensor(at + 10, at::kInt, {c.batch}, true)));
+  return a.ok();
+}
+
+// (the eleven arguments above) -> (out, lse) or None
+PyObject* attention_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(args, n, 11);
+  s4d_attention_args c = {};
+  if (!attention_args(a, 0, c)) Py_RETURN_NONE;
+  const at::Tensor& q = THPVariable_Unpack(args[0]);
+  at::Tensor out = empty(q.sizes(), q.scalar_type(), a.device()), ws;
+  at::Tensor lse = empty({c.batch, c.heads, c.queries}, at::kFloat, a.device());
   c.out = out.data_ptr();
   c.lse = lse.data_ptr<float>();
   c.workspace_bytes = attention_forward_ws_fn(&c);
@@ -230,15 +239,55 @@ PyObject* attention_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (addresses of the five functions above) -> None
+// (dout, q, k, v, out, lse, the other eight of the eleven, need_dkv, need_dslopes) -> (dq, dk, dv, dslopes) or
+// None
+PyObject* attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 16) Py_RETURN_NONE;
+  // in attention_args' order: q, k, v and the rest; then dout, out and lse
+  PyObject* const order[14] = {args[1],  args[2],  args[3],  args[6],  args[7],  args[8], args[9],
+                               args[10], args[11], args[12], args[13], args[0], args[4], args[5]};
+  Args a(order, 14, 14);
+  s4d_attention_args c = {};
+  if (!attention_args(a, 0, c) || c.dtype != S4D_DTYPE_BF16 || c.batch == 0) Py_RETURN_NONE;
+  const at::Tensor &q = THPVariable_Unpack(args[1]), &k = THPVariable_Unpack(args[2]);
+  const at::Tensor* dout = a.tensor(11);
+  if (!a.ok() || dout->scalar_type() != at::kBFloat16 || dout->sizes() != q.sizes() || !operand(a, dout, c.dout_stride))
+    Py_RETURN_NONE;
+  const at::Tensor *out = a.tensor(12, at::kBFloat16, q.sizes()), *lse = a.tensor(13, at::kFloat, {c.batch, c.heads, c.queries});
+  if (!a.ok()) Py_RETURN_NONE;
+  c.dout = dout->data_ptr(), c.out = out->data_ptr(), c.lse = lse->data_ptr<float>();
+  at::Tensor dq = empty(q.sizes(), at::kBFloat16, a.device()), dk, dv, ds, ws;
+  c.dq = dq.data_ptr();
+  if (PyObject_IsTrue(args[14]) == 1) {
+    dk = empty(k.sizes(), at::kBFloat16, a.device()), dv = empty(k.sizes(), at::kBFloat16, a.device());
+    c.dk = dk.data_ptr(), c.dv = dv.data_ptr();
+  }
+  if (c.slopes != nullptr && PyObject_IsTrue(args[15]) == 1) {
+    ds = empty(THPVariable_Unpack(args[8]).sizes(), at::kFloat, a.device());
+    c.dslopes = ds.data_ptr<float>();
+  }
+  c.workspace_bytes = attention_backward_ws_fn(&c);
+  if (c.workspace_bytes > 0) {
+    ws = empty({int64_t(c.workspace_bytes / 4)}, at::kFloat, a.device());
+    c.workspace = ws.data_ptr();
+  }
+  if (attention_backward_fn(&c, a.stream()) != S4D_OK) Py_RETURN_NONE;
+  return pack({dq, dk, dv, ds});
+  END_HANDLE_TH_ERRORS
+}
+
+// (addresses of the seven functions above) -> None
 PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long at[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", &at[0], &at[1], &at[2], &at[3], &at[4])) return nullptr;
+  unsigned long long at[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6])) return nullptr;
   norm_forward_fn = reinterpret_cast<decltype(norm_forward_fn)>(at[0]);
   norm_backward_ws_fn = reinterpret_cast<decltype(norm_backward_ws_fn)>(at[1]);
   norm_backward_fn = reinterpret_cast<decltype(norm_backward_fn)>(at[2]);
   attention_forward_ws_fn = reinterpret_cast<decltype(attention_forward_ws_fn)>(at[3]);
   attention_forward_fn = reinterpret_cast<decltype(attention_forward_fn)>(at[4]);
+  attention_backward_ws_fn = reinterpret_cast<decltype(attention_backward_ws_fn)>(at[5]);
+  attention_backward_fn = reinterpret_cast<decltype(attention_backward_fn)>(at[6]);
   Py_RETURN_NONE;
 }
 
@@ -252,6 +301,7 @@ PyMethodDef methods[] = {
     {"norm_forward", fast(norm_forward), METH_FASTCALL, nullptr},
     {"norm_backward", fast(norm_backward), METH_FASTCALL, nullptr},
     {"attention_forward", fast(attention_forward), METH_FASTCALL, nullptr},
+    {"attention_backward", fast(attention_backward), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "s4d_decoder_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -10,8 +10,8 @@ import torch.nn.functional as F
 from helpers import pcc
 from oracle import head_torch as oh
 from sparse4d_tt_b200 import _lib_decoder as lib_decoder
-from sparse4d_tt_b200 import (decoder_attention, decoder_attention_forward, decoder_norm, decoder_norm_backward,
-                              decoder_norm_forward, ops)
+from sparse4d_tt_b200 import (decoder_attention, decoder_attention_backward, decoder_attention_forward, decoder_norm,
+                              decoder_norm_backward, decoder_norm_forward, ops)
 from sparse4d_tt_b200 import synthetic as syn
 from sparse4d_tt_b200.graph import capture
 from sparse4d_tt_b200.head import HeadGraph, Sparse4DHead, preprocess_head_parameters
@@ -209,7 +209,11 @@ def test_calls_module_and_python_path_agree(cuda_device, monkeypatch):
                     *decoder_norm_backward(d.contiguous(), t, p[0], mean, rstd, need_dx=False, need_dbias=False)]
         for a in ((q, k, v), long, (q[:0], k[:0], v[:0]), (q.half(), k.half(), v.half())):
             out += decoder_attention_forward(*a)
-        out += [*decoder_attention_forward(q, k, v, **how), *decoder_attention_forward(q, k, v, scale=0.5, **row)]
+        for kw in (how, dict(row, scale=0.5), {}, dict(k_len=how["k_len"])):
+            o, lse = decoder_attention_forward(q, k, v, **kw)
+            out += [o, lse, *decoder_attention_backward(o, q, k, v, o, lse, **kw),
+                    *decoder_attention_backward(o.transpose(1, 2).contiguous().transpose(1, 2), q, k, v, o, lse, **kw,
+                                                need_dkv=False, need_dslopes=False)]
         return out
 
     class Leaves:
@@ -229,7 +233,7 @@ def test_calls_module_and_python_path_agree(cuda_device, monkeypatch):
     calls = lib_decoder.calls()
     monkeypatch.setattr(lib_decoder, "_calls", Counts())
     first = everything()
-    assert all(taken) and len(taken) == 24
+    assert all(taken) and len(taken) == 34
     monkeypatch.setattr(lib_decoder, "_calls", Leaves())
     for a, b_ in zip(first, everything(), strict=True):
         assert (a is None) == (b_ is None)
@@ -249,5 +253,9 @@ def test_calls_module_and_python_path_agree(cuda_device, monkeypatch):
                 lambda: c.attention_forward(q, k, v, None, 0.0, how["slopes"], how["q_pos"], how["q_pos"], *[None] * 3),
                 lambda: c.attention_forward(q, k, v, None, 0.0, None, None, None, how["q_segment"], None, None),
                 lambda: c.attention_forward(q, k, v, None, 5e3, *[None] * 6),
-                lambda: c.attention_forward(q, k, v, q, 0.0, *[None] * 6)):
+                lambda: c.attention_forward(q, k, v, q, 0.0, *[None] * 6),
+                lambda: c.attention_backward(q, q, k, v, q, x, None, 0.0, *[None] * 6, True, True),
+                lambda: c.attention_backward(q.half(), q, k, v, q, x, None, 0.0, *[None] * 6, True, True),
+                lambda: c.attention_backward(q, q, k, v, q, None, None, 0.0, *[None] * 6, True, True),
+                lambda: c.attention_backward(q, q, k, v)):
         assert bad() is None
