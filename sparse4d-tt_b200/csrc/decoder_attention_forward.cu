@@ -23,6 +23,11 @@
 // warps, one for the even and one for the odd tiles, each with its own O, m and l, joined at the
 // end (at D = 128 tensor memory holds one O).
 //
+// FEW: a row tile of a few rows only.  A thread that computes 64 scores is then what a tile waits for, while
+// most lanes of the products hold nothing.  So the rows are there four times, once in each quarter of the
+// lanes, and a quarter's warp weighs 16 keys of the tile (its other weights are 0); the copies have their
+// own O, m and l and are joined like the parts of a cluster.
+//
 // Few rows and many keys: the keys are cut into parts, a CTA each.  Up to eight parts are one cluster:
 // every CTA leaves its O, m and l in shared memory and each joins a share of the rows from its peers'.
 // More parts write normalised O and log-sum-exp to memory and a second launch joins them.
@@ -38,7 +43,8 @@
 namespace s4d {
 namespace {
 
-constexpr int kKeys = 64;  // keys of a tile
+constexpr int kKeys = 64;     // keys of a tile
+constexpr int kFewRows = 32;  // FEW: the rows' four copies are this far apart
 
 template <int DP>
 struct Fwd {
@@ -61,13 +67,13 @@ struct Fwd {
   static size_t smem(int64_t tiles) { return size_t(kKinds) + size_t((tiles + 15) / 16 * 16) + 1024; }
 };
 
-// 32 scores of a row, in base 2, and their maximum.
-template <int POS, bool CAP, bool MASKED>
-__device__ __forceinline__ void scores(uint32_t (&r)[32], const ScoreConst& k, float slope2, float qx, float qy,
+// CH scores of a row, in base 2, and their maximum.
+template <int POS, bool CAP, bool MASKED, int CH>
+__device__ __forceinline__ void scores(uint32_t (&r)[CH], const ScoreConst& k, float slope2, float qx, float qy,
                                        int seg, bool sees, const float* aux, float& mx) {
   const F2 x2 = f2(qx), y2 = f2(qy), nslope = f2(-slope2), k1 = f2(k.k1), c = f2(k.c), nc = f2(-k.c);
 #pragma unroll
-  for (int j4 = 0; j4 < 32; j4 += 4) {
+  for (int j4 = 0; j4 < CH; j4 += 4) {
     float4 x4, y4;
     int4 s4;
     if constexpr (POS > 0) x4 = *reinterpret_cast<const float4*>(aux + j4);
@@ -97,10 +103,10 @@ __device__ __forceinline__ void scores(uint32_t (&r)[32], const ScoreConst& k, f
 }
 
 // Their weights 2^(s - m) as 16-bit pairs, and the sum of the unrounded weights.
-template <typename T>
-__device__ __forceinline__ void weights(const uint32_t (&r)[32], F2 nbase, F2 (&sum)[2], uint32_t* w) {
+template <typename T, int CH>
+__device__ __forceinline__ void weights(const uint32_t (&r)[CH], F2 nbase, F2 (&sum)[2], uint32_t* w) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
+  for (int e = 0; e < CH / 2; ++e) {
     float a, d;
     split(add2(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), nbase), a, d);
     a = ex2(a), d = ex2(d);
@@ -109,7 +115,7 @@ __device__ __forceinline__ void weights(const uint32_t (&r)[32], F2 nbase, F2 (&
   }
 }
 
-template <typename T, int DP, int POS, bool CAP>
+template <typename T, int DP, int POS, bool CAP, bool FEW>
 __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     attention_forward_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                              const __grid_constant__ CUtensorMap vm, const AttnParams p) {
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   }
   if (warp == S::kWarps + 1) tmem_alloc(smem_u32(tmem_slot), S::kCols);
   griddep_wait();
-  const bool q_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
+  const bool q_by_tma = !FEW && kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
   if (q_by_tma && warp == S::kWarps && lane == 0) {
     mbar_expect_tx(q_full, S::kQ);
 #pragma unroll
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   if (!q_by_tma) {
     for (int c = threadIdx.x; c < kAttnRows * (DP / 8); c += S::kThreads) {
       const int r = c / (DP / 8), d = c % (DP / 8);
-      const uint32_t at = uint32_t(row0) + r;
+      const uint32_t at = uint32_t(row0) + (FEW ? r % kFewRows : r);
       uint4 v = make_uint4(0, 0, 0, 0);
       if (at < rows && d * 8 < p.dim)
         v = ldg_nc_v4(static_cast<const T*>(p.q) + b * p.q_sb + int64_t(at / rep) * p.q_sn +
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
   tc_fence_after();
   griddep_launch_dependents();  // tensor memory is allocated: a kernel behind this one cannot take it away
   const int stream = warp / 4, tid = threadIdx.x & 127;  // tid: the row, and the tensor-memory lane
-  const int64_t row = row0 + tid;
+  const int64_t row = row0 + (FEW ? tid % kFewRows : tid);
   const bool live = row < rows;
   const uint32_t i = live ? (rep == 1 ? uint32_t(row) : uint32_t(row) / rep) : 0;
   const int h = int(g * rep + (live ? uint32_t(row) - i * rep : 0));
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     __syncwarp();
   } else {
     const uint32_t lanes = uint32_t(warp % 4 * 32) << 16;
-    const bool warp_live = row0 + warp % 4 * 32 < rows;
+    const bool warp_live = FEW || row0 + warp % 4 * 32 < rows;
     const ScoreConst k(p);
     float slope2 = 0.0f, qx = 0.0f, qy = 0.0f;
     int seg = 0;       // without segments 0
@@ -323,7 +329,16 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         // With two streams a thread has 96 registers: the first half of the scores waits in tensor memory.
         uint32_t r0[32], r1[32];
         float mx = -INFINITY;
-        if constexpr (S::kStreams == 2) {
+        uint32_t rf[16];  // FEW: the warp's quarter of the keys
+        const int quarter = warp % 4;
+        if constexpr (FEW) {
+          tmem_ld16_async(tmem_s + quarter * 16, rf);
+          tmem_ld_wait(rf);
+          if (masked)
+            scores<POS, CAP, true>(rf, k, slope2, qx, qy, seg, sees, aux + quarter * 16, mx);
+          else
+            scores<POS, CAP, false>(rf, k, slope2, qx, qy, seg, sees, aux + quarter * 16, mx);
+        } else if constexpr (S::kStreams == 2) {
           tmem_ld32_async(tmem_s, r0);
           tmem_ld_wait(r0);
           if (masked)
@@ -343,10 +358,12 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
           else
             scores<POS, CAP, false>(r0, k, slope2, qx, qy, seg, sees, aux, mx);
         }
-        if (masked)
-          scores<POS, CAP, true>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
-        else
-          scores<POS, CAP, false>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
+        if constexpr (!FEW) {
+          if (masked)
+            scores<POS, CAP, true>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
+          else
+            scores<POS, CAP, false>(r1, k, slope2, qx, qy, seg, sees, aux + 32, mx);
+        }
         const bool grow = mx > m + 8.0f || (m == -INFINITY && mx > m);
         const bool any_grow = __any_sync(0xffffffffu, grow);
         if (!first_tile && (any_grow || bad))  // O is about to change outside the tensor cores
@@ -369,15 +386,24 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         }
         const F2 nbase = f2(m == -INFINITY ? 0.0f : -m);  // no key yet: every score is -inf, every weight 0
         F2 sum[2] = {f2(0.0f), f2(0.0f)};
-        uint32_t w[32];
-        weights<T>(r1, nbase, sum, w + 16);
-        if constexpr (S::kStreams == 2) {
-          tmem_st_wait();
-          tmem_ld32_async(tmem_s, r0);
-          tmem_ld_wait(r0);
+        if constexpr (FEW) {
+          // the other quarters' weights of this copy of the row are 0
+          uint32_t w[8], none[8] = {};
+          weights<T>(rf, nbase, sum, w);
+          tmem_st(tmem_s + quarter * 8, w);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) tmem_st(tmem_s + (quarter + e) % 4 * 8, none);
+        } else {
+          uint32_t w[32];
+          weights<T>(r1, nbase, sum, w + 16);
+          if constexpr (S::kStreams == 2) {
+            tmem_st_wait();
+            tmem_ld32_async(tmem_s, r0);
+            tmem_ld_wait(r0);
+          }
+          weights<T>(r0, nbase, sum, w);
+          tmem_st32(tmem_s, w);
         }
-        weights<T>(r0, nbase, sum, w);
-        tmem_st32(tmem_s, w);
         float a, d;
         split(add2(sum[0], sum[1]), a, d);
         l += a + d;
@@ -405,7 +431,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     const float total = dead ? __int_as_float(0x7fc00000) : S::kStreams == 2 ? fmaf(l, f0, l1 * f1) : l;
     const bool any0 = l != 0.0f, any1 = l1 != 0.0f;  // else tensor memory holds nothing of this row
     const int64_t out_row = (b * p.nq + i) * p.heads + h;
-    if (p.cluster > 1) {
+    if (FEW || p.cluster > 1) {
       // O (not yet divided by l) and m, l stay in shared memory for the cluster: O over the K and V tiles,
       // which nothing reads any more, 16-byte piece j of row r at j ^ (r & 7)
       if constexpr (S::kStreams == 2) barrier_sync(3, S::kWarps * 32);
@@ -439,7 +465,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
 #pragma unroll
           for (int e = 0; e < 32; ++e) f[e] = any1 ? fmaf(__uint_as_float(o[e]), f1, f[e]) : f[e];
         }
-        if (p.cluster > 1) {
+        if (FEW || p.cluster > 1) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             *reinterpret_cast<float4*>(smem + S::kK + tid * (DP * 4) + (((c * 8 + e) ^ (tid & 7)) << 4)) =
@@ -472,41 +498,42 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     tmem_dealloc(tmem, S::kCols);
   }
   if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
-  if (p.cluster == 1) return;
+  if (!FEW && p.cluster == 1) return;
 
-  // The cluster's rows: DP / 8 lanes a row, 8 columns a lane; this CTA takes rows part, part + cluster, ...
+  // The cluster's rows: DP / 8 lanes a row, 8 columns a lane; this CTA takes rows rank, rank + cluster, ...
   constexpr int kLanes = DP / 8, kRowsPerWarp = 32 / kLanes;
   const int col = lane % kLanes * 8;
-  for (int r = part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && row0 + r < rows;
+  const int rank = p.cluster > 1 ? part : 0;
+  for (int r = rank + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < (FEW ? kFewRows : kAttnRows) && row0 + r < rows;
        r += p.cluster * kRowsPerWarp * (S::kThreads / 32)) {
     const uint32_t at = uint32_t(row0) + r, qi = rep == 1 ? at : at / rep, hh = g * rep + (at - qi * rep);
     const int64_t out_row = (b * p.nq + qi) * p.heads + hh, lse_row = (int64_t(b) * p.heads + hh) * p.nq + qi;
     const uint32_t at_ml = sbase + S::kAux + r * 8, at_o = sbase + S::kK + r * (DP * 4);
     const uint32_t piece0 = at_o + (((col / 4) ^ (r & 7)) << 4), piece1 = at_o + (((col / 4 + 1) ^ (r & 7)) << 4);
-    // four peers at a time, all their loads before the first use
+    // four peers at a time (FEW: the four copies of one), all their loads before the first use
     float top = -INFINITY, total = 0.0f;
     float4 o0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o1 = o0;
-    for (int s0 = 0; s0 < p.cluster; s0 += 4) {
+    for (int s0 = 0; s0 < p.cluster; s0 += FEW ? 1 : 4) {
       float2 v[4];
       float4 x[4], y[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const uint32_t peer = min(s0 + s, p.cluster - 1);
-        v[s] = peer_f2(peer_addr(at_ml, peer));
-        x[s] = peer_f4(peer_addr(piece0, peer));
-        y[s] = peer_f4(peer_addr(piece1, peer));
+        const uint32_t peer = FEW ? s0 : min(s0 + s, p.cluster - 1), copy = FEW ? s * kFewRows : 0;
+        v[s] = peer_f2(peer_addr(at_ml + copy * 8, peer));
+        x[s] = peer_f4(peer_addr(piece0 + copy * (DP * 4), peer));
+        y[s] = peer_f4(peer_addr(piece1 + copy * (DP * 4), peer));
       }
       float high = top;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        if (s0 + s < p.cluster) high = fmaxf(high, v[s].x);
+        if (FEW || s0 + s < p.cluster) high = fmaxf(high, v[s].x);
       const float base = high == -INFINITY ? 0.0f : high, old = ex2(top - base);
       top = high;
       total *= old;
       o0.x *= old, o0.y *= old, o0.z *= old, o0.w *= old, o1.x *= old, o1.y *= old, o1.z *= old, o1.w *= old;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        if (s0 + s >= p.cluster) continue;
+        if (!FEW && s0 + s >= p.cluster) continue;
         const float w = ex2(v[s].x - base);  // 0 for a part without keys
         total = fmaf(v[s].y, w, total);
         o0.x = fmaf(w, x[s].x, o0.x), o0.y = fmaf(w, x[s].y, o0.y), o0.z = fmaf(w, x[s].z, o0.z),
@@ -516,13 +543,24 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // no key: zeros
-    if (col == 0 && p.lse != nullptr) p.lse[lse_row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+    const float lse = total == 0.0f ? -INFINITY : (top + log2f(total)) * kLn2;
+    if (FEW && p.splits != p.cluster) {  // one of many parts
+      const int64_t all = int64_t(p.batch) * p.nq * p.heads;
+      if (col == 0) p.part_lse[part * all + lse_row] = lse;
+      if (col < p.dim) {
+        float4* dst = reinterpret_cast<float4*>(p.part_o + (part * all + out_row) * p.dim + col);
+        dst[0] = make_float4(o0.x * inv, o0.y * inv, o0.z * inv, o0.w * inv);
+        dst[1] = make_float4(o1.x * inv, o1.y * inv, o1.z * inv, o1.w * inv);
+      }
+      continue;
+    }
+    if (col == 0 && p.lse != nullptr) p.lse[lse_row] = lse;
     if (col < p.dim)
       *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row * p.dim + col) =
           make_uint4(pack2<T>(o0.x * inv, o0.y * inv), pack2<T>(o0.z * inv, o0.w * inv),
                      pack2<T>(o1.x * inv, o1.y * inv), pack2<T>(o1.z * inv, o1.w * inv));
   }
-  cluster_sync();  // the peers still read this CTA's shared memory
+  if (p.cluster > 1) cluster_sync();  // the peers still read this CTA's shared memory
 }
 
 // Joins the parts of one row: o = sum_s 2^(lse_s - lse) o_s.  One warp a row, lanes along D.
@@ -559,10 +597,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
   if (lane == 0 && p.lse != nullptr) p.lse[lse_row] = total == 0.0f ? -INFINITY : base + log2f(total) * kLn2;
 }
 
-template <typename T, int DP, int POS, bool CAP>
-int launch(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
+template <typename T, int DP, int POS, bool CAP, bool FEW>
+int launch_kernel(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
   static bool smem_set[64] = {};
-  const int rc = set_kernel_smem(attention_forward_kernel<T, DP, POS, CAP>, Fwd<DP>::smem(kAttnMaxTiles),
+  const int rc = set_kernel_smem(attention_forward_kernel<T, DP, POS, CAP, FEW>, Fwd<DP>::smem(kAttnMaxTiles),
                                  "cudaFuncSetAttribute(attention_forward_kernel)", smem_set);
   if (rc != S4D_OK) return rc;
   const int64_t row_tiles = (p.nq * p.rep + kAttnRows - 1) / kAttnRows;
@@ -585,8 +623,20 @@ int launch(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
     attr[cfg.numAttrs++].val.clusterDim.z = 1;
   }
   cfg.attrs = attr;
-  return cuda_check(cudaLaunchKernelEx(&cfg, attention_forward_kernel<T, DP, POS, CAP>, m.q, m.k, m.v, p),
+  return cuda_check(cudaLaunchKernelEx(&cfg, attention_forward_kernel<T, DP, POS, CAP, FEW>, m.q, m.k, m.v, p),
                     "attention_forward_kernel launch");
+}
+
+// A row tile of eight rows or fewer is held four times where a score costs more than its product with K and
+// V: 4 x 1 query over 65,536 keys, 8 shared heads of 128, 1-D distance 215 us without, 199 with it; 8 x 1
+// over 16,384, 8 heads of 64, 2-D distance 74 and 55; 2 queries over 4 x 4,000, 8 shared heads of 128
+// 20.3 and 19.5.  Plain scores over heads of 64 lose (8 queries over 2 x 20,000, 16 heads: 35.5 and
+// 38 us), and so do more rows, which are fetched one by one (6 x 30 over 900: 10.6 and 12.8 us).
+template <typename T, int DP, int POS, bool CAP>
+int launch(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
+  if constexpr (DP > 64 || POS > 0 || CAP)
+    if (p.nq * p.rep <= 8) return launch_kernel<T, DP, POS, CAP, true>(p, m, st);
+  return launch_kernel<T, DP, POS, CAP, false>(p, m, st);
 }
 
 template <typename T, int DP>

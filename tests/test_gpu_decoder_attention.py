@@ -562,3 +562,36 @@ def test_gradients_of_parts_with_masked_values_that_are_no_numbers(cuda_device, 
     for grads in [run() for _ in range(10)] + [graph.replay()]:
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(grads, first))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D,how", [
+    (1, 1, 1, 1, 1, 128, {}), (2, 1, 70, 8, 1, 64, dict(pos=1)), (3, 2, 333, 12, 3, 72, dict(cap=12.0)),
+    (2, 8, 900, 3, 3, 64, dict(pos=2, slopes="row")), (1, 1, 9000, 4, 2, 40, dict(pos=2)), (2, 3, 64, 4, 2, 128, {}),
+    (4, 1, 5000, 8, 8, 128, dict(pos=1, k_len=[5000, 0, 1, 4097])), (2, 9, 500, 2, 2, 128, dict(pos=1)),
+])
+def test_few_rows(cuda_device, dtype, B, Nq, Nk, H, G, D, how):
+    q, k, v, how = make(B, Nq, Nk, H, G, D, dtype, **how)
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    check_forward(q, k, v, how, out, lse)
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip((out, lse), decoder_attention_forward(q, k, v, **how)))
+
+
+@pytest.mark.parametrize("Nk", [300, 3000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_with_documents_and_values_that_are_no_numbers(cuda_device, D, Nk):
+    """Documents of which a query's own lies in one quarter of a tile, a query of none, and NaN and infinity in
+    the others' values and past the valid keys."""
+    ks = torch.arange(Nk) // 13
+    ks[Nk - 100:] = -1
+    q, k, v, how = make(2, 4, Nk, 4, 2, D, pos=2, segments=([0, 3, -1, 7], ks), k_len=[Nk, 95])
+    want = decoder_attention_forward(q, k, v, **how)
+    check_forward(q, k, v, how, *want)
+    k2, v2 = k.clone(), v.clone()
+    hidden = ~torch.isin(ks, torch.tensor([0, 3, 7])).cuda()
+    k2[:, hidden], v2[:, hidden] = float("nan"), float("inf")
+    v2[1, 95:] = float("nan")
+    for _ in range(10):
+        out, lse = decoder_attention_forward(q, k2, v2, **how)
+        check_forward(q, k, v, how, out, lse)
