@@ -16,7 +16,7 @@
 // than the rows: 16,384 x 4,096 bf16 forward 69 us against 49 us.
 // Up to eight warps a row the registers are held to what lets three (backward: two) blocks of eight warps
 // share an SM: what a block waits for, the others load over.  16,384 x 4,096 bf16 both passes 172 us with
-// the compiler's choice (two and one), 158 so; 7,213 x 1,001 f16 26.9 and 25.8.
+// the compiler's choice (two and one), 158 so (136 by now); 7,213 x 1,001 f16 26.9 and 25.8.
 //
 // The sums over rows for dw and db stay in registers: a block adds its row groups through shared memory
 // and writes one fp32 partial row per block; a second launch adds the partial rows in block order.
@@ -69,9 +69,15 @@ __device__ __forceinline__ float group_sum(float v, float* red) {
     if ((threadIdx.x & 31) == 0) red[warp] = v;
     __syncthreads();
     const float* r = red + warp / W * W;
-    v = 0.0f;
+    if constexpr (W < 8) {
+      v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) v += r[i];
+      for (int i = 0; i < W; ++i) v += r[i];
+    } else {  // the unrolled loads are all issued at once and would take W registers
+      v = r[threadIdx.x % W];
+#pragma unroll
+      for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
   }
   return v;
 }
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(Group<W>::kThreads, W <= 8 ? 2 : 1) norm_backw
   const float inv = 1.0f / float(p.width);
   int buf = 0;
   // the next row's loads under way during this row's sums, where the registers allow it
-  constexpr bool kAhead = sizeof(T) == 2 && W < 16 && (VEC == 8 || K == 8);
+  constexpr bool kAhead = sizeof(T) == 2 && W < 32 && (VEC == 8 || K == 8);
   RawVec<T, VEC> rx[K], rd[K];
   auto load_row = [&](int64_t row) {
     const T* xr = static_cast<const T*>(p.x) + row * p.x_ld;
@@ -319,9 +325,19 @@ __global__ void __launch_bounds__(Group<W>::kThreads, W <= 8 ? 2 : 1) norm_backw
       if ((threadIdx.x & 31) == 0) red[buf][0][warp] = s1, red[buf][1][warp] = s2;
       __syncthreads();
       const int w0 = warp / W * W;
-      s1 = s2 = 0.0f;
+      if constexpr (W < 8) {
+        s1 = s2 = 0.0f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) s1 += red[buf][0][w0 + i], s2 += red[buf][1][w0 + i];
+        for (int i = 0; i < W; ++i) s1 += red[buf][0][w0 + i], s2 += red[buf][1][w0 + i];
+      } else {  // as in group_sum (both passes of 16,384 x 4,096 bf16 158 us with the loads, 136 so; 4,096 x
+                // 16,384 472 and 273)
+        s1 = red[buf][0][w0 + threadIdx.x % W], s2 = red[buf][1][w0 + threadIdx.x % W];
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) {
+          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+          s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+        }
+      }
     }
     if (!live) continue;
     s1 *= inv, s2 *= inv;
