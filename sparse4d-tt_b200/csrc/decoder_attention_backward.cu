@@ -285,7 +285,9 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   if (p.k_len != nullptr) valid = min(valid, max(int64_t(0), int64_t(__ldg(p.k_len + b))));
   const int first = PARTS ? own.part * int(p.tiles_per_split) : 0;  // the part's first tile of keys
   const int tiles = max(0, min(int(p.tiles_per_split), int((valid + kCols - 1) / kCols) - first));
-  const bool own_by_tma = kAttnRows % p.rep == 0;  // the tile is 128 / rep whole queries
+  // the tile is 128 / rep whole queries; nothing is fetched for a part without keys, whose row threads leave zeros
+  // for the cluster over Q and dO without waiting for anything
+  const bool gather = kAttnRows % p.rep != 0, own_by_tma = !gather && tiles > 0;
 
   if (warp == S::kWarps && lane == 0) {
     for (int s = 0; s < S::kKStages; ++s) {
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
         write_record<POS>(p, b, int(g * rep + e % rep), e / rep, -INFINITY, 0.0f, 0.0f, 0.0f, 0.0f, -1);
     }
   }
-  if (!own_by_tma) {
+  if (gather && tiles > 0) {
     for (int c = threadIdx.x; c < 2 * kAttnRows * (DP / 8); c += S::kThreads) {
       const bool is_do = c >= kAttnRows * (DP / 8);
       const int e = is_do ? c - kAttnRows * (DP / 8) : c, r = e / (DP / 8), d = e % (DP / 8);

@@ -595,3 +595,20 @@ def test_few_rows_with_documents_and_values_that_are_no_numbers(cuda_device, D, 
     for _ in range(10):
         out, lse = decoder_attention_forward(q, k2, v2, **how)
         check_forward(q, k, v, how, out, lse)
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D,how", [
+    (1, 1024, 1100, 2, 2, 64, dict(k_len=[100])), (1, 1024, 1100, 2, 2, 64, dict(k_len=[0], pos=2)),
+    (1, 1000, 1100, 2, 2, 128, dict(k_len=[100], cap=20.0)), (2, 500, 1100, 2, 2, 128, dict(k_len=[0, 500])),
+    (1, 300, 900, 6, 2, 64, dict(k_len=[70], pos=1, slopes="row")),   # Q and dO gathered, not by TMA
+    (1, 300, 3100, 2, 2, 64, dict()),                                 # 49 tiles of keys in eight parts of seven
+    (1, 3100, 200, 2, 1, 64, dict(pos=1)), (1, 3100, 200, 2, 2, 128, dict(k_len=[130])),
+])
+def test_gradients_of_parts_without_keys(cuda_device, B, Nq, Nk, H, G, D, how):
+    """Own tiles cut into parts of which some have nothing to walk: they add zeros, call after call."""
+    q, k, v, how = make(B, Nq, Nk, H, G, D, **how)
+    dout, grads = gradients(q, k, v, how)
+    check_backward(q, k, v, how, dout, grads)
+    for _ in range(30):
+        again = gradients(q, k, v, how)[1]
+        assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(grads, again))
