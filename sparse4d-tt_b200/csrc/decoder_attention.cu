@@ -160,6 +160,8 @@ AttnParams fill(const s4d_attention_args& a) {
   AttnParams p{};
   const Strides q(a.q_stride, a.batch, a.queries, a.heads);
   p.q = a.q, p.q_sb = q.b, p.q_sn = q.n, p.q_sh = q.h;
+  const Strides v(a.v_stride, a.batch, a.keys, a.kv_heads);
+  p.v = a.v, p.v_sb = v.b, p.v_sn = v.n, p.v_sh = v.h;
   p.out = a.out, p.lse = a.lse;
   p.slopes = a.slopes, p.sl_b = a.slope_stride[0], p.sl_n = a.slope_stride[1], p.sl_h = a.slope_stride[2];
   p.q_pos = a.q_pos, p.k_pos = a.k_pos, p.q_seg = a.q_segment, p.k_seg = a.k_segment, p.k_len = a.k_len;

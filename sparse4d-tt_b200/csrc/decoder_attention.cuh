@@ -28,6 +28,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct AttnParams {
   const void* q;
   int64_t q_sb, q_sn, q_sh;  // element strides of batch, row and head
+  const void* v;             // (forward)
+  int64_t v_sb, v_sn, v_sh;
   const void* dout;
   int64_t do_sb, do_sn, do_sh;
   void* out;   // [B, Nq, H, D] contiguous (backward: read)

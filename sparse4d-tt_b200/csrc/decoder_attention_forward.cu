@@ -26,7 +26,9 @@
 // FEW: a row tile of a few rows only.  A thread that computes 64 scores is then what a tile waits for, while
 // most lanes of the products hold nothing.  So the rows are there four times, once in each quarter of the
 // lanes, and a quarter's warp weighs 16 keys of the tile (its other weights are 0); the copies have their
-// own O, m and l and are joined like the parts of a cluster.
+// own O, m and l and are joined like the parts of a cluster.  Those zeros stand for keys that the row sees:
+// times an infinity they make a column of O a NaN, which is put right at the end (seen_not_finite), since to look
+// through every tile's V first took one query over 4 x 65,536 keys from 208 to 237 us.
 //
 // Few rows and many keys: the keys are cut into parts, a CTA each.  Up to eight parts are one cluster:
 // every CTA leaves its O, m and l in shared memory and each joins a share of the rows from its peers'.
@@ -112,6 +114,35 @@ __device__ __forceinline__ void weights(const uint32_t (&r)[CH], F2 nbase, F2 (&
     a = ex2(a), d = ex2(d);
     sum[e & 1] = add2(sum[e & 1], f2(a, d));
     w[e] = pack2<T>(a, d);
+  }
+}
+
+// FEW: columns [col, col + 32) of a copy's O that came out as no numbers.  Such a column is the sum of the
+// infinities and NaNs among the values of the keys that this copy weighs (16 of every 64 from key `begin`)
+// and the row sees, or has none: then another copy has them, and here any number will do.
+template <typename T>
+__device__ __forceinline__ void seen_not_finite(float (&f)[32], const AttnParams& p, int b, int g, int64_t begin, int64_t end,
+                                                int seg, bool sees, int col) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) f[e] = isfinite(f[e]) ? f[e] : 0.0f;
+  if (!sees) return;
+  const int32_t* k_seg = p.k_seg != nullptr ? p.k_seg + b * p.nk : nullptr;
+  const T* v = static_cast<const T*>(p.v) + b * p.v_sb + g * p.v_sh + col;
+#pragma unroll 1
+  for (int64_t key = begin; key < end; key = (key + 1) % 16 == 0 ? key + 1 + kKeys - 16 : key + 1) {
+    if (k_seg != nullptr && __ldg(k_seg + key) != seg) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (col + e * 8 >= p.dim) break;
+      const uint4 x = ldg_nc_v4(v + key * p.v_sn + e * 8);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 y = unpack2<T>(w[i]);
+        if (!isfinite(y.x)) f[8 * e + 2 * i] += y.x;
+        if (!isfinite(y.y)) f[8 * e + 2 * i + 1] += y.y;
+      }
+    }
   }
 }
 
@@ -464,6 +495,13 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
           tmem_ld_wait(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) f[e] = any1 ? fmaf(__uint_as_float(o[e]), f1, f[e]) : f[e];
+        }
+        if constexpr (FEW) {
+          bool finite = true;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) finite = finite && isfinite(f[e]);
+          if (!finite && live)
+            seen_not_finite<T>(f, p, b, g, first * kKeys + warp % 4 * 16, min(valid, (first + tiles) * kKeys), seg, sees, c * 32);
         }
         if (FEW || p.cluster > 1) {
 #pragma unroll

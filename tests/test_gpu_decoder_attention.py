@@ -612,3 +612,28 @@ def test_gradients_of_parts_without_keys(cuda_device, B, Nq, Nk, H, G, D, how):
     for _ in range(30):
         again = gradients(q, k, v, how)[1]
         assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Nq", [1, 4, 5, 70])  # on both sides of eight rows
+@pytest.mark.parametrize("D,pos,cap,Nk", [(64, 0, 5.0, 200), (64, 2, 0.0, 200), (128, 0, 0.0, 330), (128, 1, 0.0, 20000),
+                                          (64, 0, 0.0, 200)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_values_that_are_seen_and_no_numbers(cuda_device, D, pos, cap, Nk, Nq, dtype, bad):
+    """An infinity in a value that a row sees is that infinity in out, a NaN a NaN, in that column and no other:
+    in full tiles and in the ragged last one, whatever the number of rows."""
+    q, k, v, how = make(1, Nq, Nk, 2, 1, D, dtype, pos=pos, cap=cap)
+    if pos:
+        how["slopes"] = how["slopes"] / 20  # no weight underflows
+    clean = decoder_attention_forward(q, k, v, **how)
+    check_forward(q, k, v, how, *clean)
+    hit = {5: 3, 17: D - 1, 70: 9, Nk - 1: 12}  # key: column
+    v2 = v.clone()
+    for key, col in hit.items():
+        v2[:, key, :, col] = bad
+    cols = torch.zeros(D, dtype=torch.bool, device="cuda")
+    cols[list(hit.values())] = True
+    out, lse = decoder_attention_forward(q, k, v2, **how)
+    assert torch.equal(lse, clean[1])
+    assert torch.isnan(out[..., cols]).all() if math.isnan(bad) else (out[..., cols] == bad).all()
+    check_forward(q, k, torch.where(cols, torch.zeros_like(v), v), how, torch.where(cols, torch.zeros_like(out), out), lse)
