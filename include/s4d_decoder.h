@@ -61,7 +61,8 @@ S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int6
  *   out_i = sum_j softmax_j(s) v_j over the seen keys, 0 for a query that sees none;
  *   lse_i = log sum_j exp(s), -inf for such a query.
  * What q, k, v and the positions hold at pairs that are not seen never reaches out: an infinity or
- * a NaN there changes nothing.  Distances of two coordinates are roots of an f32 sum of squares, so
+ * a NaN there changes nothing.  An infinity in a value that is seen is one in out, unless its weight
+ * underflows in `dtype` (then it may be a NaN).  Distances of two coordinates are roots of an f32 sum of squares, so
  * differences of positions stay below 2^63.  No result overlaps an argument.
  *
  *   dtype         S4D_DTYPE_BF16 or S4D_DTYPE_F16, of q, k, v and out

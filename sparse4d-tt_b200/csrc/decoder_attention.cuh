@@ -463,11 +463,13 @@ __device__ __forceinline__ bool row_not_finite(const unsigned char* tile, int bl
   return bad;
 }
 
-// acc[lane, :] (+)= sum over the ROWS rows j of a tile with a[lane, j] != 0 of a[lane, j] tile[j, :]:
-// what mma_accumulate computes, except that a zero weight hides the row's infinities and NaNs
-// instead of turning them into NaN.  For tiles that are masked in part and hold such values.
+// acc[lane, :] (+)= sum over the rows j in [begin, end) (multiples of 16) of a tile of ROWS rows whose segment ids[j]
+// is the lane's (`seg`, when it `sees` anything) of a[lane, j] tile[j, :]: what mma_accumulate computes, except
+// that the other rows' infinities and NaNs take no part instead of being multiplied by 0.  A weight of a row that
+// is seen which came out as 0 makes them NaN, as there.  For tiles that are masked in part and hold such values.
 template <typename T, int DP, int ROWS, int STEP = 8>
-__device__ __noinline__ void accumulate_nonzero(uint32_t acc, uint32_t a, const unsigned char* tile, bool init) {
+__device__ __noinline__ void accumulate_seen(uint32_t acc, uint32_t a, const unsigned char* tile, bool init, const int* ids,
+                                             int seg, bool sees, int begin = 0, int end = ROWS) {
   for (int c = 0; c < DP / 16; ++c) {
     float o[16];
     uint32_t r[16];
@@ -476,16 +478,16 @@ __device__ __noinline__ void accumulate_nonzero(uint32_t acc, uint32_t a, const 
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = init ? 0.0f : __uint_as_float(r[i]);
     const unsigned char* block = tile + (c / 4) * (ROWS * 128);
-    for (int j0 = 0; j0 < ROWS; j0 += 16) {
+    for (int j0 = begin; j0 < end; j0 += 16) {
       uint32_t w[8];
       tmem_ld8_async(a + j0 / 16 * STEP, w);
       tmem_ld_wait(w);
 #pragma unroll
       for (int jj = 0; jj < 16; ++jj) {
+        const int j = j0 + jj;
+        if (!sees || ids[j] != seg) continue;
         const float2 pr = unpack2<T>(w[jj / 2]);
         const float weight = jj & 1 ? pr.y : pr.x;
-        if (weight == 0.0f) continue;
-        const int j = j0 + jj;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint4 v = *reinterpret_cast<const uint4*>(block + j * 128 + ((((c % 4) * 2 + h) ^ (j & 7)) << 4));

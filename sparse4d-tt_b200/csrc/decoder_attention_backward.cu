@@ -522,8 +522,9 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
         if (bad) {
           // dQ is about to change outside the tensor cores
           dead = !earlier_done<S::kBuffers>(acc_done, n, abort_flag, p.wait_limit_ns);
-          if (!dead) accumulate_nonzero<T, DP, kCols, 16>(tmem_o + lanes, tmem_s, kt, n == 0);
-          if (!dead) accumulate_nonzero<T, DP, kCols, 16>(tmem_o + DP + lanes, tmem_s + 8, kt, n == 0);
+          const int* ids = reinterpret_cast<const int*>(aux + 2 * kCols);
+          if (!dead) accumulate_seen<T, DP, kCols, 16>(tmem_o + lanes, tmem_s, kt, n == 0, ids, seg, sees);
+          if (!dead) accumulate_seen<T, DP, kCols, 16>(tmem_o + DP + lanes, tmem_s + 8, kt, n == 0, ids, seg, sees);
         }
       }
       warp_arrive(ds_full + 8 * buf.stage);
@@ -862,8 +863,9 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
           // dV and dK are about to change outside the tensor cores
           dead = !earlier_done<S::kBuffers>(acc_done, n, abort_flag, p.wait_limit_ns);
           if (!dead) {
-            accumulate_nonzero<T, DP, kCols>(tmem_dv + lanes, tmem_s, dot, n == 0);
-            accumulate_nonzero<T, DP, kCols>(tmem_dk + lanes, tmem_s + kCols, qt, n == 0);
+            const int* ids = reinterpret_cast<const int*>(aux + 5 * kCols);
+            accumulate_seen<T, DP, kCols>(tmem_dv + lanes, tmem_s, dot, n == 0, ids, seg, sees);
+            accumulate_seen<T, DP, kCols>(tmem_dk + lanes, tmem_s + kCols, qt, n == 0, ids, seg, sees);
           }
         }
       }

@@ -439,7 +439,9 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
         split(add2(sum[0], sum[1]), a, d);
         l += a + d;
         tmem_st_wait();
-        if (bad && !dead) accumulate_nonzero<T, DP, kKeys>(tmem_acc, tmem_s, vt, first_tile);
+        if (bad && !dead)  // FEW: this copy's quarter of the keys
+          accumulate_seen<T, DP, kKeys>(tmem_acc, tmem_s, vt, first_tile, reinterpret_cast<const int*>(aux + 2 * kKeys), seg,
+                                        sees, FEW ? quarter * 16 : 0, FEW ? quarter * 16 + 16 : kKeys);
       }
       warp_arrive(p_full + 8 * (n & 1));
       t = next;
@@ -620,9 +622,9 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p)
   const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
-    const float w = ex2((p.part_lse[s * rows + lse_row] - base) * kLog2e);
+    const float lse = p.part_lse[s * rows + lse_row], w = ex2((lse - base) * kLog2e);
     total += w;
-    if (mine && w != 0.0f) {  // a part without keys has weight 0
+    if (mine && lse != -INFINITY) {  // a part without keys has weight 0
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * p.dim + lane * 4);
       o[0] = fmaf(w, v.x, o[0]), o[1] = fmaf(w, v.y, o[1]), o[2] = fmaf(w, v.z, o[2]), o[3] = fmaf(w, v.w, o[3]);
     }

@@ -637,3 +637,26 @@ def test_values_that_are_seen_and_no_numbers(cuda_device, D, pos, cap, Nk, Nq, d
     assert torch.equal(lse, clean[1])
     assert torch.isnan(out[..., cols]).all() if math.isnan(bad) else (out[..., cols] == bad).all()
     check_forward(q, k, torch.where(cols, torch.zeros_like(v), v), how, torch.where(cols, torch.zeros_like(out), out), lse)
+
+
+@pytest.mark.parametrize("Nk", [100, 128, 20000])  # key 80 in a ragged tile, in a full one, in the first of many parts
+@pytest.mark.parametrize("Nq", [2, 40])
+@pytest.mark.parametrize("D", [64, 128])
+def test_seen_values_whose_weight_underflows(cuda_device, D, Nq, Nk):
+    """A NaN in a seen value is one in out also when its weight is 0 in fp32, and so is one of a query's output gradient
+    in dv: as 0 times NaN is in the definition."""
+    q, k, v, how = make(1, Nq, Nk, 1, 1, D, pos=1)
+    how["slopes"] = how["slopes"] * 0 + 1
+    how["k_pos"][:] = 300.0  # 2^-432 beside the last key
+    how["q_pos"][:], how["k_pos"][:, -1] = 0.0, 0.0
+    v[:, 80, :, 5] = math.nan
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    assert torch.isnan(out[..., 5]).all() and torch.isfinite(lse).all()
+    keep = torch.arange(D, device="cuda") != 5
+    assert torch.equal(out[..., keep], v[:, -1:, :, keep].expand(-1, Nq, -1, -1))
+    if Nk <= 128:
+        v[:, 80, :, 5] = 0.0
+        dout = torch.ones_like(q)
+        dout[:, 1, :, 3] = math.nan
+        dv = decoder_attention_backward(dout, q, k, v, *decoder_attention_forward(q, k, v, **how), **how)[2]
+        assert torch.isnan(dv[..., 3]).all() and torch.isfinite(dv[..., :3]).all() and torch.isfinite(dv[..., 4:]).all()
