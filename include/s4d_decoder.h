@@ -28,6 +28,14 @@ enum { S4D_DTYPE_F16 = 2 };
 S4D_API int s4d_decoder_abi_version(void);
 S4D_API const char* s4d_decoder_last_error(void);
 
+/* Failure detection of the attention's kernels: a wait on one of their own barriers that takes longer than this
+ * many nanoseconds gives up.  The block then sets S4D_FLAG_WAIT_TIMEOUT in the call's error_flag, waits for the
+ * copies and products that it has under way and leaves NaNs in its rows of the results (a backward pass also in
+ * the rows of dk and dv that those rows reach).  Applies to launches from the calling host thread; default
+ * 2,000,000,000 (2 s), never expected to run out.  For tests: with 0 the kernels' copies stop half way, so that
+ * waits do run out.  Returns the previous limit. */
+S4D_API uint64_t s4d_decoder_set_wait_limit_ns(uint64_t limit_ns);
+
 /* LayerNorm over rows of `width` elements (nn.LayerNorm, biased variance):
  *   y[r, :] = (x[r, :] - mean[r]) * rstd[r] * weight + bias,  rstd = 1 / sqrt(var + eps)
  *   x, y        [rows, width] of `dtype`, unit column stride, row strides x_ld / y_ld (elements;
@@ -78,7 +86,7 @@ S4D_API int s4d_norm_backward(const void* dy, int64_t dy_ld, const void* x, int6
  *   k_len         [batch] int32 or NULL (all keys); values outside 0 .. keys are clamped
  *   workspace     s4d_attention_forward_workspace_bytes(args) bytes, 16-byte aligned, used by this call
  *                 only while it runs (0 bytes: may be NULL)
- *   error_flag    int32 or NULL: S4D_FLAG_WAIT_TIMEOUT as in s4d_dfa.h
+ *   error_flag    int32 or NULL: S4D_FLAG_WAIT_TIMEOUT (see s4d_decoder_set_wait_limit_ns)
  *   softcap       0 (none), or up to 1024: a capped score is off by a few 2^-23 softcap
  * P is rounded to `dtype` for its product with v; sums and softmax statistics are f32.  Equal calls
  * give equal bits.  batch and the axes may be 0; rows of one shared head (queries * heads /

@@ -48,6 +48,7 @@ ATTENTION_ARGS = struct.Struct(
 SIGNATURES = {
     "s4d_decoder_abi_version": (_int, []),
     "s4d_decoder_last_error": (C.c_char_p, []),
+    "s4d_decoder_set_wait_limit_ns": (C.c_uint64, [C.c_uint64]),
     "s4d_attention_forward_workspace_bytes": (_sz, [C.c_char_p]),
     "s4d_attention_forward": (_int, [C.c_char_p, _p]),
     "s4d_attention_backward_workspace_bytes": (_sz, [C.c_char_p]),
@@ -59,7 +60,7 @@ SIGNATURES = {
 }
 
 # Version of include/s4d_decoder.h these bindings are written for (s4d_decoder_abi_version()).
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _lib = None

@@ -164,7 +164,7 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
     fp32 give the distance bias; ``q_segment [B, Nq]`` and ``k_segment [B, Nk]`` int32 the document
     mask; ``k_len [B]`` int32 the valid keys of each batch entry (read on the device, clamped to
     0 .. Nk).  ``out``: a contiguous tensor like ``q`` to write into (not one of the arguments).  ``error_flag`` (int32) gets
-    ``S4D_FLAG_WAIT_TIMEOUT`` should a kernel give up waiting; the results are then not valid."""
+    ``S4D_FLAG_WAIT_TIMEOUT`` should a kernel give up waiting; the rows concerned are then NaN."""
     name = "decoder_attention_forward"
     if out is None and error_flag is None:
         done = D.calls().attention_forward(q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len)

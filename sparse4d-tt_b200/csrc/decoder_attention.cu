@@ -6,6 +6,9 @@
 #include "decoder_attention.cuh"
 
 namespace s4d {
+
+unsigned long long decoder_wait_limit_ns();  // decoder_capi.cu
+
 namespace {
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -169,7 +172,7 @@ AttnParams fill(const s4d_attention_args& a) {
   p.batch = int(a.batch), p.heads = int(a.heads), p.kv_heads = int(a.kv_heads), p.rep = int(a.heads / a.kv_heads);
   p.dim = int(a.dim), p.scale = a.scale, p.cap = a.softcap;
   p.error_flag = a.error_flag;
-  p.wait_limit_ns = kWaitLimitNs;
+  p.wait_limit_ns = decoder_wait_limit_ns();
   return p;
 }
 

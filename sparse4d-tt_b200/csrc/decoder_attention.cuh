@@ -375,6 +375,11 @@ __device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity, volati
   }
 }
 
+// With a limit of 0 the warp that fetches the tiles stops half way, so that the other warps' waits do run out.
+__device__ __forceinline__ bool withheld(const AttnParams& p, int t, int tiles) {
+  return p.wait_limit_ns == 0 && 2 * (t + 1) > tiles;
+}
+
 // Warp-uniform bounded wait (the tensor-memory loads behind it are warp-collective).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           unsigned long long limit_ns) {
@@ -601,6 +606,19 @@ __device__ __forceinline__ float4 peer_f4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ int peer_int(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// Whether the flag at `addr` of any CTA of the cluster is set.
+__device__ __forceinline__ bool cluster_any(uint32_t addr, int cluster) {
+  int any = 0;
+  for (int s = 0; s < cluster; ++s) any |= peer_int(peer_addr(addr, s));
+  return any != 0;
+}
+
 // Four of the fp32 values at `addr` of every CTA of the cluster, added in the order of the ranks.
 __device__ __forceinline__ float4 cluster_sum(uint32_t addr, int cluster) {
   float4 v[8], sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -620,6 +638,13 @@ __device__ __forceinline__ float cluster_sum1(uint32_t addr, int cluster) {
     sum += v;
   }
   return sum;
+}
+
+// NaNs over a row of `dim` 16-bit values, from a CTA that gave up waiting: what it computed is not to pass for
+// a result.
+__device__ __forceinline__ void store_nans(void* base, int64_t row, int dim) {
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + row * dim);
+  for (int c = 0; c < dim / 8; ++c) dst[c] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------

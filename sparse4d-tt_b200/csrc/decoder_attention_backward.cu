@@ -203,18 +203,17 @@ template <int N>
 __device__ __forceinline__ uint32_t shared_piece(uint32_t base, int r, int j) {
   return base + r * (N * 4) + ((j ^ (r & 7)) << 4);
 }
-// ... from the accumulators (zeros when nothing was accumulated, NaN from a CTA that gave up).
+// ... from the accumulators (zeros when nothing was accumulated).
 template <int N, int STREAMS>
-__device__ __forceinline__ void share_rows(unsigned char* smem, uint32_t acc, int row, int stream, bool any, bool dead) {
+__device__ __forceinline__ void share_rows(unsigned char* smem, uint32_t acc, int row, int stream, bool any) {
   for (int c = stream; c < N / 32; c += STREAMS) {
     uint32_t o[32];
     tmem_ld32_async(acc + c * 32, o);
     tmem_ld_wait(o);
-    const uint32_t none = dead ? 0x7fc00000u : 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       *reinterpret_cast<uint4*>(smem + row * (N * 4) + (((c * 8 + e) ^ (row & 7)) << 4)) =
-          any && !dead ? make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_uint4(none, none, none, none);
+          any ? make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]) : make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   if (warp == S::kWarps) {
     int n = 0;
     Ring kr, vr;
-    for (int t = t0; t < tiles; ++n) {
+    for (int t = t0; t < tiles && !withheld(p, t, tiles); ++n) {
       // V first: its stage is free once dP is there, K's only after dQ
       if (n >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       if (lane == 0) load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, (first + t) * kCols, b);
@@ -545,15 +544,13 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     // What a row's sums and products give.  With an exact delta sum dS would be 0; the O that delta was made
     // from is rounded to 16 bits (and made from 16-bit P), so delta is short of that sum, sum dS dist is off
     // by it times sum P dist, and dQ by it times P K.
-    auto finish_row = [&](const float (&total)[3]) {
-      write_record<POS>(p, b, h, i, -lse2, -(delta + total[0]), -qx, -qy, -slope2, sees ? seg : -1);
+    auto finish_row = [&](const float (&total)[3], float add) {  // add: 0, or the NaN of a CTA that gave up
+      write_record<POS>(p, b, h, i, -lse2 + add, -(delta + total[0]), -qx, -qy, -slope2, sees ? seg : -1);
       if constexpr (POS > 0)
-        if (p.dslopes != nullptr)
-          p.dslopes[p.dslopes_by_head ? lse_row : out_row] =
-              dead ? __int_as_float(0x7fc00000) : -fmaf(-total[0], total[2], total[1]);
+        if (p.dslopes != nullptr) p.dslopes[p.dslopes_by_head ? lse_row : out_row] = add - fmaf(-total[0], total[2], total[1]);
     };
     if constexpr (!PARTS) {
-      if (live && stream == 0) finish_row(sums);
+      if (live && stream == 0) finish_row(sums, 0.0f);
       if (!dead && warp_live) {
         // dQ's columns in 32s, shared out among the streams
         for (int c = stream; c * 32 < p.dim; c += S::kStreams) {
@@ -574,19 +571,21 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
       if (stream == 0)
 #pragma unroll
         for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) total[e * kAttnRows + tid] = sums[e];
-      share_rows<2 * DP, S::kStreams>(smem, tmem_o + lanes, tid, stream, t0 < tiles, dead);
+      share_rows<2 * DP, S::kStreams>(smem, tmem_o + lanes, tid, stream, t0 < tiles);
       cluster_sync();
+      // a NaN when a CTA of the cluster gave up: all of their roles are done, and with them what sets the flag
+      const float add = cluster_any(sbase + S::kCtl + 4, p.cluster) ? __int_as_float(0x7fc00000) : 0.0f;
       if (live && stream == 0 && tid % p.cluster == own.part) {
         float v[3] = {};
 #pragma unroll
         for (int e = 0; e < (POS > 0 ? 3 : 1); ++e) v[e] = cluster_sum1(smem_u32(total + e * kAttnRows + tid), p.cluster);
-        finish_row(v);
+        finish_row(v, add);
       }
       constexpr int kLanes = DP / 8, kRowsPerWarp = 32 / kLanes;
       const int col = lane % kLanes * 8;
       for (int r = own.part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && row0 + r < rows;
            r += p.cluster * kRowsPerWarp * S::kWarps) {
-        const float short_of = cluster_sum1(smem_u32(total + r), p.cluster);
+        const float short_of = cluster_sum1(smem_u32(total + r), p.cluster) + add;
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -613,7 +612,15 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
   }
-  if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  const bool gave_up = *abort_flag;
+  if (threadIdx.x == 0 && gave_up && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  // every role is done: rows of a CTA that gave up become NaN, and through their records dK and dV
+  if (!PARTS && gave_up && warp < 4 && live) {
+    const float nan = __int_as_float(0x7fc00000);
+    store_nans(p.dq, out_row, p.dim);
+    write_record<POS>(p, b, h, i, nan, nan, -qx, -qy, -slope2, sees ? seg : -1);
+    if (POS > 0 && p.dslopes != nullptr) p.dslopes[p.dslopes_by_head ? lse_row : out_row] = nan;
+  }
   if (PARTS && p.behind) griddep_wait();  // what follows this launch follows the one ahead too
 }
 
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     if (lane == 0) {
       int n = 0, hh = work ? 0 : p.rep, t = t0;
       Ring r;
-      for (; hh < p.rep; advance(hh, t), ++n) {
+      for (; hh < p.rep && !withheld(p, t, tiles); advance(hh, t), ++n) {
         if (n >= S::kStages && !sleep_wait(empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
         const uint32_t st = sbase + S::kQ + r.stage * 2 * S::kTile, bar = full + 8 * r.stage;
         const int h = g * p.rep + hh;
@@ -877,15 +884,16 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     if (!dead && work) dead = !warp_wait(o_full, 0, abort_flag, p.wait_limit_ns);
     if constexpr (PARTS) {
       // dV and dK of this part of the queries, for the cluster
-      share_rows<2 * DP, S::kStreams>(smem, tmem_dv + lanes, tid, stream, work, dead);
+      share_rows<2 * DP, S::kStreams>(smem, tmem_dv + lanes, tid, stream, work);
       cluster_sync();
+      const bool gave_up = cluster_any(sbase + S::kCtl + 4, p.cluster);  // as in the dQ kernel
       constexpr int kLanes = 2 * DP / 8, kRowsPerWarp = 32 / kLanes;
       const int at = lane % kLanes * 8, col = at % DP;
       for (int r = own.part + p.cluster * (warp * kRowsPerWarp + lane / kLanes); r < kAttnRows && key0 + r < p.nk;
            r += p.cluster * kRowsPerWarp * S::kWarps) {
         const float4 x = cluster_sum(shared_piece<2 * DP>(sbase, r, at / 4), p.cluster);
         const float4 y = cluster_sum(shared_piece<2 * DP>(sbase, r, at / 4 + 1), p.cluster);
-        const float f = at >= DP ? p.scale : 1.0f;
+        const float f = gave_up ? __int_as_float(0x7fc00000) : at >= DP ? p.scale : 1.0f;
         if (col < p.dim)
           *reinterpret_cast<uint4*>(static_cast<T*>(at >= DP ? p.dk : p.dv) +
                                     ((b * p.nk + key0 + r) * p.kv_heads + g) * p.dim + col) =
@@ -917,7 +925,12 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
   }
-  if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  const bool gave_up = *abort_flag;
+  if (threadIdx.x == 0 && gave_up && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  if (!PARTS && gave_up && warp < 4 && live) {  // as in the dQ kernel
+    store_nans(p.dk, (b * p.nk + key) * p.kv_heads + g, p.dim);
+    store_nans(p.dv, (b * p.nk + key) * p.kv_heads + g, p.dim);
+  }
   if (PARTS && p.behind) griddep_wait();  // what follows this launch follows the one ahead too
 }
 

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
       mbar_init(p_full + 8 * s, kRowWarps);
       mbar_init(pv_done + 8 * s, 1);
     }
-    mbar_init(o_full, 1);
+    mbar_init(o_full, 2);  // the products, and the warp that issued them or gave up
     mbar_init(q_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     };
     int n = 0, t = t0;
     Ring r, slot;
-    for (; t < tiles; ++n) {
+    for (; t < tiles && !withheld(p, t, tiles); ++n) {
       const bool again = n >= S::kStages;
       if (again && !warp_wait(k_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       load_k(r.stage, slot.stage, t);
@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     }
     if (leader) {
       mma_commit(o_full);  // also on the abort path: nothing may run once tensor memory is freed
+      mbar_arrive(o_full);
       mbar_wait(o_full, 0, nullptr);
     }
     __syncwarp();
@@ -460,15 +461,15 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     }
     const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
     float f0 = S::kStreams == 2 ? ex2(m - base) : 1.0f, f1 = S::kStreams == 2 ? ex2(m1 - base) : 0.0f;
-    // a CTA that gave up makes its rows NaN
-    const float total = dead ? __int_as_float(0x7fc00000) : S::kStreams == 2 ? fmaf(l, f0, l1 * f1) : l;
+    const float total = S::kStreams == 2 ? fmaf(l, f0, l1 * f1) : l;
     const bool any0 = l != 0.0f, any1 = l1 != 0.0f;  // else tensor memory holds nothing of this row
     const int64_t out_row = (b * p.nq + i) * p.heads + h;
     if (FEW || p.cluster > 1) {
       // O (not yet divided by l) and m, l stay in shared memory for the cluster: O over the K and V tiles,
       // which nothing reads any more, 16-byte piece j of row r at j ^ (r & 7)
       if constexpr (S::kStreams == 2) barrier_sync(3, S::kWarps * 32);
-      if (stream == 0) ml[tid] = make_float2(top, total);
+      // a CTA that gave up makes its rows NaN
+      if (stream == 0) ml[tid] = make_float2(top, *abort_flag ? __int_as_float(0x7fc00000) : total);
     } else {
       const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // no key: zeros
       f0 *= inv, f1 *= inv;
@@ -537,8 +538,23 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     tc_fence_after();
     tmem_dealloc(tmem, S::kCols);
   }
-  if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
-  if (!FEW && p.cluster == 1) return;
+  // Every role is done, and with it what sets the flag.  Rows that are stored already become NaN.
+  const bool gave_up = *abort_flag;
+  if (threadIdx.x == 0 && gave_up && p.error_flag != nullptr) atomicOr(p.error_flag, S4D_FLAG_WAIT_TIMEOUT);
+  if (!FEW && p.cluster == 1) {
+    if (gave_up && threadIdx.x < kAttnRows && row0 + threadIdx.x < rows) {
+      const uint32_t at = uint32_t(row0) + threadIdx.x, qi = at / rep, hh = g * rep + at % rep;
+      const int64_t lse_row = (int64_t(b) * p.heads + hh) * p.nq + qi;
+      const float nan = __int_as_float(0x7fc00000);
+      if (p.splits > 1) {
+        p.part_lse[part * (int64_t(p.batch) * p.nq * p.heads) + lse_row] = nan;  // and so the joined row
+      } else {
+        store_nans(p.out, (b * p.nq + qi) * p.heads + hh, p.dim);
+        if (p.lse != nullptr) p.lse[lse_row] = nan;
+      }
+    }
+    return;
+  }
 
   // The cluster's rows: DP / 8 lanes a row, 8 columns a lane; this CTA takes rows rank, rank + cluster, ...
   constexpr int kLanes = DP / 8, kRowsPerWarp = 32 / kLanes;

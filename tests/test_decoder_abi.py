@@ -252,3 +252,16 @@ def test_calls_module_leaves_what_is_not_its_to_take():
     q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
     assert c.attention_forward(q, q, q, None, 0.0, *[None] * 6) is None
     assert c.attention_forward(None, None, None, None, 0.0, *[None] * 6) is None
+
+
+def test_wait_limit_is_per_thread_and_restorable(lib):
+    import threading
+
+    prev = lib.s4d_decoder_set_wait_limit_ns(12345)
+    assert prev == 2_000_000_000
+    seen = []
+    t = threading.Thread(target=lambda: seen.append(lib.s4d_decoder_set_wait_limit_ns(7)))
+    t.start()
+    t.join()
+    assert seen == [2_000_000_000]  # another thread keeps its own default
+    assert lib.s4d_decoder_set_wait_limit_ns(prev) == 12345

@@ -11,7 +11,9 @@ import pytest
 import torch
 
 from attention_ref import U, half_step, reference, score_error
+from sparse4d_tt_b200 import _lib_decoder as lib_decoder
 from sparse4d_tt_b200 import decoder_attention, decoder_attention_backward, decoder_attention_forward
+from sparse4d_tt_b200._lib import S4D_FLAG_WAIT_TIMEOUT
 from sparse4d_tt_b200.graph import capture
 
 pytestmark = pytest.mark.gpu
@@ -660,3 +662,39 @@ def test_seen_values_whose_weight_underflows(cuda_device, D, Nq, Nk):
         dout[:, 1, :, 3] = math.nan
         dv = decoder_attention_backward(dout, q, k, v, *decoder_attention_forward(q, k, v, **how), **how)[2]
         assert torch.isnan(dv[..., 3]).all() and torch.isfinite(dv[..., :3]).all() and torch.isfinite(dv[..., 4:]).all()
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D,how", [
+    (2, 900, 900, 4, 4, 64, dict(pos=2)), (1, 400, 700, 4, 2, 128, dict(cap=20.0)),      # one CTA a row tile
+    (1, 3, 300, 6, 2, 64, {}), (1, 130, 2000, 3, 3, 128, dict(pos=1, slopes="row")),     # clusters, parts in the backward pass
+    (1, 1, 700, 2, 2, 128, {}), (1, 2, 40000, 2, 1, 64, dict(pos=1)),                    # few rows, few and many parts
+    (1, 40, 40000, 1, 1, 64, {}), (2, 500, 500, 2, 2, 64, dict(segments=(ids(300, 200), ids(300, 200)), k_len=[500, 400])),
+])
+def test_waits_that_run_out(cuda_device, B, Nq, Nk, H, G, D, how):
+    """With the limit at 0 the kernels' waits give up and return: the flag's bit is set, and every element of the
+    results is a NaN or what it should be; the next call is as ever.  Without a flag the NaNs tell."""
+    q, k, v, how = make(B, Nq, Nk, H, G, D, **how)
+    lib = lib_decoder.lib()
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    dout, want = gradients(q, k, v, how)
+    clean = (out, lse, *(t for t in want if t is not None))
+    flags = torch.zeros(2, dtype=torch.int32, device="cuda")
+    leaf = q.clone().requires_grad_()
+    prev = lib.s4d_decoder_set_wait_limit_ns(0)
+    try:
+        got = (*decoder_attention_forward(q, k, v, **how, error_flag=flags[:1]),
+               *(t for t in decoder_attention_backward(dout, q, k, v, out, lse, **how, error_flag=flags[1:]) if t is not None))
+        y = decoder_attention(leaf, k, v, **how)
+        y.backward(dout)
+    finally:
+        lib.s4d_decoder_set_wait_limit_ns(prev)
+    torch.cuda.synchronize()
+    assert prev == 2_000_000_000 and flags.tolist() == [S4D_FLAG_WAIT_TIMEOUT] * 2
+    for a, b in zip(got, clean):
+        gone = torch.isnan(a)
+        assert gone.any() and torch.equal(a.masked_fill(gone, 0), b.masked_fill(gone, 0))
+    assert torch.isnan(y).any() and torch.isnan(leaf.grad).any()
+    flags.zero_()
+    again = (*decoder_attention_forward(q, k, v, **how, error_flag=flags[:1]),
+             *(t for t in decoder_attention_backward(dout, q, k, v, out, lse, **how, error_flag=flags[1:]) if t is not None))
+    assert flags.tolist() == [0, 0] and all(torch.equal(a, b) for a, b in zip(again, clean))
