@@ -394,28 +394,28 @@ __global__ void __launch_bounds__(Dq<DP>::kThreads, 1)
   const int t0 = walk.first();
 
   if (warp == S::kWarps) {
-    int n = 0;
+    int nk = 0, nv = 0;  // loads under way or done
     Ring kr, vr;
-    for (int t = t0; t < tiles && !withheld(p, t, tiles); ++n) {
+    for (int t = t0; t < tiles && !withheld(p, t, tiles);) {
       // V first: its stage is free once dP is there, K's only after dQ
-      if (n >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
+      if (nv >= S::kVStages && !warp_wait(v_empty + 8 * vr.stage, vr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       if (lane == 0) load_tile<DP, kCols>(sbase + S::kV + vr.stage * S::kTile, &vm, v_full + 8 * vr.stage, g, (first + t) * kCols, b);
-      if (n >= S::kKStages && !warp_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) {
-        mbar_wait(v_full + 8 * vr.stage, vr.parity, nullptr);  // no copy may land in a CTA that is gone
-        break;
-      }
+      ++nv;
+      if (nk >= S::kKStages && !warp_wait(k_empty + 8 * kr.stage, kr.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       if (lane == 0) load_tile<DP, kCols>(sbase + S::kK + kr.stage * S::kTile, &km, k_full + 8 * kr.stage, g, (first + t) * kCols, b);
       const int64_t key = int64_t(first + t) * kCols, at = b * p.nk + key;
       load_key_values<POS>(sbase + S::kAux + kr.stage * 3 * kCols * 4, k_full + 8 * kr.stage, p.k_pos + at * POS,
                            p.k_seg != nullptr ? p.k_seg + at : nullptr, valid - key);
+      ++nk;
       kr.next(S::kKStages);
       vr.next(S::kVStages);
       t = walk.next(t);
     }
+    // no copy may land in the memory of a CTA that is gone: the last one of each stage
     if (own_by_tma) mbar_wait(own_full, 0, nullptr);
-    for (int e = max(0, n - S::kKStages); e < n; ++e)
+    for (int e = max(0, nk - S::kKStages); e < nk; ++e)
       mbar_wait(k_full + 8 * (e % S::kKStages), (e / S::kKStages) & 1, nullptr);
-    for (int e = max(0, n - S::kVStages); e < n; ++e)
+    for (int e = max(0, nv - S::kVStages); e < nv; ++e)
       mbar_wait(v_full + 8 * (e % S::kVStages), (e / S::kVStages) & 1, nullptr);
   } else if (warp == S::kWarps + 1) {
     const uint32_t leader = elect_one();

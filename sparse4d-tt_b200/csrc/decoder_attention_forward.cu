@@ -247,27 +247,26 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, 2)
     auto load_v = [&](int s, int t) {
       if (lane == 0) load_tile<DP, kKeys>(sbase + S::kV + s * S::kTile, &vm, v_full + 8 * s, g, int((first + t) * kKeys), b);
     };
-    int n = 0, t = t0;
+    int nk = 0, nv = 0, t = t0;  // loads under way or done
     Ring r, slot;
-    for (; t < tiles && !withheld(p, t, tiles); ++n) {
-      const bool again = n >= S::kStages;
+    while (t < tiles && !withheld(p, t, tiles)) {
+      const bool again = nk >= S::kStages;
       if (again && !warp_wait(k_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       load_k(r.stage, slot.stage, t);
-      if (again && !warp_wait(v_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) {
-        // the K load is out: it may not land in the memory of a CTA that is gone
-        mbar_wait(k_full + 8 * r.stage, r.parity, nullptr);
-        break;
-      }
+      ++nk;
+      if (again && !warp_wait(v_empty + 8 * r.stage, r.parity ^ 1, abort_flag, p.wait_limit_ns)) break;
       load_v(r.stage, t);
+      ++nv;
       r.next(S::kStages);
       slot.next(S::kSlots);
       t = walk.next(t);
     }
+    // no copy may land in the memory of a CTA that is gone: the last one of each stage
     if (q_by_tma) mbar_wait(q_full, 0, nullptr);
-    for (int e = max(0, n - S::kStages); e < n; ++e) {
+    for (int e = max(0, nk - S::kStages); e < nk; ++e)
       mbar_wait(k_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
+    for (int e = max(0, nv - S::kStages); e < nv; ++e)
       mbar_wait(v_full + 8 * (e % S::kStages), (e / S::kStages) & 1, nullptr);
-    }
   } else if (warp == S::kWarps + 1) {
     // The whole warp walks the tiles, so that addresses and descriptors stay in uniform registers; one
     // lane issues.
