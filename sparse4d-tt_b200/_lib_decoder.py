@@ -16,12 +16,11 @@ import threading
 import torch
 
 from . import _lib as L
+from .build import calls_path
 
 # The in-tree build; S4D_DECODER_LIB may point at another build of the same ABI.
 LIB_PATH = os.environ.get("S4D_DECODER_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib",
                                                              "libs4d_decoder.so")
-
-CALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "s4d_decoder_calls.so")
 
 S4D_DTYPE_F16 = 2
 DTYPES = {torch.float32: L.S4D_DTYPE_F32, torch.bfloat16: L.S4D_DTYPE_BF16, torch.float16: S4D_DTYPE_F16}
@@ -100,10 +99,11 @@ def calls():
         handle = lib()
         with _lock:
             if _calls is None:
-                if not os.path.exists(CALLS_PATH):
-                    raise RuntimeError(f"{CALLS_PATH} is not built; run `python __graft_entry__.py build` "
-                                       "(or python sparse4d-tt_b200/build.py).")
-                loader = importlib.machinery.ExtensionFileLoader("s4d_decoder_calls", CALLS_PATH)
+                path = calls_path()
+                if not os.path.exists(path):
+                    raise RuntimeError(f"{path} is not built (it goes with this Python and torch); run "
+                                       "`python __graft_entry__.py build` (or python sparse4d-tt_b200/build.py).")
+                loader = importlib.machinery.ExtensionFileLoader("s4d_decoder_calls", path)
                 module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
                 loader.exec_module(module)
                 module.init(*(C.cast(getattr(handle, n), C.c_void_p).value for n in (

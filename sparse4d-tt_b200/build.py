@@ -25,7 +25,6 @@ SOURCES = ["capi.cu", "kps_project.cu", "dfa_gather.cu", "kps_noalloc.cu", "line
            "instance_bank.cu", "peer.cu", "layer_norm.cu"]
 # The decoder's operators: each (source, defines) is compiled by itself, several at a time.
 DECODER_LIB_PATH = os.path.join(LIB_DIR, "libs4d_decoder.so")
-CALLS_PATH = os.path.join(LIB_DIR, "s4d_decoder_calls.so")
 DECODER_SOURCES = [("decoder_capi.cu",), ("decoder_norm.cu",), ("decoder_attention.cu",),
                    ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=64"),
                    ("decoder_attention_forward.cu", "-DS4D_HEAD_DIM=128"),
@@ -82,24 +81,33 @@ def build_decoder(verbose_ptxas: bool = False, force: bool = False) -> str:
     return DECODER_LIB_PATH
 
 
+def calls_path() -> str:
+    """Where the module of the decoder's calls is for this Python and torch, whose internals it is compiled against: one
+    that was built for another is not taken for it."""
+    import torch
+
+    tag = f"{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    return os.path.join(LIB_DIR, f"s4d_decoder_calls.{tag.replace(os.sep, '_')}.so")
+
+
 def build_calls(force: bool = False) -> str:
     """The Python module of csrc/decoder_calls.cpp (host code against torch's headers; it needs no nvcc)."""
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    src = os.path.join(CSRC, "decoder_calls.cpp")
-    deps = [src, os.path.join(INCLUDE, "s4d_dfa.h"), os.path.join(INCLUDE, "s4d_decoder.h")]
-    if not force and os.path.exists(CALLS_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(CALLS_PATH) for d in deps):
-        return CALLS_PATH
+    src, path = os.path.join(CSRC, "decoder_calls.cpp"), calls_path()
+    deps = [src, os.path.join(INCLUDE, "s4d_dfa.h"), os.path.join(INCLUDE, "s4d_decoder.h"), os.path.abspath(__file__)]
+    if not force and os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path) for d in deps):
+        return path
     os.makedirs(LIB_DIR, exist_ok=True)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     dirs = [INCLUDE, *include_paths(), sysconfig.get_paths()["include"], cuda]
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *(a for d in dirs for a in ("-I", d)),
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", CALLS_PATH + ".tmp", src, "-L",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", path + ".tmp", src, "-L",
           os.path.join(os.path.dirname(torch.__file__), "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"],
          "s4d_decoder_calls.so", False)
-    os.replace(CALLS_PATH + ".tmp", CALLS_PATH)
-    return CALLS_PATH
+    os.replace(path + ".tmp", path)
+    return path
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> str:

@@ -265,3 +265,28 @@ def test_wait_limit_is_per_thread_and_restorable(lib):
     t.join()
     assert seen == [2_000_000_000]  # another thread keeps its own default
     assert lib.s4d_decoder_set_wait_limit_ns(prev) == 12345
+
+
+def test_calls_module_of_another_torch_is_not_taken(monkeypatch, tmp_path):
+    """The module is compiled against torch's and Python's internals: one that was built for other versions is neither
+    kept by the build nor loaded."""
+    from sparse4d_tt_b200 import build as b
+
+    built = []
+
+    def run(cmd, what, verbose):
+        built.append(cmd[cmd.index("-o") + 1])
+        open(built[-1], "w").close()
+
+    monkeypatch.setattr(b, "_run", run)
+    monkeypatch.setattr(b, "LIB_DIR", str(tmp_path))
+    first = b.build_calls()
+    assert b.build_calls() == first and len(built) == 1
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    monkeypatch.setattr(D, "_calls", None)
+    with pytest.raises(RuntimeError, match="not built"):
+        D.calls()
+    second = b.build_calls()
+    assert second != first and len(built) == 2
+    os.utime(second, (0, 0))  # older than its sources and its flags
+    assert b.build_calls() == second and len(built) == 3
