@@ -27,7 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from .attention import decoder_attention_forward
+from .attention import decoder_attention
 from .dfa import MATMUL_PRECISIONS, DeformableFeatureAggregation, _matmul_precision, preprocess_dfa_parameters
 from .graph import capture, chained_camera_terms
 
@@ -128,7 +128,7 @@ class Sparse4DHead:
     returned as fp32.
 
     ``model_config["ATTENTION_KERNEL"]``: ``"sdpa"`` (default, torch's) or ``"decoder"``
-    (``attention.decoder_attention_forward``, for bf16 and fp16).  With ``"decoder"``,
+    (``attention.decoder_attention``, for bf16 and fp16; differentiable as that is).  With ``"decoder"``,
     ``ATTENTION_DISTANCE_SLOPES`` (one number a head) subtracts slope times the distance of two
     instances in the ground plane from their score, with the anchors as they are refined from
     layer to layer; ``ATTENTION_SOFTCAP`` caps the scores; and ``forward(..., instance_group=)`` keeps
@@ -206,9 +206,8 @@ class Sparse4DHead:
         dt = self.attention_dtype
         if self.attention_kernel == "decoder":
             xy = None if self.attention_slopes is None else anchor[..., X:Z].contiguous()
-            o, _ = decoder_attention_forward(q.to(dt), k.to(dt), v.to(dt), softcap=self.attention_softcap,
-                                             slopes=self.attention_slopes, q_pos=xy, k_pos=xy, q_segment=group,
-                                             k_segment=group)
+            o = decoder_attention(q.to(dt), k.to(dt), v.to(dt), softcap=self.attention_softcap, slopes=self.attention_slopes,
+                                  q_pos=xy, k_pos=xy, q_segment=group, k_segment=group)
             o = o.reshape(bs, n, e).float()
         else:
             q, k, v = (t.transpose(1, 2) for t in (q, k, v))

@@ -134,6 +134,30 @@ def test_head_on_the_decoder_kernel_follows_sdpa(cuda_device, head_case):
     steps_agree(a, b, head_case[2].anchor.cuda(), 0.999)
 
 
+def test_head_attention_has_the_gradients_of_sdpa(cuda_device, head_case):
+    """The attention layer's gradients in its input and in the value, on either kernel: both round P, dS and the
+    results to bf16 a few times, 2^-8 of a norm each.  What has no gradient is refused, not left out."""
+    params = head_case[0]
+    heads = [Sparse4DHead("cuda:0", params, dict(BASE, ATTENTION_KERNEL=kind)) for kind in ("sdpa", "decoder")]
+    layer = heads[0].operation_order.index("gnn")
+    g = torch.Generator().manual_seed(4)
+    query, value, dout = (torch.randn(2, 300, n, generator=g).cuda() for n in (512, 512, 256))
+    anchor = torch.randn(2, 300, 11, generator=g).cuda()
+    got = []
+    for gh in heads:
+        x, v = query.clone().requires_grad_(), value.clone().requires_grad_()
+        out = gh._attention(gh.layers[layer], x, v, anchor, None)
+        got.append(torch.autograd.grad(out, (x, v), dout))
+    for a, b in zip(*got):
+        assert b.norm() > 0 and (a - b).norm() <= 2.4e-2 * a.norm()
+    biased = Sparse4DHead("cuda:0", params, dict(BASE, ATTENTION_KERNEL="decoder", ATTENTION_DISTANCE_SLOPES=[0.1] * 8))
+    with pytest.raises(ValueError, match="no gradient"):
+        biased._attention(biased.layers[layer], query, value, anchor.clone().requires_grad_(), None)
+    half = Sparse4DHead("cuda:0", params, dict(BASE, ATTENTION_KERNEL="decoder", ATTENTION_DTYPE=torch.float16))
+    with pytest.raises(TypeError, match="bfloat16"):
+        half._attention(half.layers[layer], query.clone().requires_grad_(), value, anchor, None)
+
+
 class PlainHead(Sparse4DHead):
     """The head with its attention written out in fp32 on the same rounded q, k and v."""
 
