@@ -24,6 +24,7 @@ There is no CPU path: CPU tensors are rejected.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -79,6 +80,8 @@ def _checked(name: str, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float],
                          f"{list(v.shape)}")
     if G == 0 or H % G:
         raise ValueError(f"{name}: the {H} heads must be a multiple of the {G} kv_heads")
+    if softcap and C.c_float(softcap).value == 0.0:
+        raise ValueError(f"{name}: softcap {softcap} is 0 in fp32, which would be no cap")
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"{name}: dim must be a multiple of 8 from 8 to 128, got {dim}")
     (q, qs), (k, ks), (v, vs) = _operand(q), _operand(k), _operand(v)

@@ -66,7 +66,7 @@ class Args {
     if (!ok_) return 0.0f;
     const double v = PyFloat_Check(args_[i]) || PyLong_Check(args_[i]) ? PyFloat_AsDouble(args_[i]) : NAN;
     if (PyErr_Occurred()) PyErr_Clear();
-    need(std::isfinite(v));
+    need(std::isfinite(v) && (v == 0.0 || float(v) != 0.0f));  // what fp32 makes another number of
     return float(v);
   }
   bool truth(int i) { return ok_ && PyObject_IsTrue(args_[i]) == 1; }

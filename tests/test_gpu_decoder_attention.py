@@ -698,3 +698,15 @@ def test_waits_that_run_out(cuda_device, B, Nq, Nk, H, G, D, how):
     again = (*decoder_attention_forward(q, k, v, **how, error_flag=flags[:1]),
              *(t for t in decoder_attention_backward(dout, q, k, v, out, lse, **how, error_flag=flags[1:]) if t is not None))
     assert flags.tolist() == [0, 0] and all(torch.equal(a, b) for a, b in zip(again, clean))
+
+
+def test_caps_that_are_zero_in_fp32_are_rejected(cuda_device):
+    """A positive cap that fp32 rounds to 0 means the opposite of no cap: all scores equal."""
+    q, k, v, _ = make(1, 5, 9, 2, 1, 64)
+    out, lse = decoder_attention_forward(q, k, v)
+    for call in (lambda: decoder_attention_forward(q, k, v, softcap=1e-50), lambda: decoder_attention(q, k, v, softcap=1e-50),
+                 lambda: decoder_attention_backward(out, q, k, v, out, lse, softcap=1e-50)):
+        with pytest.raises(ValueError, match="softcap"):
+            call()
+    one = decoder_attention_forward(q, k, v, scale=1e-50)[0]  # a scale that small makes them equal
+    assert torch.equal(one, decoder_attention_forward(q, k, v, scale=0.0)[0])
