@@ -141,6 +141,12 @@ class on_device:
         return False
 
 
+def in_memory(t: torch.Tensor | None) -> torch.Tensor | None:
+    """``t`` such that its memory holds its values: a copy of a view that stands for the negative of its memory (the
+    imaginary part of a conjugate)."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def same_device(name: str, first: torch.Tensor, *others) -> int:
     """The CUDA device index of ``first``, which every other tensor (None: left out) has to share."""
     index = first.get_device()

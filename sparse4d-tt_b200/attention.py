@@ -40,6 +40,7 @@ def _operand(t: Tensor) -> Tuple[Tensor, Tuple[int, ...]]:
     """``t [B, N, heads, dim]`` and its strides, such that the kernels can read it in place (unit stride along
     dim, the others positive multiples of 8, 16-byte aligned); a contiguous copy where ``t`` is not
     (an expanded tensor, for one)."""
+    t = D.in_memory(t)
     sb, sn, sh, sd = t.stride()
     b, n, h, _ = t.shape
     if (sd == 1 and t.data_ptr() % 16 == 0 and (b <= 1 or (sb > 0 and sb % 8 == 0))
@@ -85,7 +86,8 @@ def _checked(name: str, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float],
     if dim % 8 or not 8 <= dim <= 128:
         raise ValueError(f"{name}: dim must be a multiple of 8 from 8 to 128, got {dim}")
     (q, qs), (k, ks), (v, vs) = _operand(q), _operand(k), _operand(v)
-    keep = (q, k, v)
+    slopes, q_pos, k_pos = D.in_memory(slopes), D.in_memory(q_pos), D.in_memory(k_pos)
+    keep = (q, k, v, slopes, q_pos, k_pos)
     pos, slope, qp, kp = 0, (0, 0, 0, 0), 0, 0
     if slopes is not None:
         if q_pos is None or k_pos is None:
@@ -180,7 +182,7 @@ def decoder_attention_forward(q: Tensor, k: Tensor, v: Tensor, scale: Optional[f
         D.same_device(name, q, out)
         if out.dtype != q.dtype:
             raise TypeError(f"{name}: out must be {q.dtype}, got {out.dtype}")
-        if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+        if out.shape != q.shape or not out.is_contiguous() or out.is_neg() or out.data_ptr() % 16:
             raise ValueError(f"{name}: out must be a contiguous, 16-byte aligned {list(q.shape)} tensor")
         if any(t is not None and D.overlap(out, t) for t in (q, k, v, slopes, q_pos, k_pos, q_segment, k_segment, k_len)):
             raise ValueError(f"{name}: out must not share memory with the arguments")
@@ -218,6 +220,7 @@ def decoder_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, ou
             return done
     a = _checked(name, q, k, v, scale, softcap, slopes, q_pos, k_pos, q_segment, k_segment, k_len, error_flag)
     D.same_device(name, q, dout, out, lse)
+    out, lse = D.in_memory(out), D.in_memory(lse)
     B, nq, _, H = a.sizes[:4]
     if q.dtype != torch.bfloat16 or dout.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise TypeError(f"{name}: q, dout and out must be torch.bfloat16, got {q.dtype}, {dout.dtype} and {out.dtype}")

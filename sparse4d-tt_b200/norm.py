@@ -25,6 +25,7 @@ MAX_WIDTH = 16384
 def _rows(t: Tensor, width: int) -> Tuple[Tensor, int]:
     """``t [..., width]`` and the stride of its rows: ``t`` itself or a view where the strides allow it (rows
     may be strided, or one row broadcast), a contiguous copy otherwise."""
+    t = D.in_memory(t)
     if t.is_contiguous():
         return t, width
     v = t if t.dim() == 2 else t.reshape(-1, width)
@@ -64,6 +65,7 @@ def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optio
         if done is not None:
             return done
     index = D.same_device(name, x, weight, bias, out)
+    weight, bias = D.in_memory(weight), D.in_memory(bias)
     width, dtype = _width(name, x), x.dtype
     pt = torch.float32 if weight is None else _param(name, "weight", weight, dtype, width)
     if bias is not None:
@@ -76,7 +78,7 @@ def decoder_norm_forward(x: Tensor, weight: Optional[Tensor] = None, bias: Optio
         out = x.new_empty(shape)
     elif out.dtype != dtype:
         raise TypeError(f"{name}: out must be {dtype}, got {out.dtype}")
-    elif out.shape != shape or not out.is_contiguous():
+    elif out.shape != shape or not out.is_contiguous() or out.is_neg():
         raise ValueError(f"{name}: out must be a contiguous {list(shape)} tensor")
     elif (D.overlap(out, x) and (out.data_ptr() != x.data_ptr() or not x.is_contiguous())) or any(
             t is not None and D.overlap(out, t) for t in (weight, bias)):
@@ -107,6 +109,7 @@ def decoder_norm_backward(dout: Tensor, x: Tensor, weight: Optional[Tensor], mea
         if done is not None:
             return done
     index = D.same_device(name, x, dout, weight, mean, rstd)
+    weight, mean, rstd = D.in_memory(weight), D.in_memory(mean), D.in_memory(rstd)
     width, dtype, shape = _width(name, x), x.dtype, x.shape
     if dout.dtype != dtype:
         raise TypeError(f"{name}: dout must be {dtype}, got {dout.dtype}")

@@ -283,3 +283,34 @@ def test_calls_module_and_python_path_agree(cuda_device, monkeypatch):
                 lambda: c.attention_backward(q, q, k, v, q, None, None, 0.0, *[None] * 6, True, True),
                 lambda: c.attention_backward(q, q, k, v)):
         assert bad() is None
+
+
+def test_views_that_stand_for_the_negative_of_their_memory(cuda_device):
+    """The imaginary part of a conjugate is such a view; every argument may be one, and an out may not."""
+    g = torch.Generator().manual_seed(8)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    neg = lambda t: torch.complex(t * 0, -t).conj().imag if t.dtype == torch.float32 else torch._neg_view(-t)  # noqa: E731
+    assert neg(r(3)).is_neg()
+    q, k, v, dout = (r(1, n, 2, 64).bfloat16() for n in (20, 30, 30, 20))
+    how = dict(slopes=r(2).abs(), q_pos=r(1, 20, 2), k_pos=r(1, 30, 2))
+    out, lse = decoder_attention_forward(q, k, v, **how)
+    grads = decoder_attention_backward(dout, q, k, v, out, lse, **how)
+    nhow = {n: neg(t) for n, t in how.items()}
+    nout, nlse = decoder_attention_forward(neg(q), neg(k), neg(v), **nhow)
+    assert torch.equal(nout, out) and torch.equal(nlse, lse)
+    got = decoder_attention_backward(neg(dout), neg(q), neg(k), neg(v), neg(out), torch._neg_view(-lse), **nhow)
+    assert all(torch.equal(a, b) for a, b in zip(got, grads))
+    with pytest.raises(ValueError, match="out"):
+        decoder_attention_forward(q, k, v, out=torch._neg_view(out))
+    for width in (1, 24):
+        x, dy, w, b = r(7, width), r(7, width), r(width), r(width)
+        y, mean, rstd = decoder_norm_forward(x, w, b)
+        want = decoder_norm_backward(dy, x, w, mean, rstd)
+        flat = lambda t: torch._neg_view(-t)  # noqa: E731
+        for f in (neg, flat):
+            ny = decoder_norm_forward(f(x), flat(w), flat(b))
+            assert all(torch.equal(a, c) for a, c in zip(ny, (y, mean, rstd)))
+            got = decoder_norm_backward(f(dy), f(x), flat(w), flat(mean), flat(rstd))
+            assert all(torch.equal(a, c) for a, c in zip(got, want))
+        with pytest.raises(ValueError, match="out"):
+            decoder_norm_forward(x, out=flat(y))
