@@ -69,7 +69,13 @@ class Args {
     need(std::isfinite(v) && (v == 0.0 || float(v) != 0.0f));  // what fp32 makes another number of
     return float(v);
   }
-  bool truth(int i) { return ok_ && PyObject_IsTrue(args_[i]) == 1; }
+  bool truth(int i) {
+    if (!ok_) return false;
+    const int v = PyObject_IsTrue(args_[i]);
+    if (v < 0) PyErr_Clear();
+    need(v >= 0);
+    return v == 1;
+  }
   bool none(int i) const { return args_[i] == Py_None; }
 
  private:
@@ -154,9 +160,11 @@ PyObject* norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!param(a, w, x->scalar_type(), width, &type)) Py_RETURN_NONE;
   if (type == at::ScalarType::Undefined) type = at::kFloat;
   at::Tensor dx, dw, db, ws;
-  if (a.truth(5)) dx = empty(x->sizes(), x->scalar_type(), a.device());
-  if (a.truth(6)) dw = empty({width}, type, a.device());
-  if (a.truth(7)) db = empty({width}, type, a.device());
+  const bool need_dx = a.truth(5), need_dw = a.truth(6), need_db = a.truth(7);
+  if (!a.ok()) Py_RETURN_NONE;
+  if (need_dx) dx = empty(x->sizes(), x->scalar_type(), a.device());
+  if (need_dw) dw = empty({width}, type, a.device());
+  if (need_db) db = empty({width}, type, a.device());
   const size_t need = dw.defined() || db.defined() ? norm_backward_ws_fn(rows, width) : 0;
   if (need > 0) ws = empty({int64_t(need / 4)}, at::kFloat, a.device());
   auto at_of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
@@ -244,10 +252,10 @@ PyObject* attention_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 16) Py_RETURN_NONE;
-  // in attention_args' order: q, k, v and the rest; then dout, out and lse
-  PyObject* const order[14] = {args[1],  args[2],  args[3],  args[6],  args[7],  args[8], args[9],
-                               args[10], args[11], args[12], args[13], args[0], args[4], args[5]};
-  Args a(order, 14, 14);
+  // in attention_args' order: q, k, v and the rest; then dout, out, lse and what is needed
+  PyObject* const order[16] = {args[1],  args[2],  args[3],  args[6], args[7], args[8], args[9],  args[10],
+                               args[11], args[12], args[13], args[0], args[4], args[5], args[14], args[15]};
+  Args a(order, 16, 16);
   s4d_attention_args c = {};
   if (!attention_args(a, 0, c) || c.dtype != S4D_DTYPE_BF16 || c.batch == 0) Py_RETURN_NONE;
   const at::Tensor &q = THPVariable_Unpack(args[1]), &k = THPVariable_Unpack(args[2]);
@@ -255,15 +263,16 @@ PyObject* attention_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!a.ok() || dout->scalar_type() != at::kBFloat16 || dout->sizes() != q.sizes() || !operand(a, dout, c.dout_stride))
     Py_RETURN_NONE;
   const at::Tensor *out = a.tensor(12, at::kBFloat16, q.sizes()), *lse = a.tensor(13, at::kFloat, {c.batch, c.heads, c.queries});
+  const bool need_dkv = a.truth(14), need_dslopes = a.truth(15);
   if (!a.ok()) Py_RETURN_NONE;
   c.dout = dout->data_ptr(), c.out = out->data_ptr(), c.lse = lse->data_ptr<float>();
   at::Tensor dq = empty(q.sizes(), at::kBFloat16, a.device()), dk, dv, ds, ws;
   c.dq = dq.data_ptr();
-  if (PyObject_IsTrue(args[14]) == 1) {
+  if (need_dkv) {
     dk = empty(k.sizes(), at::kBFloat16, a.device()), dv = empty(k.sizes(), at::kBFloat16, a.device());
     c.dk = dk.data_ptr(), c.dv = dv.data_ptr();
   }
-  if (c.slopes != nullptr && PyObject_IsTrue(args[15]) == 1) {
+  if (c.slopes != nullptr && need_dslopes) {
     ds = empty(THPVariable_Unpack(args[8]).sizes(), at::kFloat, a.device());
     c.dslopes = ds.data_ptr<float>();
   }

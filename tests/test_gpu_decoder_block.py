@@ -314,3 +314,21 @@ def test_views_that_stand_for_the_negative_of_their_memory(cuda_device):
             assert all(torch.equal(a, c) for a, c in zip(got, want))
         with pytest.raises(ValueError, match="out"):
             decoder_norm_forward(x, out=flat(y))
+
+
+def test_needs_that_have_no_truth_value(cuda_device):
+    """What Python refuses to take for true or false is refused as Python does it."""
+    x = torch.randn(6, 32, device="cuda")
+    _, mean, rstd = decoder_norm_forward(x)
+    q = torch.randn(1, 6, 2, 64, device="cuda").bfloat16()
+    out, lse = decoder_attention_forward(q, q, q)
+    pos = dict(slopes=torch.ones(2, device="cuda"), q_pos=torch.zeros(1, 6, 1, device="cuda"),
+               k_pos=torch.zeros(1, 6, 1, device="cuda"))
+    two = torch.ones(2)
+    for call in (lambda: decoder_norm_backward(x, x, None, mean, rstd, need_dx=two),
+                 lambda: decoder_norm_backward(x, x, None, mean, rstd, need_dbias=two),
+                 lambda: decoder_attention_backward(q, q, q, q, out, lse, need_dkv=two),
+                 lambda: decoder_attention_backward(q, q, q, q, out, lse, need_dslopes=two, **pos)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()
+    assert decoder_norm_backward(x, x, None, mean, rstd, need_dx=0, need_dweight=torch.ones(1))[0] is None
