@@ -122,7 +122,7 @@ S4D_API int s4d_attention_forward(const s4d_attention_args* args, void* stream);
  *   dq       [batch, queries, heads, dim] contiguous; dk, dv [batch, keys, kv_heads, dim] contiguous, or
  *            both NULL when not wanted; all 16-byte aligned
  *   dslopes  f32, or NULL: [batch, queries, heads] when dslopes_per_row, else [heads], the sum over all
- *            rows.  Positions have no gradient.
+ *            rows (0 without a row or a batch entry).  Positions have no gradient.
  *   workspace  s4d_attention_backward_workspace_bytes(args) bytes, 16-byte aligned
  * No atomics: equal calls give equal bits.  Pairs that are not seen take no part, whatever q, k, v,
  * dout and the positions hold there; gradients of rows that see nothing or are seen by nothing are 0.

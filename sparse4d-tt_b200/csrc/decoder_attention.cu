@@ -217,6 +217,12 @@ __global__ void __launch_bounds__(1024) slope_sum_kernel(const float* rows, int 
   }
 }
 
+int launch_slope_sum(const float* rows, const s4d_attention_args& a, cudaStream_t st) {
+  return cuda_check(launch_pdl(true, slope_sum_kernel, dim3(unsigned(a.heads)), dim3(1024), 0, st, rows, int(a.batch),
+                               a.queries, int(a.heads), a.dslopes),
+                    "slope_sum_kernel launch");
+}
+
 size_t backward_workspace(const s4d_attention_args& a) {
   const size_t rows = size_t(a.batch) * size_t(a.heads);
   const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
@@ -292,14 +298,16 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   if (a.dtype != S4D_DTYPE_BF16) S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for bf16");
   if (ceil_div(a.queries, kBackwardTile) > kAttnMaxTiles || ceil_div(a.keys, kBackwardTile) > kAttnMaxTiles)
     S4D_BAD(S4D_ERR_UNSUPPORTED_SHAPE, "implemented for at most 524288 queries and keys");
-  if (a.batch == 0) return S4D_OK;
+  const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
+  cudaStream_t stm = static_cast<cudaStream_t>(stream);
+  if (a.dslopes != nullptr && a.pos_dim == 0) S4D_BAD(S4D_ERR_INVALID_ARG, "dslopes without a distance bias");
+  if (!aligned_to(a.dslopes, 4)) S4D_BAD(S4D_ERR_INVALID_ARG, "misaligned pointer");
+  if (a.batch == 0) return sum ? launch_slope_sum(nullptr, a, stm) : S4D_OK;  // zeros
   if ((a.dk == nullptr) != (a.dv == nullptr)) S4D_BAD(S4D_ERR_INVALID_ARG, "dk and dv go together");
-  if (!aligned_to(a.dout, 16) || !aligned_to(a.dq, 16) || !aligned_to(a.dk, 16) || !aligned_to(a.dv, 16) ||
-      !aligned_to(a.dslopes, 4))
+  if (!aligned_to(a.dout, 16) || !aligned_to(a.dq, 16) || !aligned_to(a.dk, 16) || !aligned_to(a.dv, 16))
     S4D_BAD(S4D_ERR_INVALID_ARG, "misaligned pointer");
   if (a.queries > 0 && (a.dout == nullptr || a.dq == nullptr || a.lse == nullptr))
     S4D_BAD(S4D_ERR_INVALID_ARG, "null dout, dq or lse");
-  if (a.dslopes != nullptr && a.pos_dim == 0) S4D_BAD(S4D_ERR_INVALID_ARG, "dslopes without a distance bias");
   if (!Strides(a.dout_stride, a.batch, a.queries, a.heads).ok(a.batch, a.queries, a.heads))
     S4D_BAD(S4D_ERR_INVALID_ARG, "strides of dout must be positive multiples of 8 elements");
   const size_t need = backward_workspace(a);
@@ -315,10 +323,8 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
   p.dq = a.dq, p.dk = a.dk, p.dv = a.dv;
   p.splits = 1;
   p.records = static_cast<float*>(a.workspace);
-  const bool sum = a.dslopes != nullptr && !a.dslopes_per_row;
   p.dslopes = sum ? p.records + a.batch * a.heads * ceil_div(a.queries, kRecordTile) * (kRecordBytes / 4) : a.dslopes;
   p.dslopes_by_head = sum;
-  cudaStream_t stm = static_cast<cudaStream_t>(stream);
   if (a.queries > 0 || a.keys > 0) {
     AttnBackwardMaps m;
     st = key_map(&m.k_tile, a, a.k, a.k_stride, kBackwardTile);
@@ -337,10 +343,7 @@ int s4d_attention_backward(const s4d_attention_args* args, void* stream) {
                        : launch_attention_backward_d128(int(a.pos_dim), p, m, stm);
     if (st != S4D_OK) return st;
   }
-  if (!sum) return S4D_OK;
-  return cuda_check(launch_pdl(true, slope_sum_kernel, dim3(unsigned(a.heads)), dim3(1024), 0, stm,
-                               static_cast<const float*>(p.dslopes), p.batch, p.nq, p.heads, a.dslopes),
-                    "slope_sum_kernel launch");
+  return sum ? launch_slope_sum(p.dslopes, a, stm) : S4D_OK;
 }
 
 }  // extern "C"

@@ -710,3 +710,15 @@ def test_caps_that_are_zero_in_fp32_are_rejected(cuda_device):
             call()
     one = decoder_attention_forward(q, k, v, scale=1e-50)[0]  # a scale that small makes them equal
     assert torch.equal(one, decoder_attention_forward(q, k, v, scale=0.0)[0])
+
+
+@pytest.mark.parametrize("batch,queries", [(0, 5), (2, 0)])
+def test_slopes_gradient_of_no_rows_is_written(cuda_device, batch, queries):
+    """The C entry's sum over no rows is 0, whatever dslopes held."""
+    ds, x, dk, dv = torch.full((6,), 7.0, device="cuda"), *(torch.zeros(4096, device="cuda") for _ in range(3))
+    a = x.data_ptr()
+    args = lib_decoder.ATTENTION_ARGS.pack(batch, queries, 3, 6, 2, 8, 1, a, a, a, *(1024, 48, 8), *(1024, 16, 8), *(1024, 16, 8), a,
+                                           a, a, 0, 0, 1, a, a, 0, 0, 0, 0, 0, 0, 0.5, 0.0, 1, 0, a, 1024, 48, 8, a,
+                                           dk.data_ptr(), dv.data_ptr(), ds.data_ptr())
+    lib_decoder.check("s4d_attention_backward", lib_decoder.lib().s4d_attention_backward(args, lib_decoder.stream_ptr(0)))
+    assert not ds.any()
