@@ -332,3 +332,65 @@ def test_needs_that_have_no_truth_value(cuda_device):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
     assert decoder_norm_backward(x, x, None, mean, rstd, need_dx=0, need_dweight=torch.ones(1))[0] is None
+
+
+def test_head_graph_over_other_groups(cuda_device, head_case):
+    """A captured pass reads the groups that it is handed, as an eager pass on them does."""
+    params, cfg, ins, packed = head_case
+    d = torch.device("cuda:0")
+    gh = Sparse4DHead("cuda:0", params, dict(BASE, ATTENTION_KERNEL="decoder", ATTENTION_DISTANCE_SLOPES=[0.1] * 8))
+    groups = [(torch.arange(900) >= at).int().expand(cfg.bs, -1).contiguous().cuda() for at in (900, 600, 128)]
+    graph = HeadGraph(gh, cfg.bs, cfg.spatial_shapes, instance_group=groups[0])
+    feed = (packed[0], ins.projection_mat.to(d), ins.image_wh.to(d), ins.anchor.to(d))
+    seen = []
+    for group in groups + groups[1:2]:
+        got = [t.clone() for t in graph.run(*feed, group)["prediction"]]
+        assert all(torch.equal(x, y) for x, y in zip(got, run(gh, head_case, instance_group=group)))
+        seen.append(got[-1])
+    assert torch.equal(seen[1], seen[3]) and not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_two_threads_and_streams_at_once(cuda_device):
+    """Calls from two host threads on two streams, each with launches of clusters (few rows, cut tiles) and without,
+    give the bits that they give alone."""
+    import threading
+
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    sets = []
+    for n, keys, dim in ((2, 4000, 64), (900, 900, 64), (1, 9000, 128), (700, 1100, 128)):
+        q, k, v = r(1, n, 4, dim).bfloat16(), r(1, keys, 2, dim).bfloat16(), r(1, keys, 2, dim).bfloat16()
+        sets.append((q, k, v, dict(slopes=r(4).abs() / 8, q_pos=r(1, n, 2), k_pos=r(1, keys, 2))))
+    x, w, b = r(3000, 300), r(300), r(300)
+
+    def work(order):
+        out = {}
+        for i in order:
+            q, k, v, how = sets[i]
+            o, lse = decoder_attention_forward(q, k, v, **how)
+            out[i] = (o, lse, *decoder_attention_backward(o, q, k, v, o, lse, **how))
+            y, mean, rstd = decoder_norm_forward(x, w, b)
+            out[i] += (y, *decoder_norm_backward(y, x, w, mean, rstd))
+        return out
+
+    want = work(range(4))
+    torch.cuda.synchronize()
+    results, errors = [], []
+
+    def thread(order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(25):
+                    results.append(work(order))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(o,)) for o in ((0, 1, 2, 3), (3, 0, 2, 1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(results) == 50
+    for got in results:
+        assert all(torch.equal(a, c) for i in range(4) for a, c in zip(got[i], want[i]))
