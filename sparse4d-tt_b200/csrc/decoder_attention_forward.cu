@@ -682,14 +682,14 @@ int launch_kernel(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st
                     "attention_forward_kernel launch");
 }
 
-// A row tile of eight rows or fewer is held four times where a score costs more than its product with K and
-// V: 4 x 1 query over 65,536 keys, 8 shared heads of 128, 1-D distance 215 us without, 199 with it; 8 x 1
-// over 16,384, 8 heads of 64, 2-D distance 74 and 55; 2 queries over 4 x 4,000, 8 shared heads of 128
-// 20.3 and 19.5.  Plain scores over heads of 64 lose (8 queries over 2 x 20,000, 16 heads: 35.5 and
-// 38 us), and so do more rows, which are fetched one by one (6 x 30 over 900: 10.6 and 12.8 us).
+// A row tile of eight rows or fewer is held four times where a score has a bias or a cap.  Graph times of 4 x 1 query
+// over 65,536 keys, 32 heads on 8 shared ones, without and with it: of 128, 2-D distance 195 and 176 us, capped
+// 193 and 171, both 261 and 175; of 64, 1-D distance 124 and 110, 2-D 145 and 104, capped 154 and 102 (heads of
+// 128 with 1-D distance 177 either way).  Plain scores lose: 164 and 168 us for heads of 128, 100 and 103 of 64.
+// So do more rows, which are fetched one by one (6 x 30 over 900: 10.6 and 12.8 us).
 template <typename T, int DP, int POS, bool CAP>
 int launch(const AttnParams& p, const AttnForwardMaps& m, cudaStream_t st) {
-  if constexpr (DP > 64 || POS > 0 || CAP)
+  if constexpr (POS > 0 || CAP)
     if (p.nq * p.rep <= 8) return launch_kernel<T, DP, POS, CAP, true>(p, m, st);
   return launch_kernel<T, DP, POS, CAP, false>(p, m, st);
 }
