@@ -132,8 +132,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Parts of the keys.  A tile of 128 rows and one shared head is one CTA.  With fewer CTAs than SMs the keys
 // are cut until every SM has one, or two when with one a part has 16 tiles of 64 keys or more: the two on
 // an SM keep more loads under way, but each of its tiles takes longer, and more parts take longer to join.
-// (2 x 16 queries over 30,000 keys, 2 shared heads of 64: 35.6 us with one CTA an SM, 42.0 with two; one
-// query over 4 x 65,536 keys, 8 shared heads of 128: 349 us with one, 175 with two.)  A part is not
+// (Graph times: 2 x 16 queries over 30,000 keys, 2 heads of 64 29.4 us with one CTA an SM, 36.2 with two; one
+// query over 4 x 65,536 keys, 32 heads of 128 on 8, 1-D distance 268 us with one, 178 with two.)  A part is not
 // cut below two tiles, one for each stream of row warps.  Up to 11 parts become at most 8, which
 // one cluster joins in shared memory: a second launch and its pass over memory cost more than a quarter
 // of the CTAs brings.

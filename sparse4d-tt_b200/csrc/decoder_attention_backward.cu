@@ -7,8 +7,8 @@
 // Two kernels, so that nothing is added by atomics and equal calls give equal bits: one owns 128
 // query rows and walks the keys (dQ, dslopes, and a record of each query for the second), one owns 128
 // keys of a shared head and walks the query rows of every head that shares them (dK and dV).  That
-// costs the two score products and the exponential a second time (7 products instead of 5), and
-// saves a pass of fp32 additions over dQ in memory.  Both have the forward kernel's roles: one score
+// costs the two score products and the exponential a second time (8 products instead of 5, with the P K
+// below), and saves a pass of fp32 additions over dQ in memory.  Both have the forward kernel's roles: one score
 // row a thread, S and dP side by side in tensor memory (64 columns each), the 16-bit P and dS
 // written back over them as the tensor-memory operand of the next products, the other operand read
 // MN-major from the same shared-memory tile that served the scores.  The products of the scores and
@@ -20,7 +20,7 @@
 // subnormal range.  delta comes from an O that is rounded too, which would weigh as much as dP itself where
 // a row's weight lies on few keys.  So the first kernel also adds R_i = sum_j dS_ij, which an exact delta
 // makes 0, and the product P K: the second kernel gets delta + R, dQ loses R P K, dslope R sum P dist
-// (8192 tokens: dq 755 us without the product, 803 with it).
+// (8192 tokens: dq 735 us without the product, 740 with it).
 //
 // What bounds it: as in the forward pass the work per score in registers (one exponential, one more
 // special-function instruction with a 2-D distance, two with a cap, and about twenty others), and the
@@ -31,11 +31,11 @@
 // are linear in the tiles, so the streams share them; the tensor cores take the tiles in order.  Twelve
 // row warps leave a thread 128 registers: it holds 16 scores and 16 dP at a time.
 //
-// Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance, before P K was added: dq 756, dk and dv
-// 862 us; with two streams and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with
-// two CTAs an SM, two streams and tiles of 32 each 930 and 1180.  Without the arithmetic of the scores dk
-// and dv take 574 us, without the products too 337; its 512 tiles of keys on 148 SMs left
-// 14 % of the slots empty until the last ones were cut (launch_tiles below).
+// Measured at 8192 tokens, 16 heads of 64 on 8, 1-D distance, calls in a CUDA graph: dq 740, dk and dv 711 us.  On the
+// way there, before P K was added and tiles were cut (launch_tiles below): dq 756, dk and dv 862 us; with two
+// streams and three tiles 807 and 908, those with 32 scores at a time 862 and 1000; with two CTAs an SM, two streams
+// and tiles of 32 each 930 and 1180.  Then dk and dv took 574 us without the arithmetic of the scores and 337 without
+// the products too.
 #include "decoder_attention.cuh"
 
 namespace s4d {
@@ -939,10 +939,11 @@ __global__ void __launch_bounds__(Dkv<DP>::kThreads, 1)
 // tile takes, are one of `kernel` beside the end of the first, cut into as many parts of the other axis as
 // there is room for clusters of that many CTAs, up to eight: each keeps its sums in shared memory and
 // joins a share of the rows.  A part keeps six tiles or more, since its start and the join take as long as
-// two.  (4 x 1800 tokens, 8 heads, 480 own tiles: forward and backward pass 406 us without, 376 us with
-// it; 8192 tokens, 512 tiles of keys: 2090 and 1988 us; 900 tokens, 64 tiles, all cut: 69 and 58.5 us.)
-// Tiles with segments differ in length and fill the SMs as they come, and are short: those are not cut (8 x
-// 1437 tokens in groups, 768 tiles: 251 us, cut 256; 900 in three groups, 64 tiles: 55.0 and 55.2 us).
+// two; the last ones get what is left, which may be none.  (Graph times of the backward pass without and with it:
+// 4 x 1800 tokens, 8 heads, 480 own tiles 309 and 280 us; 8192 tokens, 512 tiles of keys 1544 and 1452 us; 900 tokens,
+// 64 tiles, all cut 38.9 and 33.5 us.)  Tiles with segments differ in length and fill the SMs as they come, and are
+// short: those are not cut (when that was tried, both passes over 8 x 1437 tokens in groups, 768 tiles, took 251 us,
+// cut 256; 900 in three groups, 64 tiles, 55.0 and 55.2 us).
 template <typename S, typename K, typename... Maps>
 int launch_tiles(K whole_kernel, K kernel, const char* what, bool (&smem_set)[2][64], int (&fits)[64][9], AttnParams p,
                  int64_t tiles, int64_t walked, int64_t weight, cudaStream_t st, const Maps&... maps) {

@@ -11,7 +11,7 @@
 //   the others  one row a thread: scores from tensor memory, cap, bias and mask in registers (two
 //               scores an instruction), the row maximum without a shuffle, P = 2^(s - m) back over S
 //               as 16-bit pairs.
-// O is only rescaled when a row's maximum grew by more than 2^8 since the last time: P then stays
+// O is only rescaled when a row's maximum grew by more than 2^8 since the last time (a published method): P then stays
 // under 2^8, which costs no precision in a float.  P is rounded to the inputs' type because the
 // tensor cores multiply it with V in that type; l adds the unrounded values in fp32.
 //
@@ -34,12 +34,13 @@
 // every CTA leaves its O, m and l in shared memory and each joins a share of the rows from its peers'.
 // More parts write normalised O and log-sum-exp to memory and a second launch joins them.
 //
-// Measured (kernel alone, bf16 unless said): 32 x 900 tokens, 8 heads of 64, 2-D distance 213 us (212 M
-// exponentials and as many square roots: 119 us at 16 a clock); 8 x 1437, 8 heads of 64, segments 68 us;
-// 2 x 4096, 16 heads of 128 on 4, capped, f16 420 us (270 us for its three special-function instructions
-// a score); 8192 tokens, 16 heads of 64 on 8, 1-D distance 585 us.  What is left over is not one unit:
+// Measured (calls in a CUDA graph, bf16 unless said): 32 x 900 tokens, 8 heads of 64, 2-D distance 202 us (212 M
+// exponentials and as many square roots: 119 us at 16 a clock); 8 x 1437, 8 heads of 64, segments 69 us;
+// 2 x 4096, 16 heads of 128 on 4, capped, f16 392 us (270 us for its three special-function instructions
+// a score); 8192 tokens, 16 heads of 64 on 8, 1-D distance 544 us.  What is left over is not one unit:
 // when the first took 229, it took 167 with the square root taken out, 212 without exponentials, 197 without
-// products, and 105 with an empty tile loop and all its hand-overs.
+// products, and 105 with an empty tile loop and all its hand-overs.  At D <= 64 a thread's 96 registers do not hold
+// all it needs: the kernels but FEW spill 36 to 52 bytes.
 #include "decoder_attention.cuh"
 
 namespace s4d {

@@ -16,7 +16,12 @@
 // than the rows: 16,384 x 4,096 bf16 forward 69 us against 49 us.
 // Up to eight warps a row the registers are held to what lets three (backward: two) blocks of eight warps
 // share an SM: what a block waits for, the others load over.  16,384 x 4,096 bf16 both passes 172 us with
-// the compiler's choice (two and one), 158 so (136 by now); 7,213 x 1,001 f16 26.9 and 25.8.
+// the compiler's choice (two and one), 158 so; 7,213 x 1,001 f16 26.9 and 25.8.  The f32 forward kernels spill 20 to
+// 28 bytes for it and still gain where rows are long enough for the blocks to matter: 16,384 x 2,048 47.1 us with two,
+// 45.1 with three; 7,000 x 768 10.5 and 9.9; 28,800 x 512 21.4 either way; of the sizes tried only 16,384 x 4,096
+// loses (89 and 94).
+// Graph times by now, forward and backward: 16,384 x 4,096 bf16 51 and 90 us, f16 52 and 89; 28,800 x 512 f32 21 and
+// 33; 7,213 x 1,001 f16 11.5 and 17.2; 4,096 x 16,384 bf16 107 and 173.
 //
 // The sums over rows for dw and db stay in registers: a block adds its row groups through shared memory
 // and writes one fp32 partial row per block; a second launch adds the partial rows in block order.
@@ -329,8 +334,8 @@ __global__ void __launch_bounds__(Group<W>::kThreads, W <= 8 ? 2 : 1) norm_backw
         s1 = s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; ++i) s1 += red[buf][0][w0 + i], s2 += red[buf][1][w0 + i];
-      } else {  // as in group_sum (both passes of 16,384 x 4,096 bf16 158 us with the loads, 136 so; 4,096 x
-                // 16,384 472 and 273)
+      } else {  // as in group_sum (graph times of both passes, 16,384 x 4,096 bf16 158 us with the loads, 136
+                // so; 4,096 x 16,384 472 and 273)
         s1 = red[buf][0][w0 + threadIdx.x % W], s2 = red[buf][1][w0 + threadIdx.x % W];
 #pragma unroll
         for (int o = W / 2; o > 0; o >>= 1) {
